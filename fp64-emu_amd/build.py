@@ -12,6 +12,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -39,11 +41,19 @@ def _run(cmd, cwd=None):
     subprocess.run(cmd, check=True, cwd=cwd)
 
 
+# One object each, compiled side by side; the float64 product's first.
+HIP_SOURCES = ("fp64emu.hip", "f8.hip")
+
+
 def build_capi():
     hipcc = os.path.join(ROCM, "bin", "hipcc")
-    src = os.path.join(CSRC, "fp64emu.hip")
     tmp = CAPI_SO + ".tmp"
-    _run([hipcc, *HIP_FLAGS, "-shared", f"-I{INCLUDE}", src, "-o", tmp])
+    with tempfile.TemporaryDirectory() as work:
+        objects = [os.path.join(work, s + ".o") for s in HIP_SOURCES]
+        with ThreadPoolExecutor() as pool:
+            list(pool.map(_run, [[hipcc, *HIP_FLAGS, f"-I{INCLUDE}", "-c", os.path.join(CSRC, s), "-o", o]
+                                 for s, o in zip(HIP_SOURCES, objects)]))
+        _run([hipcc, *HIP_FLAGS, "-shared", *objects, "-o", tmp])
     os.replace(tmp, CAPI_SO)
     return CAPI_SO
 

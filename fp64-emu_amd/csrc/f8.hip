@@ -1,0 +1,1449 @@
+// Operands in 8-bit floating point with one float32 scale per block of 128,
+// for gfx950: the quantiser, products of such operands on the f8 matrix
+// instructions, and the gated activation whose checkpoint is held so.  The
+// entry points are those of include/fp64emu.h (fp64emu_*_f8*).
+//
+// A block with a = max(largest magnitude, 2^-110) has the scale s = a / F and
+// the codes q = rne8(x ((1 / a) F)), F the format's largest value.  The floor
+// keeps 1 / a finite for a block of zeros; the product exceeds F by at most three
+// float32 roundings, which the conversion rounds back to F.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "fp64emu.h"
+#include "status.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlk = 128;                         // elements that share a scale
+constexpr uint32_t kTinyBits = 0x08800000;        // 2^-110
+constexpr int64_t kMaxGridZ = 65535;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+typedef unsigned short v8s __attribute__((ext_vector_type(8)));
+
+__host__ __device__ constexpr float top_of(int fmt) { return fmt == FP64EMU_E4M3 ? 448.0f : 57344.0f; }
+
+// ---------------------------------------------------------------------------
+// Values in and codes out, eight at a time.
+
+__device__ __forceinline__ float bf16_value(unsigned short h) {
+  return __builtin_bit_cast(float, (uint32_t)h << 16);
+}
+__device__ __forceinline__ unsigned short bf16_round(float f) {   // nearest even; NaN stays NaN
+  const uint32_t u = __builtin_bit_cast(uint32_t, f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40);
+  return (unsigned short)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+}
+
+template <int kT>
+__device__ __forceinline__ float load1(const void* p, int64_t i) {
+  if constexpr (kT == FP64EMU_F32) return static_cast<const float*>(p)[i];
+  if constexpr (kT == FP64EMU_BF16) return bf16_value(static_cast<const unsigned short*>(p)[i]);
+  return (float)static_cast<const _Float16*>(p)[i];
+}
+template <int kT>
+__device__ __forceinline__ void store1(void* p, int64_t i, float v) {
+  if constexpr (kT == FP64EMU_F32) static_cast<float*>(p)[i] = v;
+  if constexpr (kT == FP64EMU_BF16) static_cast<unsigned short*>(p)[i] = bf16_round(v);
+  if constexpr (kT == FP64EMU_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
+}
+
+// Elements i .. i + 7 of p as floats, those from `valid` on as zeros.  vec: p
+// and every row start at multiples of 16 bytes.
+template <int kT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, int valid, bool vec, float (&v)[8]) {
+  if (vec && valid >= 8) {
+    if constexpr (kT == FP64EMU_F32) {
+      const v4f* q = reinterpret_cast<const v4f*>(static_cast<const float*>(p) + i);
+      const v4f a = q[0], b = q[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else {
+      const v8s a = *reinterpret_cast<const v8s*>(static_cast<const unsigned short*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = kT == FP64EMU_BF16 ? bf16_value(a[j])
+                                  : (float)__builtin_bit_cast(_Float16, (unsigned short)a[j]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < valid ? load1<kT>(p, i + j) : 0.0f;
+}
+
+template <int kT>
+__device__ __forceinline__ void store8(void* p, int64_t i, int valid, bool vec, const float (&v)[8]) {
+  if (vec && valid >= 8) {
+    if constexpr (kT == FP64EMU_F32) {
+      v4f* q = reinterpret_cast<v4f*>(static_cast<float*>(p) + i);
+      q[0] = v4f{v[0], v[1], v[2], v[3]};
+      q[1] = v4f{v[4], v[5], v[6], v[7]};
+    } else {
+      v8s a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        a[j] = kT == FP64EMU_BF16 ? bf16_round(v[j])
+                                  : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
+      *reinterpret_cast<v8s*>(static_cast<unsigned short*>(p) + i) = a;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < valid) store1<kT>(p, i + j, v[j]);
+}
+
+template <int kFmt>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int v = 0;
+  if constexpr (kFmt == FP64EMU_E4M3) {
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, v, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+  } else {
+    v = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, v, false);
+    v = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, v, true);
+  }
+  return (uint32_t)v;
+}
+
+// The values of four codes.
+template <int kFmt>
+__device__ __forceinline__ void values4(uint32_t w, float* v) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  v2f lo, hi;
+  if constexpr (kFmt == FP64EMU_E4M3) {
+    lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  } else {
+    lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false);
+    hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true);
+  }
+  v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
+}
+
+// Eight codes at q, the first `valid` of them.  vec: q a multiple of 8.
+__device__ __forceinline__ void put8(uint8_t* q, int valid, bool vec, v2u w) {
+  if (vec && valid >= 8) {
+    *reinterpret_cast<v2u*>(q) = w;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < valid) q[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+}
+
+// Magnitudes are compared as integers: for floats with the sign cleared that
+// is the order of their values, with NaN above infinity, so that one NaN in a
+// block becomes its maximum.
+__device__ __forceinline__ uint32_t mag(float f) { return __builtin_bit_cast(uint32_t, f) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// The maximum over the 16 lanes of a DPP row, in all of them.
+__device__ __forceinline__ uint32_t row16_max(uint32_t m) {
+  m = umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xf, 0xf, false));   // row_ror:8
+  m = umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xf, 0xf, false));
+  m = umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, false));
+  return umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float amax_of(uint32_t m) { return __builtin_bit_cast(float, umax(m, kTinyBits)); }
+
+// One quantised output as the kernels take it (an fp64emu_f8_t for one member
+// at a time); q null: not asked for.
+struct Out8 {
+  uint8_t* q;
+  float* s;
+  int64_t ld, stride, s_row, s_block, s_stride;
+  int vec;                   // q, ld and stride are multiples of 8
+};
+
+__device__ __forceinline__ void member(Out8& o, int64_t b) {
+  o.q += b * o.stride;
+  o.s += b * o.s_stride;
+}
+
+// ---------------------------------------------------------------------------
+// A 128 x 128 tile in the registers of 256 threads: thread t holds rows
+// 8 (t / 16) .. + 7 and columns 8 (t % 16) .. + 7 as v[row][column].  A row's
+// block is then 16 lanes of one DPP row, so its maximum takes four DPP steps;
+// a column's is spread over the 16 row groups: two lane exchanges and one pass
+// through LDS.  The transposed codes go through LDS too, in 8-byte chunks
+// (one thread's 8 rows of a column) whose place in the column's 128 bytes is
+// xored with the column group, so that neither the writes (16 column groups
+// of one row group) nor the reads (16 chunks of one column) collide.
+struct TileLds {
+  uint32_t colmax[4][kBlk];
+  uint8_t codes[kBlk * kBlk];
+};
+
+struct TilePlace {
+  int rg, cl;                // row and column group of the thread
+  int rows, cols;            // valid rows and columns of the tile
+};
+
+__device__ __forceinline__ TilePlace tile_place(int64_t row0, int64_t col0, int64_t M, int64_t K) {
+  return {(int)threadIdx.x >> 4, (int)threadIdx.x & 15, (int)(M - row0 < kBlk ? M - row0 : kBlk),
+          (int)(K - col0 < kBlk ? K - col0 : kBlk)};
+}
+
+// The rows' blocks of a tile at row0, block kb of the output.
+template <int kFmt>
+__device__ __forceinline__ void emit_rows(const float (&v)[8][8], const TilePlace& t, int64_t row0,
+                                          int64_t col0, int64_t kb, const Out8& o) {
+  const int left = t.cols - 8 * t.cl;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[p][j]));
+    const float a = amax_of(row16_max(m));
+    const float r = (1.0f / a) * top_of(kFmt);
+    const int row = 8 * t.rg + p;
+    if (row >= t.rows) continue;
+    const v2u w = {codes4<kFmt>(v[p][0] * r, v[p][1] * r, v[p][2] * r, v[p][3] * r),
+                   codes4<kFmt>(v[p][4] * r, v[p][5] * r, v[p][6] * r, v[p][7] * r)};
+    put8(o.q + (row0 + row) * o.ld + col0 + 8 * t.cl, left, o.vec, w);
+    if (t.cl == 0) o.s[(row0 + row) * o.s_row + kb * o.s_block] = a / top_of(kFmt);
+  }
+}
+
+// The columns' blocks: q row (col0 + column), byte row0 + row.  r[j]: F / a of
+// this thread's column j.
+template <int kFmt>
+__device__ __forceinline__ void emit_transposed(const float (&v)[8][8], const float (&r)[8],
+                                                const TilePlace& t, int64_t row0, int64_t col0,
+                                                const Out8& o, TileLds& lds) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const v2u w = {codes4<kFmt>(v[0][j] * r[j], v[1][j] * r[j], v[2][j] * r[j], v[3][j] * r[j]),
+                   codes4<kFmt>(v[4][j] * r[j], v[5][j] * r[j], v[6][j] * r[j], v[7][j] * r[j])};
+    *reinterpret_cast<v2u*>(lds.codes + (8 * t.cl + j) * kBlk + 8 * (t.rg ^ t.cl)) = w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int c = p * 16 + t.rg, chunk = t.cl;        // 16 lanes: one column's 128 bytes
+    const v2u w = *reinterpret_cast<const v2u*>(lds.codes + c * kBlk + 8 * (chunk ^ (c >> 3)));
+    if (c < t.cols) put8(o.q + (col0 + c) * o.ld + row0 + 8 * chunk, t.rows - 8 * chunk, o.vec, w);
+  }
+  __syncthreads();
+}
+
+// Column maxima of the tile into lds.colmax (over four waves); a barrier
+// stands between them and their readers.
+__device__ __forceinline__ void column_maxima(const float (&v)[8][8], const TilePlace& t, TileLds& lds) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m = umax(m, mag(v[p][j]));
+    m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+    if ((t.rg & 3) == 0) lds.colmax[t.rg >> 2][8 * t.cl + j] = m;
+  }
+  __syncthreads();
+}
+
+template <int kFmt>
+__device__ __forceinline__ void emit_cols(const float (&v)[8][8], const TilePlace& t, int64_t row0,
+                                          int64_t col0, int64_t mb, const Out8& o, TileLds& lds) {
+  column_maxima(v, t, lds);
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = 8 * t.cl + j;
+    const float a = amax_of(umax(umax(lds.colmax[0][c], lds.colmax[1][c]),
+                                 umax(lds.colmax[2][c], lds.colmax[3][c])));
+    r[j] = (1.0f / a) * top_of(kFmt);
+  }
+  if (threadIdx.x < kBlk) {
+    const int c = threadIdx.x;
+    const float a = amax_of(umax(umax(lds.colmax[0][c], lds.colmax[1][c]),
+                                 umax(lds.colmax[2][c], lds.colmax[3][c])));
+    if (c < t.cols) o.s[(col0 + c) * o.s_row + mb * o.s_block] = a / top_of(kFmt);
+  }
+  emit_transposed<kFmt>(v, r, t, row0, col0, o, lds);
+}
+
+// One scale for the whole tile, both orientations.
+template <int kFmt>
+__device__ __forceinline__ void emit_tile(const float (&v)[8][8], const TilePlace& t, int64_t row0,
+                                          int64_t col0, const Out8& rows, const Out8& cols,
+                                          TileLds& lds) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[p][j]));
+  m = row16_max(m);
+  m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+  m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+  if ((threadIdx.x & 63) == 0) lds.colmax[threadIdx.x >> 6][0] = m;
+  __syncthreads();
+  const float a = amax_of(umax(umax(lds.colmax[0][0], lds.colmax[1][0]),
+                               umax(lds.colmax[2][0], lds.colmax[3][0])));
+  const float r = (1.0f / a) * top_of(kFmt), s = a / top_of(kFmt);
+  const int64_t mb = row0 / kBlk, kb = col0 / kBlk;
+  if (rows.q) {
+    if (threadIdx.x == 0) rows.s[mb * rows.s_row + kb * rows.s_block] = s;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int row = 8 * t.rg + p;
+      const v2u w = {codes4<kFmt>(v[p][0] * r, v[p][1] * r, v[p][2] * r, v[p][3] * r),
+                     codes4<kFmt>(v[p][4] * r, v[p][5] * r, v[p][6] * r, v[p][7] * r)};
+      if (row < t.rows)
+        put8(rows.q + (row0 + row) * rows.ld + col0 + 8 * t.cl, t.cols - 8 * t.cl, rows.vec, w);
+    }
+  }
+  if (cols.q) {
+    if (threadIdx.x == 0) cols.s[kb * cols.s_row + mb * cols.s_block] = s;
+    const float rr[8] = {r, r, r, r, r, r, r, r};
+    emit_transposed<kFmt>(v, rr, t, row0, col0, cols, lds);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Quantiser.
+struct QuantArgs {
+  const void* x;
+  int64_t batch, M, K, ldx, stride_x;
+  int64_t kblocks;
+  int vec, tiles;
+  Out8 rows, cols;
+};
+
+// One work group per 128 x 128 tile (blocks along K fastest: a row of tiles
+// reads whole rows of x), every value read once.
+template <int kT, int kFmt>
+__global__ void __launch_bounds__(kThreads) quant_tile_kernel(QuantArgs g) {
+  __shared__ TileLds lds;
+  const int64_t kb = blockIdx.x % g.kblocks, mb = blockIdx.x / g.kblocks;
+  const int64_t row0 = mb * kBlk, col0 = kb * kBlk;
+  const TilePlace t = tile_place(row0, col0, g.M, g.K);
+  for (int64_t b = blockIdx.z; b < g.batch; b += gridDim.z) {
+    Out8 rows = g.rows, cols = g.cols;
+    if (rows.q) member(rows, b);
+    if (cols.q) member(cols, b);
+    float v[8][8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int row = 8 * t.rg + p;
+      const int valid = row < t.rows ? t.cols - 8 * t.cl : 0;
+      load8<kT>(g.x, b * g.stride_x + (row0 + row) * g.ldx + col0 + 8 * t.cl, valid, g.vec, v[p]);
+    }
+    if (g.tiles) {
+      emit_tile<kFmt>(v, t, row0, col0, rows, cols, lds);
+    } else {
+      if (rows.q) emit_rows<kFmt>(v, t, row0, col0, kb, rows);
+      if (cols.q) emit_cols<kFmt>(v, t, row0, col0, mb, cols, lds);
+    }
+    __syncthreads();
+  }
+}
+
+// Rows only, few of them: 16 lanes per block, so that one token's blocks
+// spread over work groups instead of filling 1 row in 128 of a tile.
+template <int kT, int kFmt>
+__global__ void __launch_bounds__(kThreads) quant_rows_kernel(QuantArgs g) {
+  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
+  const int cl = threadIdx.x & 15;
+  const int64_t row = unit / g.kblocks, kb = unit % g.kblocks;
+  const int64_t col = kb * kBlk + 8 * cl;
+  const bool live = row < g.M;
+  const int valid = live && col < g.K ? (int)(g.K - col < 8 ? g.K - col : 8) : 0;
+  for (int64_t b = blockIdx.z; b < g.batch; b += gridDim.z) {
+    Out8 o = g.rows;
+    member(o, b);
+    float v[8];
+    load8<kT>(g.x, b * g.stride_x + row * g.ldx + col, valid, g.vec, v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[j]));
+    const float a = amax_of(row16_max(m));
+    const float r = (1.0f / a) * top_of(kFmt);
+    const v2u w = {codes4<kFmt>(v[0] * r, v[1] * r, v[2] * r, v[3] * r),
+                   codes4<kFmt>(v[4] * r, v[5] * r, v[6] * r, v[7] * r)};
+    if (!live) continue;
+    put8(o.q + row * o.ld + col, valid, o.vec, w);
+    if (cl == 0) o.s[row * o.s_row + kb * o.s_block] = a / top_of(kFmt);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gated activation.  1 / (1 + e^-g): e^-g = 2^(-g log2 e) with the product's
+// rounding error carried into the result (as a relative term, ln 2 times the
+// error), so that large |g| keeps float32 accuracy with the hardware's 2^x.
+__device__ __forceinline__ float sigmoid(float g) {
+  constexpr float kL = 1.44269502f, kLlo = 1.92596303e-8f;      // log2 e = kL + kLlo
+  const float t = -g * kL;
+  const float lo = fmaf(-g, kL, -t) - g * kLlo;
+  float e = __builtin_amdgcn_exp2f(t);
+  // Outside the normal range of 2^t the term is left out: there it would be inf - inf.
+  if (fabsf(t) < 126.0f) e = fmaf(e, lo * 0.693147182f, e);
+  return 1.0f / (1.0f + e);
+}
+
+struct SwigluArgs {
+  const void* h;
+  int64_t M, F, ldh;
+  int64_t fblocks;
+  int vec;
+  void* y;
+  int64_t ldy;
+  int vec_y;
+  Out8 keep, rows, cols;
+};
+
+// One work group per 128 x 128 tile of y.
+template <int kT>
+__global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
+  constexpr int kF = FP64EMU_E4M3;
+  __shared__ TileLds lds;
+  const int64_t fb = blockIdx.x % a.fblocks, mb = blockIdx.x / a.fblocks;
+  const int64_t row0 = mb * kBlk, col0 = fb * kBlk;
+  const TilePlace t = tile_place(row0, col0, a.M, a.F);
+  float g[8][8], u[8][8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int row = 8 * t.rg + p;
+    const int valid = row < t.rows ? t.cols - 8 * t.cl : 0;
+    const int64_t i = (row0 + row) * a.ldh + col0 + 8 * t.cl;
+    load8<kT>(a.h, i, valid, a.vec, g[p]);
+    load8<kT>(a.h, i + a.F, valid, a.vec, u[p]);
+  }
+  if (a.keep.q) {
+    emit_rows<kF>(g, t, row0, col0, fb, a.keep);
+    emit_rows<kF>(u, t, row0, a.F + col0, a.fblocks + fb, a.keep);
+  }
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[p][j] = g[p][j] * sigmoid(g[p][j]) * u[p][j];
+  if (a.y) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int row = 8 * t.rg + p;
+      store8<kT>(a.y, (row0 + row) * a.ldy + col0 + 8 * t.cl, row < t.rows ? t.cols - 8 * t.cl : 0,
+                 a.vec_y, g[p]);
+    }
+  }
+  if (a.rows.q) emit_rows<kF>(g, t, row0, col0, fb, a.rows);
+  if (a.cols.q) emit_cols<kF>(g, t, row0, col0, mb, a.cols, lds);
+}
+
+struct SwigluGradArgs {
+  const void* dy;
+  int64_t M, F, ldy;
+  int64_t fblocks;
+  int vec;
+  Out8 keep;                 // read
+  void* dh;
+  int64_t ldh;
+  int vec_h;
+  Out8 rows, cols;
+};
+
+// Eight values of a kept half: codes times the block's scale.
+template <int kFmt>
+__device__ __forceinline__ void kept8(const uint8_t* q, int valid, bool vec, float s, float (&v)[8]) {
+  v2u w = {0u, 0u};
+  if (vec && valid >= 8) {
+    w = *reinterpret_cast<const v2u*>(q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < valid) w[j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
+  }
+  values4<kFmt>(w[0], v);
+  values4<kFmt>(w[1], v + 4);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] * s : 0.0f;
+}
+
+template <int kT, int kO>
+__global__ void __launch_bounds__(kThreads) swiglu_grad_kernel(SwigluGradArgs a) {
+  constexpr int kF = FP64EMU_E4M3;
+  __shared__ TileLds lds;
+  const int64_t fb = blockIdx.x % a.fblocks, mb = blockIdx.x / a.fblocks;
+  const int64_t row0 = mb * kBlk, col0 = fb * kBlk;
+  const TilePlace t = tile_place(row0, col0, a.M, a.F);
+  float dg[8][8], du[8][8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int64_t row = row0 + 8 * t.rg + p;
+    const int valid = row < a.M ? t.cols - 8 * t.cl : 0;
+    float dy[8], g[8], u[8];
+    load8<kT>(a.dy, row * a.ldy + col0 + 8 * t.cl, valid, a.vec, dy);
+    float sg = 0.0f, su = 0.0f;
+    if (valid > 0) {
+      sg = a.keep.s[row * a.keep.s_row + fb * a.keep.s_block];
+      su = a.keep.s[row * a.keep.s_row + (a.fblocks + fb) * a.keep.s_block];
+    }
+    const uint8_t* q = a.keep.q + row * a.keep.ld + col0 + 8 * t.cl;
+    kept8<kF>(q, valid, a.keep.vec, sg, g);
+    kept8<kF>(q + a.F, valid, a.keep.vec && (a.F & 7) == 0, su, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = sigmoid(g[j]);
+      du[p][j] = dy[j] * g[j] * s;
+      dg[p][j] = dy[j] * u[j] * s * fmaf(g[j], 1.0f - s, 1.0f);
+    }
+  }
+  if (a.dh) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int64_t row = row0 + 8 * t.rg + p;
+      const int valid = row < a.M ? t.cols - 8 * t.cl : 0;
+      const int64_t i = row * a.ldh + col0 + 8 * t.cl;
+      store8<kO>(a.dh, i, valid, a.vec_h, dg[p]);
+      store8<kO>(a.dh, i + a.F, valid, a.vec_h, du[p]);
+    }
+  }
+  if (a.rows.q) {
+    emit_rows<kF>(dg, t, row0, col0, fb, a.rows);
+    emit_rows<kF>(du, t, row0, a.F + col0, a.fblocks + fb, a.rows);
+  }
+  if (a.cols.q) {
+    emit_cols<kF>(dg, t, row0, col0, mb, a.cols, lds);
+    emit_cols<kF>(du, t, row0, a.F + col0, mb, a.cols, lds);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products.  out^T = B A^T on v_mfma_f32_16x16x128_f8f6f4: one instruction
+// covers one block of 128 along K, so its float32 result is scaled by
+// sA sB and added to the running sums, which stay in float32 registers.  B's
+// rows are the instruction's first operand: lane l then holds output column
+// (token) l % 16 and four successive n, so that a tile scale of B and a row
+// scale of A make one factor per lane, and the four values are one store.
+//
+// Operand order: lane l holds 32 bytes of row l % 16, at k = 32 (l / 16).
+// Which k those are to the instruction does not matter as long as A and B
+// agree, since every k of a block has the same scales.
+
+struct MmArgs {
+  const uint8_t *A, *B;
+  const float *sA, *sB;
+  void* out;
+  float* part;                       // partial sums [splits, batch, M, N] if splits > 1
+  int64_t lda, ldb, strideA, strideB;
+  int64_t sA_row, sA_blk, sA_str, sB_row, sB_blk, sB_str;
+  int64_t ldo, stride_o;
+  int64_t K;
+  int M, N, batch;
+  int nkb, splits, kb_per_split;     // blocks along K: of all, and of one split
+  int tiles_m, tiles_n;
+  int dtype, accumulate;
+  int b_tiles;                       // B's scales by tiles
+  int vec_o;                         // out's rows start at multiples of 4 elements
+};
+
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+
+// A fragment as the block's sum takes it.  Its 32 codes as they are, for one
+// v_mfma_f32_16x16x128_f8f6f4; or as bfloat16, which holds both formats'
+// values, for four v_mfma_f32_16x16x32_bf16.  The former aligns the products of
+// neighbouring k to the largest before it adds them and keeps about 13 bits below
+// it (measured: of 2^16 + 2^(16 - d) at adjacent k the second is lost from d = 14
+// on; at k eight apart it is kept to float32's own 23): an error of 2e-5 to 4e-5 of
+// a block's sum, far below the rounding of a bfloat16 or float16 result and
+// far above that of a float32 one.  The latter rounds as float32 sums do (1e-8
+// there), at half the rate and the conversions' cost.  So: the first for
+// 16-bit outputs of large products, the second for float32 ones, and where the
+// product waits for memory anyway.
+template <bool kExact, int kFmt>
+struct Frag {
+  v8i c;
+  __device__ __forceinline__ explicit Frag(const v8i& codes) : c(codes) {}
+  __device__ __forceinline__ Frag() {}
+};
+template <int kFmt>
+struct Frag<true, kFmt> {
+  v8b c[4];
+  __device__ __forceinline__ Frag() {}
+  __device__ __forceinline__ explicit Frag(const v8i& codes) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v2b w[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t x = (uint32_t)codes[2 * j + h];
+        if constexpr (kFmt == FP64EMU_E4M3) {
+          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false);
+          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true);
+        } else {
+          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, false);
+          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, true);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[j][i] = w[i >> 1][i & 1];
+    }
+  }
+};
+
+template <bool kExact, int kFB, int kFA>
+__device__ __forceinline__ v4f block_sum(const Frag<kExact, kFB>& b, const Frag<kExact, kFA>& a) {
+  v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (kExact) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.c[j], a.c[j], p, 0, 0, 0);
+  } else {
+    p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.c, a.c, p, kFB, kFA, 0, 0, 0, 0);
+  }
+  return p;
+}
+
+__device__ __forceinline__ v8i join(const v4i& a, const v4i& b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 16 bytes of a row at k, those past K as zero codes (whatever the memory
+// holds there, if it is memory at all).  Any alignment.
+__device__ __forceinline__ v4i load16_masked(const uint8_t* row, int64_t k, int64_t K) {
+  v4i v = {0, 0, 0, 0};
+  if (k + 16 <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (k + j < K) v[j >> 2] |= (int)((uint32_t)row[k + j] << (8 * (j & 3)));
+  }
+  return v;
+}
+
+// Four successive outputs (m, n .. n + 3).
+__device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v) {
+  const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
+  if (g.splits > 1) {
+    return;
+  }
+  const int64_t i = b * g.stride_o + m * g.ldo + n;
+  if (g.vec_o && valid == 4) {
+    if (g.dtype == FP64EMU_F32) {
+      v4f* o = reinterpret_cast<v4f*>(static_cast<float*>(g.out) + i);
+      if (g.accumulate) v += *o;
+      *o = v;
+    } else {
+      typedef unsigned short v4s __attribute__((ext_vector_type(4)));
+      v4s* o = reinterpret_cast<v4s*>(static_cast<unsigned short*>(g.out) + i);
+      const bool bf = g.dtype == FP64EMU_BF16;
+      if (g.accumulate) {
+        const v4s w = *o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] += bf ? bf16_value(w[j]) : (float)__builtin_bit_cast(_Float16, (unsigned short)w[j]);
+      }
+      v4s r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] = bf ? bf16_round(v[j]) : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
+      *o = r;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= valid) break;
+    float x = v[j];
+    if (g.dtype == FP64EMU_F32) {
+      if (g.accumulate) x += load1<FP64EMU_F32>(g.out, i + j);
+      store1<FP64EMU_F32>(g.out, i + j, x);
+    } else if (g.dtype == FP64EMU_BF16) {
+      if (g.accumulate) x += load1<FP64EMU_BF16>(g.out, i + j);
+      store1<FP64EMU_BF16>(g.out, i + j, x);
+    } else {
+      if (g.accumulate) x += load1<FP64EMU_F16>(g.out, i + j);
+      store1<FP64EMU_F16>(g.out, i + j, x);
+    }
+  }
+}
+
+// The partial sums of one split instead of an output.
+__device__ __forceinline__ void store_part(const MmArgs& g, int split, int64_t b, int64_t m, int64_t n, v4f v) {
+  float* o = g.part + (((int64_t)split * g.batch + b) * g.M + m) * g.N + n;
+  const int64_t left = g.N - n;
+  if (left >= 4 && (g.N & 3) == 0) {
+    *reinterpret_cast<v4f*>(o) = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < left) o[j] = v[j];
+}
+
+// Sum of the splits' partial sums, in their order.
+__global__ void __launch_bounds__(kThreads) sum_parts_kernel(MmArgs g) {
+  const int64_t row_quads = (g.N + 3) / 4, total = (int64_t)g.batch * g.M * row_quads;
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  const int splits = g.splits;
+  g.splits = 1;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += step) {
+    const int64_t bm = i / row_quads, n = (i - bm * row_quads) * 4;
+    const float* p = g.part + bm * g.N + n;
+    const int64_t one = (int64_t)g.batch * g.M * g.N, left = g.N - n;
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (left >= 4 && (g.N & 3) == 0) {
+      for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const v4f*>(p + s * one);
+    } else {
+      for (int s = 0; s < splits; ++s)
+        for (int j = 0; j < 4; ++j)
+          if (j < left) v[j] += p[s * one + j];
+    }
+    store_out(g, bm / g.M, bm % g.M, n, v);
+  }
+}
+
+// s_waitcnt: at most `vm` vector-memory operations outstanding, LDS done.
+template <int vm>
+__device__ __forceinline__ void wait_vm_lgkm0() {
+  static_assert(vm >= 0 && vm < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt((vm & 15) | (7 << 4) | (0 << 8) | ((vm >> 4) << 14));
+}
+// Barrier without the fences of __syncthreads(), which would drain the copies in flight.
+__device__ __forceinline__ void barrier_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// A buffer resource over `bytes` bytes at a work-group-uniform p.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint32_t bytes) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
+                                           __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+
+// Tiles of kBM x kBN outputs, kWM x kWN waves of (kBM / kWM) x (kBN / kWN).
+// A stage holds one block of K: kBN rows of B and kBM rows of A of 128 bytes
+// each, then their scales.  A row's eight 16-byte chunks are xored with the
+// row, so that eight lanes reading one chunk of eight rows reach eight places
+// (the copies write LDS in lane order: the lane that owns a place fetches the
+// chunk that belongs there).
+template <int kBM_, int kBN_, int kWM_, int kWN_>
+struct MmShape {
+  static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_;
+  static constexpr int kWaves = kWM * kWN, kT = 64 * kWaves;
+  static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;   // 16 x 16 tiles per wave
+  static constexpr int kCopB = kBN / 8 / kWaves, kCopA = kBM / 8 / kWaves;   // copies per wave
+  static constexpr int kCopies = kCopA + kCopB + 1;
+  static constexpr int kOffA = kBN * kBlk, kOffS = (kBN + kBM) * kBlk;
+  static constexpr int kStage = kOffS + 4 * (kBN + kBM);
+  static_assert(kT == kBM + kBN, "one scale per thread and stage");
+  static_assert(2 * kStage <= 160 * 1024, "two stages in LDS");
+};
+
+template <class S, bool kExact, int kFA, int kFB, bool kRowB>
+__device__ __forceinline__ void mm_tile(const MmArgs& g) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wm = wave % S::kWM, wn = wave / S::kWM;
+
+  // Work item: member and split, then the tile.  Work group i runs on XCD i % 8:
+  // each XCD takes a contiguous run of tiles, in panels of 8 tile rows, so that
+  // its 32 CUs share operand panels in its L2.
+  const int tiles = g.tiles_m * g.tiles_n;
+  int item;
+  {
+    const int total = (int)gridDim.x, x = (int)blockIdx.x & 7, i = (int)blockIdx.x >> 3;
+    const int q = total >> 3, r = total & 7;
+    item = x * q + (x < r ? x : r) + i;
+  }
+  const int outer = item / tiles;
+  item -= outer * tiles;
+  const int b = outer % g.batch, split = outer / g.batch;
+  constexpr int kPanel = 8;
+  const int per = kPanel * g.tiles_n, panel = item / per, left = g.tiles_m - panel * kPanel;
+  const int high = left < kPanel ? left : kPanel, in = item - panel * per;
+  const int tm = panel * kPanel + in % high, tn = in / high;
+  const int64_t m0 = (int64_t)tm * S::kBM, n0 = (int64_t)tn * S::kBN;
+  const int rowsA = (int)(g.M - m0 < S::kBM ? g.M - m0 : S::kBM);
+  const int rowsB = (int)(g.N - n0 < S::kBN ? g.N - n0 : S::kBN);
+  const int kb0 = split * g.kb_per_split;
+  const int kb1 = kb0 + g.kb_per_split < g.nkb ? kb0 + g.kb_per_split : g.nkb;
+  const int nk = kb1 - kb0;
+
+  const uint8_t* A = g.A + b * g.strideA + m0 * g.lda;
+  const uint8_t* B = g.B + b * g.strideB + n0 * g.ldb;
+  // Up to the end of the last row's last 16 bytes (rows are 16-byte aligned here).
+  const int64_t K16 = (g.K + 15) & ~(int64_t)15;
+  const __amdgpu_buffer_rsrc_t srcA = buffer_src(A, (uint32_t)((rowsA - 1) * g.lda + K16));
+  const __amdgpu_buffer_rsrc_t srcB = buffer_src(B, (uint32_t)((rowsB - 1) * g.ldb + K16));
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  uint32_t offA[S::kCopA], offB[S::kCopB];       // rows past the end repeat the last one
+#pragma unroll
+  for (int i = 0; i < S::kCopB; ++i) {
+    const int r = (i * S::kWaves + wave) * 8 + (lane >> 3);
+    offB[i] = (uint32_t)((r < rowsB ? r : rowsB - 1) * g.ldb + chunk);
+  }
+#pragma unroll
+  for (int i = 0; i < S::kCopA; ++i) {
+    const int r = (i * S::kWaves + wave) * 8 + (lane >> 3);
+    offA[i] = (uint32_t)((r < rowsA ? r : rowsA - 1) * g.lda + chunk);
+  }
+  // Thread t < kBN: the scale of B's row t; else of A's row t - kBN (whole waves of either).
+  const float* sp;
+  const bool forB = wave * 64 < S::kBN;
+  const int64_t sblk = forB ? g.sB_blk : g.sA_blk;
+  {
+    const int t = threadIdx.x;
+    if (forB) {
+      const int64_t r = n0 + (t < rowsB ? t : rowsB - 1);
+      sp = g.sB + b * g.sB_str + (kRowB ? r : r / kBlk) * g.sB_row;
+    } else {
+      const int64_t r = t - S::kBN < rowsA ? t - S::kBN : rowsA - 1;
+      sp = g.sA + b * g.sA_str + (m0 + r) * g.sA_row;
+    }
+    sp += kb0 * sblk;
+  }
+
+  // Block kb into stage st.  The block's offset is part of each lane's where it
+  // ends past K, so that the resource's bound covers it.
+  auto issue = [&](int kb, int st) {
+    lds_u8* stage = (lds_u8*)lds + st * S::kStage;
+#pragma unroll
+    for (int i = 0; i < S::kCopB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcB, stage + (i * S::kWaves + wave) * 1024, 16,
+                                               (int)offB[i] + kb * kBlk, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < S::kCopA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcA, stage + S::kOffA + (i * S::kWaves + wave) * 1024, 16,
+                                               (int)offA[i] + kb * kBlk, 0, 0, 0);
+    __builtin_amdgcn_global_load_lds(sp, stage + S::kOffS + wave * 256, 4, 0, 0);
+    sp += sblk;
+  };
+  // Codes past K in a stage become zeros (the memory there is padding or
+  // another row): thread t has row t of the stage, B's rows first.
+  const int tail = (int)(g.K & (kBlk - 1));
+  auto clear_tail = [&](int st) {
+    uint8_t* row = lds + st * S::kStage + threadIdx.x * kBlk;
+    for (int c = tail >> 4; c < 8; ++c) {
+      v4i* w = reinterpret_cast<v4i*>(row + ((c ^ (threadIdx.x & 7)) << 4));
+      v4i v = *w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int left = tail - 16 * c - 4 * j;             // bytes of this word before K
+        v[j] = left >= 4 ? v[j] : left <= 0 ? 0 : v[j] & (int)((1u << (8 * left)) - 1);
+      }
+      *w = v;
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);                       // lgkmcnt(0)
+    barrier_lds();
+  };
+
+  v4f acc[S::kTN][S::kTM];
+#pragma unroll
+  for (int x = 0; x < S::kTN; ++x)
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) acc[x][y] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int fr = lane & 15, fg = lane >> 4;
+  const int slot = ((2 * fg) ^ (fr & 7)) * 16;               // the second chunk's place is slot ^ 16
+  const int fragB = (wn * S::kTN * 16 + fr) * kBlk, fragA = S::kOffA + (wm * S::kTM * 16 + fr) * kBlk;
+  auto frag = [&](const uint8_t* stage, int base) {
+    return join(*reinterpret_cast<const v4i*>(stage + base + slot),
+                *reinterpret_cast<const v4i*>(stage + base + (slot ^ 16)));
+  };
+  Frag<kExact, kFA> fa[S::kTM];
+  v8i fb;
+  float sa[S::kTM];
+  // A's fragments and scales of a stage and B's first fragment.
+  auto open = [&](const uint8_t* stage) {
+    const float* sc = reinterpret_cast<const float*>(stage + S::kOffS);
+    fb = frag(stage, fragB);
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) fa[y] = Frag<kExact, kFA>(frag(stage, fragA + y * 16 * kBlk));
+    const float st = kRowB ? 1.0f : sc[wn * S::kTN * 16];
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) {
+      sa[y] = sc[S::kBN + wm * S::kTM * 16 + y * 16 + fr];
+      if constexpr (!kRowB) sa[y] *= st;
+    }
+  };
+  // acc[x] += the scaled block sums p.
+  auto add = [&](int x, const v4f (&p)[S::kTM], const v4f& sb) {
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[x][y][i] = fmaf(p[y][i], kRowB ? sa[y] * sb[i] : sa[y], acc[x][y][i]);
+    // Here, and not wherever the compiler finds room: it moved all of a block's
+    // sums behind its last tile, with every p kept until then.
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) asm volatile("" : "+v"(acc[x][y]));
+  };
+
+  // One barrier per block: when a wave has B's last fragment of stage i & 1 in
+  // registers and its copies of block i + 1 (issued a whole block earlier) have
+  // landed, it waits for the others; the stage is then free for block i + 2 and
+  // the next one is whole.  Inside a block, row x of tiles issues its
+  // instructions while row x - 1's sums are scaled and B's next fragment is on
+  // its way; the scheduling barriers keep the compiler from reading the
+  // fragments ahead (which spilled 75 registers).
+  issue(kb0, 0);
+  if (nk > 1) issue(kb0 + 1, 1);
+  if (nk > 1) wait_vm_lgkm0<S::kCopies>();
+  else wait_vm_lgkm0<0>();
+  barrier_lds();
+  if (tail && nk == 1 && kb1 == g.nkb) clear_tail(0);
+  open(lds);
+  for (int i = 0; i < nk; ++i) {
+    const uint8_t* stage = lds + (i & 1) * S::kStage;
+    const float* sc = reinterpret_cast<const float*>(stage + S::kOffS);
+    v4f p[2][S::kTM], sb[2];
+#pragma unroll
+    for (int x = 0; x < S::kTN; ++x) {
+      v8i next;
+      if (x + 1 < S::kTN) next = frag(stage, fragB + (x + 1) * 16 * kBlk);
+      if constexpr (kRowB)
+        sb[x & 1] = *reinterpret_cast<const v4f*>(sc + wn * S::kTN * 16 + x * 16 + 4 * fg);
+      if (x + 1 == S::kTN) {
+        wait_vm_lgkm0<0>();
+        barrier_lds();
+        if (i + 2 < nk) issue(kb0 + i + 2, i & 1);
+      }
+      const Frag<kExact, kFB> fbx(fb);
+#pragma unroll
+      for (int y = 0; y < S::kTM; ++y) p[x & 1][y] = block_sum<kExact, kFB, kFA>(fbx, fa[y]);
+      if (x > 0) add(x - 1, p[(x - 1) & 1], sb[(x - 1) & 1]);
+      if (x + 1 < S::kTN) fb = next;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    add(S::kTN - 1, p[(S::kTN - 1) & 1], sb[(S::kTN - 1) & 1]);
+    if (i + 1 < nk) {
+      if (tail && i + 2 == nk && kb1 == g.nkb) clear_tail((i + 1) & 1);
+      open(lds + ((i + 1) & 1) * S::kStage);
+    }
+  }
+
+#pragma unroll
+  for (int y = 0; y < S::kTM; ++y) {
+    const int64_t m = m0 + (wm * S::kTM + y) * 16 + fr;
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int x = 0; x < S::kTN; ++x) {
+      const int64_t n = n0 + (wn * S::kTN + x) * 16 + 4 * fg;
+      if (n >= g.N) continue;
+      if (g.splits > 1) store_part(g, split, b, m, n, acc[x][y]);
+      else store_out(g, b, m, n, acc[x][y]);
+    }
+  }
+}
+
+template <class S, bool kExact, int kFA, int kFB, bool kRowB>
+__global__ void __launch_bounds__(S::kT, 2) mm_tile_kernel(MmArgs g) {
+  mm_tile<S, kExact, kFA, kFB, kRowB>(g);
+}
+
+// Rows of any alignment into rows of a multiple of 16 bytes, 16 bytes a thread.
+__global__ void __launch_bounds__(kThreads) pack_rows_kernel(const uint8_t* q, int64_t ld, int64_t stride,
+                                                             uint8_t* to, int64_t rows, int64_t total,
+                                                             int64_t K) {
+  const int64_t chunks = (K + 15) / 16, step = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total * chunks; i += step) {
+    const int64_t r = i / chunks, c = i - r * chunks, b = r / rows;
+    const v4i v = load16_masked(q + b * stride + (r - b * rows) * ld, c * 16, K);
+    *reinterpret_cast<v4i*>(to + i * 16) = v;
+  }
+}
+
+// Few rows of A: the product reads B once and little else.  A work group has
+// kTN x 16 rows of B and all waves on them, wave w at blocks w, w + kFewWaves,
+// ... of K; fragments come straight from memory (lane l's 32 bytes are the
+// instruction's operand as they lie in the row), and the waves' sums meet in LDS.
+constexpr int kFewWaves = 8;
+
+template <int kTM, int kTN, int kU, int kFA, int kFB, bool kRowB>
+__global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
+  __shared__ v4f red[kFewWaves][kTN * kTM][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int outer = blockIdx.x / tiles, item = blockIdx.x - outer * tiles;
+  const int b = outer % g.batch, split = outer / g.batch;
+  const int64_t m0 = (int64_t)(item / g.tiles_n) * (16 * kTM), n0 = (int64_t)(item % g.tiles_n) * (16 * kTN);
+  const int kb0 = split * g.kb_per_split;
+  const int kb1 = kb0 + g.kb_per_split < g.nkb ? kb0 + g.kb_per_split : g.nkb;
+
+  const uint8_t *pa[kTM], *pb[kTN];
+  const float *sa[kTM], *sb[kTN][kRowB ? 4 : 1];
+#pragma unroll
+  for (int y = 0; y < kTM; ++y) {
+    const int64_t m = m0 + y * 16 + fr < g.M ? m0 + y * 16 + fr : g.M - 1;
+    pa[y] = g.A + b * g.strideA + m * g.lda;
+    sa[y] = g.sA + b * g.sA_str + m * g.sA_row;
+  }
+#pragma unroll
+  for (int x = 0; x < kTN; ++x) {
+    const int64_t n = n0 + x * 16 + fr < g.N ? n0 + x * 16 + fr : g.N - 1;
+    pb[x] = g.B + b * g.strideB + n * g.ldb;
+#pragma unroll
+    for (int i = 0; i < (kRowB ? 4 : 1); ++i) {
+      const int64_t r = n0 + x * 16 + (kRowB ? 4 * fg + i : 0);
+      sb[x][i] = g.sB + b * g.sB_str + (kRowB ? (r < g.N ? r : g.N - 1) : r / kBlk) * g.sB_row;
+    }
+  }
+
+  v4f acc[kTN][kTM];
+#pragma unroll
+  for (int x = 0; x < kTN; ++x)
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) acc[x][y] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto frag = [&](const uint8_t* row, int kb) {
+    const int64_t k = (int64_t)kb * kBlk + 32 * fg;
+    return join(load16_masked(row, k, g.K), load16_masked(row, k + 16, g.K));
+  };
+  auto whole = [&](const uint8_t* row, int kb) {
+    v8i v;
+    __builtin_memcpy(&v, row + (int64_t)kb * kBlk + 32 * fg, 32);
+    return v;
+  };
+  auto step = [&](const v8i (&cb)[kTN], const v8i (&ca)[kTM], int kb) {
+    Frag<true, kFA> fa[kTM];
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) fa[y] = Frag<true, kFA>(ca[y]);
+    float s[kTM];
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) s[y] = sa[y][kb * g.sA_blk];
+#pragma unroll
+    for (int x = 0; x < kTN; ++x) {
+      float t[kRowB ? 4 : 1];
+#pragma unroll
+      for (int i = 0; i < (kRowB ? 4 : 1); ++i) t[i] = sb[x][i][kb * g.sB_blk];
+      const Frag<true, kFB> fb(cb[x]);
+#pragma unroll
+      for (int y = 0; y < kTM; ++y) {
+        const v4f p = block_sum<true, kFB, kFA>(fb, fa[y]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[x][y][i] = fmaf(p[i], s[y] * t[kRowB ? i : 0], acc[x][y][i]);
+      }
+    }
+  };
+
+  const int full = (int)(g.K / kBlk) < kb1 ? (int)(g.K / kBlk) : kb1;    // blocks before it are whole
+  int kb = kb0 + wave;
+  for (; kb + (kU - 1) * kFewWaves < full; kb += kU * kFewWaves) {
+    v8i fb[kU][kTN], fa[kU][kTM];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+#pragma unroll
+      for (int x = 0; x < kTN; ++x) fb[u][x] = whole(pb[x], kb + u * kFewWaves);
+#pragma unroll
+      for (int y = 0; y < kTM; ++y) fa[u][y] = whole(pa[y], kb + u * kFewWaves);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) step(fb[u], fa[u], kb + u * kFewWaves);
+  }
+  for (; kb < kb1; kb += kFewWaves) {
+    v8i fb[kTN], fa[kTM];
+#pragma unroll
+    for (int x = 0; x < kTN; ++x) fb[x] = frag(pb[x], kb);
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) fa[y] = frag(pa[y], kb);
+    step(fb, fa, kb);
+  }
+
+#pragma unroll
+  for (int x = 0; x < kTN; ++x)
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) red[wave][x * kTM + y][lane] = acc[x][y];
+  __syncthreads();
+  for (int t = wave; t < kTN * kTM; t += kFewWaves) {
+    v4f v = red[0][t][lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) v += red[w][t][lane];
+    const int64_t m = m0 + (t % kTM) * 16 + fr, n = n0 + (t / kTM) * 16 + 4 * fg;
+    if (m >= g.M || n >= g.N) continue;
+    if (g.splits > 1) store_part(g, split, b, m, n, v);
+    else store_out(g, b, m, n, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+using Tile256 = MmShape<256, 256, 4, 2>;
+using Tile128 = MmShape<128, 128, 2, 2>;
+
+struct MmPlan {
+  int form;                  // 0: few rows, 1: 128 x 128 tiles, 2: 256 x 256 tiles
+  int tile_m, tile_n;
+  int64_t tiles_m, tiles_n;
+  int splits, kb_per_split;
+};
+
+constexpr int kCUs = 256;
+
+MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
+  MmPlan p{};
+  const int64_t nkb = (K + kBlk - 1) / kBlk;
+  auto shape = [&](int form, int tm, int tn) {
+    p.form = form;
+    p.tile_m = tm;
+    p.tile_n = tn;
+    p.tiles_m = (M + tm - 1) / tm;
+    p.tiles_n = (N + tn - 1) / tn;
+  };
+  if (M <= 64) {
+    const int tm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    shape(0, tm, M <= 16 ? 16 : 32);
+  } else {
+    shape(2, 256, 256);
+    if (dtype == FP64EMU_F32 || batch * p.tiles_m * p.tiles_n < kCUs) shape(1, 128, 128);
+  }
+  // Splits: where the tiles leave compute units idle and each split keeps
+  // at least 8 blocks of K.
+  const int64_t groups = std::max<int64_t>(batch * p.tiles_m * p.tiles_n, 1);
+  const int64_t want = p.form == 0 ? 2 * kCUs : p.form == 1 ? 2 * kCUs : kCUs;
+  int64_t s = std::min<int64_t>(std::max<int64_t>(want / groups, 1), std::max<int64_t>(nkb / 8, 1));
+  s = std::min<int64_t>(s, 32);
+  p.kb_per_split = (int)((nkb + s - 1) / s);
+  p.splits = p.kb_per_split > 0 ? (int)((nkb + p.kb_per_split - 1) / p.kb_per_split) : 1;
+  return p;
+}
+
+int check_hip(hipError_t e, const char* what) {
+  if (e == hipSuccess) return FP64EMU_OK;
+  return fp64emu_fail(FP64EMU_EHIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+int invalid(const char* msg) { return fp64emu_fail(FP64EMU_EINVAL, msg); }
+
+bool multiple(const void* p, int64_t of) { return reinterpret_cast<uintptr_t>(p) % of == 0; }
+
+int size_of(int dtype) { return dtype == FP64EMU_F32 ? 4 : 2; }
+
+bool known_dtype(int d) { return d == FP64EMU_F32 || d == FP64EMU_BF16 || d == FP64EMU_F16; }
+bool known_fmt(int f) { return f == FP64EMU_E4M3 || f == FP64EMU_E5M2; }
+
+// A quantised output of `rows` x `depth` codes, or NULL.
+int out8(const fp64emu_f8_t* f, int64_t depth, Out8* o) {
+  *o = Out8{};
+  if (!f) return FP64EMU_OK;
+  if (!f->q || !f->s) return invalid("null 8-bit operand");
+  if (!known_fmt(f->fmt)) return invalid("fmt must be FP64EMU_E4M3 or FP64EMU_E5M2");
+  if (f->ld < depth) return invalid("8-bit rows are shorter than their depth");
+  *o = Out8{f->q, f->s, f->ld, f->stride, f->s_row, f->s_block, f->s_stride,
+            multiple(f->q, 8) && f->ld % 8 == 0 && f->stride % 8 == 0};
+  return FP64EMU_OK;
+}
+
+constexpr int64_t kMaxGroups = (1ll << 31) / kThreads;    // work items of one launch stay below 2^31
+
+template <int kT, int kFmt>
+int launch_quant(const QuantArgs& g, int64_t mblocks, hipStream_t s) {
+  const unsigned z = (unsigned)std::min(g.batch, kMaxGridZ);
+  if (!g.tiles && !g.cols.q && g.M < kBlk) {
+    const int64_t units = g.M * g.kblocks;
+    quant_rows_kernel<kT, kFmt><<<dim3((unsigned)((units + 15) / 16), 1, z), kThreads, 0, s>>>(g);
+  } else {
+    quant_tile_kernel<kT, kFmt><<<dim3((unsigned)(mblocks * g.kblocks), 1, z), kThreads, 0, s>>>(g);
+  }
+  return check_hip(hipGetLastError(), "quant_f8 launch");
+}
+
+template <class S, bool kExact, int kFA, int kFB>
+void launch_tile(const MmArgs& g, unsigned groups, hipStream_t s) {
+  if (g.b_tiles) mm_tile_kernel<S, kExact, kFA, kFB, false><<<groups, S::kT, 0, s>>>(g);
+  else mm_tile_kernel<S, kExact, kFA, kFB, true><<<groups, S::kT, 0, s>>>(g);
+}
+
+template <int kTM, int kTN, int kU, int kFA, int kFB>
+void launch_few(const MmArgs& g, unsigned groups, hipStream_t s) {
+  if (g.b_tiles) mm_few_kernel<kTM, kTN, kU, kFA, kFB, false><<<groups, 64 * kFewWaves, 0, s>>>(g);
+  else mm_few_kernel<kTM, kTN, kU, kFA, kFB, true><<<groups, 64 * kFewWaves, 0, s>>>(g);
+}
+
+template <int kFA, int kFB>
+void launch_mm(const MmArgs& g, const MmPlan& p, unsigned groups, hipStream_t s) {
+  if (p.form == 2) launch_tile<Tile256, false, kFA, kFB>(g, groups, s);
+  else if (p.form == 1 && g.dtype == FP64EMU_F32) launch_tile<Tile128, true, kFA, kFB>(g, groups, s);
+  else if (p.form == 1) launch_tile<Tile128, false, kFA, kFB>(g, groups, s);
+  else if (p.tile_m == 16) launch_few<1, 1, 4, kFA, kFB>(g, groups, s);
+  else if (p.tile_m == 32) launch_few<2, 2, 2, kFA, kFB>(g, groups, s);
+  else launch_few<4, 2, 2, kFA, kFB>(g, groups, s);
+}
+
+// Whether the tile kernel can copy an operand's rows: 16-byte aligned, a tile's
+// rows within 32-bit offsets (those of the last, partial block included).
+bool copyable(const fp64emu_f8_t& f) {
+  return multiple(f.q, 16) && f.ld % 16 == 0 && f.stride % 16 == 0 && f.ld < (1ll << 32) / 256 - kBlk;
+}
+
+// Partial sums, then the rows of A and of B that are laid out again.
+struct MmRoom { size_t parts, A, B; };
+
+MmRoom mm_room(const fp64emu_mm_f8_t* p, const MmPlan& plan) {
+  MmRoom r{};
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  if (plan.splits > 1) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
+  const size_t ld = (size_t)((p->K + 15) / 16 * 16);
+  if (plan.form > 0 && !copyable(p->A)) r.A = up((size_t)(p->batch * p->M) * ld);
+  if (plan.form > 0 && !copyable(p->B)) r.B = up((size_t)(p->batch * p->N) * ld);
+  return r;
+}
+
+void pack(const fp64emu_f8_t& f, int64_t batch, int64_t rows, int64_t K, uint8_t* to, hipStream_t s) {
+  const int64_t work = batch * rows * ((K + 15) / 16);
+  const unsigned groups = (unsigned)std::min<int64_t>((work + kThreads - 1) / kThreads, 65536);
+  pack_rows_kernel<<<groups, kThreads, 0, s>>>(f.q, f.ld, f.stride, to, rows, batch * rows, K);
+}
+
+int check_mm(const fp64emu_mm_f8_t* p) {
+  if (!p) return invalid("product must not be NULL");
+  if (p->batch < 0 || p->M < 0 || p->N < 0 || p->K < 0) return invalid("shapes must be non-negative");
+  if (p->M >= (1ll << 31) - 256 || p->N >= (1ll << 31) - 256 || p->batch >= (1ll << 31) ||
+      p->K >= (1ll << 31) - kBlk)
+    return invalid("shapes must be below 2^31");
+  if (!known_dtype(p->dtype)) return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+  if (!known_fmt(p->A.fmt) || !known_fmt(p->B.fmt))
+    return invalid("fmt must be FP64EMU_E4M3 or FP64EMU_E5M2");
+  if (p->A.tiles) return invalid("A's scales are by rows");
+  return FP64EMU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp64emu_quant_f8(const void* x, int dtype, int64_t batch, int64_t M, int64_t K, int64_t ldx,
+                     int64_t stride_x, const fp64emu_f8_t* rows, const fp64emu_f8_t* cols,
+                     fp64emu_stream_t stream) {
+  if (batch < 0 || M < 0 || K < 0) return invalid("shapes must be non-negative");
+  if (!known_dtype(dtype)) return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+  if (!rows && !cols) return invalid("no output asked for");
+  if (rows && cols && (rows->tiles != cols->tiles || rows->fmt != cols->fmt))
+    return invalid("rows and cols must agree in fmt and tiles");
+  if (batch == 0 || M == 0 || K == 0) return FP64EMU_OK;
+  if (!x) return invalid("null operand pointer");
+  if (ldx < K) return invalid("rows of x are shorter than K");
+  QuantArgs g{};
+  if (int st = out8(rows, K, &g.rows)) return st;
+  if (int st = out8(cols, M, &g.cols)) return st;
+  const int64_t mblocks = (M + kBlk - 1) / kBlk;
+  g.x = x;
+  g.batch = batch;
+  g.M = M;
+  g.K = K;
+  g.ldx = ldx;
+  g.stride_x = stride_x;
+  g.kblocks = (K + kBlk - 1) / kBlk;
+  g.tiles = (rows ? rows : cols)->tiles;
+  const int sz = size_of(dtype);
+  g.vec = multiple(x, 16) && ldx * sz % 16 == 0 && stride_x * sz % 16 == 0;
+  if (mblocks > kMaxGroups / g.kblocks) return invalid("operand too large for one launch");
+  const int fmt = (rows ? rows : cols)->fmt;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define FP64EMU_QUANT(T)                                                             \
+  case T:                                                                            \
+    return fmt == FP64EMU_E4M3 ? launch_quant<T, FP64EMU_E4M3>(g, mblocks, s)        \
+                               : launch_quant<T, FP64EMU_E5M2>(g, mblocks, s);
+  switch (dtype) {
+    FP64EMU_QUANT(FP64EMU_F32)
+    FP64EMU_QUANT(FP64EMU_BF16)
+    FP64EMU_QUANT(FP64EMU_F16)
+  }
+#undef FP64EMU_QUANT
+  return invalid("dtype");
+}
+
+size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p) {
+  if (check_mm(p) || p->batch * p->M == 0 || p->N == 0 || p->K == 0) return 0;
+  const MmRoom r = mm_room(p, plan_mm(p->batch, p->M, p->N, p->K, p->dtype));
+  return r.parts + r.A + r.B;
+}
+
+int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_bytes,
+                  fp64emu_stream_t stream) {
+  if (int st = check_mm(p)) return st;
+  if (p->batch == 0 || p->M == 0 || p->N == 0) return FP64EMU_OK;
+  if (!p->out) return invalid("null operand pointer");
+  if (p->ldo < p->N) return invalid("rows of out are shorter than N");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  MmArgs g{};
+  g.out = p->out;
+  g.ldo = p->ldo;
+  g.stride_o = p->stride_o;
+  g.dtype = p->dtype;
+  g.accumulate = p->accumulate != 0;
+  g.M = (int)p->M;
+  g.N = (int)p->N;
+  g.K = p->K;
+  g.batch = (int)p->batch;
+  const int quad = 4 * size_of(p->dtype);
+  g.vec_o = multiple(p->out, quad) && p->ldo % 4 == 0 && p->stride_o % 4 == 0;
+  if (p->K == 0) {
+    // An empty sum: zeros, or out as it is.
+    if (g.accumulate) return FP64EMU_OK;
+    g.splits = 0;
+  } else {
+    if (!p->A.q || !p->A.s || !p->B.q || !p->B.s) return invalid("null 8-bit operand");
+    if (p->A.ld < p->K || p->B.ld < p->K) return invalid("8-bit rows are shorter than their depth");
+  }
+  const int64_t quads = p->batch * p->M * ((p->N + 3) / 4);
+  const unsigned sum_groups = (unsigned)std::min<int64_t>((quads + kThreads - 1) / kThreads, 65536);
+  if (p->K == 0) {
+    sum_parts_kernel<<<sum_groups, kThreads, 0, s>>>(g);
+    return check_hip(hipGetLastError(), "mm_f8 launch");
+  }
+  const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
+  const MmRoom room = mm_room(p, plan);
+  const size_t need = room.parts + room.A + room.B;
+  if (need && (!workspace || workspace_bytes < need))
+    return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_mm_f8_workspace");
+  if (need && !multiple(workspace, 16)) return invalid("workspace must be 16-byte aligned");
+  g.A = p->A.q;
+  g.B = p->B.q;
+  g.sA = p->A.s;
+  g.sB = p->B.s;
+  g.lda = p->A.ld;
+  g.ldb = p->B.ld;
+  g.strideA = p->A.stride;
+  g.strideB = p->B.stride;
+  g.sA_row = p->A.s_row;
+  g.sA_blk = p->A.s_block;
+  g.sA_str = p->A.s_stride;
+  g.sB_row = p->B.s_row;
+  g.sB_blk = p->B.s_block;
+  g.sB_str = p->B.s_stride;
+  g.part = static_cast<float*>(workspace);
+  g.nkb = (int)((p->K + kBlk - 1) / kBlk);
+  g.splits = plan.splits;
+  g.kb_per_split = plan.kb_per_split;
+  g.tiles_m = (int)plan.tiles_m;
+  g.tiles_n = (int)plan.tiles_n;
+  g.b_tiles = p->B.tiles != 0;
+  if (plan.tiles_m > kMaxGroups / plan.tiles_n / p->batch / plan.splits / 2)
+    return invalid("product too large for one launch");
+  const unsigned groups = (unsigned)(plan.tiles_m * plan.tiles_n * p->batch * plan.splits);
+  const int64_t K16 = (p->K + 15) / 16 * 16;
+  if (plan.form > 0 && K16 >= (1ll << 32) / 256 - kBlk) return invalid("K too large for one launch");
+  if (room.A) {
+    uint8_t* to = static_cast<uint8_t*>(workspace) + room.parts;
+    pack(p->A, p->batch, p->M, p->K, to, s);
+    g.A = to;
+    g.lda = K16;
+    g.strideA = p->M * K16;
+  }
+  if (room.B) {
+    uint8_t* to = static_cast<uint8_t*>(workspace) + room.parts + room.A;
+    pack(p->B, p->batch, p->N, p->K, to, s);
+    g.B = to;
+    g.ldb = K16;
+    g.strideB = p->N * K16;
+  }
+  if (p->A.fmt == FP64EMU_E4M3) {
+    if (p->B.fmt == FP64EMU_E4M3) launch_mm<FP64EMU_E4M3, FP64EMU_E4M3>(g, plan, groups, s);
+    else launch_mm<FP64EMU_E4M3, FP64EMU_E5M2>(g, plan, groups, s);
+  } else {
+    if (p->B.fmt == FP64EMU_E4M3) launch_mm<FP64EMU_E5M2, FP64EMU_E4M3>(g, plan, groups, s);
+    else launch_mm<FP64EMU_E5M2, FP64EMU_E5M2>(g, plan, groups, s);
+  }
+  if (int st = check_hip(hipGetLastError(), "mm_f8 launch")) return st;
+  if (plan.splits > 1) {
+    sum_parts_kernel<<<sum_groups, kThreads, 0, s>>>(g);
+    return check_hip(hipGetLastError(), "mm_f8 launch");
+  }
+  return FP64EMU_OK;
+}
+
+int fp64emu_swiglu_f8(const void* h, int dtype, int64_t M, int64_t F, int64_t ldh, void* y, int64_t ldy,
+                      const fp64emu_f8_t* keep, const fp64emu_f8_t* rows, const fp64emu_f8_t* cols,
+                      fp64emu_stream_t stream) {
+  if (M < 0 || F < 0) return invalid("shapes must be non-negative");
+  if (!known_dtype(dtype)) return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+  if (!y && !keep && !rows && !cols) return invalid("no output asked for");
+  for (const fp64emu_f8_t* f : {keep, rows, cols})
+    if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("outputs are e4m3 with scales by rows");
+  if (M == 0 || F == 0) return FP64EMU_OK;
+  if (!h) return invalid("null operand pointer");
+  if (ldh < 2 * F || (y && ldy < F)) return invalid("rows are shorter than their width");
+  SwigluArgs a{};
+  if (int st = out8(keep, 2 * F, &a.keep)) return st;
+  if (int st = out8(rows, F, &a.rows)) return st;
+  if (int st = out8(cols, M, &a.cols)) return st;
+  a.h = h;
+  a.M = M;
+  a.F = F;
+  a.ldh = ldh;
+  a.fblocks = (F + kBlk - 1) / kBlk;
+  a.keep.vec = a.keep.vec && F % 8 == 0;
+  const int sz = size_of(dtype);
+  a.vec = multiple(h, 16) && ldh * sz % 16 == 0 && F * sz % 16 == 0;
+  a.y = y;
+  a.ldy = ldy;
+  a.vec_y = multiple(y, 16) && ldy * sz % 16 == 0;
+  const int64_t mblocks = (M + kBlk - 1) / kBlk;
+  if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const unsigned groups = (unsigned)(mblocks * a.fblocks);
+  if (dtype == FP64EMU_F32) swiglu_kernel<FP64EMU_F32><<<groups, kThreads, 0, s>>>(a);
+  else if (dtype == FP64EMU_BF16) swiglu_kernel<FP64EMU_BF16><<<groups, kThreads, 0, s>>>(a);
+  else swiglu_kernel<FP64EMU_F16><<<groups, kThreads, 0, s>>>(a);
+  return check_hip(hipGetLastError(), "swiglu_f8 launch");
+}
+
+int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, int64_t ldy,
+                               const fp64emu_f8_t* keep, void* dh, int out_dtype, int64_t ldh,
+                               const fp64emu_f8_t* rows, const fp64emu_f8_t* cols,
+                               fp64emu_stream_t stream) {
+  if (M < 0 || F < 0) return invalid("shapes must be non-negative");
+  if (!known_dtype(dtype) || !known_dtype(out_dtype))
+    return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+  if (out_dtype != dtype && out_dtype != FP64EMU_F32)
+    return invalid("out_dtype must be dy's or FP64EMU_F32");
+  if (!dh && !rows && !cols) return invalid("no output asked for");
+  if (!keep) return invalid("null 8-bit operand");
+  for (const fp64emu_f8_t* f : {keep, rows, cols})
+    if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("operands are e4m3 with scales by rows");
+  if ((rows || cols) && F % kBlk) return invalid("quantised gradients need F as a multiple of 128");
+  if (M == 0 || F == 0) return FP64EMU_OK;
+  if (!dy) return invalid("null operand pointer");
+  if (ldy < F || (dh && ldh < 2 * F)) return invalid("rows are shorter than their width");
+  SwigluGradArgs a{};
+  if (int st = out8(keep, 2 * F, &a.keep)) return st;
+  if (int st = out8(rows, 2 * F, &a.rows)) return st;
+  if (int st = out8(cols, M, &a.cols)) return st;
+  a.dy = dy;
+  a.M = M;
+  a.F = F;
+  a.ldy = ldy;
+  a.fblocks = (F + kBlk - 1) / kBlk;
+  const int sz = size_of(dtype), so = size_of(out_dtype);
+  a.vec = multiple(dy, 16) && ldy * sz % 16 == 0;
+  a.dh = dh;
+  a.ldh = ldh;
+  a.vec_h = multiple(dh, 16) && ldh * so % 16 == 0 && F * so % 16 == 0;
+  const int64_t mblocks = (M + kBlk - 1) / kBlk;
+  if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const unsigned groups = (unsigned)(mblocks * a.fblocks);
+#define FP64EMU_GRAD(T, O)                                                               \
+  if (dtype == T && out_dtype == O) swiglu_grad_kernel<T, O><<<groups, kThreads, 0, s>>>(a);
+  FP64EMU_GRAD(FP64EMU_F32, FP64EMU_F32)
+  FP64EMU_GRAD(FP64EMU_BF16, FP64EMU_BF16)
+  FP64EMU_GRAD(FP64EMU_F16, FP64EMU_F16)
+  FP64EMU_GRAD(FP64EMU_BF16, FP64EMU_F32)
+  FP64EMU_GRAD(FP64EMU_F16, FP64EMU_F32)
+#undef FP64EMU_GRAD
+  return check_hip(hipGetLastError(), "swiglu_f8 launch");
+}
+
+}  // extern "C"

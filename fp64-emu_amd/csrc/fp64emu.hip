@@ -47,6 +47,7 @@
 
 #include "fp64emu.h"
 #include "remainder_weights.h"
+#include "status.h"
 
 namespace {
 
@@ -4392,6 +4393,8 @@ int scratch_address(void** out) {
 
 // ---------------------------------------------------------------------------
 // C ABI
+
+int fp64emu_fail(int code, const std::string& msg) { return fail(code, msg); }
 
 extern "C" {
 

@@ -5,11 +5,14 @@
 // scratch from the caching allocator on the current stream and calls the C
 // ABI of include/fp64emu.h; nothing here computes.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
 #include <algorithm>
+#include <optional>
+#include <utility>
 #include <vector>
 
 #include "fp64emu.h"
@@ -188,6 +191,227 @@ void fp64_emu_mm_timed(at::Tensor& out, at::Tensor& times, const at::Tensor& A,
                                 (size_t)ws.numel(), current_stream(A)));
 }
 
+// ---- Operands in 8-bit floating point (include/fp64emu.h, fp64emu_f8_t) ----
+namespace {
+
+int dtype_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return FP64EMU_F32;
+    case at::kBFloat16: return FP64EMU_BF16;
+    case at::kHalf: return FP64EMU_F16;
+    default: TORCH_CHECK(false, "expect float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+// q [(batch,) rows, depth] and its scales [(batch,) rows or tile rows, blocks].
+fp64emu_f8_t f8_of(const at::Tensor& q, const at::Tensor& s, const char* what) {
+  fp64emu_f8_t f{};
+  const auto type = q.scalar_type();
+  TORCH_CHECK(type == at::kFloat8_e4m3fn || type == at::kFloat8_e5m2, what,
+              ": codes are float8_e4m3fn or float8_e5m2, got ", type);
+  TORCH_CHECK(s.scalar_type() == at::kFloat, what, ": scales are float32");
+  TORCH_CHECK(q.is_cuda() && s.is_cuda() && q.device() == s.device(), what,
+              ": codes and scales must be on one GPU");
+  const int64_t d = q.dim();
+  TORCH_CHECK((d == 2 || d == 3) && s.dim() == d, what, ": codes and scales are both 2-D or both 3-D");
+  const int64_t rows = q.size(d - 2), depth = q.size(d - 1);
+  TORCH_CHECK(d == 2 || s.size(0) == q.size(0), what, ": batch of codes and scales");
+  TORCH_CHECK(s.size(d - 1) == (depth + 127) / 128, what, ": expect one scale per 128 of K, ",
+              (depth + 127) / 128, ", got ", s.size(d - 1));
+  TORCH_CHECK(s.size(d - 2) == rows || s.size(d - 2) == (rows + 127) / 128, what,
+              ": expect scales by rows or by tiles of 128 rows");
+  TORCH_CHECK(depth <= 1 || q.stride(d - 1) == 1, what, ": codes must be contiguous along K");
+  f.q = static_cast<uint8_t*>(q.data_ptr());
+  f.s = s.data_ptr<float>();
+  f.ld = rows > 1 ? q.stride(d - 2) : std::max<int64_t>(depth, (depth + 15) / 16 * 16);
+  TORCH_CHECK(f.ld >= depth, what, ": rows of codes overlap");
+  f.stride = d == 3 && q.size(0) > 1 ? q.stride(0) : 0;
+  f.s_row = s.stride(d - 2);
+  f.s_block = s.stride(d - 1);
+  f.s_stride = d == 3 ? s.stride(0) : 0;
+  f.fmt = type == at::kFloat8_e4m3fn ? FP64EMU_E4M3 : FP64EMU_E5M2;
+  f.tiles = s.size(d - 2) != rows;
+  return f;
+}
+
+// The same for outputs that may be left out (both tensors empty and undefined).
+struct MaybeF8 {
+  fp64emu_f8_t f{};
+  bool set = false;
+  MaybeF8(const std::optional<at::Tensor>& q, const std::optional<at::Tensor>& s, const char* what) {
+    TORCH_CHECK(q.has_value() == s.has_value(), what, ": codes and scales come together");
+    if (q.has_value()) {
+      f = f8_of(*q, *s, what);
+      set = true;
+    }
+  }
+  const fp64emu_f8_t* get() const { return set ? &f : nullptr; }
+};
+
+void check_rows(const at::Tensor& t, const char* what) {
+  const int64_t d = t.dim();
+  TORCH_CHECK(t.is_cuda(), what, " must be on a GPU");
+  TORCH_CHECK(t.size(d - 1) <= 1 || t.stride(d - 1) == 1, what, " must be contiguous along its rows");
+}
+
+int64_t row_stride(const at::Tensor& t) {
+  const int64_t d = t.dim(), w = t.size(d - 1);
+  const int64_t ld = t.size(d - 2) > 1 ? t.stride(d - 2) : (w + 7) / 8 * 8;
+  TORCH_CHECK(ld >= w, "rows overlap");
+  return ld;
+}
+
+void check_f8_sizes(const std::optional<at::Tensor>& q, const at::Tensor& like, at::IntArrayRef sizes,
+                    const char* msg) {
+  if (!q.has_value()) return;
+  TORCH_CHECK(q->sizes() == sizes, msg);
+  TORCH_CHECK(q->device() == like.device(), "outputs must be on the device of the input");
+}
+
+using MaybeTensor = std::optional<at::Tensor>;
+
+}  // namespace
+
+// x [(batch,) M, K] into codes by rows, by columns laid transposed, or both;
+// `tiles`: one scale for 128 x 128 (of one row block and one column block the
+// scales' shapes do not tell).
+void fp64_emu_quant_f8(const at::Tensor& x, const MaybeTensor& q, const MaybeTensor& s,
+                       const MaybeTensor& qt, const MaybeTensor& st, bool tiles) {
+  const int64_t d = x.dim();
+  TORCH_CHECK(d == 2 || d == 3, "expect x as [M, K] or [batch, M, K]");
+  check_rows(x, "x");
+  const int64_t batch = d == 3 ? x.size(0) : 1, M = x.size(d - 2), K = x.size(d - 1);
+  std::vector<int64_t> rows(x.sizes().vec()), cols(rows);
+  std::swap(cols[d - 1], cols[d - 2]);
+  check_f8_sizes(q, x, rows, "q [M, K]");
+  check_f8_sizes(qt, x, cols, "qt [K, M]");
+  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
+  for (MaybeF8* f : {&r, &c}) {
+    const int64_t n = f == &r ? M : K;
+    TORCH_CHECK(!f->set || n <= 1 || f->f.tiles == (int)tiles, "scales by ", tiles ? "tiles" : "rows",
+                " are asked for");
+    f->f.tiles = tiles;
+  }
+  const c10::DeviceGuard guard(x.device());
+  check_status(fp64emu_quant_f8(x.data_ptr(), dtype_of(x), batch, M, K, row_stride(x),
+                                d == 3 && batch > 1 ? x.stride(0) : 0, r.get(), c.get(),
+                                current_stream(x)));
+}
+
+// out[(b,) m, n] = sum_k A[(b,) m, k] B[(b,) n, k], or added to out.
+void fp64_emu_mm_f8(at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
+                    const at::Tensor& sB, bool accumulate) {
+  fp64emu_mm_f8_t p{};
+  p.A = f8_of(A, sA, "A");
+  p.B = f8_of(B, sB, "B");
+  const int64_t d = A.dim();
+  TORCH_CHECK(B.dim() == d && out.dim() == d, "A, B and out are all 2-D or all 3-D");
+  TORCH_CHECK(A.device() == B.device() && A.device() == out.device(),
+              "A, B and out must be on the same device");
+  p.batch = d == 3 ? A.size(0) : 1;
+  p.M = A.size(d - 2);
+  p.K = A.size(d - 1);
+  p.N = B.size(d - 2);
+  TORCH_CHECK(B.size(d - 1) == p.K && (d == 2 || B.size(0) == p.batch),
+              d == 2 ? "expect B as [N, K]" : "expect B as [batch, N, K]");
+  TORCH_CHECK(sA.size(d - 2) == p.M, "A's scales are by rows");
+  p.A.tiles = 0;
+  std::vector<int64_t> want{p.M, p.N};
+  if (d == 3) want.insert(want.begin(), p.batch);
+  TORCH_CHECK(out.sizes() == at::IntArrayRef(want), "out [M, N] of the product");
+  check_rows(out, "out");
+  at::assert_no_internal_overlap(out);
+  p.out = out.data_ptr();
+  p.dtype = dtype_of(out);
+  p.ldo = row_stride(out);
+  p.stride_o = d == 3 && p.batch > 1 ? out.stride(0) : 0;
+  p.accumulate = accumulate;
+  const c10::DeviceGuard guard(A.device());
+  const size_t bytes = fp64emu_mm_f8_workspace(&p);
+  at::Tensor ws;
+  if (bytes) ws = workspace(A, bytes);
+  check_status(fp64emu_mm_f8(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream(A)));
+}
+
+// y = silu(g) u of h = [g | u]; each output only where given.
+void fp64_emu_swiglu_f8(const at::Tensor& h, const MaybeTensor& y, const MaybeTensor& hq,
+                        const MaybeTensor& hs, const MaybeTensor& q, const MaybeTensor& s,
+                        const MaybeTensor& qt, const MaybeTensor& st) {
+  TORCH_CHECK(h.dim() == 2 && h.size(1) % 2 == 0, "expect h as [M, 2 F]");
+  check_rows(h, "h");
+  const int64_t M = h.size(0), F = h.size(1) / 2, FB = (F + 127) / 128;
+  check_f8_sizes(hq, h, {M, 2 * F}, "hq [M, 2 F]");
+  check_f8_sizes(q, h, {M, F}, "q [M, F]");
+  check_f8_sizes(qt, h, {F, M}, "qt [F, M]");
+  fp64emu_f8_t keep{};
+  TORCH_CHECK(hq.has_value() == hs.has_value(), "hq and hs come together");
+  if (hq.has_value()) {
+    TORCH_CHECK(hq->scalar_type() == at::kFloat8_e4m3fn && hs->scalar_type() == at::kFloat,
+                "hq float8_e4m3fn, hs float32");
+    TORCH_CHECK(hs->sizes() == at::IntArrayRef({M, 2 * FB}), "hs [M, 2 ceil(F / 128)]");
+    check_rows(*hq, "hq");
+    TORCH_CHECK(hs->device() == h.device(), "outputs must be on the device of the input");
+    keep.q = static_cast<uint8_t*>(hq->data_ptr());
+    keep.s = hs->data_ptr<float>();
+    keep.ld = row_stride(*hq);
+    keep.s_row = hs->stride(0);
+    keep.s_block = hs->stride(1);
+  }
+  if (y.has_value()) {
+    TORCH_CHECK(y->sizes() == at::IntArrayRef({M, F}) && y->scalar_type() == h.scalar_type() &&
+                    y->device() == h.device(),
+                "y [M, F] of h's type");
+    check_rows(*y, "y");
+  }
+  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
+  TORCH_CHECK(!r.set || s->size(0) == M, "q's scales are by rows");
+  TORCH_CHECK(!c.set || st->size(0) == F, "qt's scales are by rows");
+  r.f.tiles = c.f.tiles = 0;
+  const c10::DeviceGuard guard(h.device());
+  check_status(fp64emu_swiglu_f8(h.data_ptr(), dtype_of(h), M, F, row_stride(h),
+                                 y.has_value() ? y->data_ptr() : nullptr, y.has_value() ? row_stride(*y) : 0,
+                                 hq.has_value() ? &keep : nullptr, r.get(), c.get(), current_stream(h)));
+}
+
+// The gradient of fp64_emu_swiglu_f8 from what it kept.
+void fp64_emu_swiglu_f8_backward(const at::Tensor& dy, const at::Tensor& hq, const at::Tensor& hs,
+                                 const MaybeTensor& dh, const MaybeTensor& q, const MaybeTensor& s,
+                                 const MaybeTensor& qt, const MaybeTensor& st) {
+  TORCH_CHECK(dy.dim() == 2, "expect dy as [M, F]");
+  check_rows(dy, "dy");
+  const int64_t M = dy.size(0), F = dy.size(1), FB = (F + 127) / 128;
+  TORCH_CHECK(hq.sizes() == at::IntArrayRef({M, 2 * F}) && hq.scalar_type() == at::kFloat8_e4m3fn,
+              "hq float8_e4m3fn [M, 2 F]");
+  TORCH_CHECK(hs.sizes() == at::IntArrayRef({M, 2 * FB}) && hs.scalar_type() == at::kFloat,
+              "hs float32 [M, 2 ceil(F / 128)]");
+  TORCH_CHECK(hq.device() == dy.device() && hs.device() == dy.device(),
+              "dy, hq and hs must be on the same device");
+  check_rows(hq, "hq");
+  fp64emu_f8_t keep{};
+  keep.q = static_cast<uint8_t*>(hq.data_ptr());
+  keep.s = hs.data_ptr<float>();
+  keep.ld = row_stride(hq);
+  keep.s_row = hs.stride(0);
+  keep.s_block = hs.stride(1);
+  check_f8_sizes(q, dy, {M, 2 * F}, "q [M, 2 F]");
+  check_f8_sizes(qt, dy, {2 * F, M}, "qt [2 F, M]");
+  int out_dtype = dtype_of(dy);
+  if (dh.has_value()) {
+    TORCH_CHECK(dh->sizes() == at::IntArrayRef({M, 2 * F}) && dh->device() == dy.device(), "dh [M, 2 F]");
+    check_rows(*dh, "dh");
+    out_dtype = dtype_of(*dh);
+  }
+  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
+  TORCH_CHECK(!r.set || s->size(0) == M, "q's scales are by rows");
+  TORCH_CHECK(!c.set || st->size(0) == 2 * F, "qt's scales are by rows");
+  r.f.tiles = c.f.tiles = 0;
+  const c10::DeviceGuard guard(dy.device());
+  check_status(fp64emu_swiglu_f8_backward(dy.data_ptr(), dtype_of(dy), M, F, row_stride(dy), &keep,
+                                          dh.has_value() ? dh->data_ptr() : nullptr, out_dtype,
+                                          dh.has_value() ? row_stride(*dh) : 0, r.get(), c.get(),
+                                          current_stream(dy)));
+}
+
 TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_maxp() -> int", &fp64_emu_maxp);
   ops.def("fp64_emu_mm(Tensor! out, Tensor A, Tensor B, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
@@ -195,6 +419,10 @@ TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_mm_nt(Tensor! out, Tensor A, Tensor Bt, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
   ops.def("fp64_emu_bmm_nt(Tensor! out, Tensor A, Tensor Bt, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
   ops.def("fp64_emu_mm_timed(Tensor! out, Tensor! times, Tensor A, Tensor B, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
+  ops.def("fp64_emu_quant_f8(Tensor x, Tensor(a!)? q, Tensor(b!)? s, Tensor(c!)? qt, Tensor(d!)? st, bool tiles) -> ()");
+  ops.def("fp64_emu_mm_f8(Tensor(a!) out, Tensor A, Tensor sA, Tensor B, Tensor sB, bool accumulate) -> ()");
+  ops.def("fp64_emu_swiglu_f8(Tensor h, Tensor(a!)? y, Tensor(b!)? hq, Tensor(c!)? hs, Tensor(d!)? q, Tensor(e!)? s, Tensor(f!)? qt, Tensor(g!)? st) -> ()");
+  ops.def("fp64_emu_swiglu_f8_backward(Tensor dy, Tensor hq, Tensor hs, Tensor(a!)? dh, Tensor(b!)? q, Tensor(c!)? s, Tensor(d!)? qt, Tensor(e!)? st) -> ()");
 }
 
 // PyTorch-ROCm keeps the CUDA dispatch key for HIP devices.
@@ -204,4 +432,8 @@ TORCH_LIBRARY_IMPL(fp64_emu, CUDA, ops) {
   ops.impl("fp64_emu_mm_nt", &fp64_emu_mm_nt);
   ops.impl("fp64_emu_bmm_nt", &fp64_emu_bmm_nt);
   ops.impl("fp64_emu_mm_timed", &fp64_emu_mm_timed);
+  ops.impl("fp64_emu_quant_f8", &fp64_emu_quant_f8);
+  ops.impl("fp64_emu_mm_f8", &fp64_emu_mm_f8);
+  ops.impl("fp64_emu_swiglu_f8", &fp64_emu_swiglu_f8);
+  ops.impl("fp64_emu_swiglu_f8_backward", &fp64_emu_swiglu_f8_backward);
 }

@@ -24,6 +24,8 @@ import torch
 
 from ._ops import ops
 from . import _meta  # noqa: F401  (fake kernels for torch.compile)
+from .f8 import (bmm_f8, linear_f8, mm_f8, quant_f8, quant_f8_tiles, swiglu_ckpt_f8, swiglu_f8,
+                 swiglu_f8_backward)
 
 # Pairwise-coprime moduli up to the balanced int8 ceiling of 256, largest
 # first; torch-ext/fp64_emu/__init__.py:20-22.
@@ -196,4 +198,6 @@ def plan(K: int, bits: int = 53) -> int:
     raise ValueError(f"K={K} at bits={bits} needs more range than {_MAXP} primes give")
 
 
-__all__ = ["mm", "mm_nt", "bmm", "bmm_nt", "mm_timed", "plan", "plan_config", "range_bits"]
+__all__ = ["mm", "mm_nt", "bmm", "bmm_nt", "mm_timed", "plan", "plan_config", "range_bits",
+           "quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",
+           "linear_f8", "swiglu_ckpt_f8"]

@@ -11,7 +11,8 @@ def _noop(*args, **kwargs):
 
 
 for _name in ("fp64_emu_mm", "fp64_emu_bmm", "fp64_emu_mm_nt", "fp64_emu_bmm_nt",
-              "fp64_emu_mm_timed"):
+              "fp64_emu_mm_timed", "fp64_emu_quant_f8", "fp64_emu_mm_f8", "fp64_emu_swiglu_f8",
+              "fp64_emu_swiglu_f8_backward"):
     _packet = getattr(ops, _name, None)
     _qual = getattr(_packet, "_qualified_op_name", None) if _packet is not None else None
     if _qual is None:

@@ -25,7 +25,9 @@ EXPORTS = ("fp64emu_maxp", "fp64emu_last_error", "fp64emu_workspace_size",
            "fp64emu_mm_nt", "fp64emu_bmm", "fp64emu_bmm_nt", "fp64emu_mm_timed",
            "fp64emu_mm_nt_events", "fp64emu_bmm_nt_events", "fp64emu_mm_nt_noalloc",
            "fp64emu_product_workspace", "fp64emu_product", "fp64emu_layout",
-           "fp64emu_ddgemm_nt", "fp64emu_probe_mfma", "fp64emu_probe_stream")
+           "fp64emu_ddgemm_nt", "fp64emu_probe_mfma", "fp64emu_probe_stream", "fp64emu_quant_f8",
+           "fp64emu_mm_f8_workspace", "fp64emu_mm_f8", "fp64emu_swiglu_f8",
+           "fp64emu_swiglu_f8_backward")
 
 NOALLOC_SCRATCH_BYTES = 64 << 20   # FP64EMU_NOALLOC_SCRATCH_BYTES
 
@@ -56,6 +58,20 @@ class Product(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("batch", "M", "N", "K")] + [
             ("b_kn", ctypes.c_int), ("primes", ctypes.c_void_p), ("nprimes", ctypes.c_int),
             ("exact", ctypes.c_int), ("bits", ctypes.c_int64), ("use_corr", ctypes.c_int)]
+
+
+class F8(ctypes.Structure):
+    """Mirror of fp64emu_f8_t."""
+    _fields_ = [("q", ctypes.c_void_p), ("s", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("ld", "stride", "s_row", "s_block", "s_stride")] + [
+            ("fmt", ctypes.c_int), ("tiles", ctypes.c_int)]
+
+
+class MmF8(ctypes.Structure):
+    """Mirror of fp64emu_mm_f8_t."""
+    _fields_ = [("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("stride_o", ctypes.c_int64),
+                ("dtype", ctypes.c_int), ("accumulate", ctypes.c_int), ("A", F8), ("B", F8)] + [
+                    (n, ctypes.c_int64) for n in ("batch", "M", "N", "K")]
 
 
 _LIB = None
@@ -103,6 +119,17 @@ def lib():
     L.fp64emu_probe_mfma.restype = i32
     L.fp64emu_probe_stream.argtypes = [vp, vp, i64, i32, vp]
     L.fp64emu_probe_stream.restype = i32
+    f8 = ctypes.POINTER(F8)
+    L.fp64emu_quant_f8.argtypes = [vp, i32, i64, i64, i64, i64, i64, f8, f8, vp]
+    L.fp64emu_quant_f8.restype = i32
+    L.fp64emu_mm_f8_workspace.argtypes = [ctypes.POINTER(MmF8)]
+    L.fp64emu_mm_f8_workspace.restype = sz
+    L.fp64emu_mm_f8.argtypes = [ctypes.POINTER(MmF8), vp, sz, vp]
+    L.fp64emu_mm_f8.restype = i32
+    L.fp64emu_swiglu_f8.argtypes = [vp, i32, i64, i64, i64, vp, i64, f8, f8, f8, vp]
+    L.fp64emu_swiglu_f8.restype = i32
+    L.fp64emu_swiglu_f8_backward.argtypes = [vp, i32, i64, i64, i64, f8, vp, i32, i64, f8, f8, vp]
+    L.fp64emu_swiglu_f8_backward.restype = i32
     _LIB = L
     return L
 

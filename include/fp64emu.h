@@ -288,6 +288,71 @@ int fp64emu_probe_mfma(int32_t* acc_out, unsigned long long* clocks, const int8_
 int fp64emu_probe_stream(double* dst, const double* src, int64_t n, int mode,
                          fp64emu_stream_t stream);
 
+/* ---- Operands in 8-bit floating point, one float32 scale per block of 128
+ * (no reference counterpart).  A matrix of `rows` x `depth` is held as codes
+ * q (OCP e4m3 or e5m2) and scales s, x ~ q s, where a block is 128 successive
+ * elements of a row, or a tile of 128 x 128 elements.  With
+ * a = max(largest magnitude of the block, 2^-110) and F the format's largest
+ * value (448, 57344): s = a / F, q = x ((1 / a) F) rounded to the nearest code,
+ * every step a float32 operation rounded once.  A block that holds an infinity
+ * or a NaN stands for NaN throughout.  Strides count elements; the innermost
+ * stride of q is 1. ---- */
+
+enum { FP64EMU_E4M3 = 0, FP64EMU_E5M2 = 1 };                   /* fmt */
+enum { FP64EMU_F32 = 0, FP64EMU_BF16 = 1, FP64EMU_F16 = 2 };   /* dtype */
+
+typedef struct {
+  uint8_t* q;               /* [batch, rows, depth] codes */
+  float* s;                 /* scale of row r (or tile row r), block k: s[r s_row + k s_block] */
+  int64_t ld, stride;       /* of q: row to row, member to member */
+  int64_t s_row, s_block, s_stride;
+  int fmt;
+  int tiles;                /* 0: one scale per row and block; 1: per 128 rows and block */
+} fp64emu_f8_t;
+
+/* x [batch, M, K] (rows ldx apart, members stride_x apart) into `rows`, blocks
+ * along K: q [batch, M, K]; and / or into `cols`, blocks along M and q laid
+ * transposed: q [batch, K, M].  Either may be NULL.  With tiles set (in both
+ * alike) the two hold the same tiles' scales. */
+int fp64emu_quant_f8(const void* x, int dtype, int64_t batch, int64_t M, int64_t K, int64_t ldx,
+                     int64_t stride_x, const fp64emu_f8_t* rows /* host */,
+                     const fp64emu_f8_t* cols /* host */, fp64emu_stream_t stream);
+
+/* out[b, m, n] = sum_k A[b, m, k] B[b, n, k] (+ out[b, m, n] if accumulate), A
+ * with scales by rows, B by rows or tiles; sums in float32, out rounded once. */
+typedef struct {
+  void* out;                /* [batch, M, N], innermost stride 1 */
+  int64_t ldo, stride_o;
+  int dtype, accumulate;
+  fp64emu_f8_t A, B;        /* [batch, M, K], [batch, N, K] */
+  int64_t batch, M, N, K;
+} fp64emu_mm_f8_t;
+
+/* Workspace of fp64emu_mm_f8 (0 for most shapes: float32 partial sums where few
+ * output tiles make it split the depth).  The call needs that much.  Two calls
+ * with the same arguments give the same bits. */
+size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p);
+
+int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_bytes,
+                  fp64emu_stream_t stream);
+
+/* y = silu(g) u for h = [g | u] of M rows and 2F columns (rows ldh apart), each output
+ * only where asked for: `y` [M, F] in h's dtype; `rows` and `cols`, y quantised as by
+ * fp64emu_quant_f8 from its float32 value; `keep`, h itself as [M, 2F] codes
+ * with blocks along F in each half, scales [M, 2 ceil(F / 128)]. */
+int fp64emu_swiglu_f8(const void* h, int dtype, int64_t M, int64_t F, int64_t ldh, void* y,
+                      int64_t ldy, const fp64emu_f8_t* keep, const fp64emu_f8_t* rows,
+                      const fp64emu_f8_t* cols, fp64emu_stream_t stream);
+
+/* Its gradient at the values g', u' that `keep` stands for: [dg | du] =
+ * [dy u' s (1 + g' (1 - s)) | dy g' s], s = 1 / (1 + exp(-g')), of dy [M, F]: `dh`
+ * [M, 2F] in out_dtype; `rows` [M, 2F] and `cols` [2F, M] quantised from the float32
+ * values, for F a multiple of 128. */
+int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, int64_t ldy,
+                               const fp64emu_f8_t* keep, void* dh, int out_dtype, int64_t ldh,
+                               const fp64emu_f8_t* rows, const fp64emu_f8_t* cols,
+                               fp64emu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
