@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <utility>
 
 #include "fp64emu.h"
 #include "status.h"
@@ -34,15 +35,15 @@ typedef unsigned short v8s __attribute__((ext_vector_type(8)));
 __host__ __device__ constexpr float top_of(int fmt) { return fmt == FP64EMU_E4M3 ? 448.0f : 57344.0f; }
 
 // ---------------------------------------------------------------------------
-// Values in and codes out, eight at a time.
+// Values in and codes out, eight at a time.  Rows start anywhere: accesses of
+// eight elements are unaligned ones (the hardware splits those that need it),
+// and only a row's last, partial eight go element by element.
 
 __device__ __forceinline__ float bf16_value(unsigned short h) {
   return __builtin_bit_cast(float, (uint32_t)h << 16);
 }
 __device__ __forceinline__ unsigned short bf16_round(float f) {   // nearest even; NaN stays NaN
-  const uint32_t u = __builtin_bit_cast(uint32_t, f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40);
-  return (unsigned short)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+  return __builtin_bit_cast(unsigned short, (__bf16)f);
 }
 
 template <int kT>
@@ -58,48 +59,23 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
   if constexpr (kT == FP64EMU_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
-// Elements i .. i + 7 of p as floats, those from `valid` on as zeros.  vec: p
-// and every row start at multiples of 16 bytes.
 template <int kT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, int valid, bool vec, float (&v)[8]) {
-  if (vec && valid >= 8) {
+__device__ __forceinline__ void store8(void* p, int64_t i, int valid, const float (&v)[8]) {
+  if (valid >= 8) {
     if constexpr (kT == FP64EMU_F32) {
-      const v4f* q = reinterpret_cast<const v4f*>(static_cast<const float*>(p) + i);
-      const v4f a = q[0], b = q[1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-    } else {
-      const v8s a = *reinterpret_cast<const v8s*>(static_cast<const unsigned short*>(p) + i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = kT == FP64EMU_BF16 ? bf16_value(a[j])
-                                  : (float)__builtin_bit_cast(_Float16, (unsigned short)a[j]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < valid ? load1<kT>(p, i + j) : 0.0f;
-}
-
-template <int kT>
-__device__ __forceinline__ void store8(void* p, int64_t i, int valid, bool vec, const float (&v)[8]) {
-  if (vec && valid >= 8) {
-    if constexpr (kT == FP64EMU_F32) {
-      v4f* q = reinterpret_cast<v4f*>(static_cast<float*>(p) + i);
-      q[0] = v4f{v[0], v[1], v[2], v[3]};
-      q[1] = v4f{v[4], v[5], v[6], v[7]};
+      __builtin_memcpy(static_cast<float*>(p) + i, v, 32);
     } else {
       v8s a;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         a[j] = kT == FP64EMU_BF16 ? bf16_round(v[j])
                                   : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
-      *reinterpret_cast<v8s*>(static_cast<unsigned short*>(p) + i) = a;
+      __builtin_memcpy(static_cast<unsigned short*>(p) + i, &a, 16);
     }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 7; ++j)
     if (j < valid) store1<kT>(p, i + j, v[j]);
 }
 
@@ -131,15 +107,26 @@ __device__ __forceinline__ void values4(uint32_t w, float* v) {
   v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
 }
 
-// Eight codes at q, the first `valid` of them.  vec: q a multiple of 8.
-__device__ __forceinline__ void put8(uint8_t* q, int valid, bool vec, v2u w) {
-  if (vec && valid >= 8) {
-    *reinterpret_cast<v2u*>(q) = w;
+// Eight codes, the first `valid` of them.
+__device__ __forceinline__ void put8(uint8_t* q, int valid, v2u w) {
+  if (valid >= 8) {
+    __builtin_memcpy(q, &w, 8);
     return;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < valid) q[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+  uint64_t v = (uint64_t)w[1] << 32 | w[0];
+#pragma unroll 1
+  for (int j = 0; j < valid; ++j, v >>= 8) q[j] = (uint8_t)v;
+}
+__device__ __forceinline__ v2u get8(const uint8_t* q, int valid) {
+  v2u w = {0u, 0u};
+  if (valid >= 8) {
+    __builtin_memcpy(&w, q, 8);
+    return w;
+  }
+  uint64_t v = 0;
+#pragma unroll 1
+  for (int j = valid - 1; j >= 0; --j) v = v << 8 | q[j];
+  return v2u{(uint32_t)v, (uint32_t)(v >> 32)};
 }
 
 // Magnitudes are compared as integers: for floats with the sign cleared that
@@ -147,6 +134,93 @@ __device__ __forceinline__ void put8(uint8_t* q, int valid, bool vec, v2u w) {
 // block becomes its maximum.
 __device__ __forceinline__ uint32_t mag(float f) { return __builtin_bit_cast(uint32_t, f) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t umax16(uint32_t a, uint32_t b) {   // of each half
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2s, a),
+                                                                __builtin_bit_cast(v2s, b)));
+}
+
+// Eight rows of eight elements of x as they came, in a thread's registers.
+// Column magnitudes come as kWords words of the values' own width (two to a
+// word in 16 bits), so that their joining takes half the steps there.
+template <int kT>
+struct Held {
+  static constexpr int kWords = 4;
+  v4u w[8];
+  __device__ __forceinline__ void load(int p, const void* x, int64_t i, int valid) {
+    const unsigned short* q = static_cast<const unsigned short*>(x) + i;
+    if (valid >= 8) {
+      __builtin_memcpy(&w[p], q, 16);
+      return;
+    }
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int j = valid - 1; j >= 0; --j) {
+      hi = hi << 16 | lo >> 48;
+      lo = lo << 16 | q[j];
+    }
+    w[p] = v4u{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+  // Makes the compiler unpack the words again instead of keeping 64 floats beside
+  // them from one use to the next (198 registers instead of 104 in the quantiser).
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) asm volatile("" : "+v"(w[p]));
+  }
+  static __device__ __forceinline__ float value(uint32_t h) {
+    return kT == FP64EMU_BF16 ? bf16_value((unsigned short)h)
+                              : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+  }
+  __device__ __forceinline__ float at(int p, int j) const { return value(w[p][j >> 1] >> (16 * (j & 1))); }
+  static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return umax16(a, b); }
+  // The magnitude of column j in the words' column word, as a float's bits.
+  static __device__ __forceinline__ uint32_t bits(uint32_t word, int j) {
+    return __builtin_bit_cast(uint32_t, value(word >> (16 * (j & 1)) & 0xffffu));
+  }
+  __device__ __forceinline__ uint32_t row_mag(int p) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) m = umax16(m, w[p][d] & 0x7fff7fffu);
+    return __builtin_bit_cast(uint32_t, value(umax(m & 0xffffu, m >> 16)));
+  }
+  __device__ __forceinline__ uint32_t col_word(int d) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m = umax16(m, w[p][d] & 0x7fff7fffu);
+    return m;
+  }
+};
+
+template <>
+struct Held<FP64EMU_F32> {
+  static constexpr int kWords = 8;
+  float v[8][8];
+  __device__ __forceinline__ void load(int p, const void* x, int64_t i, int valid) {
+    const float* q = static_cast<const float*>(x) + i;
+    if (valid >= 8) {
+      __builtin_memcpy(v[p], q, 32);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[p][j] = j < valid ? q[j] : 0.0f;
+  }
+  __device__ __forceinline__ void again() {}
+  __device__ __forceinline__ float at(int p, int j) const { return v[p][j]; }
+  static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return umax(a, b); }
+  static __device__ __forceinline__ uint32_t bits(uint32_t word, int) { return word; }
+  __device__ __forceinline__ uint32_t row_mag(int p) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[p][j]));
+    return m;
+  }
+  __device__ __forceinline__ uint32_t col_word(int d) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m = umax(m, mag(v[p][d]));
+    return m;
+  }
+};
 
 // The maximum over the 16 lanes of a DPP row, in all of them.
 __device__ __forceinline__ uint32_t row16_max(uint32_t m) {
@@ -155,7 +229,41 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t m) {
   m = umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, false));
   return umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
 }
+// Lane kLane of each DPP row, in all of the row.
+template <int kLane>
+__device__ __forceinline__ float row16_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + kLane,
+                                                              0xf, 0xf, false));   // row_newbcast
+}
+template <class Fn, int... kP>
+__device__ __forceinline__ void each_row(const Fn& fn, std::integer_sequence<int, kP...>) {
+  (fn(std::integral_constant<int, kP>{}), ...);
+}
 __device__ __forceinline__ float amax_of(uint32_t m) { return __builtin_bit_cast(float, umax(m, kTinyBits)); }
+
+// F / a as (1 / a) F, both rounded.  1 / a: the hardware's reciprocal (within one
+// ulp) and one Newton step, y + y (1 - a y) with fused multiply-adds, which rounds
+// correctly (checked for all 2^23 significands; the exponent does not matter
+// while 1 / a is normal); a division (ten instructions and more) past that.
+template <int kFmt>
+__device__ __forceinline__ float inverse_scale(float a) {
+  float y;
+  if (a <= 0x1p125f) {
+    y = __builtin_amdgcn_rcpf(a);
+    y = fmaf(fmaf(-a, y, 1.0f), y, y);
+  } else {
+    y = 1.0f / a;
+  }
+  return y * top_of(kFmt);
+}
+// a / F, rounded once: F is a constant, the quotient's first guess off by an ulp at
+// most, the remainder a - F q exact (a >= 2^-110), so the correction rounds correctly.
+template <int kFmt>
+__device__ __forceinline__ float scale_of(float a) {
+  constexpr float inv = 1.0f / top_of(kFmt);
+  const float q = a * inv;
+  return a < __builtin_inff() ? fmaf(fmaf(-top_of(kFmt), q, a), inv, q) : a;
+}
 
 // One quantised output as the kernels take it (an fp64emu_f8_t for one member
 // at a time); q null: not asked for.
@@ -163,7 +271,6 @@ struct Out8 {
   uint8_t* q;
   float* s;
   int64_t ld, stride, s_row, s_block, s_stride;
-  int vec;                   // q, ld and stride are multiples of 8
 };
 
 __device__ __forceinline__ void member(Out8& o, int64_t b) {
@@ -173,13 +280,13 @@ __device__ __forceinline__ void member(Out8& o, int64_t b) {
 
 // ---------------------------------------------------------------------------
 // A 128 x 128 tile in the registers of 256 threads: thread t holds rows
-// 8 (t / 16) .. + 7 and columns 8 (t % 16) .. + 7 as v[row][column].  A row's
-// block is then 16 lanes of one DPP row, so its maximum takes four DPP steps;
-// a column's is spread over the 16 row groups: two lane exchanges and one pass
-// through LDS.  The transposed codes go through LDS too, in 8-byte chunks
-// (one thread's 8 rows of a column) whose place in the column's 128 bytes is
-// xored with the column group, so that neither the writes (16 column groups
-// of one row group) nor the reads (16 chunks of one column) collide.
+// 8 (t / 16) .. + 7 and columns 8 (t % 16) .. + 7.  A row's block is then 16
+// lanes of one DPP row, so its maximum takes four DPP steps; a column's is
+// spread over the 16 row groups: two lane exchanges and one pass through LDS.
+// The transposed codes go through LDS too, in 8-byte chunks (one thread's 8 rows
+// of a column) whose place in the column's 128 bytes is xored with the column
+// group, so that neither the writes (16 column groups of one row group) nor the
+// reads (16 chunks of one column) collide.
 struct TileLds {
   uint32_t colmax[4][kBlk];
   uint8_t codes[kBlk * kBlk];
@@ -188,6 +295,7 @@ struct TileLds {
 struct TilePlace {
   int rg, cl;                // row and column group of the thread
   int rows, cols;            // valid rows and columns of the tile
+  __device__ __forceinline__ int valid(int p) const { return 8 * rg + p < rows ? cols - 8 * cl : 0; }
 };
 
 __device__ __forceinline__ TilePlace tile_place(int64_t row0, int64_t col0, int64_t M, int64_t K) {
@@ -195,95 +303,87 @@ __device__ __forceinline__ TilePlace tile_place(int64_t row0, int64_t col0, int6
           (int)(K - col0 < kBlk ? K - col0 : kBlk)};
 }
 
-// The rows' blocks of a tile at row0, block kb of the output.
-template <int kFmt>
-__device__ __forceinline__ void emit_rows(const float (&v)[8][8], const TilePlace& t, int64_t row0,
-                                          int64_t col0, int64_t kb, const Out8& o) {
-  const int left = t.cols - 8 * t.cl;
-#pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[p][j]));
-    const float a = amax_of(row16_max(m));
-    const float r = (1.0f / a) * top_of(kFmt);
-    const int row = 8 * t.rg + p;
-    if (row >= t.rows) continue;
-    const v2u w = {codes4<kFmt>(v[p][0] * r, v[p][1] * r, v[p][2] * r, v[p][3] * r),
-                   codes4<kFmt>(v[p][4] * r, v[p][5] * r, v[p][6] * r, v[p][7] * r)};
-    put8(o.q + (row0 + row) * o.ld + col0 + 8 * t.cl, left, o.vec, w);
-    if (t.cl == 0) o.s[(row0 + row) * o.s_row + kb * o.s_block] = a / top_of(kFmt);
-  }
+template <int kFmt, class H>
+__device__ __forceinline__ v2u row_codes(const H& v, int p, float r) {
+  return v2u{codes4<kFmt>(v.at(p, 0) * r, v.at(p, 1) * r, v.at(p, 2) * r, v.at(p, 3) * r),
+             codes4<kFmt>(v.at(p, 4) * r, v.at(p, 5) * r, v.at(p, 6) * r, v.at(p, 7) * r)};
 }
 
-// The columns' blocks: q row (col0 + column), byte row0 + row.  r[j]: F / a of
+// The rows' blocks of a tile at row0, block kb of the output.
+template <int kFmt, class H>
+__device__ __forceinline__ void emit_rows(const H& v, const TilePlace& t, int64_t row0, int64_t col0,
+                                          int64_t kb, const Out8& o) {
+  uint8_t* q = o.q + (row0 + 8 * t.rg) * o.ld + col0 + 8 * t.cl;
+  float mine = 0.0f;         // lane cl < 8 of the row group writes row cl's scale
+#pragma unroll
+  for (int p = 0; p < 8; ++p, q += o.ld) {
+    const float a = amax_of(row16_max(v.row_mag(p)));
+    mine = t.cl == p ? a : mine;
+    put8(q, t.valid(p), row_codes<kFmt>(v, p, inverse_scale<kFmt>(a)));
+  }
+  if (t.cl < 8 && 8 * t.rg + t.cl < t.rows)
+    o.s[(row0 + 8 * t.rg + t.cl) * o.s_row + kb * o.s_block] = scale_of<kFmt>(mine);
+}
+
+// The columns' codes: q row (col0 + column), byte row0 + row.  r[j]: F / a of
 // this thread's column j.
-template <int kFmt>
-__device__ __forceinline__ void emit_transposed(const float (&v)[8][8], const float (&r)[8],
-                                                const TilePlace& t, int64_t row0, int64_t col0,
-                                                const Out8& o, TileLds& lds) {
+template <int kFmt, class H>
+__device__ __forceinline__ void emit_transposed(const H& v, const float (&r)[8], const TilePlace& t,
+                                                int64_t row0, int64_t col0, const Out8& o, TileLds& lds) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const v2u w = {codes4<kFmt>(v[0][j] * r[j], v[1][j] * r[j], v[2][j] * r[j], v[3][j] * r[j]),
-                   codes4<kFmt>(v[4][j] * r[j], v[5][j] * r[j], v[6][j] * r[j], v[7][j] * r[j])};
+    const v2u w = {codes4<kFmt>(v.at(0, j) * r[j], v.at(1, j) * r[j], v.at(2, j) * r[j], v.at(3, j) * r[j]),
+                   codes4<kFmt>(v.at(4, j) * r[j], v.at(5, j) * r[j], v.at(6, j) * r[j], v.at(7, j) * r[j])};
     *reinterpret_cast<v2u*>(lds.codes + (8 * t.cl + j) * kBlk + 8 * (t.rg ^ t.cl)) = w;
   }
   __syncthreads();
+  const int chunk = t.cl, left = t.rows - 8 * chunk;       // 16 lanes: one column's 128 bytes
+  uint8_t* q = o.q + (col0 + t.rg) * o.ld + row0 + 8 * chunk;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int c = p * 16 + t.rg, chunk = t.cl;        // 16 lanes: one column's 128 bytes
+  for (int p = 0; p < 8; ++p, q += 16 * o.ld) {
+    const int c = p * 16 + t.rg;
     const v2u w = *reinterpret_cast<const v2u*>(lds.codes + c * kBlk + 8 * (chunk ^ (c >> 3)));
-    if (c < t.cols) put8(o.q + (col0 + c) * o.ld + row0 + 8 * chunk, t.rows - 8 * chunk, o.vec, w);
+    if (c < t.cols) put8(q, left, w);
   }
-  __syncthreads();
 }
 
-// Column maxima of the tile into lds.colmax (over four waves); a barrier
-// stands between them and their readers.
-__device__ __forceinline__ void column_maxima(const float (&v)[8][8], const TilePlace& t, TileLds& lds) {
+template <int kFmt, class H>
+__device__ __forceinline__ void emit_cols(const H& v, const TilePlace& t, int64_t row0, int64_t col0,
+                                          int64_t mb, const Out8& o, TileLds& lds) {
+  constexpr int kW = H::kWords, kPer = 8 / kW;               // columns per word
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int p = 0; p < 8; ++p) m = umax(m, mag(v[p][j]));
-    m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-    if ((t.rg & 3) == 0) lds.colmax[t.rg >> 2][8 * t.cl + j] = m;
+  for (int d = 0; d < kW; ++d) {
+    uint32_t m = v.col_word(d);
+    m = H::join(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = H::join(m, (uint32_t)__shfl_xor((int)m, 32));
+    if ((t.rg & 3) == 0) lds.colmax[t.rg >> 2][kW * t.cl + d] = m;
   }
   __syncthreads();
-}
-
-template <int kFmt>
-__device__ __forceinline__ void emit_cols(const float (&v)[8][8], const TilePlace& t, int64_t row0,
-                                          int64_t col0, int64_t mb, const Out8& o, TileLds& lds) {
-  column_maxima(v, t, lds);
+  auto joined = [&](int word) {
+    return H::join(H::join(lds.colmax[0][word], lds.colmax[1][word]),
+                   H::join(lds.colmax[2][word], lds.colmax[3][word]));
+  };
   float r[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = 8 * t.cl + j;
-    const float a = amax_of(umax(umax(lds.colmax[0][c], lds.colmax[1][c]),
-                                 umax(lds.colmax[2][c], lds.colmax[3][c])));
-    r[j] = (1.0f / a) * top_of(kFmt);
+  for (int d = 0; d < kW; ++d) {
+    const uint32_t m = joined(kW * t.cl + d);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      r[kPer * d + e] = inverse_scale<kFmt>(amax_of(H::bits(m, e)));
   }
-  if (threadIdx.x < kBlk) {
-    const int c = threadIdx.x;
-    const float a = amax_of(umax(umax(lds.colmax[0][c], lds.colmax[1][c]),
-                                 umax(lds.colmax[2][c], lds.colmax[3][c])));
-    if (c < t.cols) o.s[(col0 + c) * o.s_row + mb * o.s_block] = a / top_of(kFmt);
-  }
+  const int c = threadIdx.x;
+  if (c < t.cols)
+    o.s[(col0 + c) * o.s_row + mb * o.s_block] = scale_of<kFmt>(amax_of(H::bits(joined(c / kPer), c % kPer)));
   emit_transposed<kFmt>(v, r, t, row0, col0, o, lds);
 }
 
 // One scale for the whole tile, both orientations.
-template <int kFmt>
-__device__ __forceinline__ void emit_tile(const float (&v)[8][8], const TilePlace& t, int64_t row0,
-                                          int64_t col0, const Out8& rows, const Out8& cols,
-                                          TileLds& lds) {
+template <int kFmt, class H>
+__device__ __forceinline__ void emit_tile(const H& v, const TilePlace& t, int64_t row0, int64_t col0,
+                                          const Out8& rows, const Out8& cols, TileLds& lds) {
   uint32_t m = 0;
 #pragma unroll
-  for (int p = 0; p < 8; ++p)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[p][j]));
+  for (int p = 0; p < 8; ++p) m = umax(m, v.row_mag(p));
   m = row16_max(m);
   m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
   m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
@@ -291,18 +391,13 @@ __device__ __forceinline__ void emit_tile(const float (&v)[8][8], const TilePlac
   __syncthreads();
   const float a = amax_of(umax(umax(lds.colmax[0][0], lds.colmax[1][0]),
                                umax(lds.colmax[2][0], lds.colmax[3][0])));
-  const float r = (1.0f / a) * top_of(kFmt), s = a / top_of(kFmt);
+  const float r = inverse_scale<kFmt>(a), s = scale_of<kFmt>(a);
   const int64_t mb = row0 / kBlk, kb = col0 / kBlk;
   if (rows.q) {
     if (threadIdx.x == 0) rows.s[mb * rows.s_row + kb * rows.s_block] = s;
+    uint8_t* q = rows.q + (row0 + 8 * t.rg) * rows.ld + col0 + 8 * t.cl;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const int row = 8 * t.rg + p;
-      const v2u w = {codes4<kFmt>(v[p][0] * r, v[p][1] * r, v[p][2] * r, v[p][3] * r),
-                     codes4<kFmt>(v[p][4] * r, v[p][5] * r, v[p][6] * r, v[p][7] * r)};
-      if (row < t.rows)
-        put8(rows.q + (row0 + row) * rows.ld + col0 + 8 * t.cl, t.cols - 8 * t.cl, rows.vec, w);
-    }
+    for (int p = 0; p < 8; ++p, q += rows.ld) put8(q, t.valid(p), row_codes<kFmt>(v, p, r));
   }
   if (cols.q) {
     if (threadIdx.x == 0) cols.s[kb * cols.s_row + mb * cols.s_block] = s;
@@ -315,38 +410,35 @@ __device__ __forceinline__ void emit_tile(const float (&v)[8][8], const TilePlac
 // Quantiser.
 struct QuantArgs {
   const void* x;
-  int64_t batch, M, K, ldx, stride_x;
+  int64_t batch0, M, K, ldx, stride_x;                     // batch0: member of blockIdx.z = 0
   int64_t kblocks;
-  int vec, tiles;
   Out8 rows, cols;
 };
 
+enum { kRows = 1, kCols = 2, kTiles = 4 };                 // what a call asks for
+
 // One work group per 128 x 128 tile (blocks along K fastest: a row of tiles
 // reads whole rows of x), every value read once.
-template <int kT, int kFmt>
-__global__ void __launch_bounds__(kThreads) quant_tile_kernel(QuantArgs g) {
+template <int kT, int kFmt, int kForm>
+__global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 3 : 4) quant_tile_kernel(QuantArgs g) {
   __shared__ TileLds lds;
-  const int64_t kb = blockIdx.x % g.kblocks, mb = blockIdx.x / g.kblocks;
+  const uint32_t kblocks = (uint32_t)g.kblocks;
+  const int64_t kb = blockIdx.x % kblocks, mb = blockIdx.x / kblocks;
   const int64_t row0 = mb * kBlk, col0 = kb * kBlk;
   const TilePlace t = tile_place(row0, col0, g.M, g.K);
-  for (int64_t b = blockIdx.z; b < g.batch; b += gridDim.z) {
-    Out8 rows = g.rows, cols = g.cols;
-    if (rows.q) member(rows, b);
-    if (cols.q) member(cols, b);
-    float v[8][8];
+  const int64_t b = g.batch0 + blockIdx.z;
+  if (g.rows.q) member(g.rows, b);
+  if (g.cols.q) member(g.cols, b);
+  Held<kT> v;
+  int64_t i = b * g.stride_x + (row0 + 8 * t.rg) * g.ldx + col0 + 8 * t.cl;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const int row = 8 * t.rg + p;
-      const int valid = row < t.rows ? t.cols - 8 * t.cl : 0;
-      load8<kT>(g.x, b * g.stride_x + (row0 + row) * g.ldx + col0 + 8 * t.cl, valid, g.vec, v[p]);
-    }
-    if (g.tiles) {
-      emit_tile<kFmt>(v, t, row0, col0, rows, cols, lds);
-    } else {
-      if (rows.q) emit_rows<kFmt>(v, t, row0, col0, kb, rows);
-      if (cols.q) emit_cols<kFmt>(v, t, row0, col0, mb, cols, lds);
-    }
-    __syncthreads();
+  for (int p = 0; p < 8; ++p, i += g.ldx) v.load(p, g.x, i, t.valid(p));
+  if constexpr (kForm & kTiles) {
+    emit_tile<kFmt>(v, t, row0, col0, g.rows, g.cols, lds);
+  } else {
+    if constexpr (kForm & kRows) emit_rows<kFmt>(v, t, row0, col0, kb, g.rows);
+    v.again();
+    if constexpr (kForm & kCols) emit_cols<kFmt>(v, t, row0, col0, mb, g.cols, lds);
   }
 }
 
@@ -356,26 +448,19 @@ template <int kT, int kFmt>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(QuantArgs g) {
   const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
   const int cl = threadIdx.x & 15;
-  const int64_t row = unit / g.kblocks, kb = unit % g.kblocks;
+  const int64_t row = (uint32_t)unit / (uint32_t)g.kblocks, kb = unit - row * g.kblocks;
   const int64_t col = kb * kBlk + 8 * cl;
   const bool live = row < g.M;
   const int valid = live && col < g.K ? (int)(g.K - col < 8 ? g.K - col : 8) : 0;
-  for (int64_t b = blockIdx.z; b < g.batch; b += gridDim.z) {
-    Out8 o = g.rows;
-    member(o, b);
-    float v[8];
-    load8<kT>(g.x, b * g.stride_x + row * g.ldx + col, valid, g.vec, v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = umax(m, mag(v[j]));
-    const float a = amax_of(row16_max(m));
-    const float r = (1.0f / a) * top_of(kFmt);
-    const v2u w = {codes4<kFmt>(v[0] * r, v[1] * r, v[2] * r, v[3] * r),
-                   codes4<kFmt>(v[4] * r, v[5] * r, v[6] * r, v[7] * r)};
-    if (!live) continue;
-    put8(o.q + row * o.ld + col, valid, o.vec, w);
-    if (cl == 0) o.s[row * o.s_row + kb * o.s_block] = a / top_of(kFmt);
-  }
+  const int64_t b = g.batch0 + blockIdx.z;
+  Out8 o = g.rows;
+  member(o, b);
+  Held<kT> v;
+  v.load(0, g.x, b * g.stride_x + row * g.ldx + col, valid);
+  const float a = amax_of(row16_max(v.row_mag(0)));
+  if (!live) return;
+  put8(o.q + row * o.ld + col, valid, row_codes<kFmt>(v, 0, inverse_scale<kFmt>(a)));
+  if (cl == 0) o.s[row * o.s_row + kb * o.s_block] = scale_of<kFmt>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -389,17 +474,15 @@ __device__ __forceinline__ float sigmoid(float g) {
   float e = __builtin_amdgcn_exp2f(t);
   // Outside the normal range of 2^t the term is left out: there it would be inf - inf.
   if (fabsf(t) < 126.0f) e = fmaf(e, lo * 0.693147182f, e);
-  return 1.0f / (1.0f + e);
+  return __builtin_amdgcn_rcpf(1.0f + e);                       // within one ulp
 }
 
 struct SwigluArgs {
   const void* h;
   int64_t M, F, ldh;
   int64_t fblocks;
-  int vec;
   void* y;
   int64_t ldy;
-  int vec_y;
   Out8 keep, rows, cols;
 };
 
@@ -408,113 +491,107 @@ template <int kT>
 __global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
   constexpr int kF = FP64EMU_E4M3;
   __shared__ TileLds lds;
-  const int64_t fb = blockIdx.x % a.fblocks, mb = blockIdx.x / a.fblocks;
+  const uint32_t fblocks = (uint32_t)a.fblocks;
+  const int64_t fb = blockIdx.x % fblocks, mb = blockIdx.x / fblocks;
   const int64_t row0 = mb * kBlk, col0 = fb * kBlk;
   const TilePlace t = tile_place(row0, col0, a.M, a.F);
-  float g[8][8], u[8][8];
+  Held<FP64EMU_F32> y;
+  {
+    Held<kT> g, u;
+    int64_t i = (row0 + 8 * t.rg) * a.ldh + col0 + 8 * t.cl;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int row = 8 * t.rg + p;
-    const int valid = row < t.rows ? t.cols - 8 * t.cl : 0;
-    const int64_t i = (row0 + row) * a.ldh + col0 + 8 * t.cl;
-    load8<kT>(a.h, i, valid, a.vec, g[p]);
-    load8<kT>(a.h, i + a.F, valid, a.vec, u[p]);
+    for (int p = 0; p < 8; ++p, i += a.ldh) {
+      g.load(p, a.h, i, t.valid(p));
+      u.load(p, a.h, i + a.F, t.valid(p));
+    }
+    if (a.keep.q) {
+      emit_rows<kF>(g, t, row0, col0, fb, a.keep);
+      emit_rows<kF>(u, t, row0, a.F + col0, a.fblocks + fb, a.keep);
+      g.again();
+      u.again();
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y.v[p][j] = g.at(p, j) * sigmoid(g.at(p, j)) * u.at(p, j);
   }
-  if (a.keep.q) {
-    emit_rows<kF>(g, t, row0, col0, fb, a.keep);
-    emit_rows<kF>(u, t, row0, a.F + col0, a.fblocks + fb, a.keep);
-  }
-#pragma unroll
-  for (int p = 0; p < 8; ++p)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) g[p][j] = g[p][j] * sigmoid(g[p][j]) * u[p][j];
   if (a.y) {
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const int row = 8 * t.rg + p;
-      store8<kT>(a.y, (row0 + row) * a.ldy + col0 + 8 * t.cl, row < t.rows ? t.cols - 8 * t.cl : 0,
-                 a.vec_y, g[p]);
-    }
+    for (int p = 0; p < 8; ++p)
+      store8<kT>(a.y, (row0 + 8 * t.rg + p) * a.ldy + col0 + 8 * t.cl, t.valid(p), y.v[p]);
   }
-  if (a.rows.q) emit_rows<kF>(g, t, row0, col0, fb, a.rows);
-  if (a.cols.q) emit_cols<kF>(g, t, row0, col0, mb, a.cols, lds);
+  if (a.rows.q) emit_rows<kF>(y, t, row0, col0, fb, a.rows);
+  if (a.cols.q) emit_cols<kF>(y, t, row0, col0, mb, a.cols, lds);
 }
 
 struct SwigluGradArgs {
   const void* dy;
   int64_t M, F, ldy;
   int64_t fblocks;
-  int vec;
   Out8 keep;                 // read
   void* dh;
   int64_t ldh;
-  int vec_h;
   Out8 rows, cols;
 };
 
-// Eight values of a kept half: codes times the block's scale.
-template <int kFmt>
-__device__ __forceinline__ void kept8(const uint8_t* q, int valid, bool vec, float s, float (&v)[8]) {
-  v2u w = {0u, 0u};
-  if (vec && valid >= 8) {
-    w = *reinterpret_cast<const v2u*>(q);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < valid) w[j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
-  }
-  values4<kFmt>(w[0], v);
-  values4<kFmt>(w[1], v + 4);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] * s : 0.0f;
-}
-
+// One work group per 128 x 128 tile of dy.
 template <int kT, int kO>
-__global__ void __launch_bounds__(kThreads) swiglu_grad_kernel(SwigluGradArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) swiglu_grad_kernel(SwigluGradArgs a) {
   constexpr int kF = FP64EMU_E4M3;
   __shared__ TileLds lds;
-  const int64_t fb = blockIdx.x % a.fblocks, mb = blockIdx.x / a.fblocks;
+  const uint32_t fblocks = (uint32_t)a.fblocks;
+  const int64_t fb = blockIdx.x % fblocks, mb = blockIdx.x / fblocks;
   const int64_t row0 = mb * kBlk, col0 = fb * kBlk;
   const TilePlace t = tile_place(row0, col0, a.M, a.F);
-  float dg[8][8], du[8][8];
+  Held<kT> dy;
+  v2u g[8], u[8];
+  // Lane cl of a row group has row cl % 8's scale, of g in the lower eight lanes
+  // and of u in the upper ones: broadcast within the DPP row where it is used.
+  float scales = 0.0f;
+  if (8 * t.rg + (t.cl & 7) < t.rows)
+    scales = a.keep.s[(row0 + 8 * t.rg + (t.cl & 7)) * a.keep.s_row +
+                      (t.cl < 8 ? fb : a.fblocks + fb) * a.keep.s_block];
+  {
+    int64_t i = (row0 + 8 * t.rg) * a.ldy + col0 + 8 * t.cl;
+    const uint8_t* q = a.keep.q + (row0 + 8 * t.rg) * a.keep.ld + col0 + 8 * t.cl;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int64_t row = row0 + 8 * t.rg + p;
-    const int valid = row < a.M ? t.cols - 8 * t.cl : 0;
-    float dy[8], g[8], u[8];
-    load8<kT>(a.dy, row * a.ldy + col0 + 8 * t.cl, valid, a.vec, dy);
-    float sg = 0.0f, su = 0.0f;
-    if (valid > 0) {
-      sg = a.keep.s[row * a.keep.s_row + fb * a.keep.s_block];
-      su = a.keep.s[row * a.keep.s_row + (a.fblocks + fb) * a.keep.s_block];
+    for (int p = 0; p < 8; ++p, i += a.ldy, q += a.keep.ld) {
+      const int valid = t.valid(p);
+      dy.load(p, a.dy, i, valid);
+      g[p] = get8(q, valid);
+      u[p] = get8(q + a.F, valid);
     }
-    const uint8_t* q = a.keep.q + row * a.keep.ld + col0 + 8 * t.cl;
-    kept8<kF>(q, valid, a.keep.vec, sg, g);
-    kept8<kF>(q + a.F, valid, a.keep.vec && (a.F & 7) == 0, su, u);
+  }
+  Held<FP64EMU_F32> d[2];                                   // dg, du
+  auto row = [&](auto P) {
+    constexpr int p = decltype(P)::value;
+    const float sg = row16_lane<p>(scales), su = row16_lane<8 + p>(scales);
+    float gv[8], uv[8];
+    values4<kF>(g[p][0], gv);
+    values4<kF>(g[p][1], gv + 4);
+    values4<kF>(u[p][0], uv);
+    values4<kF>(u[p][1], uv + 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float s = sigmoid(g[j]);
-      du[p][j] = dy[j] * g[j] * s;
-      dg[p][j] = dy[j] * u[j] * s * fmaf(g[j], 1.0f - s, 1.0f);
+      const float x = gv[j] * sg, s = sigmoid(x), ds = dy.at(p, j) * s;
+      d[1].v[p][j] = ds * x;
+      d[0].v[p][j] = ds * (uv[j] * su) * fmaf(x, 1.0f - s, 1.0f);
     }
-  }
-  if (a.dh) {
+  };
+  each_row(row, std::make_integer_sequence<int, 8>{});
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const int64_t row = row0 + 8 * t.rg + p;
-      const int valid = row < a.M ? t.cols - 8 * t.cl : 0;
-      const int64_t i = row * a.ldh + col0 + 8 * t.cl;
-      store8<kO>(a.dh, i, valid, a.vec_h, dg[p]);
-      store8<kO>(a.dh, i + a.F, valid, a.vec_h, du[p]);
+  for (int half = 0; half < 2; ++half) {
+    const int64_t at = half ? a.F : 0, block = half ? a.fblocks : 0;
+    if (a.dh) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        store8<kO>(a.dh, (row0 + 8 * t.rg + p) * a.ldh + at + col0 + 8 * t.cl, t.valid(p), d[half].v[p]);
     }
-  }
-  if (a.rows.q) {
-    emit_rows<kF>(dg, t, row0, col0, fb, a.rows);
-    emit_rows<kF>(du, t, row0, a.F + col0, a.fblocks + fb, a.rows);
-  }
-  if (a.cols.q) {
-    emit_cols<kF>(dg, t, row0, col0, mb, a.cols, lds);
-    emit_cols<kF>(du, t, row0, a.F + col0, mb, a.cols, lds);
+    if (a.rows.q) emit_rows<kF>(d[half], t, row0, at + col0, block + fb, a.rows);
+    if (a.cols.q) {
+      emit_cols<kF>(d[half], t, row0, at + col0, mb, a.cols, lds);
+      __syncthreads();
+    }
   }
 }
 
@@ -1140,23 +1217,32 @@ int out8(const fp64emu_f8_t* f, int64_t depth, Out8* o) {
   if (!f->q || !f->s) return invalid("null 8-bit operand");
   if (!known_fmt(f->fmt)) return invalid("fmt must be FP64EMU_E4M3 or FP64EMU_E5M2");
   if (f->ld < depth) return invalid("8-bit rows are shorter than their depth");
-  *o = Out8{f->q, f->s, f->ld, f->stride, f->s_row, f->s_block, f->s_stride,
-            multiple(f->q, 8) && f->ld % 8 == 0 && f->stride % 8 == 0};
+  *o = Out8{f->q, f->s, f->ld, f->stride, f->s_row, f->s_block, f->s_stride};
   return FP64EMU_OK;
 }
 
 constexpr int64_t kMaxGroups = (1ll << 31) / kThreads;    // work items of one launch stay below 2^31
 
 template <int kT, int kFmt>
-int launch_quant(const QuantArgs& g, int64_t mblocks, hipStream_t s) {
-  const unsigned z = (unsigned)std::min(g.batch, kMaxGridZ);
-  if (!g.tiles && !g.cols.q && g.M < kBlk) {
-    const int64_t units = g.M * g.kblocks;
-    quant_rows_kernel<kT, kFmt><<<dim3((unsigned)((units + 15) / 16), 1, z), kThreads, 0, s>>>(g);
-  } else {
-    quant_tile_kernel<kT, kFmt><<<dim3((unsigned)(mblocks * g.kblocks), 1, z), kThreads, 0, s>>>(g);
+int launch_quant(QuantArgs g, int64_t batch, int64_t mblocks, bool tiles, hipStream_t s) {
+  for (; g.batch0 < batch; g.batch0 += kMaxGridZ) {
+    const unsigned z = (unsigned)std::min(batch - g.batch0, kMaxGridZ);
+    const dim3 grid((unsigned)(mblocks * g.kblocks), 1, z);
+    if (tiles) {
+      quant_tile_kernel<kT, kFmt, kTiles><<<grid, kThreads, 0, s>>>(g);
+    } else if (!g.cols.q && g.M < kBlk) {
+      const int64_t units = g.M * g.kblocks;
+      quant_rows_kernel<kT, kFmt><<<dim3((unsigned)((units + 15) / 16), 1, z), kThreads, 0, s>>>(g);
+    } else if (!g.cols.q) {
+      quant_tile_kernel<kT, kFmt, kRows><<<grid, kThreads, 0, s>>>(g);
+    } else if (!g.rows.q) {
+      quant_tile_kernel<kT, kFmt, kCols><<<grid, kThreads, 0, s>>>(g);
+    } else {
+      quant_tile_kernel<kT, kFmt, kRows | kCols><<<grid, kThreads, 0, s>>>(g);
+    }
+    if (int st = check_hip(hipGetLastError(), "quant_f8 launch")) return st;
   }
-  return check_hip(hipGetLastError(), "quant_f8 launch");
+  return FP64EMU_OK;
 }
 
 template <class S, bool kExact, int kFA, int kFB>
@@ -1239,22 +1325,19 @@ int fp64emu_quant_f8(const void* x, int dtype, int64_t batch, int64_t M, int64_t
   if (int st = out8(cols, M, &g.cols)) return st;
   const int64_t mblocks = (M + kBlk - 1) / kBlk;
   g.x = x;
-  g.batch = batch;
   g.M = M;
   g.K = K;
   g.ldx = ldx;
   g.stride_x = stride_x;
   g.kblocks = (K + kBlk - 1) / kBlk;
-  g.tiles = (rows ? rows : cols)->tiles;
-  const int sz = size_of(dtype);
-  g.vec = multiple(x, 16) && ldx * sz % 16 == 0 && stride_x * sz % 16 == 0;
+  const bool tiles = (rows ? rows : cols)->tiles != 0;
   if (mblocks > kMaxGroups / g.kblocks) return invalid("operand too large for one launch");
   const int fmt = (rows ? rows : cols)->fmt;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define FP64EMU_QUANT(T)                                                             \
   case T:                                                                            \
-    return fmt == FP64EMU_E4M3 ? launch_quant<T, FP64EMU_E4M3>(g, mblocks, s)        \
-                               : launch_quant<T, FP64EMU_E5M2>(g, mblocks, s);
+    return fmt == FP64EMU_E4M3 ? launch_quant<T, FP64EMU_E4M3>(g, batch, mblocks, tiles, s)        \
+                               : launch_quant<T, FP64EMU_E5M2>(g, batch, mblocks, tiles, s);
   switch (dtype) {
     FP64EMU_QUANT(FP64EMU_F32)
     FP64EMU_QUANT(FP64EMU_BF16)
@@ -1384,12 +1467,8 @@ int fp64emu_swiglu_f8(const void* h, int dtype, int64_t M, int64_t F, int64_t ld
   a.F = F;
   a.ldh = ldh;
   a.fblocks = (F + kBlk - 1) / kBlk;
-  a.keep.vec = a.keep.vec && F % 8 == 0;
-  const int sz = size_of(dtype);
-  a.vec = multiple(h, 16) && ldh * sz % 16 == 0 && F * sz % 16 == 0;
   a.y = y;
   a.ldy = ldy;
-  a.vec_y = multiple(y, 16) && ldy * sz % 16 == 0;
   const int64_t mblocks = (M + kBlk - 1) / kBlk;
   if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -1426,11 +1505,8 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
   a.F = F;
   a.ldy = ldy;
   a.fblocks = (F + kBlk - 1) / kBlk;
-  const int sz = size_of(dtype), so = size_of(out_dtype);
-  a.vec = multiple(dy, 16) && ldy * sz % 16 == 0;
   a.dh = dh;
   a.ldh = ldh;
-  a.vec_h = multiple(dh, 16) && ldh * so % 16 == 0 && F * so % 16 == 0;
   const int64_t mblocks = (M + kBlk - 1) / kBlk;
   if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
