@@ -527,31 +527,37 @@ __global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
 struct SwigluGradArgs {
   const void* dy;
   int64_t M, F, ldy;
-  int64_t fblocks;
+  int64_t fblocks, tiles;
   Out8 keep;                 // read
   void* dh;
   int64_t ldh;
   Out8 rows, cols;
 };
 
-// One work group per 128 x 128 tile of dy.
+// Two work groups per 128 x 128 tile of dy, one for dg's tile and one for du's
+// (which needs no u): both tiles' values at once took 256 registers and 110 us
+// at 8192 x 4096, where this takes half of them.  The two are eight groups apart,
+// on one XCD, whose L2 then has what both read.
 template <int kT, int kO>
-__global__ void __launch_bounds__(kThreads, 2) swiglu_grad_kernel(SwigluGradArgs a) {
+__global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) swiglu_grad_kernel(SwigluGradArgs a) {
   constexpr int kF = FP64EMU_E4M3;
   __shared__ TileLds lds;
-  const uint32_t fblocks = (uint32_t)a.fblocks;
-  const int64_t fb = blockIdx.x % fblocks, mb = blockIdx.x / fblocks;
+  const bool up = blockIdx.x & 8;                            // du's half
+  const uint32_t tile = (blockIdx.x >> 4) * 8 + (blockIdx.x & 7), fblocks = (uint32_t)a.fblocks;
+  if (tile >= a.tiles) return;
+  const int64_t fb = tile % fblocks, mb = tile / fblocks;
   const int64_t row0 = mb * kBlk, col0 = fb * kBlk;
   const TilePlace t = tile_place(row0, col0, a.M, a.F);
-  Held<kT> dy;
-  v2u g[8], u[8];
   // Lane cl of a row group has row cl % 8's scale, of g in the lower eight lanes
   // and of u in the upper ones: broadcast within the DPP row where it is used.
   float scales = 0.0f;
   if (8 * t.rg + (t.cl & 7) < t.rows)
     scales = a.keep.s[(row0 + 8 * t.rg + (t.cl & 7)) * a.keep.s_row +
                       (t.cl < 8 ? fb : a.fblocks + fb) * a.keep.s_block];
+  Held<FP64EMU_F32> d;
   {
+    Held<kT> dy;
+    v2u g[8], u[8];
     int64_t i = (row0 + 8 * t.rg) * a.ldy + col0 + 8 * t.cl;
     const uint8_t* q = a.keep.q + (row0 + 8 * t.rg) * a.keep.ld + col0 + 8 * t.cl;
 #pragma unroll
@@ -559,40 +565,32 @@ __global__ void __launch_bounds__(kThreads, 2) swiglu_grad_kernel(SwigluGradArgs
       const int valid = t.valid(p);
       dy.load(p, a.dy, i, valid);
       g[p] = get8(q, valid);
-      u[p] = get8(q + a.F, valid);
+      u[p] = get8(q + a.F, up ? 0 : valid);
     }
+    auto row = [&](auto P) {
+      constexpr int p = decltype(P)::value;
+      const float sg = row16_lane<p>(scales), su = row16_lane<8 + p>(scales);
+      float gv[8], uv[8];
+      values4<kF>(g[p][0], gv);
+      values4<kF>(g[p][1], gv + 4);
+      values4<kF>(u[p][0], uv);
+      values4<kF>(u[p][1], uv + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = gv[j] * sg, s = sigmoid(x), ds = dy.at(p, j) * s;
+        d.v[p][j] = up ? ds * x : ds * (uv[j] * su) * fmaf(x, 1.0f - s, 1.0f);
+      }
+    };
+    each_row(row, std::make_integer_sequence<int, 8>{});
   }
-  Held<FP64EMU_F32> d[2];                                   // dg, du
-  auto row = [&](auto P) {
-    constexpr int p = decltype(P)::value;
-    const float sg = row16_lane<p>(scales), su = row16_lane<8 + p>(scales);
-    float gv[8], uv[8];
-    values4<kF>(g[p][0], gv);
-    values4<kF>(g[p][1], gv + 4);
-    values4<kF>(u[p][0], uv);
-    values4<kF>(u[p][1], uv + 4);
+  const int64_t at = up ? a.F : 0, block = up ? a.fblocks : 0;
+  if (a.dh) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = gv[j] * sg, s = sigmoid(x), ds = dy.at(p, j) * s;
-      d[1].v[p][j] = ds * x;
-      d[0].v[p][j] = ds * (uv[j] * su) * fmaf(x, 1.0f - s, 1.0f);
-    }
-  };
-  each_row(row, std::make_integer_sequence<int, 8>{});
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int64_t at = half ? a.F : 0, block = half ? a.fblocks : 0;
-    if (a.dh) {
-#pragma unroll
-      for (int p = 0; p < 8; ++p)
-        store8<kO>(a.dh, (row0 + 8 * t.rg + p) * a.ldh + at + col0 + 8 * t.cl, t.valid(p), d[half].v[p]);
-    }
-    if (a.rows.q) emit_rows<kF>(d[half], t, row0, at + col0, block + fb, a.rows);
-    if (a.cols.q) {
-      emit_cols<kF>(d[half], t, row0, at + col0, mb, a.cols, lds);
-      __syncthreads();
-    }
+    for (int p = 0; p < 8; ++p)
+      store8<kO>(a.dh, (row0 + 8 * t.rg + p) * a.ldh + at + col0 + 8 * t.cl, t.valid(p), d.v[p]);
   }
+  if (a.rows.q) emit_rows<kF>(d, t, row0, at + col0, block + fb, a.rows);
+  if (a.cols.q) emit_cols<kF>(d, t, row0, at + col0, mb, a.cols, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -1508,9 +1506,10 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
   a.dh = dh;
   a.ldh = ldh;
   const int64_t mblocks = (M + kBlk - 1) / kBlk;
-  if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
+  if (mblocks > kMaxGroups / 4 / a.fblocks) return invalid("operand too large for one launch");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const unsigned groups = (unsigned)(mblocks * a.fblocks);
+  a.tiles = mblocks * a.fblocks;
+  const unsigned groups = (unsigned)((a.tiles + 7) / 8 * 16);
 #define FP64EMU_GRAD(T, O)                                                               \
   if (dtype == T && out_dtype == O) swiglu_grad_kernel<T, O><<<groups, kThreads, 0, s>>>(a);
   FP64EMU_GRAD(FP64EMU_F32, FP64EMU_F32)
