@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "fp64emu.h"
@@ -805,10 +806,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 
 // Tiles of kBM x kBN outputs, kWM x kWN waves of (kBM / kWM) x (kBN / kWN).
 // A stage holds one block of K: kBN rows of B and kBM rows of A of 128 bytes
-// each, then their scales.  A row's eight 16-byte chunks are xored with the
-// row, so that eight lanes reading one chunk of eight rows reach eight places
-// (the copies write LDS in lane order: the lane that owns a place fetches the
-// chunk that belongs there).
+// each, then their scales.  A lane's fragment is 16-byte chunks l / 16 and
+// l / 16 + 4 of row l % 16.  LDS serves a 16-byte read of 64 lanes sixteen at a time
+// over its 256 bytes of banks, lanes 0-3, 12-15 and 20-27 first, 4-11, 16-19 and 28-31
+// next; chunk c of row r lies at place c ^ (r / 2 % 8) of the row's eight, which gives
+// each such sixteen sixteen places (c ^ r % 8 with chunks 2 (l / 16) and + 1 met twice in
+// each and cost a third of LDS's cycles).  The copies write LDS in lane order: the lane
+// that owns a place fetches the chunk that belongs there.
 template <int kBM_, int kBN_, int kWM_, int kWN_>
 struct MmShape {
   static constexpr int kBM = kBM_, kBN = kBN_, kWM = kWM_, kWN = kWN_;
@@ -824,7 +828,9 @@ struct MmShape {
 
 template <class S, bool kExact, int kFA, int kFB, bool kRowB>
 __device__ __forceinline__ void mm_tile(const MmArgs& g) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::kStage];
+  // The two stages, or the waves' rows of out.
+  constexpr int kOut = S::kWaves * S::kTM * 16 * (S::kTN * 16 * (kExact ? 4 : 2) + 16);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kOut > 2 * S::kStage ? kOut : 2 * S::kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
@@ -859,7 +865,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   const int64_t K16 = (g.K + 15) & ~(int64_t)15;
   const __amdgpu_buffer_rsrc_t srcA = buffer_src(A, (uint32_t)((rowsA - 1) * g.lda + K16));
   const __amdgpu_buffer_rsrc_t srcB = buffer_src(B, (uint32_t)((rowsB - 1) * g.ldb + K16));
-  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  const int chunk = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;   // of rows 8 (2 i + wave % 2) + lane / 8
   uint32_t offA[S::kCopA], offB[S::kCopB];       // rows past the end repeat the last one
 #pragma unroll
   for (int i = 0; i < S::kCopB; ++i) {
@@ -889,26 +895,35 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
 
   // Block kb into stage st.  The block's offset is part of each lane's where it
   // ends past K, so that the resource's bound covers it.
-  auto issue = [&](int kb, int st) {
+  constexpr int kAll = S::kCopA + S::kCopB;
+  auto copy = [&](int kb, int st, int c) {
     lds_u8* stage = (lds_u8*)lds + st * S::kStage;
-#pragma unroll
-    for (int i = 0; i < S::kCopB; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcB, stage + (i * S::kWaves + wave) * 1024, 16,
-                                               (int)offB[i] + kb * kBlk, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < S::kCopA; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcA, stage + S::kOffA + (i * S::kWaves + wave) * 1024, 16,
-                                               (int)offA[i] + kb * kBlk, 0, 0, 0);
-    __builtin_amdgcn_global_load_lds(sp, stage + S::kOffS + wave * 256, 4, 0, 0);
+    if (c < S::kCopB)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcB, stage + (c * S::kWaves + wave) * 1024, 16,
+                                               (int)offB[c] + kb * kBlk, 0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(srcA, stage + S::kOffA + ((c - S::kCopB) * S::kWaves + wave) * 1024, 16,
+                                               (int)offA[c - S::kCopB] + kb * kBlk, 0, 0, 0);
+  };
+  auto copy_scales = [&](int st) {
+    __builtin_amdgcn_global_load_lds(sp, (lds_u8*)lds + st * S::kStage + S::kOffS + wave * 256, 4, 0, 0);
     sp += sblk;
   };
+  constexpr int kParts = 4, kPer = (kAll + kParts - 1) / kParts;
+  auto issue = [&](int kb, int st, int part) {
+#pragma unroll
+    for (int c = 0; c < kAll; ++c)
+      if (c / kPer == part) copy(kb, st, c);
+    if (part == 0) copy_scales(st);
+  };
+
   // Codes past K in a stage become zeros (the memory there is padding or
   // another row): thread t has row t of the stage, B's rows first.
   const int tail = (int)(g.K & (kBlk - 1));
   auto clear_tail = [&](int st) {
     uint8_t* row = lds + st * S::kStage + threadIdx.x * kBlk;
     for (int c = tail >> 4; c < 8; ++c) {
-      v4i* w = reinterpret_cast<v4i*>(row + ((c ^ (threadIdx.x & 7)) << 4));
+      v4i* w = reinterpret_cast<v4i*>(row + ((c ^ ((threadIdx.x >> 1) & 7)) << 4));
       v4i v = *w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -928,94 +943,158 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     for (int y = 0; y < S::kTM; ++y) acc[x][y] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int fr = lane & 15, fg = lane >> 4;
-  const int slot = ((2 * fg) ^ (fr & 7)) * 16;               // the second chunk's place is slot ^ 16
+  const int slot = (fg ^ (fr >> 1)) * 16;                    // chunk fg; chunk fg + 4 is at slot ^ 64
   const int fragB = (wn * S::kTN * 16 + fr) * kBlk, fragA = S::kOffA + (wm * S::kTM * 16 + fr) * kBlk;
   auto frag = [&](const uint8_t* stage, int base) {
     return join(*reinterpret_cast<const v4i*>(stage + base + slot),
-                *reinterpret_cast<const v4i*>(stage + base + (slot ^ 16)));
+                *reinterpret_cast<const v4i*>(stage + base + (slot ^ 64)));
   };
   Frag<kExact, kFA> fa[S::kTM];
   v8i fb;
   float sa[S::kTM];
-  // A's fragments and scales of a stage and B's first fragment.
-  auto open = [&](const uint8_t* stage) {
+  auto scale_a = [&](const uint8_t* stage, int y) {
     const float* sc = reinterpret_cast<const float*>(stage + S::kOffS);
-    fb = frag(stage, fragB);
-#pragma unroll
-    for (int y = 0; y < S::kTM; ++y) fa[y] = Frag<kExact, kFA>(frag(stage, fragA + y * 16 * kBlk));
-    const float st = kRowB ? 1.0f : sc[wn * S::kTN * 16];
-#pragma unroll
-    for (int y = 0; y < S::kTM; ++y) {
-      sa[y] = sc[S::kBN + wm * S::kTM * 16 + y * 16 + fr];
-      if constexpr (!kRowB) sa[y] *= st;
-    }
+    const float s = sc[S::kBN + wm * S::kTM * 16 + y * 16 + fr];
+    return kRowB ? s : s * sc[wn * S::kTN * 16];
   };
-  // acc[x] += the scaled block sums p.
-  auto add = [&](int x, const v4f (&p)[S::kTM], const v4f& sb) {
+  auto scale_b = [&](const uint8_t* stage, int x) {
+    return *reinterpret_cast<const v4f*>(stage + S::kOffS + 4 * (wn * S::kTN * 16 + x * 16 + 4 * fg));
+  };
+  // acc[x][y] += the scaled block sum p.
+  auto add = [&](int x, int y, const v4f& p, const v4f& sb) {
 #pragma unroll
-    for (int y = 0; y < S::kTM; ++y)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        acc[x][y][i] = fmaf(p[y][i], kRowB ? sa[y] * sb[i] : sa[y], acc[x][y][i]);
+    for (int i = 0; i < 4; ++i)
+      acc[x][y][i] = fmaf(p[i], kRowB ? sa[y] * sb[i] : sa[y], acc[x][y][i]);
     // Here, and not wherever the compiler finds room: it moved all of a block's
     // sums behind its last tile, with every p kept until then.
-#pragma unroll
-    for (int y = 0; y < S::kTM; ++y) asm volatile("" : "+v"(acc[x][y]));
+    asm volatile("" : "+v"(acc[x][y]));
   };
 
-  // One barrier per block: when a wave has B's last fragment of stage i & 1 in
-  // registers and its copies of block i + 1 (issued a whole block earlier) have
-  // landed, it waits for the others; the stage is then free for block i + 2 and
-  // the next one is whole.  Inside a block, row x of tiles issues its
-  // instructions while row x - 1's sums are scaled and B's next fragment is on
-  // its way; the scheduling barriers keep the compiler from reading the
-  // fragments ahead (which spilled 75 registers).
-  issue(kb0, 0);
-  if (nk > 1) issue(kb0 + 1, 1);
-  if (nk > 1) wait_vm_lgkm0<S::kCopies>();
-  else wait_vm_lgkm0<0>();
+  // One barrier per block, before its last row of tiles: when a wave has B's last
+  // fragment of stage i & 1 in registers and its copies of block i + 1 (issued a
+  // whole block earlier) have landed, it waits for the others; the stage is then
+  // free for block i + 2 and the next one is whole, and the last row's matrix
+  // instructions cover the reads of the next block's fragments, each of A's as
+  // its register comes free.  Row x of tiles issues its matrix instructions
+  // while row x - 1's sums are scaled and B's next fragment is on its way; the
+  // scheduling barriers keep the compiler from reading the fragments ahead (which
+  // spilled 75 registers).
+  for (int part = 0; part < kParts; ++part) issue(kb0, 0, part);
+  wait_vm_lgkm0<0>();
+  if (nk > 1) issue(kb0 + 1, 1, 0);
   barrier_lds();
   if (tail && nk == 1 && kb1 == g.nkb) clear_tail(0);
-  open(lds);
+  fb = frag(lds, fragB);
+#pragma unroll
+  for (int y = 0; y < S::kTM; ++y) {
+    fa[y] = Frag<kExact, kFA>(frag(lds, fragA + y * 16 * kBlk));
+    sa[y] = scale_a(lds, y);
+  }
   for (int i = 0; i < nk; ++i) {
     const uint8_t* stage = lds + (i & 1) * S::kStage;
-    const float* sc = reinterpret_cast<const float*>(stage + S::kOffS);
+    const uint8_t* after = lds + ((i + 1) & 1) * S::kStage;
     v4f p[2][S::kTM], sb[2];
+    float sa_next[S::kTM];
+    constexpr int kLast = S::kTN - 1;
 #pragma unroll
     for (int x = 0; x < S::kTN; ++x) {
       v8i next;
-      if (x + 1 < S::kTN) next = frag(stage, fragB + (x + 1) * 16 * kBlk);
-      if constexpr (kRowB)
-        sb[x & 1] = *reinterpret_cast<const v4f*>(sc + wn * S::kTN * 16 + x * 16 + 4 * fg);
-      if (x + 1 == S::kTN) {
+      if constexpr (kRowB) sb[x & 1] = scale_b(stage, x);
+      if (x == kLast) {
         wait_vm_lgkm0<0>();
         barrier_lds();
-        if (i + 2 < nk) issue(kb0 + i + 2, i & 1);
+        if (i + 2 < nk) issue(kb0 + i + 2, i & 1, 0);
+        if (tail && i + 2 == nk && kb1 == g.nkb) clear_tail((i + 1) & 1);
+        next = frag(after, fragB);                           // (past the last block: unused)
+      } else {
+        next = frag(stage, fragB + (x + 1) * 16 * kBlk);
       }
+      if (x + 1 < kParts && i + 1 < nk) issue(kb0 + i + 1, (i + 1) & 1, x + 1);
       const Frag<kExact, kFB> fbx(fb);
 #pragma unroll
-      for (int y = 0; y < S::kTM; ++y) p[x & 1][y] = block_sum<kExact, kFB, kFA>(fbx, fa[y]);
-      if (x > 0) add(x - 1, p[(x - 1) & 1], sb[(x - 1) & 1]);
-      if (x + 1 < S::kTN) fb = next;
+      for (int y = 0; y < S::kTM; ++y) {
+        p[x & 1][y] = block_sum<kExact, kFB, kFA>(fbx, fa[y]);
+        if (x == kLast) {
+          fa[y] = Frag<kExact, kFA>(frag(after, fragA + y * 16 * kBlk));
+          sa_next[y] = scale_a(after, y);
+        }
+        if (x > 0) add(x - 1, y, p[(x - 1) & 1][y], sb[(x - 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fb = next;
       __builtin_amdgcn_sched_barrier(0);
     }
-    add(S::kTN - 1, p[(S::kTN - 1) & 1], sb[(S::kTN - 1) & 1]);
-    if (i + 1 < nk) {
-      if (tail && i + 2 == nk && kb1 == g.nkb) clear_tail((i + 1) & 1);
-      open(lds + ((i + 1) & 1) * S::kStage);
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) {
+      add(kLast, y, p[kLast & 1][y], sb[kLast & 1]);
+      sa[y] = sa_next[y];
     }
   }
 
+  if (g.splits > 1 || (!kExact && g.accumulate)) {
 #pragma unroll
-  for (int y = 0; y < S::kTM; ++y) {
-    const int64_t m = m0 + (wm * S::kTM + y) * 16 + fr;
-    if (m >= g.M) continue;
+    for (int y = 0; y < S::kTM; ++y) {
+      const int64_t m = m0 + (wm * S::kTM + y) * 16 + fr;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int x = 0; x < S::kTN; ++x) {
+        const int64_t n = n0 + (wn * S::kTN + x) * 16 + 4 * fg;
+        if (n >= g.N) continue;
+        if (g.splits > 1) store_part(g, split, b, m, n, acc[x][y]);
+        else store_out(g, b, m, n, acc[x][y]);
+      }
+    }
+    return;
+  }
+  // Through LDS, so that a store writes whole lines of out: four values of a
+  // lane are 8 or 16 bytes of a row, and storing them as they lie (32 or 64 bytes of a
+  // line at a time) cost 12 us a tile where this costs REPLACED.  Each wave has its own
+  // room: its rows of out, 16 bytes apart beyond their length so that neither side
+  // meets a bank twice.
+  using T = std::conditional_t<kExact, float, unsigned short>;
+  constexpr int kRow = S::kTN * 16 * (int)sizeof(T) + 16, kEach = 16 / (int)sizeof(T);
+  constexpr int kLanes = S::kTN * 16 / kEach;                  // lanes of one row
+  barrier_lds();                                             // every wave is done with the stages
+  uint8_t* room = lds + wave * (S::kTM * 16 * kRow);
+#pragma unroll
+  for (int y = 0; y < S::kTM; ++y)
 #pragma unroll
     for (int x = 0; x < S::kTN; ++x) {
-      const int64_t n = n0 + (wn * S::kTN + x) * 16 + 4 * fg;
-      if (n >= g.N) continue;
-      if (g.splits > 1) store_part(g, split, b, m, n, acc[x][y]);
-      else store_out(g, b, m, n, acc[x][y]);
+      T w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kExact) w[i] = acc[x][y][i];
+        else w[i] = g.dtype == FP64EMU_BF16 ? bf16_round(acc[x][y][i])
+                                            : __builtin_bit_cast(unsigned short, (_Float16)acc[x][y][i]);
+      }
+      __builtin_memcpy(__builtin_assume_aligned(room + (y * 16 + fr) * kRow + (x * 16 + 4 * fg) * sizeof(T),
+                                                4 * sizeof(T)), w, 4 * sizeof(T));
+    }
+  const int64_t n = n0 + wn * S::kTN * 16 + (lane % kLanes) * kEach;
+  const int valid = (int)(g.N - n < kEach ? g.N - n : kEach);
+  int64_t m = m0 + wm * S::kTM * 16 + lane / kLanes;
+  T* to = static_cast<T*>(g.out) + b * g.stride_o + m * g.ldo + n;
+  const uint8_t* from = room + (lane / kLanes) * kRow + (lane % kLanes) * 16;
+  constexpr int kRows = 64 / kLanes;                         // rows of one store
+#pragma unroll
+  for (int r = 0; r < S::kTM * 16; r += kRows, m += kRows, to += kRows * g.ldo) {
+    T w[kEach];
+    __builtin_memcpy(w, __builtin_assume_aligned(from + r * kRow, 16), 16);
+    if (m >= g.M) continue;
+    if (valid == kEach) {
+      if constexpr (kExact) {
+        if (g.accumulate) {
+          T old[kEach];
+          __builtin_memcpy(old, to, 16);
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) w[j] += old[j];
+        }
+      }
+      __builtin_memcpy(to, w, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach - 1; ++j)
+        if (j < valid) to[j] = kExact && g.accumulate ? w[j] + to[j] : w[j];
     }
   }
 }
