@@ -111,7 +111,8 @@ __device__ __forceinline__ void values4(uint32_t w, float* v) {
 // Eight codes, the first `valid` of them.
 __device__ __forceinline__ void put8(uint8_t* q, int valid, v2u w) {
   if (valid >= 8) {
-    __builtin_memcpy(q, &w, 8);
+    typedef v2u v2u_any __attribute__((aligned(1)));
+    __builtin_nontemporal_store(w, reinterpret_cast<v2u_any*>(q));
     return;
   }
   uint64_t v = (uint64_t)w[1] << 32 | w[0];
@@ -826,6 +827,88 @@ struct MmShape {
   static_assert(2 * kStage <= 160 * 1024, "two stages in LDS");
 };
 
+// Four successive elements at p, of which `valid` exist: to and from T[4].
+template <class T>
+__device__ __forceinline__ void put4(T* p, int valid, const T (&w)[4]) {
+  if (valid >= 4) {
+    __builtin_memcpy(p, w, sizeof(w));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < valid) p[j] = w[j];
+}
+template <class T>
+__device__ __forceinline__ void get4(const T* p, int valid, T (&w)[4]) {
+  if (valid >= 4) {
+    __builtin_memcpy(w, p, sizeof(w));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j) w[j] = j < valid ? p[j] : T{};
+}
+
+// An item's outputs (or partial sums) from the accumulators, a row of tiles at a
+// time: T float (kForm 0), bfloat16 (1) or float16 (2).
+template <class S, int kForm>
+__device__ __forceinline__ void store_rows(const v4f (&acc)[S::kTN][S::kTM], void* out, int64_t ld, int rows,
+                                           int cols, bool accumulate) {
+  using T = std::conditional_t<kForm == 0, float, unsigned short>;
+  T* p = static_cast<T*>(out);
+#pragma unroll
+  for (int y = 0; y < S::kTM; ++y, p += 16 * ld) {
+    if (y * 16 < rows) {
+      T old[S::kTN][4];
+      if (accumulate) {
+#pragma unroll
+        for (int x = 0; x < S::kTN; ++x) get4(p + x * 16, cols - x * 16, old[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < S::kTN; ++x) {
+        T w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = acc[x][y][i];
+          if constexpr (kForm == 0) {
+            w[i] = accumulate ? v + old[x][i] : v;
+          } else if constexpr (kForm == 1) {
+            w[i] = bf16_round(accumulate ? v + bf16_value(old[x][i]) : v);
+          } else {
+            if (accumulate) v += (float)__builtin_bit_cast(_Float16, old[x][i]);
+            w[i] = __builtin_bit_cast(unsigned short, (_Float16)v);
+          }
+        }
+        put4(p + x * 16, cols - x * 16, w);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// From (m, n) on, a lane's first output.
+template <class S, bool kExact>
+__device__ __forceinline__ void store_tile(const MmArgs& g, int64_t m, int64_t n, int b, int split,
+                                           const v4f (&acc)[S::kTN][S::kTM]) {
+  const int rows = (int)(g.M - m), cols = (int)(g.N - n);
+  const int64_t at = b * g.stride_o + m * g.ldo + n;
+  if (g.splits > 1)
+    store_rows<S, 0>(acc, g.part + (((int64_t)split * g.batch + b) * g.M + m) * g.N + n, g.N, rows, cols, false);
+  else if (kExact)
+    store_rows<S, 0>(acc, static_cast<float*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+  else if (g.dtype == FP64EMU_BF16)
+    store_rows<S, 1>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+  else
+    store_rows<S, 2>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+}
+
+// 16 bytes anywhere, not kept in the caches: what nothing here reads again.
+__device__ __forceinline__ void store16_past(void* p, const void* w) {
+  typedef v4u v4u_any __attribute__((aligned(2)));
+  v4u v;
+  __builtin_memcpy(&v, w, 16);
+  __builtin_nontemporal_store(v, static_cast<v4u_any*>(p));
+}
+
 template <class S, bool kExact, int kFA, int kFB, bool kRowB>
 __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   // The two stages, or the waves' rows of out.
@@ -1032,25 +1115,14 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   }
 
   if (g.splits > 1 || (!kExact && g.accumulate)) {
-#pragma unroll
-    for (int y = 0; y < S::kTM; ++y) {
-      const int64_t m = m0 + (wm * S::kTM + y) * 16 + fr;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int x = 0; x < S::kTN; ++x) {
-        const int64_t n = n0 + (wn * S::kTN + x) * 16 + 4 * fg;
-        if (n >= g.N) continue;
-        if (g.splits > 1) store_part(g, split, b, m, n, acc[x][y]);
-        else store_out(g, b, m, n, acc[x][y]);
-      }
-    }
+    store_tile<S, kExact>(g, m0 + wm * S::kTM * 16 + fr, n0 + wn * S::kTN * 16 + 4 * fg, b, split, acc);
     return;
   }
-  // Through LDS, so that a store writes whole lines of out: four values of a
-  // lane are 8 or 16 bytes of a row, and storing them as they lie (32 or 64 bytes of a
-  // line at a time) cost 12 us a tile where this costs REPLACED.  Each wave has its own
-  // room: its rows of out, 16 bytes apart beyond their length so that neither side
-  // meets a bank twice.
+  // Through LDS, so that a store writes whole lines of out past the caches: 8192 x
+  // 8192 x 1024 took 104 us with the four values of a lane stored as they lie (8 or 16
+  // bytes of a row), 108 us with whole lines, 89 us with whole lines and non-temporal
+  // stores.  Each wave has its own room: its rows of out, 16 bytes apart beyond
+  // their length so that neither side meets a bank twice.
   using T = std::conditional_t<kExact, float, unsigned short>;
   constexpr int kRow = S::kTN * 16 * (int)sizeof(T) + 16, kEach = 16 / (int)sizeof(T);
   constexpr int kLanes = S::kTN * 16 / kEach;                  // lanes of one row
@@ -1090,7 +1162,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
           for (int j = 0; j < kEach; ++j) w[j] += old[j];
         }
       }
-      __builtin_memcpy(to, w, 16);
+      store16_past(to, w);
     } else {
 #pragma unroll
       for (int j = 0; j < kEach - 1; ++j)
