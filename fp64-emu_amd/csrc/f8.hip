@@ -823,7 +823,8 @@ struct MmShape {
   static constexpr int kCopies = kCopA + kCopB + 1;
   static constexpr int kOffA = kBN * kBlk, kOffS = (kBN + kBM) * kBlk;
   static constexpr int kStage = kOffS + 4 * (kBN + kBM);
-  static_assert(kT == kBM + kBN, "one scale per thread and stage");
+  static_assert(kTM == 4, "four tiles a row");
+  static_assert(kT >= kBM + kBN && kBN % 64 == 0 && kBM % 64 == 0, "one scale per thread and stage");
   static_assert(2 * kStage <= 160 * 1024, "two stages in LDS");
 };
 
@@ -989,6 +990,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
                                                (int)offA[c - S::kCopB] + kb * kBlk, 0, 0, 0);
   };
   auto copy_scales = [&](int st) {
+    if (wave * 64 >= S::kBN + S::kBM) return;
     __builtin_amdgcn_global_load_lds(sp, (lds_u8*)lds + st * S::kStage + S::kOffS + wave * 256, 4, 0, 0);
     sp += sblk;
   };
@@ -1005,7 +1007,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   const int tail = (int)(g.K & (kBlk - 1));
   auto clear_tail = [&](int st) {
     uint8_t* row = lds + st * S::kStage + threadIdx.x * kBlk;
-    for (int c = tail >> 4; c < 8; ++c) {
+    for (int c = (int)threadIdx.x < S::kBN + S::kBM ? tail >> 4 : 8; c < 8; ++c) {
       v4i* w = reinterpret_cast<v4i*>(row + ((c ^ ((threadIdx.x >> 1) & 7)) << 4));
       v4i v = *w;
 #pragma unroll
@@ -1079,6 +1081,10 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     v4f p[2][S::kTM], sb[2];
     float sa_next[S::kTM];
     constexpr int kLast = S::kTN - 1;
+    auto refill = [&](int y) {
+      fa[y] = Frag<kExact, kFA>(frag(after, fragA + y * 16 * kBlk));
+      sa_next[y] = scale_a(after, y);
+    };
 #pragma unroll
     for (int x = 0; x < S::kTN; ++x) {
       v8i next;
@@ -1094,15 +1100,25 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
       }
       if (x + 1 < kParts && i + 1 < nk) issue(kb0 + i + 1, (i + 1) & 1, x + 1);
       const Frag<kExact, kFB> fbx(fb);
+      // Step s of four: a quarter of K of every tile (bfloat16; a tile's own four follow
+      // each other four instructions apart, not back to back), or tile s.
 #pragma unroll
-      for (int y = 0; y < S::kTM; ++y) {
-        p[x & 1][y] = block_sum<kExact, kFB, kFA>(fbx, fa[y]);
-        if (x == kLast) {
-          fa[y] = Frag<kExact, kFA>(frag(after, fragA + y * 16 * kBlk));
-          sa_next[y] = scale_a(after, y);
+      for (int s = 0; s < 4; ++s) {
+        if constexpr (kExact) {
+#pragma unroll
+          for (int y = 0; y < S::kTM; ++y)
+            p[x & 1][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                fbx.c[s], fa[y].c[s], s == 0 ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : p[x & 1][y], 0, 0, 0);
+        } else {
+          p[x & 1][s] = block_sum<kExact, kFB, kFA>(fbx, fa[s]);
         }
-        if (x > 0) add(x - 1, y, p[(x - 1) & 1][y], sb[(x - 1) & 1]);
+        if (x == kLast && !kExact) refill(s);
+        if (x > 0) add(x - 1, s, p[(x - 1) & 1][s], sb[(x - 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
+      }
+      if (x == kLast && kExact) {
+#pragma unroll
+        for (int y = 0; y < S::kTM; ++y) refill(y);
       }
       fb = next;
       __builtin_amdgcn_sched_barrier(0);
@@ -1306,6 +1322,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
 // Host side.
 
 using Tile256 = MmShape<256, 256, 4, 2>;
+using TileWide = MmShape<128, 256, 2, 4>;
 using Tile128 = MmShape<128, 128, 2, 2>;
 
 struct MmPlan {
@@ -1331,8 +1348,9 @@ MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
     const int tm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
     shape(0, tm, M <= 16 ? 16 : 32);
   } else {
-    shape(2, 256, 256);
-    if (dtype == FP64EMU_F32 || batch * p.tiles_m * p.tiles_n < kCUs) shape(1, 128, 128);
+    if (dtype == FP64EMU_F32) shape(3, 128, 256);
+    else shape(2, 256, 256);
+    if (batch * p.tiles_m * p.tiles_n < kCUs) shape(1, 128, 128);
   }
   // Splits: where the tiles leave compute units idle and each split keeps
   // at least 8 blocks of K.
@@ -1409,6 +1427,7 @@ void launch_few(const MmArgs& g, unsigned groups, hipStream_t s) {
 template <int kFA, int kFB>
 void launch_mm(const MmArgs& g, const MmPlan& p, unsigned groups, hipStream_t s) {
   if (p.form == 2) launch_tile<Tile256, false, kFA, kFB>(g, groups, s);
+  else if (p.form == 3) launch_tile<TileWide, true, kFA, kFB>(g, groups, s);
   else if (p.form == 1 && g.dtype == FP64EMU_F32) launch_tile<Tile128, true, kFA, kFB>(g, groups, s);
   else if (p.form == 1) launch_tile<Tile128, false, kFA, kFB>(g, groups, s);
   else if (p.tile_m == 16) launch_few<1, 1, 4, kFA, kFB>(g, groups, s);

@@ -234,20 +234,6 @@ fp64emu_f8_t f8_of(const at::Tensor& q, const at::Tensor& s, const char* what) {
   return f;
 }
 
-// The same for outputs that may be left out (both tensors empty and undefined).
-struct MaybeF8 {
-  fp64emu_f8_t f{};
-  bool set = false;
-  MaybeF8(const std::optional<at::Tensor>& q, const std::optional<at::Tensor>& s, const char* what) {
-    TORCH_CHECK(q.has_value() == s.has_value(), what, ": codes and scales come together");
-    if (q.has_value()) {
-      f = f8_of(*q, *s, what);
-      set = true;
-    }
-  }
-  const fp64emu_f8_t* get() const { return set ? &f : nullptr; }
-};
-
 void check_rows(const at::Tensor& t, const char* what) {
   const int64_t d = t.dim();
   TORCH_CHECK(t.is_cuda(), what, " must be on a GPU");
@@ -261,46 +247,59 @@ int64_t row_stride(const at::Tensor& t) {
   return ld;
 }
 
-void check_f8_sizes(const std::optional<at::Tensor>& q, const at::Tensor& like, at::IntArrayRef sizes,
-                    const char* msg) {
-  if (!q.has_value()) return;
-  TORCH_CHECK(q->sizes() == sizes, msg);
-  TORCH_CHECK(q->device() == like.device(), "outputs must be on the device of the input");
-}
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
-using MaybeTensor = std::optional<at::Tensor>;
-
-}  // namespace
-
-// x [(batch,) M, K] into codes by rows, by columns laid transposed, or both;
-// `tiles`: one scale for 128 x 128 (of one row block and one column block the
-// scales' shapes do not tell).
-void fp64_emu_quant_f8(const at::Tensor& x, const MaybeTensor& q, const MaybeTensor& s,
-                       const MaybeTensor& qt, const MaybeTensor& st, bool tiles) {
-  const int64_t d = x.dim();
-  TORCH_CHECK(d == 2 || d == 3, "expect x as [M, K] or [batch, M, K]");
-  check_rows(x, "x");
-  const int64_t batch = d == 3 ? x.size(0) : 1, M = x.size(d - 2), K = x.size(d - 1);
-  std::vector<int64_t> rows(x.sizes().vec()), cols(rows);
-  std::swap(cols[d - 1], cols[d - 2]);
-  check_f8_sizes(q, x, rows, "q [M, K]");
-  check_f8_sizes(qt, x, cols, "qt [K, M]");
-  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
-  for (MaybeF8* f : {&r, &c}) {
-    const int64_t n = f == &r ? M : K;
-    TORCH_CHECK(!f->set || n <= 1 || f->f.tiles == (int)tiles, "scales by ", tiles ? "tiles" : "rows",
-                " are asked for");
-    f->f.tiles = tiles;
+// A new quantised matrix [(batch,) rows, depth]: codes in rows of a multiple of 16
+// bytes, which the product copies fastest, scales stored block by block, in the
+// order it reads them.
+struct NewF8 {
+  at::Tensor q, s;
+  fp64emu_f8_t f{};
+  NewF8(const at::Tensor& like, const int64_t* batch, int64_t rows, int64_t depth, int64_t scale_rows,
+        int64_t blocks, at::ScalarType fmt, bool tiles) {
+    const int64_t ld = (depth + 15) / 16 * 16, n = batch ? *batch : 1;
+    const at::TensorOptions on = like.options();
+    if (batch) {
+      q = at::empty({n, rows, ld}, on.dtype(fmt));
+      s = at::empty_strided({n, scale_rows, blocks}, {scale_rows * blocks, 1, scale_rows}, on.dtype(at::kFloat));
+    } else {
+      q = at::empty({rows, ld}, on.dtype(fmt));
+      s = at::empty_strided({scale_rows, blocks}, {1, scale_rows}, on.dtype(at::kFloat));
+    }
+    if (ld != depth) q = q.narrow(-1, 0, depth);
+    f.q = static_cast<uint8_t*>(q.data_ptr());
+    f.s = s.data_ptr<float>();
+    f.ld = ld;
+    f.stride = rows * ld;
+    f.s_row = 1;
+    f.s_block = scale_rows;
+    f.s_stride = scale_rows * blocks;
+    f.fmt = fmt == at::kFloat8_e4m3fn ? FP64EMU_E4M3 : FP64EMU_E5M2;
+    f.tiles = tiles;
   }
-  const c10::DeviceGuard guard(x.device());
-  check_status(fp64emu_quant_f8(x.data_ptr(), dtype_of(x), batch, M, K, row_stride(x),
-                                d == 3 && batch > 1 ? x.stride(0) : 0, r.get(), c.get(),
-                                current_stream(x)));
+};
+
+fp64emu_f8_t kept_of(const at::Tensor& like, const at::Tensor& hq, const at::Tensor& hs, int64_t M, int64_t F) {
+  TORCH_CHECK(hq.sizes() == at::IntArrayRef({M, 2 * F}) && hq.scalar_type() == at::kFloat8_e4m3fn,
+              "hq float8_e4m3fn [M, 2 F]");
+  TORCH_CHECK(hs.sizes() == at::IntArrayRef({M, 2 * blocks_of(F)}) && hs.scalar_type() == at::kFloat,
+              "hs float32 [M, 2 ceil(F / 128)]");
+  TORCH_CHECK(hq.device() == like.device() && hs.device() == like.device(),
+              "dy, hq and hs must be on the same device");
+  check_rows(hq, "hq");
+  fp64emu_f8_t f{};
+  f.q = static_cast<uint8_t*>(hq.data_ptr());
+  f.s = hs.data_ptr<float>();
+  f.ld = row_stride(hq);
+  f.s_row = hs.stride(0);
+  f.s_block = hs.stride(1);
+  return f;
 }
 
-// out[(b,) m, n] = sum_k A[(b,) m, k] B[(b,) n, k], or added to out.
-void fp64_emu_mm_f8(at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
-                    const at::Tensor& sB, bool accumulate) {
+constexpr int64_t kPlain = 0, kRows = 1, kBoth = 2;    // what form an activation's result takes
+
+void product_f8(const at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
+                const at::Tensor& sB, bool accumulate) {
   fp64emu_mm_f8_t p{};
   p.A = f8_of(A, sA, "A");
   p.B = f8_of(B, sB, "B");
@@ -316,11 +315,9 @@ void fp64_emu_mm_f8(at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, 
               d == 2 ? "expect B as [N, K]" : "expect B as [batch, N, K]");
   TORCH_CHECK(sA.size(d - 2) == p.M, "A's scales are by rows");
   p.A.tiles = 0;
-  std::vector<int64_t> want{p.M, p.N};
-  if (d == 3) want.insert(want.begin(), p.batch);
-  TORCH_CHECK(out.sizes() == at::IntArrayRef(want), "out [M, N] of the product");
+  TORCH_CHECK(out.size(d - 2) == p.M && out.size(d - 1) == p.N && (d == 2 || out.size(0) == p.batch),
+              "out [M, N] of the product");
   check_rows(out, "out");
-  at::assert_no_internal_overlap(out);
   p.out = out.data_ptr();
   p.dtype = dtype_of(out);
   p.ldo = row_stride(out);
@@ -333,83 +330,121 @@ void fp64_emu_mm_f8(at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, 
   check_status(fp64emu_mm_f8(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream(A)));
 }
 
-// y = silu(g) u of h = [g | u]; each output only where given.
-void fp64_emu_swiglu_f8(const at::Tensor& h, const MaybeTensor& y, const MaybeTensor& hq,
-                        const MaybeTensor& hs, const MaybeTensor& q, const MaybeTensor& s,
-                        const MaybeTensor& qt, const MaybeTensor& st) {
-  TORCH_CHECK(h.dim() == 2 && h.size(1) % 2 == 0, "expect h as [M, 2 F]");
-  check_rows(h, "h");
-  const int64_t M = h.size(0), F = h.size(1) / 2, FB = (F + 127) / 128;
-  check_f8_sizes(hq, h, {M, 2 * F}, "hq [M, 2 F]");
-  check_f8_sizes(q, h, {M, F}, "q [M, F]");
-  check_f8_sizes(qt, h, {F, M}, "qt [F, M]");
-  fp64emu_f8_t keep{};
-  TORCH_CHECK(hq.has_value() == hs.has_value(), "hq and hs come together");
-  if (hq.has_value()) {
-    TORCH_CHECK(hq->scalar_type() == at::kFloat8_e4m3fn && hs->scalar_type() == at::kFloat,
-                "hq float8_e4m3fn, hs float32");
-    TORCH_CHECK(hs->sizes() == at::IntArrayRef({M, 2 * FB}), "hs [M, 2 ceil(F / 128)]");
-    check_rows(*hq, "hq");
-    TORCH_CHECK(hs->device() == h.device(), "outputs must be on the device of the input");
-    keep.q = static_cast<uint8_t*>(hq->data_ptr());
-    keep.s = hs->data_ptr<float>();
-    keep.ld = row_stride(*hq);
-    keep.s_row = hs->stride(0);
-    keep.s_block = hs->stride(1);
+}  // namespace
+
+// x [(batch,) M, K] into (q, s) by rows, (qt, st) by columns laid transposed, or
+// both; `tiles`: one scale for 128 x 128.
+std::vector<at::Tensor> fp64_emu_quant_f8(const at::Tensor& x, bool rows, bool cols, bool tiles,
+                                          at::ScalarType fmt) {
+  const int64_t d = x.dim();
+  TORCH_CHECK(d == 2 || d == 3, "expect x as [M, K] or [batch, M, K]");
+  TORCH_CHECK(fmt == at::kFloat8_e4m3fn || fmt == at::kFloat8_e5m2, "fmt must be float8_e4m3fn or float8_e5m2");
+  const at::Tensor v = x.size(d - 1) <= 1 || x.stride(d - 1) == 1 ? x : x.contiguous();
+  check_rows(v, "x");
+  const int dtype = dtype_of(v);
+  const int64_t batch = d == 3 ? v.size(0) : 1, M = v.size(d - 2), K = v.size(d - 1);
+  const int64_t MB = blocks_of(M), KB = blocks_of(K), *b = d == 3 ? &batch : nullptr;
+  const c10::DeviceGuard guard(v.device());
+  std::optional<NewF8> r, c;
+  std::vector<at::Tensor> out;
+  if (rows) {
+    r.emplace(v, b, M, K, tiles ? MB : M, KB, fmt, tiles);
+    out.insert(out.end(), {r->q, r->s});
   }
-  if (y.has_value()) {
-    TORCH_CHECK(y->sizes() == at::IntArrayRef({M, F}) && y->scalar_type() == h.scalar_type() &&
-                    y->device() == h.device(),
-                "y [M, F] of h's type");
-    check_rows(*y, "y");
+  if (cols) {
+    c.emplace(v, b, K, M, tiles ? KB : K, MB, fmt, tiles);
+    out.insert(out.end(), {c->q, c->s});
   }
-  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
-  TORCH_CHECK(!r.set || s->size(0) == M, "q's scales are by rows");
-  TORCH_CHECK(!c.set || st->size(0) == F, "qt's scales are by rows");
-  r.f.tiles = c.f.tiles = 0;
-  const c10::DeviceGuard guard(h.device());
-  check_status(fp64emu_swiglu_f8(h.data_ptr(), dtype_of(h), M, F, row_stride(h),
-                                 y.has_value() ? y->data_ptr() : nullptr, y.has_value() ? row_stride(*y) : 0,
-                                 hq.has_value() ? &keep : nullptr, r.get(), c.get(), current_stream(h)));
+  check_status(fp64emu_quant_f8(v.data_ptr(), dtype, batch, M, K, row_stride(v),
+                                batch > 1 ? v.stride(0) : 0, r ? &r->f : nullptr, c ? &c->f : nullptr,
+                                current_stream(v)));
+  return out;
 }
 
-// The gradient of fp64_emu_swiglu_f8 from what it kept.
-void fp64_emu_swiglu_f8_backward(const at::Tensor& dy, const at::Tensor& hq, const at::Tensor& hs,
-                                 const MaybeTensor& dh, const MaybeTensor& q, const MaybeTensor& s,
-                                 const MaybeTensor& qt, const MaybeTensor& st) {
-  TORCH_CHECK(dy.dim() == 2, "expect dy as [M, F]");
-  check_rows(dy, "dy");
-  const int64_t M = dy.size(0), F = dy.size(1), FB = (F + 127) / 128;
-  TORCH_CHECK(hq.sizes() == at::IntArrayRef({M, 2 * F}) && hq.scalar_type() == at::kFloat8_e4m3fn,
-              "hq float8_e4m3fn [M, 2 F]");
-  TORCH_CHECK(hs.sizes() == at::IntArrayRef({M, 2 * FB}) && hs.scalar_type() == at::kFloat,
-              "hs float32 [M, 2 ceil(F / 128)]");
-  TORCH_CHECK(hq.device() == dy.device() && hs.device() == dy.device(),
-              "dy, hq and hs must be on the same device");
-  check_rows(hq, "hq");
-  fp64emu_f8_t keep{};
-  keep.q = static_cast<uint8_t*>(hq.data_ptr());
-  keep.s = hs.data_ptr<float>();
-  keep.ld = row_stride(hq);
-  keep.s_row = hs.stride(0);
-  keep.s_block = hs.stride(1);
-  check_f8_sizes(q, dy, {M, 2 * F}, "q [M, 2 F]");
-  check_f8_sizes(qt, dy, {2 * F, M}, "qt [2 F, M]");
-  int out_dtype = dtype_of(dy);
-  if (dh.has_value()) {
-    TORCH_CHECK(dh->sizes() == at::IntArrayRef({M, 2 * F}) && dh->device() == dy.device(), "dh [M, 2 F]");
-    check_rows(*dh, "dh");
-    out_dtype = dtype_of(*dh);
+// sum_k A[(b,) m, k] B[(b,) n, k] as a new tensor of `dtype`.
+at::Tensor fp64_emu_mm_f8(const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B, const at::Tensor& sB,
+                          at::ScalarType dtype) {
+  const int64_t d = A.dim();
+  TORCH_CHECK((d == 2 || d == 3) && B.dim() == d, "A, B and out are all 2-D or all 3-D");
+  const at::TensorOptions on = A.options().dtype(dtype);
+  const at::Tensor out = d == 3 ? at::empty({A.size(0), A.size(1), B.size(1)}, on)
+                                : at::empty({A.size(0), B.size(0)}, on);
+  product_f8(out, A, sA, B, sB, false);
+  return out;
+}
+
+// The same into out, or added to it.
+void fp64_emu_mm_f8_out(at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
+                        const at::Tensor& sB, bool accumulate) {
+  at::assert_no_internal_overlap(out);
+  product_f8(out, A, sA, B, sB, accumulate);
+}
+
+// y = silu(g) u of h = [g | u]: y, or its (q, s), or (q, s, qt, st); then, with
+// keep, (hq, hs).
+std::vector<at::Tensor> fp64_emu_swiglu_f8(const at::Tensor& h, int64_t quant, bool keep) {
+  TORCH_CHECK(h.dim() == 2 && h.size(1) % 2 == 0, "expect h as [M, 2 F]");
+  TORCH_CHECK(quant >= kPlain && quant <= kBoth, "quant: 0 plain, 1 rows, 2 both");
+  const at::Tensor v = h.size(1) <= 1 || h.stride(1) == 1 ? h : h.contiguous();
+  check_rows(v, "h");
+  const int dtype = dtype_of(v);
+  const int64_t M = v.size(0), F = v.size(1) / 2, FB = blocks_of(F);
+  const c10::DeviceGuard guard(v.device());
+  std::optional<NewF8> r, c, k;
+  at::Tensor y;
+  std::vector<at::Tensor> out;
+  if (quant == kPlain) {
+    y = at::empty({M, F}, v.options());
+    out.push_back(y);
+  } else {
+    r.emplace(v, nullptr, M, F, M, FB, at::kFloat8_e4m3fn, false);
+    out.insert(out.end(), {r->q, r->s});
   }
-  MaybeF8 r(q, s, "q"), c(qt, st, "qt");
-  TORCH_CHECK(!r.set || s->size(0) == M, "q's scales are by rows");
-  TORCH_CHECK(!c.set || st->size(0) == 2 * F, "qt's scales are by rows");
-  r.f.tiles = c.f.tiles = 0;
-  const c10::DeviceGuard guard(dy.device());
-  check_status(fp64emu_swiglu_f8_backward(dy.data_ptr(), dtype_of(dy), M, F, row_stride(dy), &keep,
-                                          dh.has_value() ? dh->data_ptr() : nullptr, out_dtype,
-                                          dh.has_value() ? row_stride(*dh) : 0, r.get(), c.get(),
-                                          current_stream(dy)));
+  if (quant == kBoth) {
+    c.emplace(v, nullptr, F, M, F, blocks_of(M), at::kFloat8_e4m3fn, false);
+    out.insert(out.end(), {c->q, c->s});
+  }
+  if (keep) {
+    k.emplace(v, nullptr, M, 2 * F, M, 2 * FB, at::kFloat8_e4m3fn, false);
+    out.insert(out.end(), {k->q, k->s});
+  }
+  check_status(fp64emu_swiglu_f8(v.data_ptr(), dtype, M, F, row_stride(v), y.defined() ? y.data_ptr() : nullptr, F,
+                                 k ? &k->f : nullptr, r ? &r->f : nullptr, c ? &c->f : nullptr,
+                                 current_stream(v)));
+  return out;
+}
+
+// The gradient of fp64_emu_swiglu_f8 from what it kept: dh, or its (q, s), or (q, s, qt, st).
+std::vector<at::Tensor> fp64_emu_swiglu_f8_backward(const at::Tensor& dy, const at::Tensor& hq,
+                                                    const at::Tensor& hs, int64_t quant) {
+  TORCH_CHECK(dy.dim() == 2, "expect dy as [M, F]");
+  TORCH_CHECK(quant >= kPlain && quant <= kBoth, "quant: 0 plain, 1 rows, 2 both");
+  const at::Tensor v = dy.size(1) <= 1 || dy.stride(1) == 1 ? dy : dy.contiguous();
+  check_rows(v, "dy");
+  const int dtype = dtype_of(v);
+  const int64_t M = v.size(0), F = v.size(1);
+  const fp64emu_f8_t keep = kept_of(v, hq, hs, M, F);
+  const c10::DeviceGuard guard(v.device());
+  // Blocks of the whole 2 F that straddle the halves are quantised in a pass of
+  // their own, from float32 so that nothing is rounded twice.
+  const bool straddle = quant != kPlain && F % 128 != 0;
+  if (quant == kPlain || straddle) {
+    const at::Tensor dh = at::empty({M, 2 * F}, straddle ? v.options().dtype(at::kFloat) : v.options());
+    check_status(fp64emu_swiglu_f8_backward(v.data_ptr(), dtype, M, F, row_stride(v), &keep, dh.data_ptr(),
+                                            dtype_of(dh), 2 * F, nullptr, nullptr, current_stream(v)));
+    if (!straddle) return {dh};
+    return fp64_emu_quant_f8(dh, true, quant == kBoth, false, at::kFloat8_e4m3fn);
+  }
+  std::optional<NewF8> r, c;
+  r.emplace(v, nullptr, M, 2 * F, M, blocks_of(2 * F), at::kFloat8_e4m3fn, false);
+  std::vector<at::Tensor> out{r->q, r->s};
+  if (quant == kBoth) {
+    c.emplace(v, nullptr, 2 * F, M, 2 * F, blocks_of(M), at::kFloat8_e4m3fn, false);
+    out.insert(out.end(), {c->q, c->s});
+  }
+  check_status(fp64emu_swiglu_f8_backward(v.data_ptr(), dtype, M, F, row_stride(v), &keep, nullptr, dtype, 0,
+                                          &r->f, c ? &c->f : nullptr, current_stream(v)));
+  return out;
 }
 
 TORCH_LIBRARY(fp64_emu, ops) {
@@ -419,10 +454,11 @@ TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_mm_nt(Tensor! out, Tensor A, Tensor Bt, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
   ops.def("fp64_emu_bmm_nt(Tensor! out, Tensor A, Tensor Bt, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
   ops.def("fp64_emu_mm_timed(Tensor! out, Tensor! times, Tensor A, Tensor B, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
-  ops.def("fp64_emu_quant_f8(Tensor x, Tensor(a!)? q, Tensor(b!)? s, Tensor(c!)? qt, Tensor(d!)? st, bool tiles) -> ()");
-  ops.def("fp64_emu_mm_f8(Tensor(a!) out, Tensor A, Tensor sA, Tensor B, Tensor sB, bool accumulate) -> ()");
-  ops.def("fp64_emu_swiglu_f8(Tensor h, Tensor(a!)? y, Tensor(b!)? hq, Tensor(c!)? hs, Tensor(d!)? q, Tensor(e!)? s, Tensor(f!)? qt, Tensor(g!)? st) -> ()");
-  ops.def("fp64_emu_swiglu_f8_backward(Tensor dy, Tensor hq, Tensor hs, Tensor(a!)? dh, Tensor(b!)? q, Tensor(c!)? s, Tensor(d!)? qt, Tensor(e!)? st) -> ()");
+  ops.def("fp64_emu_quant_f8(Tensor x, bool rows, bool cols, bool tiles, ScalarType fmt) -> Tensor[]");
+  ops.def("fp64_emu_mm_f8(Tensor A, Tensor sA, Tensor B, Tensor sB, ScalarType dtype) -> Tensor");
+  ops.def("fp64_emu_mm_f8_out(Tensor(a!) out, Tensor A, Tensor sA, Tensor B, Tensor sB, bool accumulate) -> ()");
+  ops.def("fp64_emu_swiglu_f8(Tensor h, int quant, bool keep) -> Tensor[]");
+  ops.def("fp64_emu_swiglu_f8_backward(Tensor dy, Tensor hq, Tensor hs, int quant) -> Tensor[]");
 }
 
 // PyTorch-ROCm keeps the CUDA dispatch key for HIP devices.
@@ -434,6 +470,7 @@ TORCH_LIBRARY_IMPL(fp64_emu, CUDA, ops) {
   ops.impl("fp64_emu_mm_timed", &fp64_emu_mm_timed);
   ops.impl("fp64_emu_quant_f8", &fp64_emu_quant_f8);
   ops.impl("fp64_emu_mm_f8", &fp64_emu_mm_f8);
+  ops.impl("fp64_emu_mm_f8_out", &fp64_emu_mm_f8_out);
   ops.impl("fp64_emu_swiglu_f8", &fp64_emu_swiglu_f8);
   ops.impl("fp64_emu_swiglu_f8_backward", &fp64_emu_swiglu_f8_backward);
 }

@@ -26,34 +26,27 @@ from ._ops import ops
 
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BLOCK = 128
-_QUANT = (None, "rows", "both")
+_FORMS = {None: 0, "rows": 1, "both": 2}
 
-
-def _blocks(n):
-    return -(-n // BLOCK)
-
-
-def _codes(like, batch, rows, depth, fmt):
-    """Room for codes in rows of a multiple of 16 bytes, which the product copies fastest."""
-    q = torch.empty((*batch, rows, -(-depth // 16) * 16), dtype=fmt, device=like.device)
-    return q if depth % 16 == 0 else q[..., :depth]
-
-
-def _scales(like, batch, rows, blocks):
-    """Scales stored block by block, in the order the product reads them."""
-    s = torch.empty((*batch, blocks, rows), dtype=torch.float32, device=like.device)
-    return s.transpose(-1, -2)
-
-
-def _along_rows(x):
-    return x if x.size(-1) <= 1 or x.stride(-1) == 1 else x.contiguous()
+# The overloads themselves: resolving a packet's overload costs a microsecond a call.
+_quant = ops.fp64_emu_quant_f8.default
+_mm = ops.fp64_emu_mm_f8.default
+_mm_out = ops.fp64_emu_mm_f8_out.default
+_swiglu = ops.fp64_emu_swiglu_f8.default
+_swiglu_backward = ops.fp64_emu_swiglu_f8_backward.default
 
 
 def _check_x(x, fmt):
     if x.dim() not in (2, 3):
         raise ValueError(f"expect x as [M, K] or [batch, M, K], got {tuple(x.shape)}")
-    if fmt not in (E4M3, E5M2):
+    if fmt is not E4M3 and fmt is not E5M2:
         raise ValueError(f"fmt must be float8_e4m3fn or float8_e5m2, got {fmt}")
+
+
+def _form(quant):
+    if quant not in _FORMS:
+        raise ValueError(f"quant must be one of {tuple(_FORMS)}, got {quant!r}")
+    return _FORMS[quant]
 
 
 def quant_f8(x: torch.Tensor, rows: bool = True, cols: bool = False, fmt: torch.dtype = E4M3):
@@ -61,18 +54,12 @@ def quant_f8(x: torch.Tensor, rows: bool = True, cols: bool = False, fmt: torch.
 
     rows: (q, s) with blocks along K, q [.., M, K]; cols: (qt, st) with blocks
     along M and the codes laid transposed, qt [.., K, M]; with both
-    (q, s, qt, st), from one pass over x."""
+    (q, s, qt, st), from one pass over x.  Codes come in rows of a multiple of
+    16 bytes, scales stored block by block."""
     _check_x(x, fmt)
     if not (rows or cols):
         raise ValueError("neither rows nor cols are asked for")
-    *batch, M, K = x.shape
-    q = s = qt = st = None
-    if rows:
-        q, s = _codes(x, batch, M, K, fmt), _scales(x, batch, M, _blocks(K))
-    if cols:
-        qt, st = _codes(x, batch, K, M, fmt), _scales(x, batch, K, _blocks(M))
-    ops.fp64_emu_quant_f8(_along_rows(x), q, s, qt, st, False)
-    return (q, s, qt, st) if rows and cols else (q, s) if rows else (qt, st)
+    return tuple(_quant(x, rows, cols, False, fmt))
 
 
 def quant_f8_tiles(x: torch.Tensor, transposed: bool = False, fmt: torch.dtype = E4M3):
@@ -80,13 +67,7 @@ def quant_f8_tiles(x: torch.Tensor, transposed: bool = False, fmt: torch.dtype =
     `transposed` (q, s, qt, st), the same values laid out as x^T.  The form of
     a weight, whose forward product and input gradient read it both ways."""
     _check_x(x, fmt)
-    *batch, M, K = x.shape
-    q, s = _codes(x, batch, M, K, fmt), _scales(x, batch, _blocks(M), _blocks(K))
-    qt = st = None
-    if transposed:
-        qt, st = _codes(x, batch, K, M, fmt), _scales(x, batch, _blocks(K), _blocks(M))
-    ops.fp64_emu_quant_f8(_along_rows(x), q, s, qt, st, True)
-    return (q, s, qt, st) if transposed else (q, s)
+    return tuple(_quant(x, True, transposed, True, fmt))
 
 
 def _product(dim, A, sA, B, sB, out_dtype, out, accumulate):
@@ -95,8 +76,8 @@ def _product(dim, A, sA, B, sB, out_dtype, out, accumulate):
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((*A.shape[:-1], B.size(-2)), dtype=out_dtype, device=A.device)
-    ops.fp64_emu_mm_f8(out, A, sA, B, sB, accumulate)
+        return _mm(A, sA, B, sB, out_dtype)
+    _mm_out(out, A, sA, B, sB, accumulate)
     return out
 
 
@@ -105,7 +86,8 @@ def mm_f8(A: torch.Tensor, sA: torch.Tensor, B: torch.Tensor, sB: torch.Tensor,
           accumulate: bool = False) -> torch.Tensor:
     """C = A @ B^T of quantised A [M, K] and B [N, K], A's scales by rows, B's by
     rows or tiles.  out: where to (float32, bfloat16 or float16, rows any
-    distance apart); accumulate: C is added to it, the sum rounded once."""
+    distance apart; out_dtype is then out's); accumulate: C is added to it, the
+    sum rounded once."""
     return _product(2, A, sA, B, sB, out_dtype, out, accumulate)
 
 
@@ -124,47 +106,21 @@ def swiglu_f8(h: torch.Tensor, quant: str = None, keep: bool = True):
     quantised from its float32 values.  keep: then also (hq, hs), h by blocks of
     128 along each half in e4m3 (scales [M, 2 ceil(F / 128)]): the checkpoint
     swiglu_f8_backward takes, a byte for each element of h."""
-    if quant not in _QUANT:
-        raise ValueError(f"quant must be one of {_QUANT}, got {quant!r}")
+    form = _form(quant)
     if h.dim() != 2 or h.size(1) % 2:
         raise ValueError(f"expect h as [M, 2 F], got {tuple(h.shape)}")
-    M, F = h.size(0), h.size(1) // 2
-    y = q = s = qt = st = hq = hs = None
-    if quant is None:
-        y = torch.empty((M, F), dtype=h.dtype, device=h.device)
-    else:
-        q, s = _codes(h, (), M, F, E4M3), _scales(h, (), M, _blocks(F))
-        if quant == "both":
-            qt, st = _codes(h, (), F, M, E4M3), _scales(h, (), F, _blocks(M))
-    if keep:
-        hq, hs = _codes(h, (), M, 2 * F, E4M3), _scales(h, (), M, 2 * _blocks(F))
-    ops.fp64_emu_swiglu_f8(_along_rows(h), y, hq, hs, q, s, qt, st)
-    return tuple(t for t in (y, q, s, qt, st, hq, hs) if t is not None)
+    return tuple(_swiglu(h, form, keep))
 
 
 def swiglu_f8_backward(dy: torch.Tensor, hq: torch.Tensor, hs: torch.Tensor, quant: str = None):
     """The gradient of swiglu_f8 for dy [M, F], taken at the values its checkpoint
     (hq, hs) stands for.  quant None: dh [M, 2 F] in dy's type; "rows": (q, s);
     "both": (q, s, qt, st), quantised from the float32 values."""
-    if quant not in _QUANT:
-        raise ValueError(f"quant must be one of {_QUANT}, got {quant!r}")
+    form = _form(quant)
     if dy.dim() != 2:
         raise ValueError(f"expect dy as [M, F], got {tuple(dy.shape)}")
-    M, F = dy.shape
-    dy = _along_rows(dy)
-    if quant is None or F % BLOCK:
-        # Blocks of the whole 2 F that straddle the halves are quantised in a pass of
-        # their own, from float32 so that nothing is rounded twice.
-        dh = torch.empty((M, 2 * F), dtype=dy.dtype if quant is None else torch.float32,
-                         device=dy.device)
-        ops.fp64_emu_swiglu_f8_backward(dy, hq, hs, dh, None, None, None, None)
-        return dh if quant is None else quant_f8(dh, cols=quant == "both")
-    q, s = _codes(dy, (), M, 2 * F, E4M3), _scales(dy, (), M, _blocks(2 * F))
-    qt = st = None
-    if quant == "both":
-        qt, st = _codes(dy, (), 2 * F, M, E4M3), _scales(dy, (), 2 * F, _blocks(M))
-    ops.fp64_emu_swiglu_f8_backward(dy, hq, hs, None, q, s, qt, st)
-    return (q, s) if qt is None else (q, s, qt, st)
+    got = _swiglu_backward(dy, hq, hs, form)
+    return got[0] if form == 0 else tuple(got)
 
 
 class _Linear(torch.autograd.Function):
@@ -215,7 +171,7 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tenso
     return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))))
 
 
-class _Swiglu(torch.autograd.Function):
+class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h):
         y, *kept = swiglu_f8(h.reshape(-1, h.size(-1)), keep=ctx.needs_input_grad[0])
@@ -233,7 +189,7 @@ def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
     backward pass reads an 8-bit checkpoint of h instead of h."""
     if h.dim() < 1 or h.size(-1) % 2:
         raise ValueError(f"expect h as [.., 2 F], got {tuple(h.shape)}")
-    return _Swiglu.apply(h)
+    return _SwigluCkpt.apply(h)
 
 
 __all__ = ["quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",
