@@ -438,31 +438,49 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 3 : 4) quant_til
   if constexpr (kForm & kTiles) {
     emit_tile<kFmt>(v, t, row0, col0, g.rows, g.cols, lds);
   } else {
-    if constexpr (kForm & kRows) emit_rows<kFmt>(v, t, row0, col0, kb, g.rows);
-    v.again();
-    if constexpr (kForm & kCols) emit_cols<kFmt>(v, t, row0, col0, mb, g.cols, lds);
+    if constexpr (kForm & kRows) {
+      emit_rows<kFmt>(v, t, row0, col0, kb, g.rows);
+      v.again();
+    }
+    emit_cols<kFmt>(v, t, row0, col0, mb, g.cols, lds);
   }
 }
 
-// Rows only, few of them: 16 lanes per block, so that one token's blocks
-// spread over work groups instead of filling 1 row in 128 of a tile.
+// Rows only: 16 lanes per block, so that one token's blocks spread over work groups
+// instead of filling 1 row in 128 of a tile.
+struct Unit {
+  int64_t row, kb, col;      // block kb of a row; the lane's first column
+  int cl, valid;
+};
+// Unit i of `rows` rows of `blocks` blocks of a matrix of K columns.
+__device__ __forceinline__ Unit unit_at(int64_t i, int64_t blocks, int64_t K) {
+  Unit u;
+  u.row = (uint64_t)i >> 31 ? i / blocks : (int64_t)((uint32_t)i / (uint32_t)blocks);
+  u.kb = i - u.row * blocks;
+  u.cl = threadIdx.x & 15;
+  u.col = u.kb * kBlk + 8 * u.cl;
+  u.valid = (int)(K - u.col < 8 ? K - u.col : 8);
+  return u;
+}
+// A unit's codes and scale from a lane's eight values.
+template <int kFmt, class H>
+__device__ __forceinline__ void emit_unit(const H& v, const Unit& u, int64_t col, int64_t kb, const Out8& o) {
+  const float a = amax_of(row16_max(v.row_mag(0)));
+  put8(o.q + u.row * o.ld + col, u.valid, row_codes<kFmt>(v, 0, inverse_scale<kFmt>(a)));
+  if (u.cl == 0) o.s[u.row * o.s_row + kb * o.s_block] = scale_of<kFmt>(a);
+}
+
 template <int kT, int kFmt>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(QuantArgs g) {
-  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-  const int cl = threadIdx.x & 15;
-  const int64_t row = (uint32_t)unit / (uint32_t)g.kblocks, kb = unit - row * g.kblocks;
-  const int64_t col = kb * kBlk + 8 * cl;
-  const bool live = row < g.M;
-  const int valid = live && col < g.K ? (int)(g.K - col < 8 ? g.K - col : 8) : 0;
-  const int64_t b = g.batch0 + blockIdx.z;
+  const int64_t b = g.batch0 + blockIdx.z, units = g.M * g.kblocks;
   Out8 o = g.rows;
   member(o, b);
-  Held<kT> v;
-  v.load(0, g.x, b * g.stride_x + row * g.ldx + col, valid);
-  const float a = amax_of(row16_max(v.row_mag(0)));
-  if (!live) return;
-  put8(o.q + row * o.ld + col, valid, row_codes<kFmt>(v, 0, inverse_scale<kFmt>(a)));
-  if (cl == 0) o.s[row * o.s_row + kb * o.s_block] = scale_of<kFmt>(a);
+  for (int64_t i = blockIdx.x * 16 + (threadIdx.x >> 4); i < units; i += gridDim.x * 16) {
+    const Unit u = unit_at(i, g.kblocks, g.K);
+    Held<kT> v;
+    v.load(0, g.x, b * g.stride_x + u.row * g.ldx + u.col, u.valid);
+    emit_unit<kFmt>(v, u, u.col, u.kb, o);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -524,6 +542,28 @@ __global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
   }
   if (a.rows.q) emit_rows<kF>(y, t, row0, col0, fb, a.rows);
   if (a.cols.q) emit_cols<kF>(y, t, row0, col0, mb, a.cols, lds);
+}
+
+// Without columns to write: a block of a row on 16 lanes.
+template <int kT>
+__global__ void __launch_bounds__(kThreads) swiglu_rows_kernel(SwigluArgs a) {
+  constexpr int kF = FP64EMU_E4M3;
+  const int64_t units = a.M * a.fblocks;
+  for (int64_t i = blockIdx.x * 16 + (threadIdx.x >> 4); i < units; i += gridDim.x * 16) {
+    const Unit t = unit_at(i, a.fblocks, a.F);
+    Held<kT> g, u;
+    g.load(0, a.h, t.row * a.ldh + t.col, t.valid);
+    u.load(0, a.h, t.row * a.ldh + a.F + t.col, t.valid);
+    if (a.keep.q) {
+      emit_unit<kF>(g, t, t.col, t.kb, a.keep);
+      emit_unit<kF>(u, t, a.F + t.col, a.fblocks + t.kb, a.keep);
+    }
+    Held<FP64EMU_F32> y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y.v[0][j] = g.at(0, j) * sigmoid(g.at(0, j)) * u.at(0, j);
+    if (a.y) store8<kT>(a.y, t.row * a.ldy + t.col, t.valid, y.v[0]);
+    if (a.rows.q) emit_unit<kF>(y, t, t.col, t.kb, a.rows);
+  }
 }
 
 struct SwigluGradArgs {
@@ -593,6 +633,42 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) swiglu_gr
   }
   if (a.rows.q) emit_rows<kF>(d, t, row0, at + col0, block + fb, a.rows);
   if (a.cols.q) emit_cols<kF>(d, t, row0, at + col0, mb, a.cols, lds);
+}
+
+// Without columns to write: a block of a row on 16 lanes, both halves.
+template <int kT, int kO>
+__global__ void __launch_bounds__(kThreads) swiglu_grad_rows_kernel(SwigluGradArgs a) {
+  constexpr int kF = FP64EMU_E4M3;
+  const int64_t units = a.M * a.fblocks;
+  for (int64_t i = blockIdx.x * 16 + (threadIdx.x >> 4); i < units; i += gridDim.x * 16) {
+    const Unit t = unit_at(i, a.fblocks, a.F);
+    Held<kT> dy;
+    dy.load(0, a.dy, t.row * a.ldy + t.col, t.valid);
+    const uint8_t* q = a.keep.q + t.row * a.keep.ld + t.col;
+    const v2u g = get8(q, t.valid), u = get8(q + a.F, t.valid);
+    const float* s = a.keep.s + t.row * a.keep.s_row;
+    const float sg = s[t.kb * a.keep.s_block], su = s[(a.fblocks + t.kb) * a.keep.s_block];
+    Held<FP64EMU_F32> dg, du;
+    float gv[8], uv[8];
+    values4<kF>(g[0], gv);
+    values4<kF>(g[1], gv + 4);
+    values4<kF>(u[0], uv);
+    values4<kF>(u[1], uv + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = gv[j] * sg, sig = sigmoid(x), ds = dy.at(0, j) * sig;
+      du.v[0][j] = ds * x;
+      dg.v[0][j] = ds * (uv[j] * su) * fmaf(x, 1.0f - sig, 1.0f);
+    }
+    if (a.dh) {
+      store8<kO>(a.dh, t.row * a.ldh + t.col, t.valid, dg.v[0]);
+      store8<kO>(a.dh, t.row * a.ldh + a.F + t.col, t.valid, du.v[0]);
+    }
+    if (a.rows.q) {
+      emit_unit<kF>(dg, t, t.col, t.kb, a.rows);
+      emit_unit<kF>(du, t, a.F + t.col, a.fblocks + t.kb, a.rows);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1390,6 +1466,11 @@ int out8(const fp64emu_f8_t* f, int64_t depth, Out8* o) {
 
 constexpr int64_t kMaxGroups = (1ll << 31) / kThreads;    // work items of one launch stay below 2^31
 
+// Work groups for a matrix's blocks of rows, 16 each.
+unsigned unit_groups(int64_t rows, int64_t blocks) {
+  return (unsigned)std::min<int64_t>((rows * blocks + 15) / 16, 1 << 20);
+}
+
 template <int kT, int kFmt>
 int launch_quant(QuantArgs g, int64_t batch, int64_t mblocks, bool tiles, hipStream_t s) {
   for (; g.batch0 < batch; g.batch0 += kMaxGridZ) {
@@ -1397,11 +1478,8 @@ int launch_quant(QuantArgs g, int64_t batch, int64_t mblocks, bool tiles, hipStr
     const dim3 grid((unsigned)(mblocks * g.kblocks), 1, z);
     if (tiles) {
       quant_tile_kernel<kT, kFmt, kTiles><<<grid, kThreads, 0, s>>>(g);
-    } else if (!g.cols.q && g.M < kBlk) {
-      const int64_t units = g.M * g.kblocks;
-      quant_rows_kernel<kT, kFmt><<<dim3((unsigned)((units + 15) / 16), 1, z), kThreads, 0, s>>>(g);
     } else if (!g.cols.q) {
-      quant_tile_kernel<kT, kFmt, kRows><<<grid, kThreads, 0, s>>>(g);
+      quant_rows_kernel<kT, kFmt><<<dim3(unit_groups(g.M, g.kblocks), 1, z), kThreads, 0, s>>>(g);
     } else if (!g.rows.q) {
       quant_tile_kernel<kT, kFmt, kCols><<<grid, kThreads, 0, s>>>(g);
     } else {
@@ -1641,9 +1719,18 @@ int fp64emu_swiglu_f8(const void* h, int dtype, int64_t M, int64_t F, int64_t ld
   if (mblocks > kMaxGroups / a.fblocks) return invalid("operand too large for one launch");
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const unsigned groups = (unsigned)(mblocks * a.fblocks);
-  if (dtype == FP64EMU_F32) swiglu_kernel<FP64EMU_F32><<<groups, kThreads, 0, s>>>(a);
-  else if (dtype == FP64EMU_BF16) swiglu_kernel<FP64EMU_BF16><<<groups, kThreads, 0, s>>>(a);
-  else swiglu_kernel<FP64EMU_F16><<<groups, kThreads, 0, s>>>(a);
+  const unsigned few = unit_groups(M, a.fblocks);
+#define FP64EMU_SWIGLU(T)                                            \
+  case T:                                                            \
+    if (cols) swiglu_kernel<T><<<groups, kThreads, 0, s>>>(a);       \
+    else swiglu_rows_kernel<T><<<few, kThreads, 0, s>>>(a);          \
+    break;
+  switch (dtype) {
+    FP64EMU_SWIGLU(FP64EMU_F32)
+    FP64EMU_SWIGLU(FP64EMU_BF16)
+    FP64EMU_SWIGLU(FP64EMU_F16)
+  }
+#undef FP64EMU_SWIGLU
   return check_hip(hipGetLastError(), "swiglu_f8 launch");
 }
 
@@ -1680,8 +1767,12 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   a.tiles = mblocks * a.fblocks;
   const unsigned groups = (unsigned)((a.tiles + 7) / 8 * 16);
-#define FP64EMU_GRAD(T, O)                                                               \
-  if (dtype == T && out_dtype == O) swiglu_grad_kernel<T, O><<<groups, kThreads, 0, s>>>(a);
+  const unsigned few = unit_groups(M, a.fblocks);
+#define FP64EMU_GRAD(T, O)                                              \
+  if (dtype == T && out_dtype == O) {                                   \
+    if (cols) swiglu_grad_kernel<T, O><<<groups, kThreads, 0, s>>>(a);  \
+    else swiglu_grad_rows_kernel<T, O><<<few, kThreads, 0, s>>>(a);     \
+  }
   FP64EMU_GRAD(FP64EMU_F32, FP64EMU_F32)
   FP64EMU_GRAD(FP64EMU_BF16, FP64EMU_BF16)
   FP64EMU_GRAD(FP64EMU_F16, FP64EMU_F16)
