@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <string>
 #include <type_traits>
@@ -762,17 +763,33 @@ __device__ __forceinline__ v8i join(const v4i& a, const v4i& b) {
 }
 
 // 16 bytes of a row at k, those past K as zero codes (whatever the memory
-// holds there, if it is memory at all).  Any alignment.
+// holds there, if it is memory at all).  Any alignment.  A row's last, partial 16
+// are its last 16 bytes moved down.
 __device__ __forceinline__ v4i load16_masked(const uint8_t* row, int64_t k, int64_t K) {
-  v4i v = {0, 0, 0, 0};
   if (k + 16 <= K) {
+    v4i v;
     __builtin_memcpy(&v, row + k, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (k + j < K) v[j >> 2] |= (int)((uint32_t)row[k + j] << (8 * (j & 3)));
+    return v;
   }
-  return v;
+  uint64_t w[2] = {0, 0};
+  if (k < K && K >= 16) {
+    __builtin_memcpy(w, row + K - 16, 16);
+    const int drop = 8 * (int)(k + 16 - K);                  // bits, 8 .. 120
+    if (drop < 64) {
+      w[0] = w[0] >> drop | w[1] << (64 - drop);
+      w[1] >>= drop;
+    } else {
+      w[0] = w[1] >> (drop - 64);
+      w[1] = 0;
+    }
+  } else if (k < K) {
+#pragma unroll 1
+    for (int64_t j = K - 1; j >= k; --j) {
+      w[1] = w[1] << 8 | w[0] >> 56;
+      w[0] = w[0] << 8 | row[j];
+    }
+  }
+  return v4i{(int)w[0], (int)(w[0] >> 32), (int)w[1], (int)(w[1] >> 32)};
 }
 
 // Four successive outputs (m, n .. n + 3).
@@ -1401,8 +1418,10 @@ using Tile256 = MmShape<256, 256, 4, 2>;
 using TileWide = MmShape<128, 256, 2, 4>;
 using Tile128 = MmShape<128, 128, 2, 2>;
 
+enum { kFew = 0, kSquare128 = 1, kSquare256 = 2, kWide = 3 };   // forms of a product
+
 struct MmPlan {
-  int form;                  // 0: few rows, 1: 128 x 128 tiles, 2: 256 x 256 tiles
+  int form;
   int tile_m, tile_n;
   int64_t tiles_m, tiles_n;
   int splits, kb_per_split;
@@ -1410,33 +1429,57 @@ struct MmPlan {
 
 constexpr int kCUs = 256;
 
-MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
-  MmPlan p{};
-  const int64_t nkb = (K + kBlk - 1) / kBlk;
-  auto shape = [&](int form, int tm, int tn) {
-    p.form = form;
-    p.tile_m = tm;
-    p.tile_n = tn;
-    p.tiles_m = (M + tm - 1) / tm;
-    p.tiles_n = (N + tn - 1) / tn;
-  };
-  if (M <= 64) {
-    const int tm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    shape(0, tm, M <= 16 ? 16 : 32);
-  } else {
-    if (dtype == FP64EMU_F32) shape(3, 128, 256);
-    else shape(2, 256, 256);
-    if (batch * p.tiles_m * p.tiles_n < kCUs) shape(1, 128, 128);
+// A form's time in microseconds, launch included: `groups` work groups of `steps`
+// blocks of K each.  Constants from 40 shapes of 1 to 8192 rows and columns and 512 to
+// 100000 deep in every form and split (bfloat16 and float32 outputs), which it
+// meets within a quarter where two forms are close: a work group's blocks take this
+// long with one group to a CU, and longer where the groups of all CUs share the
+// caches' rate or two share a CU.
+double mm_time(int form, int tile_m, bool exact, double groups, double steps) {
+  const double share = std::min(groups, (double)kCUs) / kCUs;
+  switch (form) {
+    case kFew: {               // eight waves, a block each
+      const double per = tile_m == 16 ? 0.85 : tile_m == 32 ? 2.6 : 3.0;
+      return 2.5 + std::ceil(groups / (tile_m == 16 ? 2 * kCUs : kCUs)) * (0.7 + per * std::ceil(steps / 8));
+    }
+    case kSquare128: {         // two groups to a CU, the last round's perhaps one
+      const double one = exact ? 1.37 : 0.98, two = exact ? 1.86 : 1.12;
+      const double full = std::floor(groups / (2 * kCUs)), rest = groups - full * 2 * kCUs;
+      return 2.5 + full * (1.5 + two * steps) + (rest > 0 ? 1.5 + (rest <= kCUs ? one : two) * steps : 0.0);
+    }
+    case kSquare256:
+      return 1.0 + std::ceil(groups / kCUs) * (5.0 + (1.3 + 0.4 * share) * steps);
+    default:
+      return 2.0 + std::ceil(groups / kCUs) * (5.0 + 1.75 * steps);
   }
-  // Splits: where the tiles leave compute units idle and each split keeps
-  // at least 8 blocks of K.
-  const int64_t groups = std::max<int64_t>(batch * p.tiles_m * p.tiles_n, 1);
-  const int64_t want = p.form == 0 ? 2 * kCUs : p.form == 1 ? 2 * kCUs : kCUs;
-  int64_t s = std::min<int64_t>(std::max<int64_t>(want / groups, 1), std::max<int64_t>(nkb / 8, 1));
-  s = std::min<int64_t>(s, 32);
-  p.kb_per_split = (int)((nkb + s - 1) / s);
-  p.splits = p.kb_per_split > 0 ? (int)((nkb + p.kb_per_split - 1) / p.kb_per_split) : 1;
-  return p;
+}
+
+// The form and the number of K splits that take least by mm_time; a split adds a
+// launch and its partial sums' way to memory and back.
+MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
+  const bool exact = dtype == FP64EMU_F32;
+  const int64_t nkb = (K + kBlk - 1) / kBlk;
+  MmPlan best{};
+  double least = 1e300;
+  auto consider = [&](int form, int tm, int tn) {
+    const int64_t tiles_m = (M + tm - 1) / tm, tiles_n = (N + tn - 1) / tn;
+    for (int64_t s = 1; s <= 32; s *= 2) {
+      if (s > 1 && nkb < 2 * s) break;
+      const int64_t per = (nkb + s - 1) / s;
+      double t = mm_time(form, tm, exact, (double)(batch * tiles_m * tiles_n) * (double)s, (double)per);
+      if (s > 1) t += 3.0 + 8.0 * (double)s * (double)(batch * M) * (double)N / 4e6;
+      if (t >= least) continue;
+      least = t;
+      best = MmPlan{form, tm, tn, tiles_m, tiles_n, per > 0 ? (int)((nkb + per - 1) / per) : 1, (int)per};
+    }
+  };
+  if (M <= 16) consider(kFew, 16, 16);
+  else if (M <= 32) consider(kFew, 32, 32);
+  else consider(kFew, 64, 32);
+  consider(kSquare128, 128, 128);
+  if (exact) consider(kWide, 128, 256);
+  else consider(kSquare256, 256, 256);
+  return best;
 }
 
 int check_hip(hipError_t e, const char* what) {
@@ -1504,13 +1547,14 @@ void launch_few(const MmArgs& g, unsigned groups, hipStream_t s) {
 
 template <int kFA, int kFB>
 void launch_mm(const MmArgs& g, const MmPlan& p, unsigned groups, hipStream_t s) {
-  if (p.form == 2) launch_tile<Tile256, false, kFA, kFB>(g, groups, s);
-  else if (p.form == 3) launch_tile<TileWide, true, kFA, kFB>(g, groups, s);
-  else if (p.form == 1 && g.dtype == FP64EMU_F32) launch_tile<Tile128, true, kFA, kFB>(g, groups, s);
-  else if (p.form == 1) launch_tile<Tile128, false, kFA, kFB>(g, groups, s);
+  const bool exact = g.dtype == FP64EMU_F32;
+  if (p.form == kSquare256) launch_tile<Tile256, false, kFA, kFB>(g, groups, s);
+  else if (p.form == kWide) launch_tile<TileWide, true, kFA, kFB>(g, groups, s);
+  else if (p.form == kSquare128 && exact) launch_tile<Tile128, true, kFA, kFB>(g, groups, s);
+  else if (p.form == kSquare128) launch_tile<Tile128, false, kFA, kFB>(g, groups, s);
   else if (p.tile_m == 16) launch_few<1, 1, 4, kFA, kFB>(g, groups, s);
   else if (p.tile_m == 32) launch_few<2, 2, 2, kFA, kFB>(g, groups, s);
-  else launch_few<4, 2, 2, kFA, kFB>(g, groups, s);
+  else launch_few<4, 2, 1, kFA, kFB>(g, groups, s);
 }
 
 // Whether the tile kernel can copy an operand's rows: 16-byte aligned, a tile's
@@ -1527,8 +1571,8 @@ MmRoom mm_room(const fp64emu_mm_f8_t* p, const MmPlan& plan) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   if (plan.splits > 1) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
   const size_t ld = (size_t)((p->K + 15) / 16 * 16);
-  if (plan.form > 0 && !copyable(p->A)) r.A = up((size_t)(p->batch * p->M) * ld);
-  if (plan.form > 0 && !copyable(p->B)) r.B = up((size_t)(p->batch * p->N) * ld);
+  if (plan.form != kFew && !copyable(p->A)) r.A = up((size_t)(p->batch * p->M) * ld);
+  if (plan.form != kFew && !copyable(p->B)) r.B = up((size_t)(p->batch * p->N) * ld);
   return r;
 }
 
@@ -1663,7 +1707,7 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
     return invalid("product too large for one launch");
   const unsigned groups = (unsigned)(plan.tiles_m * plan.tiles_n * p->batch * plan.splits);
   const int64_t K16 = (p->K + 15) / 16 * 16;
-  if (plan.form > 0 && K16 >= (1ll << 32) / 256 - kBlk) return invalid("K too large for one launch");
+  if (plan.form != kFew && K16 >= (1ll << 32) / 256 - kBlk) return invalid("K too large for one launch");
   if (room.A) {
     uint8_t* to = static_cast<uint8_t*>(workspace) + room.parts;
     pack(p->A, p->batch, p->M, p->K, to, s);
