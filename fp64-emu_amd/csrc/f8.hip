@@ -1077,10 +1077,10 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     lds_u8* stage = (lds_u8*)lds + st * S::kStage;
     if (c < S::kCopB)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(srcB, stage + (c * S::kWaves + wave) * 1024, 16,
-                                               (int)offB[c] + kb * kBlk, 0, 0, 0);
+                                               (int)(offB[c] + (uint32_t)kb * kBlk), 0, 0, 0);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(srcA, stage + S::kOffA + ((c - S::kCopB) * S::kWaves + wave) * 1024, 16,
-                                               (int)offA[c - S::kCopB] + kb * kBlk, 0, 0, 0);
+                                               (int)(offA[c - S::kCopB] + (uint32_t)kb * kBlk), 0, 0, 0);
   };
   auto copy_scales = [&](int st) {
     if (wave * 64 >= S::kBN + S::kBM) return;

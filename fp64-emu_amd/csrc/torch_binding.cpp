@@ -203,6 +203,14 @@ int dtype_of(const at::Tensor& t) {
   }
 }
 
+// t where its rows are contiguous and do not overlap (those of an expanded tensor do),
+// else a contiguous copy.
+at::Tensor in_rows(const at::Tensor& t) {
+  const int64_t d = t.dim(), w = t.size(d - 1);
+  const bool fine = (w <= 1 || t.stride(d - 1) == 1) && (t.size(d - 2) <= 1 || t.stride(d - 2) >= w);
+  return fine ? t : t.contiguous();
+}
+
 // q [(batch,) rows, depth] and its scales [(batch,) rows or tile rows, blocks].
 fp64emu_f8_t f8_of(const at::Tensor& q, const at::Tensor& s, const char* what) {
   fp64emu_f8_t f{};
@@ -220,7 +228,6 @@ fp64emu_f8_t f8_of(const at::Tensor& q, const at::Tensor& s, const char* what) {
               (depth + 127) / 128, ", got ", s.size(d - 1));
   TORCH_CHECK(s.size(d - 2) == rows || s.size(d - 2) == (rows + 127) / 128, what,
               ": expect scales by rows or by tiles of 128 rows");
-  TORCH_CHECK(depth <= 1 || q.stride(d - 1) == 1, what, ": codes must be contiguous along K");
   f.q = static_cast<uint8_t*>(q.data_ptr());
   f.s = s.data_ptr<float>();
   f.ld = rows > 1 ? q.stride(d - 2) : std::max<int64_t>(depth, (depth + 15) / 16 * 16);
@@ -300,9 +307,11 @@ constexpr int64_t kPlain = 0, kRows = 1, kBoth = 2;    // what form an activatio
 
 void product_f8(const at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
                 const at::Tensor& sB, bool accumulate) {
+  TORCH_CHECK(A.dim() >= 2 && B.dim() >= 2 && out.dim() >= 2, "A, B and out are all 2-D or all 3-D");
+  const at::Tensor qa = in_rows(A), qb = in_rows(B);
   fp64emu_mm_f8_t p{};
-  p.A = f8_of(A, sA, "A");
-  p.B = f8_of(B, sB, "B");
+  p.A = f8_of(qa, sA, "A");
+  p.B = f8_of(qb, sB, "B");
   const int64_t d = A.dim();
   TORCH_CHECK(B.dim() == d && out.dim() == d, "A, B and out are all 2-D or all 3-D");
   TORCH_CHECK(A.device() == B.device() && A.device() == out.device(),
@@ -339,7 +348,7 @@ std::vector<at::Tensor> fp64_emu_quant_f8(const at::Tensor& x, bool rows, bool c
   const int64_t d = x.dim();
   TORCH_CHECK(d == 2 || d == 3, "expect x as [M, K] or [batch, M, K]");
   TORCH_CHECK(fmt == at::kFloat8_e4m3fn || fmt == at::kFloat8_e5m2, "fmt must be float8_e4m3fn or float8_e5m2");
-  const at::Tensor v = x.size(d - 1) <= 1 || x.stride(d - 1) == 1 ? x : x.contiguous();
+  const at::Tensor v = in_rows(x);
   check_rows(v, "x");
   const int dtype = dtype_of(v);
   const int64_t batch = d == 3 ? v.size(0) : 1, M = v.size(d - 2), K = v.size(d - 1);
@@ -385,7 +394,7 @@ void fp64_emu_mm_f8_out(at::Tensor& out, const at::Tensor& A, const at::Tensor& 
 std::vector<at::Tensor> fp64_emu_swiglu_f8(const at::Tensor& h, int64_t quant, bool keep) {
   TORCH_CHECK(h.dim() == 2 && h.size(1) % 2 == 0, "expect h as [M, 2 F]");
   TORCH_CHECK(quant >= kPlain && quant <= kBoth, "quant: 0 plain, 1 rows, 2 both");
-  const at::Tensor v = h.size(1) <= 1 || h.stride(1) == 1 ? h : h.contiguous();
+  const at::Tensor v = in_rows(h);
   check_rows(v, "h");
   const int dtype = dtype_of(v);
   const int64_t M = v.size(0), F = v.size(1) / 2, FB = blocks_of(F);
@@ -419,11 +428,12 @@ std::vector<at::Tensor> fp64_emu_swiglu_f8_backward(const at::Tensor& dy, const 
                                                     const at::Tensor& hs, int64_t quant) {
   TORCH_CHECK(dy.dim() == 2, "expect dy as [M, F]");
   TORCH_CHECK(quant >= kPlain && quant <= kBoth, "quant: 0 plain, 1 rows, 2 both");
-  const at::Tensor v = dy.size(1) <= 1 || dy.stride(1) == 1 ? dy : dy.contiguous();
+  const at::Tensor v = in_rows(dy);
   check_rows(v, "dy");
   const int dtype = dtype_of(v);
   const int64_t M = v.size(0), F = v.size(1);
-  const fp64emu_f8_t keep = kept_of(v, hq, hs, M, F);
+  const at::Tensor codes = in_rows(hq);
+  const fp64emu_f8_t keep = kept_of(v, codes, hs, M, F);
   const c10::DeviceGuard guard(v.device());
   // Blocks of the whole 2 F that straddle the halves are quantised in a pass of
   // their own, from float32 so that nothing is rounded twice.

@@ -201,6 +201,35 @@ def test_mm_layouts(dev, shape):
             assert (out.as_strided((M, 2), (N + 5, 1), 0) == -7).all()
 
 
+def test_expanded_and_transposed_inputs(dev):
+    """Rows that lie on each other (an expanded tensor's) and columns that lie apart: as their copies."""
+    _say("expanded")
+    x = _randn((1, 400), 31).to(dev).expand(140, 400)
+    for a, b in zip(fp64_emu.quant_f8(x, cols=True), fp64_emu.quant_f8(x.contiguous(), cols=True)):
+        assert torch.equal(a.float(), b.float())
+    for y, w in ((x, x.contiguous()), (_randn((400, 140), 32).to(dev).t(), None)):
+        w = y.contiguous() if w is None else w
+        for a, b in zip(fp64_emu.swiglu_f8(y), fp64_emu.swiglu_f8(w)):
+            assert torch.equal(a.float(), b.float())
+    _, hq, hs = fp64_emu.swiglu_f8(x)
+    dy = torch.ones(1, 200, device=dev).expand(140, 200)
+    assert torch.equal(fp64_emu.swiglu_f8_backward(dy, hq[:1].expand(140, 400), hs[:1].expand(140, 4)),
+                       fp64_emu.swiglu_f8_backward(dy.contiguous(), hq, hs))
+    qa, sa = operand((1, 300), 33, device=dev)
+    qb, sb = operand((200, 300), 34, device=dev)
+    want = fp64_emu.mm_f8(qa, sa, qb, sb).expand(150, 200)
+    turned = qb.view(torch.uint8).t().contiguous().t().view(E4M3)
+    assert not turned.is_contiguous()
+    for b in (qb, turned):
+        got = fp64_emu.mm_f8(qa.expand(150, 300), sa.expand(150, 3), b, sb)
+        assert (got.double() - want.double()).abs().max() <= want.abs().max() * 2.0 ** -7
+    x = _randn((60, 256), 35).to(dev).requires_grad_()
+    w = _randn((128, 256), 36, F32).to(dev).requires_grad_()
+    (dx,) = torch.autograd.grad(fp64_emu.linear_f8(x, w).sum(), x)       # an expanded gradient
+    (want,) = torch.autograd.grad(fp64_emu.linear_f8(x, w), x, torch.ones(60, 128, device=dev, dtype=BF16))
+    assert torch.equal(dx, want)
+
+
 def test_mm_nothing_to_do(dev):
     _say("mm empty")
     def e(r, k, fmt=E4M3):
@@ -210,6 +239,11 @@ def test_mm_nothing_to_do(dev):
     out = torch.full((5, 7), 3.0, device=dev)
     assert (fp64_emu.mm_f8(*e(5, 0), *e(7, 0), out=out, accumulate=True) == 3).all()
     assert (fp64_emu.mm_f8(*e(5, 0), *e(7, 0), out=out) == 0).all()
+    x = torch.empty(0, 256, device=dev, dtype=BF16, requires_grad=True)
+    w = torch.ones(128, 256, device=dev, requires_grad=True)
+    y = fp64_emu.linear_f8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+    assert y.shape == (0, 128) and dx.shape == x.shape and (dw == 0).all()
     assert [t.shape for t in fp64_emu.quant_f8(torch.empty(0, 300, device=dev), cols=True)] == [
         (0, 300), (0, 3), (300, 0), (300, 0)]
     assert fp64_emu.swiglu_f8(torch.empty(0, 8, device=dev))[0].shape == (0, 4)
@@ -522,7 +556,6 @@ def test_refusals(dev):
             (lambda: fp64_emu.mm_f8(q, s, w, ws, out=torch.empty(4, 299, device=dev)), "out"),
             (lambda: fp64_emu.mm_f8(q, s, w, ws, out=torch.empty(1, 300, device=dev).expand(4, 300)), "overlap|memory"),
             (lambda: fp64_emu.mm_f8(q, s, w, ws, out_dtype=torch.float64), "expect float32"),
-            (lambda: fp64_emu.mm_f8(q, s, w.t().contiguous().t(), ws), "contiguous along K"),
             (lambda: fp64_emu.swiglu_f8_backward(x, q, s), "hq"),
             (lambda: fp64_emu.swiglu_f8_backward(x[:, :128], q, s[:, :1]), "hs")]:
         with pytest.raises(RuntimeError, match=msg):
