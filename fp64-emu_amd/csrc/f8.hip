@@ -1257,25 +1257,42 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   T* to = static_cast<T*>(g.out) + b * g.stride_o + m * g.ldo + n;
   const uint8_t* from = room + (lane / kLanes) * kRow + (lane % kLanes) * 16;
   constexpr int kRows = 64 / kLanes;                         // rows of one store
+  // What out holds, read whole before the first store: one by one, each store's
+  // rows would wait for memory (16 times a tile).
+  constexpr int kSteps = kExact ? S::kTM * 16 / kRows : 1;
+  T old[kSteps][kEach];
+  if constexpr (kExact) {
+    if (g.accumulate) {
 #pragma unroll
-  for (int r = 0; r < S::kTM * 16; r += kRows, m += kRows, to += kRows * g.ldo) {
-    T w[kEach];
-    __builtin_memcpy(w, __builtin_assume_aligned(from + r * kRow, 16), 16);
-    if (m >= g.M) continue;
-    if (valid == kEach) {
-      if constexpr (kExact) {
-        if (g.accumulate) {
-          T old[kEach];
-          __builtin_memcpy(old, to, 16);
+      for (int i = 0; i < kSteps; ++i) {
+        const T* q = to + (int64_t)i * kRows * g.ldo;
+        if (m + i * kRows >= g.M) break;
+        if (valid == kEach) {
+          __builtin_memcpy(old[i], q, 16);
+        } else {
 #pragma unroll
-          for (int j = 0; j < kEach; ++j) w[j] += old[j];
+          for (int j = 0; j < kEach - 1; ++j) old[i][j] = j < valid ? q[j] : T{};
         }
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::kTM * 16 / kRows; ++i, m += kRows, to += kRows * g.ldo) {
+    T w[kEach];
+    __builtin_memcpy(w, __builtin_assume_aligned(from + i * kRows * kRow, 16), 16);
+    if (m >= g.M) continue;
+    if constexpr (kExact) {
+      if (g.accumulate) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) w[j] += old[i][j];
+      }
+    }
+    if (valid == kEach) {
       store16_past(to, w);
     } else {
 #pragma unroll
       for (int j = 0; j < kEach - 1; ++j)
-        if (j < valid) to[j] = kExact && g.accumulate ? w[j] + to[j] : w[j];
+        if (j < valid) to[j] = w[j];
     }
   }
 }
