@@ -1367,24 +1367,32 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
     __builtin_memcpy(&v, row + (int64_t)kb * kBlk + 32 * fg, 32);
     return v;
   };
-  auto step = [&](const v8i (&cb)[kTN], const v8i (&ca)[kTM], int kb) {
+  // A block's operands as they are loaded, all of them before the first is used.
+  struct Block {
+    v8i b[kTN], a[kTM];
+    float sa[kTM], sb[kTN][kRowB ? 4 : 1];
+  };
+  auto scales = [&](Block& o, int kb) {
+#pragma unroll
+    for (int y = 0; y < kTM; ++y) o.sa[y] = sa[y][kb * g.sA_blk];
+#pragma unroll
+    for (int x = 0; x < kTN; ++x)
+#pragma unroll
+      for (int i = 0; i < (kRowB ? 4 : 1); ++i) o.sb[x][i] = sb[x][i][kb * g.sB_blk];
+  };
+  auto step = [&](const Block& o) {
     Frag<true, kFA> fa[kTM];
 #pragma unroll
-    for (int y = 0; y < kTM; ++y) fa[y] = Frag<true, kFA>(ca[y]);
-    float s[kTM];
-#pragma unroll
-    for (int y = 0; y < kTM; ++y) s[y] = sa[y][kb * g.sA_blk];
+    for (int y = 0; y < kTM; ++y) fa[y] = Frag<true, kFA>(o.a[y]);
 #pragma unroll
     for (int x = 0; x < kTN; ++x) {
-      float t[kRowB ? 4 : 1];
-#pragma unroll
-      for (int i = 0; i < (kRowB ? 4 : 1); ++i) t[i] = sb[x][i][kb * g.sB_blk];
-      const Frag<true, kFB> fb(cb[x]);
+      const Frag<true, kFB> fb(o.b[x]);
 #pragma unroll
       for (int y = 0; y < kTM; ++y) {
         const v4f p = block_sum<true, kFB, kFA>(fb, fa[y]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[x][y][i] = fmaf(p[i], s[y] * t[kRowB ? i : 0], acc[x][y][i]);
+        for (int i = 0; i < 4; ++i)
+          acc[x][y][i] = fmaf(p[i], o.sa[y] * o.sb[x][kRowB ? i : 0], acc[x][y][i]);
       }
     }
   };
@@ -1392,24 +1400,27 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   const int full = (int)(g.K / kBlk) < kb1 ? (int)(g.K / kBlk) : kb1;    // blocks before it are whole
   int kb = kb0 + wave;
   for (; kb + (kU - 1) * kFewWaves < full; kb += kU * kFewWaves) {
-    v8i fb[kU][kTN], fa[kU][kTM];
+    Block o[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
 #pragma unroll
-      for (int x = 0; x < kTN; ++x) fb[u][x] = whole(pb[x], kb + u * kFewWaves);
+      for (int x = 0; x < kTN; ++x) o[u].b[x] = whole(pb[x], kb + u * kFewWaves);
 #pragma unroll
-      for (int y = 0; y < kTM; ++y) fa[u][y] = whole(pa[y], kb + u * kFewWaves);
+      for (int y = 0; y < kTM; ++y) o[u].a[y] = whole(pa[y], kb + u * kFewWaves);
+      scales(o[u], kb + u * kFewWaves);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) step(fb[u], fa[u], kb + u * kFewWaves);
+    for (int u = 0; u < kU; ++u) step(o[u]);
   }
   for (; kb < kb1; kb += kFewWaves) {
-    v8i fb[kTN], fa[kTM];
+    Block o;
 #pragma unroll
-    for (int x = 0; x < kTN; ++x) fb[x] = frag(pb[x], kb);
+    for (int x = 0; x < kTN; ++x) o.b[x] = frag(pb[x], kb);
 #pragma unroll
-    for (int y = 0; y < kTM; ++y) fa[y] = frag(pa[y], kb);
-    step(fb, fa, kb);
+    for (int y = 0; y < kTM; ++y) o.a[y] = frag(pa[y], kb);
+    scales(o, kb);
+    step(o);
   }
 
 #pragma unroll
@@ -1456,7 +1467,7 @@ double mm_time(int form, int tile_m, bool exact, double groups, double steps) {
   const double share = std::min(groups, (double)kCUs) / kCUs;
   switch (form) {
     case kFew: {               // eight waves, a block each
-      const double per = tile_m == 16 ? 0.85 : tile_m == 32 ? 2.6 : 3.0;
+      const double per = tile_m == 16 ? 0.85 : tile_m == 32 ? 1.8 : 3.0;
       return 2.5 + std::ceil(groups / (tile_m == 16 ? 2 * kCUs : kCUs)) * (0.7 + per * std::ceil(steps / 8));
     }
     case kSquare128: {         // two groups to a CU, the last round's perhaps one
@@ -1570,7 +1581,7 @@ void launch_mm(const MmArgs& g, const MmPlan& p, unsigned groups, hipStream_t s)
   else if (p.form == kSquare128 && exact) launch_tile<Tile128, true, kFA, kFB>(g, groups, s);
   else if (p.form == kSquare128) launch_tile<Tile128, false, kFA, kFB>(g, groups, s);
   else if (p.tile_m == 16) launch_few<1, 1, 4, kFA, kFB>(g, groups, s);
-  else if (p.tile_m == 32) launch_few<2, 2, 2, kFA, kFB>(g, groups, s);
+  else if (p.tile_m == 32) launch_few<2, 2, 1, kFA, kFB>(g, groups, s);
   else launch_few<4, 2, 1, kFA, kFB>(g, groups, s);
 }
 
