@@ -421,7 +421,10 @@ struct QuantArgs {
 enum { kRows = 1, kCols = 2, kTiles = 4 };                 // what a call asks for
 
 // One work group per 128 x 128 tile (blocks along K fastest: a row of tiles
-// reads whole rows of x), every value read once.
+// reads whole rows of x), every value read once.  Bound by its bytes: 8192 x 8192
+// bfloat16 into rows and columns 60 us, 4.6 TB/s where a large copy reaches 5.2.
+// A float32 2049 x 4097 into tiles both ways 15 us against 10 at that rate: 561
+// groups, two or three to a CU, all reading first and all writing last.
 template <int kT, int kFmt, int kForm>
 __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 3 : 4) quant_tile_kernel(QuantArgs g) {
   __shared__ TileLds lds;
@@ -448,7 +451,8 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 3 : 4) quant_til
 }
 
 // Rows only: 16 lanes per block, so that one token's blocks spread over work groups
-// instead of filling 1 row in 128 of a tile.
+// instead of filling 1 row in 128 of a tile.  1 x 8192: 2.3 us, one memory round trip
+// and a launch.
 struct Unit {
   int64_t row, kb, col;      // block kb of a row; the lane's first column
   int cl, valid;
@@ -507,7 +511,8 @@ struct SwigluArgs {
   Out8 keep, rows, cols;
 };
 
-// One work group per 128 x 128 tile of y.
+// One work group per 128 x 128 tile of y.  Bound by its bytes: 8192 x 4096 with the
+// checkpoint and y both ways 61 us, 4.5 TB/s of the copy's 5.2.
 template <int kT>
 __global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
   constexpr int kF = FP64EMU_E4M3;
@@ -545,7 +550,8 @@ __global__ void __launch_bounds__(kThreads) swiglu_kernel(SwigluArgs a) {
   if (a.cols.q) emit_cols<kF>(y, t, row0, col0, mb, a.cols, lds);
 }
 
-// Without columns to write: a block of a row on 16 lanes.
+// Without columns to write: a block of a row on 16 lanes.  1 x 4096: 2.3 us, where a
+// tile's work group took 6.4.
 template <int kT>
 __global__ void __launch_bounds__(kThreads) swiglu_rows_kernel(SwigluArgs a) {
   constexpr int kF = FP64EMU_E4M3;
@@ -580,7 +586,9 @@ struct SwigluGradArgs {
 // Two work groups per 128 x 128 tile of dy, one for dg's tile and one for du's
 // (which needs no u): both tiles' values at once took 256 registers and 110 us
 // at 8192 x 4096, where this takes half of them.  The two are eight groups apart,
-// on one XCD, whose L2 then has what both read.
+// on one XCD, whose L2 then has what both read.  8192 x 4096 both ways 73 us, 3.7 TB/s:
+// 65 with the sigmoid left out and 50 without the columns, so the transposed
+// codes' way through LDS and their stores hold it most.
 template <int kT, int kO>
 __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) swiglu_grad_kernel(SwigluGradArgs a) {
   constexpr int kF = FP64EMU_E4M3;
@@ -636,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) swiglu_gr
   if (a.cols.q) emit_cols<kF>(d, t, row0, at + col0, mb, a.cols, lds);
 }
 
-// Without columns to write: a block of a row on 16 lanes, both halves.
+// Without columns to write: a block of a row on 16 lanes, both halves.  333 x 777:
+// 3.9 us, where tiles took 11.3.
 template <int kT, int kO>
 __global__ void __launch_bounds__(kThreads) swiglu_grad_rows_kernel(SwigluGradArgs a) {
   constexpr int kF = FP64EMU_E4M3;
@@ -899,6 +908,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 }
 
 // Tiles of kBM x kBN outputs, kWM x kWN waves of (kBM / kWM) x (kBN / kWN).
+//
+// 8192^3 to bfloat16 on 256 x 256 tiles: 453-465 us, 2.4 PFLOP/s, where the library's f8
+// product with one scale for each matrix takes 354.  What it is made of, by leaving parts
+// out on the same inputs: matrix instructions and scaling FMAs on registers 348 us (the
+// power limit: 294 on zeros, the instructions' own rate 234), with the LDS reads 354, with
+// the copies 410, with the stores 455.  Waits and the barrier cost nothing measurable.
+// The FMAs hide behind the matrix instructions up to four or five vector
+// instructions each; scales by rows on both sides take eight.
+//
+// Exact products on 256 x 128 tiles: 4096 x 4096 x 8192, scales by rows on both sides, 248 us
+// (1.1 PFLOP/s), by tiles 222; the library's bfloat16 product reaches 1.6.  Bound by vector
+// instructions: 128 conversions, 64 FMAs and 64 products of scales a wave and block for 64 matrix
+// instructions, which hide three each.  Converting once per work group instead, through
+// LDS, left too few registers to hide its phases: 325 us.
+//
 // A stage holds one block of K: kBN rows of B and kBM rows of A of 128 bytes
 // each, then their scales.  A lane's fragment is 16-byte chunks l / 16 and
 // l / 16 + 4 of row l % 16.  LDS serves a 16-byte read of 64 lanes sixteen at a time
@@ -1318,6 +1342,10 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const uint8_t* q, i
 // kTN x 16 rows of B and all waves on them, wave w at blocks w, w + kFewWaves,
 // ... of K; fragments come straight from memory (lane l's 32 bytes are the
 // instruction's operand as they lie in the row), and the waves' sums meet in LDS.
+// All of an iteration's operands and scales are loaded before the first is used (one
+// token through 8192 x 8192: 14.9 us without that fence, 13.2 with it).  Bound by B's
+// bytes there, at 5.1 TB/s; by the latency of its few iterations where the product is
+// small (333 x 501 x 777: 6.3 us, 11.2 on 128 x 128 tiles).
 constexpr int kFewWaves = 8;
 
 template <int kTM, int kTN, int kU, int kFA, int kFB, bool kRowB>
@@ -1458,11 +1486,13 @@ struct MmPlan {
 constexpr int kCUs = 256;
 
 // A form's time in microseconds, launch included: `groups` work groups of `steps`
-// blocks of K each.  Constants from 40 shapes of 1 to 8192 rows and columns and 512 to
-// 100000 deep in every form and split (bfloat16 and float32 outputs), which it
-// meets within a quarter where two forms are close: a work group's blocks take this
-// long with one group to a CU, and longer where the groups of all CUs share the
-// caches' rate or two share a CU.
+// blocks of K each.  The constants are fitted to 34 shapes of 1 to 8192 rows and columns
+// and 512 to 100000 deep, run in every form and split with bfloat16 and float32
+// outputs: a work group's blocks take this long with one group to a CU, longer where the
+// groups of all CUs share the caches' rate or two share a CU.  By it each of
+// them took the fastest form and split or one within a tenth (512 x 512 x 4096: few rows, two
+// splits 12.7 us, 128 x 128 tiles with four 16.8; 2048^3: 128 x 128 tiles 19.4, 256 x 256 27.8;
+// 3000^3: 42.6 the other way, 57.5).
 double mm_time(int form, int tile_m, bool exact, double groups, double steps) {
   const double share = std::min(groups, (double)kCUs) / kCUs;
   switch (form) {
