@@ -909,18 +909,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 
 // Tiles of kBM x kBN outputs, kWM x kWN waves of (kBM / kWM) x (kBN / kWN).
 //
-// 8192^3 to bfloat16 on 256 x 256 tiles: 453-465 us, 2.4 PFLOP/s, where the library's f8
-// product with one scale for each matrix takes 354.  What it is made of, by leaving parts
-// out on the same inputs: matrix instructions and scaling FMAs on registers 348 us (the
-// power limit: 294 on zeros, the instructions' own rate 234), with the LDS reads 354, with
-// the copies 410, with the stores 455.  Waits and the barrier cost nothing measurable.
-// The FMAs hide behind the matrix instructions up to four or five vector
-// instructions each; scales by rows on both sides take eight.
+// 8192^3 to bfloat16 on 256 x 256 tiles: 447-465 us, 2.4 PFLOP/s, where the library's f8
+// product with one scale for each matrix takes 354-357.  What it is made of, by leaving
+// parts out on the same inputs: matrix instructions and scaling FMAs on registers 348 us
+// (294 on zeros, so the power limit; the matrix units' own cycles come to 253 at 2.07 GHz), with
+// the LDS reads 354, with the copies 460.  Without its stores it took 429 where it took 466
+// with them, before whole non-temporal lines gave 12 to 14 of those back.  The wait for
+// the copies costs 6, the barrier nothing measurable.
+// The FMAs hide behind the matrix instructions up to four vector instructions each;
+// scales by rows on both sides take eight.
 //
 // Exact products on 256 x 128 tiles: 4096 x 4096 x 8192, scales by rows on both sides, 248 us
 // (1.1 PFLOP/s), by tiles 222; the library's bfloat16 product reaches 1.6.  Bound by vector
 // instructions: 128 conversions, 64 FMAs and 64 products of scales a wave and block for 64 matrix
-// instructions, which hide three each.  Converting once per work group instead, through
+// instructions, which hide one each.  Converting once per work group instead, through
 // LDS, left too few registers to hide its phases: 325 us.
 //
 // A stage holds one block of K: kBN rows of B and kBM rows of A of 128 bytes
@@ -929,7 +931,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 // over its 256 bytes of banks, lanes 0-3, 12-15 and 20-27 first, 4-11, 16-19 and 28-31
 // next; chunk c of row r lies at place c ^ (r / 2 % 8) of the row's eight, which gives
 // each such sixteen sixteen places (c ^ r % 8 with chunks 2 (l / 16) and + 1 met twice in
-// each and cost a third of LDS's cycles).  The copies write LDS in lane order: the lane
+// each and took 5.0e7 of 1.06e8 LDS cycles; now 1.6e6 of 6.2e7, the epilogue's).  The copies write LDS in lane order: the lane
 // that owns a place fetches the chunk that belongs there.
 template <int kBM_, int kBN_, int kWM_, int kWN_>
 struct MmShape {
@@ -1486,19 +1488,25 @@ struct MmPlan {
 constexpr int kCUs = 256;
 
 // A form's time in microseconds, launch included: `groups` work groups of `steps`
-// blocks of K each.  The constants are fitted to 34 shapes of 1 to 8192 rows and columns
-// and 512 to 100000 deep, run in every form and split with bfloat16 and float32
-// outputs: a work group's blocks take this long with one group to a CU, longer where the
-// groups of all CUs share the caches' rate or two share a CU.  By it each of
-// them took the fastest form and split or one within a tenth (512 x 512 x 4096: few rows, two
-// splits 12.7 us, 128 x 128 tiles with four 16.8; 2048^3: 128 x 128 tiles 19.4, 256 x 256 27.8;
-// 3000^3: 42.6 the other way, 57.5).
-double mm_time(int form, int tile_m, bool exact, double groups, double steps) {
+// blocks of K each, `reach` the operands' bytes as often as the eight XCDs' L2 fetch them.
+// A work group's blocks take this long with one group to a CU, longer where the groups of
+// all CUs share the caches' rate or two share a CU; few rows are also held by what they
+// fetch (8192 x 64 x 8192 to float32: 37 us, the 128 x 128 tiles with eight splits 28).
+// Fitted to 32 shapes of 1 to 8192 rows and columns and 512 to 100000 deep, to bfloat16
+// and to float32, in the forms and splits that suit each: of those 64 runs 63 come within
+// 5% of their fastest and the last, 1024^3 to bfloat16, within 8%.  Of 52 runs on 26
+// other shapes, which served only to choose between equally good constants, 45 come
+// within 5% and the worst within 14%.  It is off for 16-bit products of at most 256 deep
+// with more than 32 rows, which take 128 x 128 tiles: 300 x 300 x 256 6.8 us, 3.9 in few rows.
+// Both sides: 512 x 512 x 4096 in few rows with two splits 12.5 us, on 128 x 128 tiles with
+// four 16.8; 2048^3 on 128 x 128 tiles 19.4, 256 x 256 27.7; 3000^3 42.5 the other way, 58.0.
+double mm_time(int form, int tile_m, bool exact, double groups, double steps, double reach) {
   const double share = std::min(groups, (double)kCUs) / kCUs;
   switch (form) {
     case kFew: {               // eight waves, a block each
-      const double per = tile_m == 16 ? 0.85 : tile_m == 32 ? 1.8 : 3.0;
-      return 2.5 + std::ceil(groups / (tile_m == 16 ? 2 * kCUs : kCUs)) * (0.7 + per * std::ceil(steps / 8));
+      const double per = tile_m == 16 ? 0.7 : tile_m == 32 ? 1.2 : 2.6;
+      const double rounds = std::ceil(groups / (tile_m == 16 ? 2 * kCUs : kCUs));
+      return 2.5 + std::max(rounds * (1.0 + per * std::ceil(steps / 8)), reach / 5e6);
     }
     case kSquare128: {         // two groups to a CU, the last round's perhaps one
       const double one = exact ? 1.37 : 0.98, two = exact ? 1.86 : 1.12;
@@ -1521,11 +1529,13 @@ MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
   double least = 1e300;
   auto consider = [&](int form, int tm, int tn) {
     const int64_t tiles_m = (M + tm - 1) / tm, tiles_n = (N + tn - 1) / tn;
+    const double reach = (double)batch * (double)K * ((double)M * (double)std::min<int64_t>(tiles_n, 8) +
+                                                      (double)N * (double)std::min<int64_t>(tiles_m, 8));
     for (int64_t s = 1; s <= 32; s *= 2) {
       if (s > 1 && nkb < 2 * s) break;
       const int64_t per = (nkb + s - 1) / s;
-      double t = mm_time(form, tm, exact, (double)(batch * tiles_m * tiles_n) * (double)s, (double)per);
-      if (s > 1) t += 3.0 + 8.0 * (double)s * (double)(batch * M) * (double)N / 4e6;
+      double t = mm_time(form, tm, exact, (double)(batch * tiles_m * tiles_n) * (double)s, (double)per, reach);
+      if (s > 1) t += 1.5 + 0.25 * (double)s + 7.0 * (double)s * (double)(batch * M) * (double)N / 4e6;
       if (t >= least) continue;
       least = t;
       best = MmPlan{form, tm, tn, tiles_m, tiles_n, per > 0 ? (int)((nkb + per - 1) / per) : 1, (int)per};
