@@ -713,6 +713,28 @@ struct MmArgs {
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
+// A block's sum has to come out where the scales' own product leaves float32's range (2^-80 by
+// 2^-70, or 2^70 by 2^60 beside codes of zero).
+//
+// Split scales, for any: 2^x and s / 2^x, x the exponent kept to -110 .. 100.  The matrix
+// instructions take 2^x with the codes, exactly, and the block's sum meets only the
+// product of the two remainders, 1 to 4 for scales in that range.  In that range of x every
+// code's value is a normal bfloat16, and what goes beyond it (zero, denormal, infinite
+// scales) stays in the remainder.
+struct Split { float power, rest; };
+__device__ __forceinline__ Split split_scale(float s) {
+  const uint32_t e =
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(fabsf(s), 0x1p-110f, 0x1p100f)) & 0x7f800000u;
+  return {__builtin_bit_cast(float, e), s * __builtin_bit_cast(float, 0x7f000000u - e)};
+}
+
+// One frame, for scales whose product is below 2^24: the sums are kept at 2^40 times their size.
+// A block's sum is at most 2^39 (128 products of two e5m2 codes), so a product of scales that is denormal
+// at that size belongs to a result that is denormal at its own, and 2^24 blocks of at most 2^64 2^39
+// stay finite.  Both scales below 2^12 will do, too.
+constexpr float kFrame = 0x1p40f, kFrameTop = 0x1p64f;       // of the products of scales, at 2^40 times
+constexpr float kFrameTopA = 0x1p52f, kFrameTopB = 0x1p12f;  // of A's scales, at 2^40 times, and of B's
+
 // A fragment as the block's sum takes it.  Its 32 codes as they are, for one
 // v_mfma_f32_16x16x128_f8f6f4; or as bfloat16, which holds both formats'
 // values, for four v_mfma_f32_16x16x32_bf16.  The former aligns the products of
@@ -724,17 +746,22 @@ typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 // there), at half the rate and the conversions' cost.  So: the first for
 // 16-bit outputs of large products, the second for float32 ones, and where the
 // product waits for memory anyway.
+// `power`: 2^x of the lane's row, if the scales are split.
 template <bool kExact, int kFmt>
 struct Frag {
   v8i c;
+  int x;                             // the exponent as the instruction has it: 2^(x - 127)
   __device__ __forceinline__ explicit Frag(const v8i& codes) : c(codes) {}
+  __device__ __forceinline__ Frag(const v8i& codes, float power)
+      : c(codes), x(__builtin_bit_cast(int, power) >> 23) {}
   __device__ __forceinline__ Frag() {}
 };
 template <int kFmt>
 struct Frag<true, kFmt> {
   v8b c[4];
   __device__ __forceinline__ Frag() {}
-  __device__ __forceinline__ explicit Frag(const v8i& codes) {
+  __device__ __forceinline__ explicit Frag(const v8i& codes) : Frag(codes, 1.0f) {}
+  __device__ __forceinline__ Frag(const v8i& codes, float power) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v2b w[4];
@@ -742,11 +769,11 @@ struct Frag<true, kFmt> {
       for (int h = 0; h < 2; ++h) {
         const uint32_t x = (uint32_t)codes[2 * j + h];
         if constexpr (kFmt == FP64EMU_E4M3) {
-          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false);
-          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true);
+          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, power, false);
+          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, power, true);
         } else {
-          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, false);
-          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, true);
+          w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, power, false);
+          w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, power, true);
         }
       }
 #pragma unroll
@@ -755,12 +782,14 @@ struct Frag<true, kFmt> {
   }
 };
 
-template <bool kExact, int kFB, int kFA>
+template <bool kSplit, bool kExact, int kFB, int kFA>
 __device__ __forceinline__ v4f block_sum(const Frag<kExact, kFB>& b, const Frag<kExact, kFA>& a) {
   v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
   if constexpr (kExact) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.c[j], a.c[j], p, 0, 0, 0);
+  } else if constexpr (kSplit) {
+    p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.c, a.c, p, kFB, kFA, 0, b.x, 0, a.x);
   } else {
     p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.c, a.c, p, kFB, kFA, 0, 0, 0, 0);
   }
@@ -889,6 +918,7 @@ __device__ __forceinline__ void wait_vm_lgkm0() {
   static_assert(vm >= 0 && vm < 64, "vmcnt field");
   __builtin_amdgcn_s_waitcnt((vm & 15) | (7 << 4) | (0 << 8) | ((vm >> 4) << 14));
 }
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xc07f); }   // LDS done
 // Barrier without the fences of __syncthreads(), which would drain the copies in flight.
 __device__ __forceinline__ void barrier_lds() {
   asm volatile("" ::: "memory");
@@ -939,7 +969,6 @@ struct MmShape {
   static constexpr int kWaves = kWM * kWN, kT = 64 * kWaves;
   static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;   // 16 x 16 tiles per wave
   static constexpr int kCopB = kBN / 8 / kWaves, kCopA = kBM / 8 / kWaves;   // copies per wave
-  static constexpr int kCopies = kCopA + kCopB + 1;
   static constexpr int kOffA = kBN * kBlk, kOffS = (kBN + kBM) * kBlk;
   static constexpr int kStage = kOffS + 4 * (kBN + kBM);
   static_assert(kTM == 4, "four tiles a row");
@@ -1156,13 +1185,25 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   Frag<kExact, kFA> fa[S::kTM];
   v8i fb;
   float sa[S::kTM];
+  auto scale = [&](const uint8_t* stage, int row) { return reinterpret_cast<const float*>(stage + S::kOffS)[row]; };
+  const int rowA = S::kBN + wm * S::kTM * 16 + fr, rowB = wn * S::kTN * 16;
   auto scale_a = [&](const uint8_t* stage, int y) {
-    const float* sc = reinterpret_cast<const float*>(stage + S::kOffS);
-    const float s = sc[S::kBN + wm * S::kTM * 16 + y * 16 + fr];
-    return kRowB ? s : s * sc[wn * S::kTN * 16];
+    return scale(stage, rowA + y * 16) * (kRowB ? kFrame : kFrame * scale(stage, rowB));
   };
   auto scale_b = [&](const uint8_t* stage, int x) {
-    return *reinterpret_cast<const v4f*>(stage + S::kOffS + 4 * (wn * S::kTN * 16 + x * 16 + 4 * fg));
+    return *reinterpret_cast<const v4f*>(stage + S::kOffS + 4 * (rowB + x * 16 + 4 * fg));
+  };
+  // Whether the wave's scales of the block fit the frame (not where one is NaN); far: its largest of B.
+  auto far_b = [&](const uint8_t* stage) {
+    float f = 0.0f;
+    for (int r = 0; kRowB && r < S::kTN * 16; r += 64) f += fabsf(scale(stage, rowB + r + lane));
+    return f;
+  };
+  float far = 0.0f;
+  auto fits = [&] {
+    const float a = fabsf(sa[0]) + fabsf(sa[1]) + fabsf(sa[2]) + fabsf(sa[3]);
+    const bool in = kRowB ? a < kFrameTopA && far < kFrameTopB : a < kFrameTop;
+    return __builtin_amdgcn_ballot_w64(!in) == 0;
   };
   // acc[x][y] += the scaled block sum p.
   auto add = [&](int x, int y, const v4f& p, const v4f& sb) {
@@ -1194,13 +1235,27 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     fa[y] = Frag<kExact, kFA>(frag(lds, fragA + y * 16 * kBlk));
     sa[y] = scale_a(lds, y);
   }
-  for (int i = 0; i < nk; ++i) {
+  far = far_b(lds);
+  // Block i in the frame, or with split scales, whose A comes from the stage again.
+  auto block = [&](auto split, int i) {
+    constexpr bool kSplit = decltype(split)::value;
     const uint8_t* stage = lds + (i & 1) * S::kStage;
     const uint8_t* after = lds + ((i + 1) & 1) * S::kStage;
     v4f p[2][S::kTM], sb[2];
-    float sa_next[S::kTM];
+    float sa_next[S::kTM], power_b = 1.0f;
     constexpr int kLast = S::kTN - 1;
+    if constexpr (kSplit) {
+      const Split one = split_scale(scale(stage, rowB));       // of a tile of B
+      power_b = one.power;
+#pragma unroll
+      for (int y = 0; y < S::kTM; ++y) {
+        const Split a = split_scale(scale(stage, rowA + y * 16));
+        fa[y] = Frag<kExact, kFA>(frag(stage, fragA + y * 16 * kBlk), a.power);
+        sa[y] = kRowB ? a.rest : a.rest * one.rest;
+      }
+    }
     auto refill = [&](int y) {
+      if constexpr (kSplit) return;
       fa[y] = Frag<kExact, kFA>(frag(after, fragA + y * 16 * kBlk));
       sa_next[y] = scale_a(after, y);
     };
@@ -1208,17 +1263,25 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     for (int x = 0; x < S::kTN; ++x) {
       v8i next;
       if constexpr (kRowB) sb[x & 1] = scale_b(stage, x);
+      if constexpr (kRowB && kSplit) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sb[x & 1][e] = split_scale(sb[x & 1][e]).rest;
+        power_b = split_scale(scale(stage, rowB + x * 16 + fr)).power;
+      }
       if (x == kLast) {
         wait_vm_lgkm0<0>();
         barrier_lds();
         if (i + 2 < nk) issue(kb0 + i + 2, i & 1, 0);
         if (tail && i + 2 == nk && kb1 == g.nkb) clear_tail((i + 1) & 1);
         next = frag(after, fragB);                           // (past the last block: unused)
+        if constexpr (!kSplit) far = far_b(after);
       } else {
         next = frag(stage, fragB + (x + 1) * 16 * kBlk);
       }
       if (x + 1 < kParts && i + 1 < nk) issue(kb0 + i + 1, (i + 1) & 1, x + 1);
-      const Frag<kExact, kFB> fbx(fb);
+      Frag<kExact, kFB> fbx;
+      if constexpr (kSplit) fbx = Frag<kExact, kFB>(fb, power_b);
+      else fbx = Frag<kExact, kFB>(fb);
       // Step s of four: a quarter of K of every tile (bfloat16; a tile's own four follow
       // each other four instructions apart, not back to back), or tile s.
 #pragma unroll
@@ -1229,7 +1292,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
             p[x & 1][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                 fbx.c[s], fa[y].c[s], s == 0 ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : p[x & 1][y], 0, 0, 0);
         } else {
-          p[x & 1][s] = block_sum<kExact, kFB, kFA>(fbx, fa[s]);
+          p[x & 1][s] = block_sum<kSplit, kExact, kFB, kFA>(fbx, fa[s]);
         }
         if (x == kLast && !kExact) refill(s);
         if (x > 0) add(x - 1, s, p[(x - 1) & 1][s], sb[(x - 1) & 1]);
@@ -1245,9 +1308,19 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
 #pragma unroll
     for (int y = 0; y < S::kTM; ++y) {
       add(kLast, y, p[kLast & 1][y], sb[kLast & 1]);
-      sa[y] = sa_next[y];
+      if constexpr (!kSplit) sa[y] = sa_next[y];
     }
-  }
+  };
+  // A wave that meets larger scales takes its sums out of the frame and stays with split ones:
+  // with them for every block, 8192^3 to bfloat16 took 472 us where the frame takes 434, to
+  // float32 949 where it takes 914, mostly the instructions' scale operands' own issue slots.
+  int done = 0;
+  for (; done < nk && fits(); ++done) block(std::false_type{}, done);
+#pragma unroll
+  for (int x = 0; x < S::kTN; ++x)
+#pragma unroll
+    for (int y = 0; y < S::kTM; ++y) acc[x][y] *= 1.0f / kFrame;
+  for (; done < nk; ++done) block(std::true_type{}, done);
 
   if (g.splits > 1 || (!kExact && g.accumulate)) {
     store_tile<S, kExact>(g, m0 + wm * S::kTM * 16 + fr, n0 + wn * S::kTN * 16 + 4 * fg, b, split, acc);
@@ -1364,7 +1437,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   const int kb1 = kb0 + g.kb_per_split < g.nkb ? kb0 + g.kb_per_split : g.nkb;
 
   const uint8_t *pa[kTM], *pb[kTN];
-  const float *sa[kTM], *sb[kTN][kRowB ? 4 : 1];
+  const float *sa[kTM], *sb[kTN][kRowB ? 5 : 1];             // rows 4 fg + i of the outputs, then the fragment's row fr
 #pragma unroll
   for (int y = 0; y < kTM; ++y) {
     const int64_t m = m0 + y * 16 + fr < g.M ? m0 + y * 16 + fr : g.M - 1;
@@ -1376,8 +1449,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
     const int64_t n = n0 + x * 16 + fr < g.N ? n0 + x * 16 + fr : g.N - 1;
     pb[x] = g.B + b * g.strideB + n * g.ldb;
 #pragma unroll
-    for (int i = 0; i < (kRowB ? 4 : 1); ++i) {
-      const int64_t r = n0 + x * 16 + (kRowB ? 4 * fg + i : 0);
+    for (int i = 0; i < (kRowB ? 5 : 1); ++i) {
+      const int64_t r = n0 + x * 16 + (!kRowB ? 0 : i < 4 ? 4 * fg + i : fr);
       sb[x][i] = g.sB + b * g.sB_str + (kRowB ? (r < g.N ? r : g.N - 1) : r / kBlk) * g.sB_row;
     }
   }
@@ -1400,7 +1473,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   // A block's operands as they are loaded, all of them before the first is used.
   struct Block {
     v8i b[kTN], a[kTM];
-    float sa[kTM], sb[kTN][kRowB ? 4 : 1];
+    float sa[kTM], sb[kTN][kRowB ? 5 : 1];
   };
   auto scales = [&](Block& o, int kb) {
 #pragma unroll
@@ -1408,21 +1481,29 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
 #pragma unroll
     for (int x = 0; x < kTN; ++x)
 #pragma unroll
-      for (int i = 0; i < (kRowB ? 4 : 1); ++i) o.sb[x][i] = sb[x][i][kb * g.sB_blk];
+      for (int i = 0; i < (kRowB ? 5 : 1); ++i) o.sb[x][i] = sb[x][i][kb * g.sB_blk];
   };
   auto step = [&](const Block& o) {
     Frag<true, kFA> fa[kTM];
+    float ra[kTM];
 #pragma unroll
-    for (int y = 0; y < kTM; ++y) fa[y] = Frag<true, kFA>(o.a[y]);
+    for (int y = 0; y < kTM; ++y) {
+      const Split sc = split_scale(o.sa[y]);
+      ra[y] = sc.rest;
+      fa[y] = Frag<true, kFA>(o.a[y], sc.power);
+    }
 #pragma unroll
     for (int x = 0; x < kTN; ++x) {
-      const Frag<true, kFB> fb(o.b[x]);
+      float rb[kRowB ? 4 : 1];
+#pragma unroll
+      for (int i = 0; i < (kRowB ? 4 : 1); ++i) rb[i] = split_scale(o.sb[x][i]).rest;
+      const Frag<true, kFB> fb(o.b[x], split_scale(o.sb[x][kRowB ? 4 : 0]).power);
 #pragma unroll
       for (int y = 0; y < kTM; ++y) {
-        const v4f p = block_sum<true, kFB, kFA>(fb, fa[y]);
+        const v4f p = block_sum<true, true, kFB, kFA>(fb, fa[y]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          acc[x][y][i] = fmaf(p[i], o.sa[y] * o.sb[x][kRowB ? i : 0], acc[x][y][i]);
+          acc[x][y][i] = fmaf(p[i], ra[y] * rb[kRowB ? i : 0], acc[x][y][i]);
       }
     }
   };
