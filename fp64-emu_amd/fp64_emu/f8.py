@@ -21,6 +21,7 @@ No reference counterpart: the reference's products are float64 ones.  The
 work runs in hand-written gfx950 kernels; host tensors are refused.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._ops import ops
 
@@ -141,6 +142,7 @@ class _Linear(torch.autograd.Function):
         return mm_f8(q, s, wq, ws, out_dtype=x.dtype).view(*x.shape[:-1], w.size(0))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         xqt, xst, wqt, wst = ctx.saved_tensors
         rows = dy.reshape(-1, dy.size(-1))
@@ -155,7 +157,7 @@ class _Linear(torch.autograd.Function):
 
 def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tensor:
     """y = x @ w^T for x [.., K] and w [N, K], in x's type, by 8-bit products:
-    x by rows, w by tiles.  Differentiable in x and w; what is kept for w's
+    x by rows, w by tiles.  Differentiable once, in x and w; what is kept for w's
     gradient is x in 8 bits (blocks along its rows' direction), not x.  Gradients:
     dx = dy w with dy by rows, dw = dy^T x with dy and x by columns.
 
@@ -180,12 +182,13 @@ class _SwigluCkpt(torch.autograd.Function):
         return y.view(*h.shape[:-1], y.size(1))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         return swiglu_f8_backward(dy.reshape(-1, dy.size(-1)), *ctx.saved_tensors).view(ctx.shape)
 
 
 def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
-    """y = silu(g) u for h = [.., g | u] in h's type, differentiable: its
+    """y = silu(g) u for h = [.., g | u] in h's type, differentiable once: its
     backward pass reads an 8-bit checkpoint of h instead of h."""
     if h.dim() < 1 or h.size(-1) % 2:
         raise ValueError(f"expect h as [.., 2 F], got {tuple(h.shape)}")

@@ -1,0 +1,72 @@
+"""CPU tier: the 8-bit operators and autograd.  The layer's and the checkpoint's autograd forms run on host
+stand-ins of the ops (the tests' plain forms); the ops themselves are seen with fake tensors."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import fp64_emu
+from fp64_emu import f8
+from f8_util import BLOCK, E4M3, quantised, values
+
+F32 = torch.float32
+
+
+def _quant(x, rows, cols, tiles, fmt):
+    CALLS.append(("quant", rows, cols, tiles))
+    tall, out = BLOCK if tiles else 1, []
+    if rows:
+        out += quantised(x, fmt, tall)
+    if cols:
+        out += quantised(x.t(), fmt, tall)
+    return out
+
+
+def _mm(A, sA, B, sB, dtype):
+    return (values(A, sA) @ values(B, sB).t()).to(dtype)
+
+
+def _kept(h):
+    F = h.shape[1] // 2
+    halves = [quantised(v, E4M3) for v in (h[:, :F], h[:, F:])]
+    return [torch.cat([a.view(torch.uint8) for a, _ in halves], 1).view(E4M3), torch.cat([s for _, s in halves], 1)]
+
+
+def _swiglu(h, quant, keep):
+    CALLS.append(("swiglu", keep))
+    g, u = h.detach().double().chunk(2, 1)
+    return [(g * torch.sigmoid(g) * u).to(h.dtype)] + (_kept(h) if keep else [])
+
+
+def _swiglu_backward(dy, hq, hs, quant):
+    F, blocks = dy.shape[1], hs.shape[1] // 2
+    g, u = values(hq[:, :F], hs[:, :blocks]), values(hq[:, F:], hs[:, blocks:])
+    s = torch.sigmoid(g)
+    return [torch.cat((dy * u * s * (1 + g * (1 - s)), dy * g * s), 1).to(dy.dtype)]
+
+
+CALLS = []
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The ops on the host, and what they were asked for."""
+    CALLS.clear()
+    for name, fn in (("_quant", _quant), ("_mm", _mm), ("_swiglu", _swiglu), ("_swiglu_backward", _swiglu_backward)):
+        monkeypatch.setattr(f8, name, fn)
+    return CALLS
+
+
+def _leaf(*shape, seed=0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).requires_grad_()
+
+
+def test_second_derivatives_are_refused(host):
+    """The backward passes are not differentiable: a penalty on a gradient fails instead of losing its term."""
+    x, w = _leaf(8, 256), _leaf(40, 256, seed=1)
+    (dx,) = torch.autograd.grad(fp64_emu.linear_f8(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.square().sum().backward()
+    h = _leaf(8, 256, seed=2)
+    (dh,) = torch.autograd.grad(fp64_emu.swiglu_ckpt_f8(h).square().sum(), h, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dh.square().sum().backward()
