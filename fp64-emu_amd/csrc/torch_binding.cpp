@@ -8,6 +8,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -484,3 +485,40 @@ TORCH_LIBRARY_IMPL(fp64_emu, CUDA, ops) {
   ops.impl("fp64_emu_swiglu_f8", &fp64_emu_swiglu_f8);
   ops.impl("fp64_emu_swiglu_f8_backward", &fp64_emu_swiglu_f8_backward);
 }
+
+// None of the 8-bit ops has a derivative: a result that would need one raises in the
+// backward pass, an `out` that would need one at once.
+namespace {
+
+using MmOut = void(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool);
+
+const c10::TypedOperatorHandle<MmOut>& mm_out_handle() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("fp64_emu::fp64_emu_mm_f8_out", "").typed<MmOut>();
+  return op;
+}
+
+void mm_f8_out_autograd(c10::DispatchKeySet keys, at::Tensor& out, const at::Tensor& A, const at::Tensor& sA,
+                        const at::Tensor& B, const at::Tensor& sB, bool accumulate) {
+  if (at::GradMode::is_enabled())
+    for (const at::Tensor* t : {(const at::Tensor*)&out, &A, &sA, &B, &sB})
+      TORCH_CHECK(!t->requires_grad(), "the derivative for a product into out is not implemented, ",
+                  "but one of its arguments requires a gradient");
+  mm_out_handle().redispatch(keys & c10::after_autograd_keyset, out, A, sA, B, sB, accumulate);
+}
+
+void mm_f8_out_written(c10::DispatchKeySet keys, at::Tensor& out, const at::Tensor& A, const at::Tensor& sA,
+                       const at::Tensor& B, const at::Tensor& sB, bool accumulate) {
+  mm_out_handle().redispatch(keys & c10::after_ADInplaceOrView_keyset, out, A, sA, B, sB, accumulate);
+  out.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+TORCH_LIBRARY_IMPL(fp64_emu, Autograd, ops) {
+  for (const char* name : {"fp64_emu_quant_f8", "fp64_emu_mm_f8", "fp64_emu_swiglu_f8", "fp64_emu_swiglu_f8_backward"})
+    ops.impl(name, torch::autograd::autogradNotImplementedFallback());
+  ops.impl("fp64_emu_mm_f8_out", &mm_f8_out_autograd);
+}
+
+TORCH_LIBRARY_IMPL(fp64_emu, ADInplaceOrView, ops) { ops.impl("fp64_emu_mm_f8_out", &mm_f8_out_written); }

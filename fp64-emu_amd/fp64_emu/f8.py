@@ -17,6 +17,10 @@ Products take their operands' rows along K, so a gradient needs its operands
 quantised along another dimension; the quantiser's "cols" form gives blocks
 along M with the codes laid transposed, in the same pass over x.
 
+Differentiable are linear_f8 and swiglu_ckpt_f8, once.  The other functions have no
+derivative: given tensors that require a gradient, their results raise in a
+backward pass, and a product into `out` raises at once.
+
 No reference counterpart: the reference's products are float64 ones.  The
 work runs in hand-written gfx950 kernels; host tensors are refused.
 """

@@ -70,3 +70,37 @@ def test_second_derivatives_are_refused(host):
     (dh,) = torch.autograd.grad(fp64_emu.swiglu_ckpt_f8(h).square().sum(), h, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dh.square().sum().backward()
+
+
+def test_ops_without_a_gradient_say_so():
+    """The operators' results carry a gradient function that raises (NotImplemented), not one that warns and gives
+    nothing; the passes that would reach it run on the GPU tier."""
+    with FakeTensorMode():
+        h = torch.empty(4, 512, device="cuda", requires_grad=True)
+        q, s = (torch.empty(4, 256, dtype=E4M3, device="cuda"), torch.empty(4, 2, device="cuda", requires_grad=True))
+        for call in (lambda: fp64_emu.quant_f8(h)[1], lambda: fp64_emu.quant_f8_tiles(h)[1],
+                     lambda: fp64_emu.mm_f8(q, s, q, s.detach(), out_dtype=F32),
+                     lambda: fp64_emu.bmm_f8(q[None], s[None], q[None], s.detach()[None], out_dtype=F32),
+                     lambda: fp64_emu.swiglu_f8(h, keep=False)[0],
+                     lambda: fp64_emu.swiglu_f8_backward(h, torch.empty(4, 1024, dtype=E4M3, device="cuda"),
+                                                         torch.empty(4, 8, device="cuda"))):
+            assert call().grad_fn.name().endswith("::NotImplemented")
+            with torch.no_grad():
+                assert not call().requires_grad
+
+
+def test_out_counts_as_written():
+    """A product into `out` raises its version; an out or scales that require a gradient are refused."""
+    with FakeTensorMode():
+        q, s = torch.empty(4, 256, dtype=E4M3, device="cuda"), torch.empty(4, 2, device="cuda")
+        out = torch.empty(4, 4, device="cuda")
+        before = out._version
+        fp64_emu.mm_f8(q, s, q, s, out=out, accumulate=True)
+        assert out._version == before + 1
+        leaf = torch.empty(4, 4, device="cuda", requires_grad=True)
+        for o, scales in ((leaf, s), (leaf * 2, s), (out, s.clone().requires_grad_())):
+            with pytest.raises(RuntimeError, match="requires a gradient"):
+                fp64_emu.mm_f8(q, scales, q, s, out=o)
+        with torch.no_grad():
+            fp64_emu.mm_f8(q, s, q, s, out=leaf)
+            assert leaf._version == 1

@@ -18,3 +18,27 @@ def test_second_derivatives_are_refused(dev):
     (dh,) = torch.autograd.grad(fp64_emu.swiglu_ckpt_f8(x).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dh.square().sum().backward()
+
+
+def test_ops_without_a_gradient_say_so(dev):
+    print("case no gradient", flush=True)
+    h = torch.randn(40, 512, device=dev, requires_grad=True)
+    q, s = fp64_emu.quant_f8(h.detach())
+    _, hq, hs = fp64_emu.swiglu_f8(h.detach())
+    scales = s.clone().requires_grad_()
+    for call in (lambda: fp64_emu.quant_f8(h)[1], lambda: fp64_emu.quant_f8_tiles(h)[1],
+                 lambda: fp64_emu.mm_f8(q, scales, q, s, out_dtype=F32),
+                 lambda: fp64_emu.bmm_f8(q[None], scales[None], q[None], s[None], out_dtype=F32),
+                 lambda: fp64_emu.swiglu_f8(h, keep=False)[0],
+                 lambda: fp64_emu.swiglu_f8_backward(h[:, :256], hq, hs)):
+        with pytest.raises(RuntimeError, match="not implemented"):
+            call().sum().backward()
+    out = torch.zeros(40, 40, device=dev)
+    kept = torch.ones(40, 40, device=dev, requires_grad=True) * out
+    assert out._version == 0
+    fp64_emu.mm_f8(q, s, q, s, out=out)
+    assert out._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        kept.sum().backward()                  # it had saved out
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        fp64_emu.mm_f8(q, scales, q, s, out=out)
