@@ -130,10 +130,11 @@ def swiglu_f8_backward(dy: torch.Tensor, hq: torch.Tensor, hs: torch.Tensor, qua
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, wq, ws, wqt, wst):
+    def forward(ctx, x, w, wq, ws, wqt, wst, grad):
         K = x.size(-1)
         rows = x.reshape(-1, K)
-        wants_x, wants_w = ctx.needs_input_grad[:2]
+        # (needs_input_grad does not heed no_grad, and in here gradients are always off.)
+        wants_x, wants_w = (grad and n for n in ctx.needs_input_grad[:2])
         q, s, *kept = quant_f8(rows, cols=wants_w)
         if wq is None:
             wq, ws, *across = quant_f8_tiles(w.detach(), transposed=wants_x)
@@ -156,7 +157,7 @@ class _Linear(torch.autograd.Function):
             dx = mm_f8(got[0], got[1], wqt, wst, out_dtype=ctx.x_dtype).view(ctx.shape)
         if xqt is not None:
             dw = mm_f8(got[-2], got[-1], xqt, xst, out_dtype=ctx.w_dtype)
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tensor:
@@ -166,7 +167,7 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tenso
     dx = dy w with dy by rows, dw = dy^T x with dy and x by columns.
 
     wq: quant_f8_tiles(w, transposed=True) made earlier, for weights that stay
-    (without the transposed half where x needs no gradient)."""
+    (without the transposed half where x needs no gradient, or under no_grad)."""
     if x.dim() < 1 or w.dim() != 2 or x.size(-1) != w.size(1):
         raise ValueError(f"expect x [.., K] and w [N, K], got {tuple(x.shape)} and {tuple(w.shape)}")
     wq = tuple(wq) if wq is not None else ()
@@ -174,13 +175,13 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tenso
         raise ValueError("wq: what quant_f8_tiles gives, two or four tensors")
     if wq and wq[0].shape != w.shape:
         raise ValueError(f"wq is of another weight: {tuple(wq[0].shape)} and {tuple(w.shape)}")
-    return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))))
+    return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))), torch.is_grad_enabled())
 
 
 class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h):
-        y, *kept = swiglu_f8(h.reshape(-1, h.size(-1)), keep=ctx.needs_input_grad[0])
+    def forward(ctx, h, grad):
+        y, *kept = swiglu_f8(h.reshape(-1, h.size(-1)), keep=grad and ctx.needs_input_grad[0])
         ctx.save_for_backward(*kept)
         ctx.shape = h.shape
         return y.view(*h.shape[:-1], y.size(1))
@@ -188,7 +189,7 @@ class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return swiglu_f8_backward(dy.reshape(-1, dy.size(-1)), *ctx.saved_tensors).view(ctx.shape)
+        return swiglu_f8_backward(dy.reshape(-1, dy.size(-1)), *ctx.saved_tensors).view(ctx.shape), None
 
 
 def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
@@ -196,7 +197,7 @@ def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
     backward pass reads an 8-bit checkpoint of h instead of h."""
     if h.dim() < 1 or h.size(-1) % 2:
         raise ValueError(f"expect h as [.., 2 F], got {tuple(h.shape)}")
-    return _SwigluCkpt.apply(h)
+    return _SwigluCkpt.apply(h, torch.is_grad_enabled())
 
 
 __all__ = ["quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",

@@ -104,3 +104,22 @@ def test_out_counts_as_written():
         with torch.no_grad():
             fp64_emu.mm_f8(q, s, q, s, out=leaf)
             assert leaf._version == 1
+
+
+def test_nothing_is_kept_without_gradients(host):
+    """Under no_grad a layer of parameters quantises what the forward product reads and no more, and takes a
+    weight without its transposed half."""
+    x, w = _leaf(8, 256), _leaf(40, 256, seed=1)
+    wq = tuple(_quant(w, True, False, True, E4M3))
+    want = fp64_emu.linear_f8(x, w).detach()
+    for off in (torch.no_grad, torch.inference_mode):
+        host.clear()
+        with off():
+            assert torch.equal(fp64_emu.linear_f8(x, w), want)
+            assert host == [("quant", True, False, False), ("quant", True, False, True)]
+            assert torch.equal(fp64_emu.linear_f8(x, w, wq), want)
+            host.clear()
+            fp64_emu.swiglu_ckpt_f8(x)
+            assert host == [("swiglu", False)]
+    with pytest.raises(ValueError, match="transposed half"):
+        fp64_emu.linear_f8(x, w, wq)
