@@ -24,6 +24,8 @@ backward pass, and a product into `out` raises at once.
 No reference counterpart: the reference's products are float64 ones.  The
 work runs in hand-written gfx950 kernels; host tensors are refused.
 """
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -128,11 +130,15 @@ def swiglu_f8_backward(dy: torch.Tensor, hq: torch.Tensor, hs: torch.Tensor, qua
     return got[0] if form == 0 else tuple(got)
 
 
+def _as_rows(t):
+    """t [.., K] as [rows, K]; the count is written out, since with K = 0 it cannot be inferred."""
+    return t.reshape(math.prod(t.shape[:-1]), t.size(-1))
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, wq, ws, wqt, wst, grad):
-        K = x.size(-1)
-        rows = x.reshape(-1, K)
+        rows = _as_rows(x)
         # (needs_input_grad does not heed no_grad, and in here gradients are always off.)
         wants_x, wants_w = (grad and n for n in ctx.needs_input_grad[:2])
         q, s, *kept = quant_f8(rows, cols=wants_w)
@@ -150,7 +156,7 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         xqt, xst, wqt, wst = ctx.saved_tensors
-        rows = dy.reshape(-1, dy.size(-1))
+        rows = _as_rows(dy)
         dx = dw = None
         got = quant_f8(rows, rows=wqt is not None, cols=xqt is not None)
         if wqt is not None:
@@ -181,7 +187,7 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tenso
 class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, grad):
-        y, *kept = swiglu_f8(h.reshape(-1, h.size(-1)), keep=grad and ctx.needs_input_grad[0])
+        y, *kept = swiglu_f8(_as_rows(h), keep=grad and ctx.needs_input_grad[0])
         ctx.save_for_backward(*kept)
         ctx.shape = h.shape
         return y.view(*h.shape[:-1], y.size(1))
@@ -189,7 +195,7 @@ class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return swiglu_f8_backward(dy.reshape(-1, dy.size(-1)), *ctx.saved_tensors).view(ctx.shape), None
+        return swiglu_f8_backward(_as_rows(dy), *ctx.saved_tensors).view(ctx.shape), None
 
 
 def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:

@@ -123,3 +123,19 @@ def test_nothing_is_kept_without_gradients(host):
             assert host == [("swiglu", False)]
     with pytest.raises(ValueError, match="transposed half"):
         fp64_emu.linear_f8(x, w, wq)
+
+
+def test_empty_last_dimension(host):
+    """No elements to sum: zeros; no rows and no outputs: empty results, and gradients of their shapes."""
+    for shape, n in (((3, 4, 0), 5), ((0, 4, 256), 5), ((3, 256), 0), ((0, 0), 0)):
+        x, w = _leaf(*shape), _leaf(n, shape[-1], seed=1)
+        y = fp64_emu.linear_f8(x, w)
+        assert y.shape == (*shape[:-1], n) and (y == 0).all()
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert dx.shape == x.shape and dw.shape == w.shape and (dx == 0).all() and (dw == 0).all()
+    for shape in ((3, 4, 0), (0, 256), (0, 0)):
+        h = _leaf(*shape)
+        y = fp64_emu.swiglu_ckpt_f8(h)
+        assert y.shape == (*shape[:-1], shape[-1] // 2)
+        (dh,) = torch.autograd.grad(y, h, torch.ones_like(y))
+        assert dh.shape == h.shape

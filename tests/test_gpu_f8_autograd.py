@@ -42,3 +42,30 @@ def test_ops_without_a_gradient_say_so(dev):
         kept.sum().backward()                  # it had saved out
     with pytest.raises(RuntimeError, match="requires a gradient"):
         fp64_emu.mm_f8(q, scales, q, s, out=out)
+
+
+def test_empty_last_dimension(dev):
+    for shape, n in (((3, 4, 0), 5), ((0, 4, 256), 5), ((3, 256), 0), ((0, 0), 0)):
+        print("case empty", shape, n, flush=True)
+        x, w = torch.ones(shape, device=dev, requires_grad=True), torch.ones(n, shape[-1], device=dev, requires_grad=True)
+        y = fp64_emu.linear_f8(x, w)
+        assert y.shape == (*shape[:-1], n) and (y == 0).all()
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert dx.shape == x.shape and dw.shape == w.shape and (dx == 0).all() and (dw == 0).all()
+    for shape in ((3, 4, 0), (0, 256), (0, 0)):
+        h = torch.ones(shape, device=dev, requires_grad=True)
+        y = fp64_emu.swiglu_ckpt_f8(h)
+        assert y.shape == (*shape[:-1], shape[-1] // 2)
+        (dh,) = torch.autograd.grad(y, h, torch.ones_like(y))
+        assert dh.shape == h.shape
+
+
+def test_nothing_is_kept_without_gradients(dev):
+    print("case no_grad", flush=True)
+    x, w = (torch.randn(40, 256, device=dev, requires_grad=True) for _ in range(2))
+    wq = fp64_emu.quant_f8_tiles(w.detach())
+    want, y = fp64_emu.linear_f8(x, w).detach(), fp64_emu.swiglu_ckpt_f8(x).detach()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            assert torch.equal(fp64_emu.linear_f8(x, w), want) and torch.equal(fp64_emu.linear_f8(x, w, wq), want)
+            assert torch.equal(fp64_emu.swiglu_ckpt_f8(x), y)
