@@ -1601,8 +1601,13 @@ double mm_time(int form, int tile_m, bool exact, double groups, double steps, do
   }
 }
 
-// The form and the number of K splits that take least by mm_time; a split adds a
-// launch and its partial sums' way to memory and back.
+constexpr int64_t kMaxGroups = (1ll << 31) / kThreads;    // work items of one launch stay below 2^31
+// Rows of operands that the tile kernels copy: a tile's 256 within 32-bit offsets, those of the last,
+// partial block included.
+constexpr int64_t kMaxTileRow = (1ll << 32) / 256 - kBlk;
+
+// The form and the number of K splits that take least by mm_time, of those that one launch
+// holds (splits = 0: none); a split adds a launch and its partial sums' way to memory and back.
 MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
   const bool exact = dtype == FP64EMU_F32;
   const int64_t nkb = (K + kBlk - 1) / kBlk;
@@ -1610,10 +1615,12 @@ MmPlan plan_mm(int64_t batch, int64_t M, int64_t N, int64_t K, int dtype) {
   double least = 1e300;
   auto consider = [&](int form, int tm, int tn) {
     const int64_t tiles_m = (M + tm - 1) / tm, tiles_n = (N + tn - 1) / tn;
+    if (form != kFew && (K + 15) / 16 * 16 >= kMaxTileRow) return;
     const double reach = (double)batch * (double)K * ((double)M * (double)std::min<int64_t>(tiles_n, 8) +
                                                       (double)N * (double)std::min<int64_t>(tiles_m, 8));
     for (int64_t s = 1; s <= 32; s *= 2) {
       if (s > 1 && nkb < 2 * s) break;
+      if (tiles_m > kMaxGroups / 2 / tiles_n / batch / s) break;
       const int64_t per = (nkb + s - 1) / s;
       double t = mm_time(form, tm, exact, (double)(batch * tiles_m * tiles_n) * (double)s, (double)per, reach);
       if (s > 1) t += 1.5 + 0.25 * (double)s + 7.0 * (double)s * (double)(batch * M) * (double)N / 4e6;
@@ -1655,8 +1662,6 @@ int out8(const fp64emu_f8_t* f, int64_t depth, Out8* o) {
   *o = Out8{f->q, f->s, f->ld, f->stride, f->s_row, f->s_block, f->s_stride};
   return FP64EMU_OK;
 }
-
-constexpr int64_t kMaxGroups = (1ll << 31) / kThreads;    // work items of one launch stay below 2^31
 
 // Work groups for a matrix's blocks of rows, 16 each.
 unsigned unit_groups(int64_t rows, int64_t blocks) {
@@ -1706,10 +1711,9 @@ void launch_mm(const MmArgs& g, const MmPlan& p, unsigned groups, hipStream_t s)
   else launch_few<4, 2, 1, kFA, kFB>(g, groups, s);
 }
 
-// Whether the tile kernel can copy an operand's rows: 16-byte aligned, a tile's
-// rows within 32-bit offsets (those of the last, partial block included).
+// Whether the tile kernels can copy an operand's rows as they lie.
 bool copyable(const fp64emu_f8_t& f) {
-  return multiple(f.q, 16) && f.ld % 16 == 0 && f.stride % 16 == 0 && f.ld < (1ll << 32) / 256 - kBlk;
+  return multiple(f.q, 16) && f.ld % 16 == 0 && f.stride % 16 == 0 && f.ld < kMaxTileRow;
 }
 
 // Partial sums, then the rows of A and of B that are laid out again.
@@ -1788,7 +1792,9 @@ int fp64emu_quant_f8(const void* x, int dtype, int64_t batch, int64_t M, int64_t
 
 size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p) {
   if (check_mm(p) || p->batch * p->M == 0 || p->N == 0 || p->K == 0) return 0;
-  const MmRoom r = mm_room(p, plan_mm(p->batch, p->M, p->N, p->K, p->dtype));
+  const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
+  if (plan.splits == 0) return 0;
+  const MmRoom r = mm_room(p, plan);
   return r.parts + r.A + r.B;
 }
 
@@ -1826,6 +1832,7 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
     return check_hip(hipGetLastError(), "mm_f8 launch");
   }
   const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
+  if (plan.splits == 0) return invalid("product too large for one launch");
   const MmRoom room = mm_room(p, plan);
   const size_t need = room.parts + room.A + room.B;
   if (need && (!workspace || workspace_bytes < need))
@@ -1852,11 +1859,8 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
   g.tiles_m = (int)plan.tiles_m;
   g.tiles_n = (int)plan.tiles_n;
   g.b_tiles = p->B.tiles != 0;
-  if (plan.tiles_m > kMaxGroups / plan.tiles_n / p->batch / plan.splits / 2)
-    return invalid("product too large for one launch");
   const unsigned groups = (unsigned)(plan.tiles_m * plan.tiles_n * p->batch * plan.splits);
   const int64_t K16 = (p->K + 15) / 16 * 16;
-  if (plan.form != kFew && K16 >= (1ll << 32) / 256 - kBlk) return invalid("K too large for one launch");
   if (room.A) {
     uint8_t* to = static_cast<uint8_t*>(workspace) + room.parts;
     pack(p->A, p->batch, p->M, p->K, to, s);

@@ -1,0 +1,29 @@
+"""CPU tier: which kernel a product of 8-bit operands takes, and what it asks for: the rule runs on
+the host."""
+import ctypes
+
+from fp64_emu import capi
+
+BF16 = 1
+
+
+def _product(M, N, K, batch=1, dtype=BF16, ld=None):
+    a, b = (capi.F8(0x1000, 0x1000, K if ld is None else ld, 0, 1, r, 0, 0, 0) for r in (M, N))
+    return capi.MmF8(0x1000, N, 0, dtype, 0, a, b, batch, M, N, K)
+
+
+def test_any_depth_has_a_kernel():
+    """Tile kernels hold a row's offset in 32 bits (2^24 codes); deeper products take few rows, whatever their
+    other sizes, and ask for no room to lay their operands out again: partial sums alone, 32 of them at most."""
+    L = capi.lib()
+    for K in (2 ** 24 - 300, 2 ** 24 - 256, 2 ** 24, 17_000_000, 2 ** 31 - 256):
+        for M, N in ((1, 1000), (1000, 1000), (4096, 8192)):
+            for dtype in (0, 1, 2):
+                p = _product(M, N, K, dtype=dtype, ld=-(-K // 16) * 16)
+                need = L.fp64emu_mm_f8_workspace(ctypes.byref(p))
+                assert need <= 32 * 4 * M * N + 256, (M, N, K, need)
+                # Short of its room, the call says so; no depth is refused for itself.
+                p.out = 0x1000
+                if need:
+                    assert L.fp64emu_mm_f8(ctypes.byref(p), None, 0, None) == 2
+                    assert b"workspace too small" in L.fp64emu_last_error()
