@@ -1798,6 +1798,19 @@ size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p) {
   return r.parts + r.A + r.B;
 }
 
+int fp64emu_mm_f8_plan(const fp64emu_mm_f8_t* p, fp64emu_mm_f8_plan_t* out) {
+  if (!out) return invalid("plan must not be NULL");
+  *out = fp64emu_mm_f8_plan_t{};
+  if (int st = check_mm(p)) return st;
+  if (p->batch * p->M == 0 || p->N == 0 || p->K == 0) return FP64EMU_OK;
+  const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
+  if (plan.splits == 0) return invalid("product too large for one launch");
+  const bool tiles = plan.form != kFew;
+  *out = {plan.tile_m, plan.tile_n, plan.splits, !tiles || p->dtype == FP64EMU_F32, tiles && !copyable(p->A),
+          tiles && !copyable(p->B)};
+  return FP64EMU_OK;
+}
+
 int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_bytes,
                   fp64emu_stream_t stream) {
   if (int st = check_mm(p)) return st;

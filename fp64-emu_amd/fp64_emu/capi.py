@@ -26,7 +26,7 @@ EXPORTS = ("fp64emu_maxp", "fp64emu_last_error", "fp64emu_workspace_size",
            "fp64emu_mm_nt_events", "fp64emu_bmm_nt_events", "fp64emu_mm_nt_noalloc",
            "fp64emu_product_workspace", "fp64emu_product", "fp64emu_layout",
            "fp64emu_ddgemm_nt", "fp64emu_probe_mfma", "fp64emu_probe_stream", "fp64emu_quant_f8",
-           "fp64emu_mm_f8_workspace", "fp64emu_mm_f8", "fp64emu_swiglu_f8",
+           "fp64emu_mm_f8_workspace", "fp64emu_mm_f8_plan", "fp64emu_mm_f8", "fp64emu_swiglu_f8",
            "fp64emu_swiglu_f8_backward")
 
 NOALLOC_SCRATCH_BYTES = 64 << 20   # FP64EMU_NOALLOC_SCRATCH_BYTES
@@ -72,6 +72,11 @@ class MmF8(ctypes.Structure):
     _fields_ = [("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("stride_o", ctypes.c_int64),
                 ("dtype", ctypes.c_int), ("accumulate", ctypes.c_int), ("A", F8), ("B", F8)] + [
                     (n, ctypes.c_int64) for n in ("batch", "M", "N", "K")]
+
+
+class MmF8Plan(ctypes.Structure):
+    """Mirror of fp64emu_mm_f8_plan_t."""
+    _fields_ = [(n, ctypes.c_int) for n in ("tile_m", "tile_n", "splits", "exact", "relaid_a", "relaid_b")]
 
 
 _LIB = None
@@ -124,6 +129,8 @@ def lib():
     L.fp64emu_quant_f8.restype = i32
     L.fp64emu_mm_f8_workspace.argtypes = [ctypes.POINTER(MmF8)]
     L.fp64emu_mm_f8_workspace.restype = sz
+    L.fp64emu_mm_f8_plan.argtypes = [ctypes.POINTER(MmF8), ctypes.POINTER(MmF8Plan)]
+    L.fp64emu_mm_f8_plan.restype = i32
     L.fp64emu_mm_f8.argtypes = [ctypes.POINTER(MmF8), vp, sz, vp]
     L.fp64emu_mm_f8.restype = i32
     L.fp64emu_swiglu_f8.argtypes = [vp, i32, i64, i64, i64, vp, i64, f8, f8, f8, vp]
@@ -147,6 +154,16 @@ def layout(batch, M, N, K, nprimes, use_corr):
     out = Layout()
     _check(lib().fp64emu_layout(batch, M, N, K, nprimes, int(bool(use_corr)), ctypes.byref(out)))
     return out
+
+
+def mm_f8_plan(M, N, K, dtype, batch=1, ld=None):
+    """fp64emu_mm_f8_plan of a product of these sizes and dtype (0, 1, 2: float32, bfloat16, float16),
+    rows of codes ld apart (default: as the quantiser lays them out)."""
+    ld = (K + 15) // 16 * 16 if ld is None else ld
+    a, b = (F8(None, None, ld, r * ld, 1, r, 0, 0, 0) for r in (M, N))
+    p, plan = MmF8(None, N, M * N, dtype, 0, a, b, batch, M, N, K), MmF8Plan()
+    _check(lib().fp64emu_mm_f8_plan(ctypes.byref(p), ctypes.byref(plan)))
+    return plan
 
 
 def workspace_size(batch, M, N, K, nprimes, use_corr):

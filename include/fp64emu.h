@@ -329,12 +329,22 @@ typedef struct {
 } fp64emu_mm_f8_t;
 
 /* Workspace of fp64emu_mm_f8 (0 for most shapes: float32 partial sums where few
- * output tiles make it split the depth).  The call needs that much.  Two calls
+ * output tiles make it split the depth, rows of operands that a tile kernel cannot
+ * copy as they lie).  The call needs that much.  Two calls
  * with the same arguments give the same bits. */
 size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p);
 
 int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_bytes,
                   fp64emu_stream_t stream);
+
+/* How a product runs: tiles of tile_m x tile_n outputs (with tile_m <= 64 straight from memory, else
+ * through LDS), the depth in `splits` parts, block sums exact or not, an operand's rows laid out
+ * again first or not.  A rule on the sizes, dtype and the operands' alignment; zeros for an empty product. */
+typedef struct {
+  int tile_m, tile_n, splits, exact, relaid_a, relaid_b;
+} fp64emu_mm_f8_plan_t;
+
+int fp64emu_mm_f8_plan(const fp64emu_mm_f8_t* p, fp64emu_mm_f8_plan_t* plan);
 
 /* y = silu(g) u for h = [g | u] of M rows and 2F columns (rows ldh apart), each output
  * only where asked for: `y` [M, F] in h's dtype; `rows` and `cols`, y quantised as by

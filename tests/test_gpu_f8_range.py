@@ -13,7 +13,7 @@ BF16, FP16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 # Few rows (16, 32 and 64 of A), 128 x 128 tiles, 256 x 256 or 128 x 256 tiles, split depths.
 SHAPES = [(1, 200, 1024), (20, 96, 1024), (50, 130, 1000), (300, 260, 200), (2048, 2048, 1024),
-          (4096, 4096, 1024), (3, 64, 40000)]
+          (4096, 4096, 1024), (2000, 2100, 8200), (3, 64, 40000)]
 
 
 def _like(shape, seed, power):
