@@ -1908,10 +1908,10 @@ int fp64emu_swiglu_f8(const void* h, int dtype, int64_t M, int64_t F, int64_t ld
                       fp64emu_stream_t stream) {
   if (M < 0 || F < 0) return invalid("shapes must be non-negative");
   if (!known_dtype(dtype)) return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
-  if (!y && !keep && !rows && !cols) return invalid("no output asked for");
   for (const fp64emu_f8_t* f : {keep, rows, cols})
     if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("outputs are e4m3 with scales by rows");
   if (M == 0 || F == 0) return FP64EMU_OK;
+  if (!y && !keep && !rows && !cols) return invalid("no output asked for");
   if (!h) return invalid("null operand pointer");
   if (ldh < 2 * F || (y && ldy < F)) return invalid("rows are shorter than their width");
   SwigluArgs a{};
@@ -1953,12 +1953,12 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
     return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
   if (out_dtype != dtype && out_dtype != FP64EMU_F32)
     return invalid("out_dtype must be dy's or FP64EMU_F32");
-  if (!dh && !rows && !cols) return invalid("no output asked for");
   if (!keep) return invalid("null 8-bit operand");
   for (const fp64emu_f8_t* f : {keep, rows, cols})
     if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("operands are e4m3 with scales by rows");
   if ((rows || cols) && F % kBlk) return invalid("quantised gradients need F as a multiple of 128");
   if (M == 0 || F == 0) return FP64EMU_OK;
+  if (!dh && !rows && !cols) return invalid("no output asked for");
   if (!dy) return invalid("null operand pointer");
   if (ldy < F || (dh && ldh < 2 * F)) return invalid("rows are shorter than their width");
   SwigluGradArgs a{};

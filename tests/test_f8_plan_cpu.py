@@ -1,5 +1,5 @@
 """CPU tier: which kernel a product of 8-bit operands takes, and what it asks for: the rule runs on
-the host."""
+the host.  And calls with nothing to do."""
 import ctypes
 
 import pytest
@@ -57,3 +57,12 @@ def test_any_depth_has_a_kernel():
                 if need:
                     assert L.fp64emu_mm_f8(ctypes.byref(p), None, 0, None) == 2
                     assert b"workspace too small" in L.fp64emu_last_error()
+
+
+def test_empty_activation():
+    """No rows or no columns: nothing to do, whatever of the outputs is NULL (an empty tensor's memory is)."""
+    L = capi.lib()
+    for M, F in ((0, 256), (4, 0), (0, 0)):
+        assert L.fp64emu_swiglu_f8(None, BF16, M, F, 2 * F, None, F, None, None, None, None) == 0
+        keep = capi.F8(None, None, 2 * F, 0, 1, M, 0, 0, 0)
+        assert L.fp64emu_swiglu_f8_backward(None, BF16, M, F, F, ctypes.byref(keep), None, BF16, 2 * F, None, None, None) == 0

@@ -69,3 +69,18 @@ def test_nothing_is_kept_without_gradients(dev):
         with off():
             assert torch.equal(fp64_emu.linear_f8(x, w), want) and torch.equal(fp64_emu.linear_f8(x, w, wq), want)
             assert torch.equal(fp64_emu.swiglu_ckpt_f8(x), y)
+
+
+def test_empty_activation(dev):
+    """With no elements each form gives its empty results."""
+    for M, F in ((0, 256), (5, 0), (0, 0)):
+        print("case empty activation", M, F, flush=True)
+        h, dy = torch.empty(M, 2 * F, device=dev), torch.empty(M, F, device=dev)
+        for keep in (False, True):
+            for quant in (None, "rows", "both"):
+                y, *_ = fp64_emu.swiglu_f8(h, quant=quant, keep=keep)
+                assert y.shape == (M, F)
+        _, hq, hs = fp64_emu.swiglu_f8(h)
+        assert fp64_emu.swiglu_f8_backward(dy, hq, hs).shape == (M, 2 * F)
+        q, s, qt, st = fp64_emu.swiglu_f8_backward(dy, hq, hs, quant="both")
+        assert q.shape == (M, 2 * F) and qt.shape == (2 * F, M)
