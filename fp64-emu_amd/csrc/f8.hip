@@ -1350,6 +1350,11 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
       __builtin_memcpy(__builtin_assume_aligned(room + (y * 16 + fr) * kRow + (x * 16 + 4 * fg) * sizeof(T),
                                                 4 * sizeof(T)), w, 4 * sizeof(T));
     }
+  // Other lanes of the wave read these rows: not before they are written, whatever the
+  // compiler can tell of the addresses (the LDS itself keeps a wave's order).
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int64_t n = n0 + wn * S::kTN * 16 + (lane % kLanes) * kEach;
   const int valid = (int)(g.N - n < kEach ? g.N - n : kEach);
   int64_t m = m0 + wm * S::kTM * 16 + lane / kLanes;
