@@ -165,7 +165,8 @@ struct Held {
     w[p] = v4u{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
   }
   // Makes the compiler unpack the words again instead of keeping 64 floats beside
-  // them from one use to the next (198 registers instead of 104 in the quantiser).
+  // them from one use to the next (bfloat16: 59 registers, not 120, in the quantiser both
+  // ways, 127, not 234, in the activation).
   __device__ __forceinline__ void again() {
 #pragma unroll
     for (int p = 0; p < 8; ++p) asm volatile("" : "+v"(w[p]));
@@ -833,9 +834,6 @@ __device__ __forceinline__ v4i load16_masked(const uint8_t* row, int64_t k, int6
 // Four successive outputs (m, n .. n + 3).
 __device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v) {
   const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
-  if (g.splits > 1) {
-    return;
-  }
   const int64_t i = b * g.stride_o + m * g.ldo + n;
   if (g.vec_o && valid == 4) {
     if (g.dtype == FP64EMU_F32) {
@@ -997,18 +995,18 @@ __device__ __forceinline__ void get4(const T* p, int valid, T (&w)[4]) {
   for (int j = 0; j < 3; ++j) w[j] = j < valid ? p[j] : T{};
 }
 
-// An item's outputs (or partial sums) from the accumulators, a row of tiles at a
-// time: T float (kForm 0), bfloat16 (1) or float16 (2).
+// An item's partial sums (kForm 0), or what it adds to bfloat16 (1) or float16 (2)
+// outputs, from the accumulators, a row of tiles at a time.
 template <class S, int kForm>
 __device__ __forceinline__ void store_rows(const v4f (&acc)[S::kTN][S::kTM], void* out, int64_t ld, int rows,
-                                           int cols, bool accumulate) {
+                                           int cols) {
   using T = std::conditional_t<kForm == 0, float, unsigned short>;
   T* p = static_cast<T*>(out);
 #pragma unroll
   for (int y = 0; y < S::kTM; ++y, p += 16 * ld) {
     if (y * 16 < rows) {
       T old[S::kTN][4];
-      if (accumulate) {
+      if constexpr (kForm != 0) {
 #pragma unroll
         for (int x = 0; x < S::kTN; ++x) get4(p + x * 16, cols - x * 16, old[x]);
       }
@@ -1017,15 +1015,13 @@ __device__ __forceinline__ void store_rows(const v4f (&acc)[S::kTN][S::kTM], voi
         T w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v = acc[x][y][i];
-          if constexpr (kForm == 0) {
-            w[i] = accumulate ? v + old[x][i] : v;
-          } else if constexpr (kForm == 1) {
-            w[i] = bf16_round(accumulate ? v + bf16_value(old[x][i]) : v);
-          } else {
-            if (accumulate) v += (float)__builtin_bit_cast(_Float16, old[x][i]);
-            w[i] = __builtin_bit_cast(unsigned short, (_Float16)v);
-          }
+          const float v = acc[x][y][i];
+          if constexpr (kForm == 0)
+            w[i] = v;
+          else if constexpr (kForm == 1)
+            w[i] = bf16_round(v + bf16_value(old[x][i]));
+          else
+            w[i] = __builtin_bit_cast(unsigned short, (_Float16)(v + (float)__builtin_bit_cast(_Float16, old[x][i])));
         }
         put4(p + x * 16, cols - x * 16, w);
       }
@@ -1040,14 +1036,12 @@ __device__ __forceinline__ void store_tile(const MmArgs& g, int64_t m, int64_t n
                                            const v4f (&acc)[S::kTN][S::kTM]) {
   const int rows = (int)(g.M - m), cols = (int)(g.N - n);
   const int64_t at = b * g.stride_o + m * g.ldo + n;
-  if (g.splits > 1)
-    store_rows<S, 0>(acc, g.part + (((int64_t)split * g.batch + b) * g.M + m) * g.N + n, g.N, rows, cols, false);
-  else if (kExact)
-    store_rows<S, 0>(acc, static_cast<float*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+  if (kExact || g.splits > 1)          // (whole float32 sums take the way through LDS)
+    store_rows<S, 0>(acc, g.part + (((int64_t)split * g.batch + b) * g.M + m) * g.N + n, g.N, rows, cols);
   else if (g.dtype == FP64EMU_BF16)
-    store_rows<S, 1>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+    store_rows<S, 1>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols);
   else
-    store_rows<S, 2>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols, g.accumulate);
+    store_rows<S, 2>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols);
 }
 
 // 16 bytes anywhere, not kept in the caches: what nothing here reads again.
