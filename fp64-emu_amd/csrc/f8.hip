@@ -741,12 +741,14 @@ constexpr float kFrameTopA = 0x1p52f, kFrameTopB = 0x1p12f;  // of A's scales, a
 // values, for four v_mfma_f32_16x16x32_bf16.  The former aligns the products of
 // neighbouring k to the largest before it adds them and keeps about 13 bits below
 // it (measured: of 2^16 + 2^(16 - d) at adjacent k the second is lost from d = 14
-// on; at k eight apart it is kept to float32's own 23): an error of 2e-5 to 4e-5 of
-// a block's sum, far below the rounding of a bfloat16 or float16 result and
-// far above that of a float32 one.  The latter rounds as float32 sums do (1e-8
+// on; at k eight apart it is kept to float32's own 23): typically 2e-5 to 4e-5 of
+// a block's sum in norm, at most eight products' 2^-13 each, 2^-10 of the sum of magnitudes.
+// Beside the rounding of a bfloat16 result (1.6e-3) that is nothing, beside a float16 one's
+// (2.1e-4) one per cent more error, and far above a float32 one's; where blocks cancel
+// it is relative to them and not to the result.  The latter rounds as float32 sums do (1e-8
 // there), at half the rate and the conversions' cost.  So: the first for
 // 16-bit outputs of large products, the second for float32 ones, and where the
-// product waits for memory anyway.
+// product waits for memory anyway.  A caller who needs the second asks for float32.
 // `power`: 2^x of the lane's row, if the scales are split.
 template <bool kExact, int kFmt>
 struct Frag {

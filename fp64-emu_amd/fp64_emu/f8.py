@@ -11,8 +11,13 @@ value (448, 57344), s = a / F and q = x ((1 / a) F) rounded to the nearest code,
 each step one float32 operation.  A block that holds an infinity or a NaN
 stands for NaN throughout.
 
-A product's sums are float32: one block of K is summed by the matrix
-instruction, scaled by both blocks' scales and added to the running sum.
+A product sums a block of K by matrix instructions, scales that by both blocks'
+scales and adds it to a running float32 sum.  With a float32 output a block's sum
+is a float32 one, too.  With a 16-bit output of more than a few rows it comes from
+the 8-bit instruction, which keeps a product to about 13 bits below the largest
+beside it: typically 2e-5 to 4e-5 of a block's sum (a float16 result rounds by 2e-4, a bfloat16
+one by 2e-3), at most 2^-10 of the sum of magnitudes, and relative to the blocks where
+they cancel.  A caller who needs more takes out_dtype=torch.float32 and rounds.
 Products take their operands' rows along K, so a gradient needs its operands
 quantised along another dimension; the quantiser's "cols" form gives blocks
 along M with the codes laid transposed, in the same pass over x.
@@ -94,7 +99,8 @@ def mm_f8(A: torch.Tensor, sA: torch.Tensor, B: torch.Tensor, sB: torch.Tensor,
     """C = A @ B^T of quantised A [M, K] and B [N, K], A's scales by rows, B's by
     rows or tiles.  out: where to (float32, bfloat16 or float16, rows any
     distance apart; out_dtype is then out's); accumulate: C is added to it, the
-    sum rounded once."""
+    sum rounded once.  16-bit outputs of more than a few rows take less exact sums of a
+    block than float32 ones (the module's notes say how much)."""
     return _product(2, A, sA, B, sB, out_dtype, out, accumulate)
 
 
