@@ -939,7 +939,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 
 // Tiles of kBM x kBN outputs, kWM x kWN waves of (kBM / kWM) x (kBN / kWN).
 //
-// 8192^3 to bfloat16 on 256 x 256 tiles: 447-465 us, 2.4 PFLOP/s, where the library's f8
+// 8192^3 to bfloat16 on 256 x 256 tiles: 467-471 us, 2.3 PFLOP/s, where the library's f8
 // product with one scale for each matrix takes 354-357.  What it is made of, by leaving
 // parts out on the same inputs: matrix instructions and scaling FMAs on registers 348 us
 // (294 on zeros, so the power limit; the matrix units' own cycles come to 253 at 2.07 GHz), with
@@ -947,13 +947,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_src(const void* p, uint
 // with them, before whole non-temporal lines gave 12 to 14 of those back.  The wait for
 // the copies costs 6, the barrier nothing measurable.
 // The FMAs hide behind the matrix instructions up to four vector instructions each;
-// scales by rows on both sides take eight.
+// scales by rows on both sides take eight (8192^3 546 us).
 //
-// Exact products on 256 x 128 tiles: 4096 x 4096 x 8192, scales by rows on both sides, 248 us
-// (1.1 PFLOP/s), by tiles 222; the library's bfloat16 product reaches 1.6.  Bound by vector
+// Exact products on 128 x 256 tiles: 4096 x 4096 x 8192, scales by rows on both sides, 264 us
+// (1.0 PFLOP/s), by tiles 245; the library's bfloat16 product reaches 1.6.  Bound by vector
 // instructions: 128 conversions, 64 FMAs and 64 products of scales a wave and block for 64 matrix
 // instructions, which hide one each.  Converting once per work group instead, through
-// LDS, left too few registers to hide its phases: 325 us.
+// LDS, left too few registers to hide its phases: 325 us, where registers took 248.
 //
 // A stage holds one block of K: kBN rows of B and kBM rows of A of 128 bytes
 // each, then their scales.  A lane's fragment is 16-byte chunks l / 16 and
@@ -1419,9 +1419,9 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const uint8_t* q, i
 // ... of K; fragments come straight from memory (lane l's 32 bytes are the
 // instruction's operand as they lie in the row), and the waves' sums meet in LDS.
 // All of an iteration's operands and scales are loaded before the first is used (one
-// token through 8192 x 8192: 14.9 us without that fence, 13.2 with it).  Bound by B's
+// token through 8192 x 8192: 14.9 us without that fence, 13.1 with it).  Bound by B's
 // bytes there, at 5.1 TB/s; by the latency of its few iterations where the product is
-// small (333 x 501 x 777: 6.3 us, 11.2 on 128 x 128 tiles).
+// small (333 x 501 x 777: 6.4 us, 11.2 on 128 x 128 tiles).
 constexpr int kFewWaves = 8;
 
 template <int kTM, int kTN, int kU, int kFA, int kFB, bool kRowB>
@@ -1576,10 +1576,12 @@ constexpr int kCUs = 256;
 // fetch (8192 x 64 x 8192 to float32: 37 us, the 128 x 128 tiles with eight splits 28).
 // Fitted to 32 shapes of 1 to 8192 rows and columns and 512 to 100000 deep, to bfloat16
 // and to float32, in the forms and splits that suit each: of those 64 runs 63 come within
-// 5% of their fastest and the last, 1024^3 to bfloat16, within 8%.  Of 52 runs on 26
-// other shapes, which served only to choose between equally good constants, 45 come
-// within 5% and the worst within 14%.  It is off for 16-bit products of at most 256 deep
-// with more than 32 rows, which take 128 x 128 tiles: 300 x 300 x 256 6.8 us, 3.9 in few rows.
+// 5% of their fastest and the last, 1024^3 to bfloat16, within 10%.  Of 54 runs on 27
+// other shapes, which served only to choose between equally good constants, 47 come
+// within 5%, six within 14%, and 300 x 300 x 256 to bfloat16 takes 6.6 us where few rows take
+// 3.9, as 16-bit products of at most 256 deep with more than 32 rows do.  Weights that do not
+// stay in the caches were not among them, and it is off there: 1 x 28672 x 8192 takes 128 x 128
+// tiles with two splits, 54 us, few rows 40; 1 x 128256 x 4096 108, 88.
 // Both sides: 512 x 512 x 4096 in few rows with two splits 12.5 us, on 128 x 128 tiles with
 // four 16.8; 2048^3 on 128 x 128 tiles 19.4, 256 x 256 27.7; 3000^3 42.5 the other way, 58.0.
 double mm_time(int form, int tile_m, bool exact, double groups, double steps, double reach) {
