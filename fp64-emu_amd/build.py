@@ -42,7 +42,7 @@ def _run(cmd, cwd=None):
 
 
 # One object each, compiled side by side; the float64 product's first.
-HIP_SOURCES = ("fp64emu.hip", "f8.hip")
+HIP_SOURCES = ("fp64emu.hip", "f8.hip", "f8_norm.hip", "f8_pointwise.hip")
 
 
 def build_capi():

@@ -3,6 +3,7 @@
 // instructions, and the gated activation whose checkpoint is held so.  The
 // entry points are those of include/fp64emu.h (fp64emu_*_f8*).
 
+#include "f8_act.h"
 #include "f8_common.h"
 
 namespace {
@@ -263,7 +264,7 @@ struct MmArgs {
   const uint8_t *A, *B;
   const float *sA, *sB;
   void* out;
-  float* part;                       // partial sums [splits, batch, M, N] if splits > 1
+  float* part;                       // partial sums [splits, batch, M, N], or null
   int64_t lda, ldb, strideA, strideB;
   int64_t sA_row, sA_blk, sA_str, sB_row, sB_blk, sB_str;
   int64_t ldo, stride_o;
@@ -274,6 +275,12 @@ struct MmArgs {
   int dtype, accumulate;
   int b_tiles;                       // B's scales by tiles
   int vec_o;                         // out's rows start at multiples of 4 elements
+  // What a product's sums go through before they are rounded: + bias, (kept,) act, + residual.
+  int epilogue;                      // any of it
+  int act, bias_type;
+  const void *bias, *residual;       // residual and keep have out's dtype
+  void* keep;
+  int64_t bias_stride, ld_res, stride_res, ld_keep, stride_keep;
 };
 
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -398,48 +405,73 @@ __device__ __forceinline__ v4i load16_masked(const uint8_t* row, int64_t k, int6
   return v4i{(int)w[0], (int)(w[0] >> 32), (int)w[1], (int)(w[1] >> 32)};
 }
 
-// Four successive outputs (m, n .. n + 3).
-__device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v) {
-  const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
-  const int64_t i = b * g.stride_o + m * g.ldo + n;
-  if (g.vec_o && valid == 4) {
-    if (g.dtype == FP64EMU_F32) {
-      v4f* o = reinterpret_cast<v4f*>(static_cast<float*>(g.out) + i);
-      if (g.accumulate) v += *o;
-      *o = v;
-    } else {
-      typedef unsigned short v4s __attribute__((ext_vector_type(4)));
-      v4s* o = reinterpret_cast<v4s*>(static_cast<unsigned short*>(g.out) + i);
-      const bool bf = g.dtype == FP64EMU_BF16;
-      if (g.accumulate) {
-        const v4s w = *o;
+// Four successive elements of a float32, bfloat16 or float16 array, the first `valid` of them (the
+// others 0); `vec`: all four of them at an aligned place.
+__device__ __forceinline__ v4f read4(int type, const void* p, int64_t i, int valid, bool vec) {
+  v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (type == FP64EMU_F32) {
+    if (vec) return *reinterpret_cast<const v4f*>(static_cast<const float*>(p) + i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] += bf ? bf16_value(w[j]) : (float)__builtin_bit_cast(_Float16, (unsigned short)w[j]);
-      }
-      v4s r;
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) v[j] = load1<FP64EMU_F32>(p, i + j);
+    return v;
+  }
+  typedef unsigned short v4s __attribute__((ext_vector_type(4)));
+  const unsigned short* q = static_cast<const unsigned short*>(p) + i;
+  v4s w = {0, 0, 0, 0};
+  if (vec) {
+    w = *reinterpret_cast<const v4s*>(q);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        r[j] = bf ? bf16_round(v[j]) : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
-      *o = r;
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) w[j] = q[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = type == FP64EMU_BF16 ? bf16_value(w[j]) : (float)__builtin_bit_cast(_Float16, (unsigned short)w[j]);
+  return v;
+}
+__device__ __forceinline__ void write4(int type, void* p, int64_t i, int valid, bool vec, v4f v) {
+  if (type == FP64EMU_F32) {
+    if (vec) {
+      *reinterpret_cast<v4f*>(static_cast<float*>(p) + i) = v;
+      return;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) store1<FP64EMU_F32>(p, i + j, v[j]);
+    return;
+  }
+  typedef unsigned short v4s __attribute__((ext_vector_type(4)));
+  unsigned short* q = static_cast<unsigned short*>(p) + i;
+  v4s r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r[j] = type == FP64EMU_BF16 ? bf16_round(v[j]) : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
+  if (vec) {
+    *reinterpret_cast<v4s*>(q) = r;
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= valid) break;
-    float x = v[j];
-    if (g.dtype == FP64EMU_F32) {
-      if (g.accumulate) x += load1<FP64EMU_F32>(g.out, i + j);
-      store1<FP64EMU_F32>(g.out, i + j, x);
-    } else if (g.dtype == FP64EMU_BF16) {
-      if (g.accumulate) x += load1<FP64EMU_BF16>(g.out, i + j);
-      store1<FP64EMU_BF16>(g.out, i + j, x);
-    } else {
-      if (g.accumulate) x += load1<FP64EMU_F16>(g.out, i + j);
-      store1<FP64EMU_F16>(g.out, i + j, x);
-    }
+  for (int j = 0; j < 4; ++j)
+    if (j < valid) q[j] = r[j];
+}
+
+// Four successive outputs (m, n .. n + 3).
+__device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v) {
+  const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
+  const bool vec = g.vec_o && valid == 4;    // of every operand of the epilogue, too
+  const int64_t i = b * g.stride_o + m * g.ldo + n;
+  if (g.epilogue) {
+    if (g.bias) v += read4(g.bias_type, g.bias, b * g.bias_stride + n, valid, vec);
+    if (g.keep) write4(g.dtype, g.keep, b * g.stride_keep + m * g.ld_keep + n, valid, vec, v);
+    float a[4] = {v[0], v[1], v[2], v[3]};
+    activate(g.act, a);
+    v = v4f{a[0], a[1], a[2], a[3]};
+    if (g.residual) v += read4(g.dtype, g.residual, b * g.stride_res + m * g.ld_res + n, valid, vec);
   }
+  if (g.accumulate) v += read4(g.dtype, g.out, i, valid, vec);
+  write4(g.dtype, g.out, i, valid, vec, v);
 }
 
 // The partial sums of one split instead of an output.
@@ -603,7 +635,7 @@ __device__ __forceinline__ void store_tile(const MmArgs& g, int64_t m, int64_t n
                                            const v4f (&acc)[S::kTN][S::kTM]) {
   const int rows = (int)(g.M - m), cols = (int)(g.N - n);
   const int64_t at = b * g.stride_o + m * g.ldo + n;
-  if (kExact || g.splits > 1)          // (whole float32 sums take the way through LDS)
+  if (kExact || g.part)                // (whole float32 sums take the way through LDS)
     store_rows<S, 0>(acc, g.part + (((int64_t)split * g.batch + b) * g.M + m) * g.N + n, g.N, rows, cols);
   else if (g.dtype == FP64EMU_BF16)
     store_rows<S, 1>(acc, static_cast<unsigned short*>(g.out) + at, g.ldo, rows, cols);
@@ -619,7 +651,123 @@ __device__ __forceinline__ void store16_past(void* p, const void* w) {
   __builtin_nontemporal_store(v, static_cast<v4u_any*>(p));
 }
 
-template <class S, bool kExact, int kFA, int kFB, bool kRowB>
+// A tile's sums through the epilogue: + bias where they lie in registers, then in float32 through the
+// wave's room in LDS, half of its rows at a time, so that what is kept, the residual and the
+// output go by whole lines.  The activation works there in a loop of its own, once in the code for
+// all of a half's values (unrolled over the registers its five forms would not fit the
+// instruction cache); the residual's lines are read before it and used after it.
+template <class S, bool kExact>
+__device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64_t m0, int64_t n0, int b, int wave, int lane,
+                                            v4f (&acc)[S::kTN][S::kTM]) {
+  using T = std::conditional_t<kExact, float, unsigned short>;
+  constexpr int kEach = 16 / (int)sizeof(T), kLanes = S::kTN * 16 / kEach, kRows = 64 / kLanes;
+  constexpr int kHalf = S::kTM / 2, kSteps = kHalf * 16 / kRows;
+  constexpr int kRow = S::kTN * 16 * 4 + 16;                   // (rows 16 bytes apart: see mm_tile's)
+  static_assert(S::kWaves * kHalf * 16 * kRow <= 2 * S::kStage, "the waves' rooms in the stages'");
+  const int fr = lane & 15, fg = lane >> 4;
+  uint8_t* room = lds + wave * (kHalf * 16 * kRow);
+  if (g.bias) {
+#pragma unroll
+    for (int x = 0; x < S::kTN; ++x) {
+      const int64_t n = n0 + x * 16 + 4 * fg, left = g.N - n;
+      const v4f bias = read4(g.bias_type, g.bias, b * g.bias_stride + n, (int)(left < 4 ? left : 4), g.vec_o && left >= 4);
+#pragma unroll
+      for (int y = 0; y < S::kTM; ++y) acc[x][y] += bias;
+    }
+  }
+  // Other lanes of the wave read what a lane wrote: not before it is written, whatever the
+  // compiler can tell of the addresses (the LDS itself keeps a wave's order).
+  auto handed = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  auto round = [&](const float (&v)[kEach], T (&w)[kEach]) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if constexpr (kExact) w[j] = v[j];
+      else w[j] = g.dtype == FP64EMU_BF16 ? bf16_round(v[j]) : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
+    }
+  };
+  const int64_t n = n0 + (lane % kLanes) * kEach;
+  const int valid = (int)(g.N - n < kEach ? g.N - n : kEach);
+  auto put_line = [&](void* out, int64_t i, const T (&w)[kEach]) {
+    T* to = static_cast<T*>(out) + i;
+    if (valid == kEach) {
+      store16_past(to, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach - 1; ++j)
+        if (j < valid) to[j] = w[j];
+    }
+  };
+  uint8_t* const line = room + (lane / kLanes) * kRow + (lane % kLanes) * kEach * 4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int64_t first = m0 + half * kHalf * 16 + lane / kLanes;    // step i: row first + i kRows
+    T old[kSteps][kEach];
+    if (g.residual) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int64_t m = first + i * kRows;
+        const T* q = static_cast<const T*>(g.residual) + b * g.stride_res + m * g.ld_res + n;
+        if (m >= g.M) break;
+        if (valid == kEach) {
+          __builtin_memcpy(old[i], q, 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kEach - 1; ++j) old[i][j] = j < valid ? q[j] : T{};
+        }
+      }
+    }
+    if (half) handed();                                        // the first half's lines are read
+#pragma unroll
+    for (int y = 0; y < kHalf; ++y)
+#pragma unroll
+      for (int x = 0; x < S::kTN; ++x)
+        *reinterpret_cast<v4f*>(room + (y * 16 + fr) * kRow + (x * 16 + 4 * fg) * 4) = acc[x][half * kHalf + y];
+    handed();
+    auto get = [&](int i, float (&v)[kEach]) {
+      __builtin_memcpy(v, __builtin_assume_aligned(line + i * kRows * kRow, 16), 4 * kEach);
+    };
+    if (g.keep || g.act) {
+#pragma unroll 1
+      for (int i = 0; i < kSteps; ++i) {
+        const int64_t m = first + i * kRows;
+        float v[kEach];
+        get(i, v);
+        if (g.keep && m < g.M) {
+          T w[kEach];
+          round(v, w);
+          put_line(g.keep, b * g.stride_keep + m * g.ld_keep + n, w);
+        }
+        activate(g.act, v);
+        __builtin_memcpy(__builtin_assume_aligned(line + i * kRows * kRow, 16), v, 4 * kEach);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t m = first + i * kRows;
+      float v[kEach];
+      get(i, v);
+      if (m >= g.M) continue;
+      if (g.residual) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          if constexpr (kExact) v[j] += old[i][j];
+          else v[j] += g.dtype == FP64EMU_BF16 ? bf16_value(old[i][j])
+                                               : (float)__builtin_bit_cast(_Float16, old[i][j]);
+        }
+      }
+      T w[kEach];
+      round(v, w);
+      put_line(g.out, b * g.stride_o + m * g.ldo + n, w);
+    }
+  }
+}
+
+// kEpilogue: a kernel of its own, so that the plain one keeps its registers.
+template <class S, bool kExact, int kFA, int kFB, bool kRowB, bool kEpilogue>
 __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   // The two stages, or the waves' rows of out.
   constexpr int kOut = S::kWaves * S::kTM * 16 * (S::kTN * 16 * (kExact ? 4 : 2) + 16);
@@ -883,8 +1031,13 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     for (int y = 0; y < S::kTM; ++y) acc[x][y] *= 1.0f / kFrame;
   for (; done < nk; ++done) block(std::true_type{}, done);
 
-  if (g.splits > 1 || (!kExact && g.accumulate)) {
+  if (g.part || (!kExact && g.accumulate)) {
     store_tile<S, kExact>(g, m0 + wm * S::kTM * 16 + fr, n0 + wn * S::kTN * 16 + 4 * fg, b, split, acc);
+    return;
+  }
+  if constexpr (kEpilogue) {
+    barrier_lds();                                           // every wave is done with the stages
+    finish_tile<S, kExact>(g, lds, m0 + wm * S::kTM * 16, n0 + wn * S::kTN * 16, b, wave, lane, acc);
     return;
   }
   // Through LDS, so that a store writes whole lines of out past the caches: 8192 x
@@ -962,9 +1115,9 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   }
 }
 
-template <class S, bool kExact, int kFA, int kFB, bool kRowB>
+template <class S, bool kExact, int kFA, int kFB, bool kRowB, bool kEpilogue>
 __global__ void __launch_bounds__(S::kT, 2) mm_tile_kernel(MmArgs g) {
-  mm_tile<S, kExact, kFA, kFB, kRowB>(g);
+  mm_tile<S, kExact, kFA, kFB, kRowB, kEpilogue>(g);
 }
 
 // Rows of any alignment into rows of a multiple of 16 bytes, 16 bytes a thread.
@@ -1225,10 +1378,23 @@ int launch_quant(QuantArgs g, int64_t batch, int64_t mblocks, bool tiles, hipStr
   return FP64EMU_OK;
 }
 
+// Operands whose tile kernels finish a product with an epilogue themselves: e4m3 on both sides, what
+// activations and weights are held in.  With e5m2 (gradients) the sums go through the
+// workspace, as with splits, at 8 bytes an output more.
+template <int kFA, int kFB>
+constexpr bool kFusedFmt = kFA == FP64EMU_E4M3 && kFB == FP64EMU_E4M3;
+
 template <class S, bool kExact, int kFA, int kFB>
 void launch_tile(const MmArgs& g, unsigned groups, hipStream_t s) {
-  if (g.b_tiles) mm_tile_kernel<S, kExact, kFA, kFB, false><<<groups, S::kT, 0, s>>>(g);
-  else mm_tile_kernel<S, kExact, kFA, kFB, true><<<groups, S::kT, 0, s>>>(g);
+  if constexpr (kFusedFmt<kFA, kFB>) {
+    if (g.epilogue && !g.part) {
+      if (g.b_tiles) mm_tile_kernel<S, kExact, kFA, kFB, false, true><<<groups, S::kT, 0, s>>>(g);
+      else mm_tile_kernel<S, kExact, kFA, kFB, true, true><<<groups, S::kT, 0, s>>>(g);
+      return;
+    }
+  }
+  if (g.b_tiles) mm_tile_kernel<S, kExact, kFA, kFB, false, false><<<groups, S::kT, 0, s>>>(g);
+  else mm_tile_kernel<S, kExact, kFA, kFB, true, false><<<groups, S::kT, 0, s>>>(g);
 }
 
 template <int kTM, int kTN, int kU, int kFA, int kFB>
@@ -1257,10 +1423,11 @@ bool copyable(const fp64emu_f8_t& f) {
 // Partial sums, then the rows of A and of B that are laid out again.
 struct MmRoom { size_t parts, A, B; };
 
-MmRoom mm_room(const fp64emu_mm_f8_t* p, const MmPlan& plan) {
+MmRoom mm_room(const fp64emu_mm_f8_t* p, const MmPlan& plan, bool epilogue) {
   MmRoom r{};
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  if (plan.splits > 1) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
+  const bool fused = p->A.fmt == FP64EMU_E4M3 && p->B.fmt == FP64EMU_E4M3;       // kFusedFmt
+  if (plan.splits > 1 || (epilogue && plan.form != kFew && !fused)) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
   const size_t ld = (size_t)((p->K + 15) / 16 * 16);
   if (plan.form != kFew && !copyable(p->A)) r.A = up((size_t)(p->batch * p->M) * ld);
   if (plan.form != kFew && !copyable(p->B)) r.B = up((size_t)(p->batch * p->N) * ld);
@@ -1328,11 +1495,13 @@ int fp64emu_quant_f8(const void* x, int dtype, int64_t batch, int64_t M, int64_t
   return invalid("dtype");
 }
 
-size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p) {
+size_t fp64emu_mm_f8_workspace(const fp64emu_mm_f8_t* p) { return fp64emu_mm_f8_epilogue_workspace(p, nullptr); }
+
+size_t fp64emu_mm_f8_epilogue_workspace(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e) {
   if (check_mm(p) || p->batch * p->M == 0 || p->N == 0 || p->K == 0) return 0;
   const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
   if (plan.splits == 0) return 0;
-  const MmRoom r = mm_room(p, plan);
+  const MmRoom r = mm_room(p, plan, e != nullptr);
   return r.parts + r.A + r.B;
 }
 
@@ -1351,7 +1520,17 @@ int fp64emu_mm_f8_plan(const fp64emu_mm_f8_t* p, fp64emu_mm_f8_plan_t* out) {
 
 int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_bytes,
                   fp64emu_stream_t stream) {
+  return fp64emu_mm_f8_epilogue(p, nullptr, workspace, workspace_bytes, stream);
+}
+
+int fp64emu_mm_f8_epilogue(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e, void* workspace,
+                           size_t workspace_bytes, fp64emu_stream_t stream) {
   if (int st = check_mm(p)) return st;
+  if (e) {
+    if (!known_act(e->act)) return invalid("act must be one of FP64EMU_ACT_*");
+    if (!known_dtype(e->bias_dtype)) return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+    if (p->accumulate) return invalid("an epilogue does not accumulate: out as its residual does");
+  }
   if (p->batch == 0 || p->M == 0 || p->N == 0) return FP64EMU_OK;
   if (!p->out) return invalid("null operand pointer");
   if (p->ldo < p->N) return invalid("rows of out are shorter than N");
@@ -1368,6 +1547,27 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
   g.batch = (int)p->batch;
   const int quad = 4 * size_of(p->dtype);
   g.vec_o = multiple(p->out, quad) && p->ldo % 4 == 0 && p->stride_o % 4 == 0;
+  if (e) {
+    if ((e->residual && e->ld_residual < p->N) || (e->keep && e->ld_keep < p->N))
+      return invalid("rows of residual or keep are shorter than N");
+    g.epilogue = 1;
+    g.act = e->act;
+    g.bias = e->bias;
+    g.bias_type = e->bias_dtype;
+    g.bias_stride = e->bias_stride;
+    g.residual = e->residual;
+    g.ld_res = e->ld_residual;
+    g.stride_res = e->stride_residual;
+    g.keep = e->keep;
+    g.ld_keep = e->ld_keep;
+    g.stride_keep = e->stride_keep;
+    const auto fours = [](const void* q, int size, int64_t ld, int64_t stride) {
+      return !q || (multiple(q, 4 * size) && ld % 4 == 0 && stride % 4 == 0);
+    };
+    g.vec_o = g.vec_o && fours(e->bias, size_of(e->bias_dtype), 0, e->bias_stride) &&
+              fours(e->residual, quad / 4, e->ld_residual, e->stride_residual) &&
+              fours(e->keep, quad / 4, e->ld_keep, e->stride_keep);
+  }
   if (p->K == 0) {
     // An empty sum: zeros, or out as it is.
     if (g.accumulate) return FP64EMU_OK;
@@ -1384,7 +1584,7 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
   }
   const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
   if (plan.splits == 0) return invalid("product too large for one launch");
-  const MmRoom room = mm_room(p, plan);
+  const MmRoom room = mm_room(p, plan, e != nullptr);
   const size_t need = room.parts + room.A + room.B;
   if (need && (!workspace || workspace_bytes < need))
     return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_mm_f8_workspace");
@@ -1403,7 +1603,7 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
   g.sB_row = p->B.s_row;
   g.sB_blk = p->B.s_block;
   g.sB_str = p->B.s_stride;
-  g.part = static_cast<float*>(workspace);
+  g.part = room.parts ? static_cast<float*>(workspace) : nullptr;
   g.nkb = (int)((p->K + kBlk - 1) / kBlk);
   g.splits = plan.splits;
   g.kb_per_split = plan.kb_per_split;
@@ -1434,7 +1634,7 @@ int fp64emu_mm_f8(const fp64emu_mm_f8_t* p, void* workspace, size_t workspace_by
     else launch_mm<FP64EMU_E5M2, FP64EMU_E5M2>(g, plan, groups, s);
   }
   if (int st = check_hip(hipGetLastError(), "mm_f8 launch")) return st;
-  if (plan.splits > 1) {
+  if (g.part) {
     sum_parts_kernel<<<sum_groups, kThreads, 0, s>>>(g);
     return check_hip(hipGetLastError(), "mm_f8 launch");
   }

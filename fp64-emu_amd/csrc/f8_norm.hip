@@ -1,0 +1,860 @@
+// Norms before and after a block, fused with the block's gate, dropout and residual, for
+// gfx950: the residual stream's next value and its norm, plain or as the next product's
+// 8-bit operand, and the gradient of both.  The entry points are fp64emu_norm_f8*.
+//
+// With i(v) = (mean(v^2) + eps)^-1/2 over a row of D elements:
+//
+//   z = y i(y) post,  v = scale r + gate drop(z),  x = v i(v) w
+//
+// (z = y without post, v = r without y.)  v is rounded once, where it is stored as the
+// new stream; x is taken from the unrounded one.
+
+#include "f8_common.h"
+#include "f8_drop.h"
+#include "f8_sums.h"
+
+namespace {
+
+struct NormArgs {
+  const void *r, *y, *gate, *w, *post;
+  const int64_t* rng;
+  int64_t M, D, ld_r, ld_y, ld_gate;         // ld_gate 0: one gate for all rows
+  int64_t blocks;                            // of 128 along a row
+  int w_type, post_type, gate_type;
+  uint32_t threshold;
+  float scale, eps;
+  void* out;                                 // the new stream
+  void* x;
+  int64_t ld_out, ld_x;
+  float* stats;                              // i(v), then i(y), M each
+  Out8 rows, cols;
+};
+
+struct NormGradArgs {
+  const void *dx, *dr;
+  int64_t ld_dx, ld_dr;
+  void *dr_out, *dy, *dgates;
+  int64_t ld_dr_out, ld_dy, ld_dgates;
+  float *dw, *dpost, *dgate;                 // [D], or a group's part of them, [groups][D] each
+  float* c1;                                 // rows of any length: a row's first mean
+};
+
+// Eight elements from i on, those past `valid` as zeros.
+template <int kT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, int valid, float (&v)[8]) {
+  Held<kT> h;
+  h.load(0, p, i, valid);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = h.at(0, j);
+}
+// The same of any type, or ones.
+__device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, int valid, float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 1.0f;
+  } else if (type == FP64EMU_F32) {
+    load8<FP64EMU_F32>(p, i, valid, v);
+  } else if (type == FP64EMU_BF16) {
+    load8<FP64EMU_BF16>(p, i, valid, v);
+  } else {
+    load8<FP64EMU_F16>(p, i, valid, v);
+  }
+}
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, false));
+}
+// The sum over the 16 lanes of a DPP row, the same bits in all of them.
+__device__ __forceinline__ float row16_sum(float v) {
+  v += dpp<0x128>(v);                        // row_ror:8
+  v += dpp<0x124>(v);
+  v += dpp<0x122>(v);
+  return v + dpp<0x121>(v);
+}
+
+// Eight elements of a row as they came.
+template <int kT>
+struct Eight {
+  Held<kT> h;
+  __device__ __forceinline__ void load(const void* p, int64_t i, int valid) { h.load(0, p, i, valid); }
+  __device__ __forceinline__ float at(int j) const { return h.at(0, j); }
+  // Makes the compiler unpack the words again instead of keeping eight floats beside them.
+  __device__ __forceinline__ void again() {
+    if constexpr (kT != FP64EMU_F32) asm volatile("" : "+v"(h.w[0]));
+  }
+};
+
+// How a launch lays rows on threads: kT threads a row, eight elements each (so 16 neighbouring
+// lanes hold a block of 128), work groups of 256 threads or one row.
+template <int kT_>
+struct RowShape {
+  static constexpr int kT = kT_, kGroup = kT > kThreads ? kT : kThreads, kRows = kGroup / kT;
+};
+
+// Sums over the threads of a row, in all of them; `turn` alternates from call to call, so that one
+// barrier is enough.
+template <int kT, int kN, int kGroup>
+struct RowSum {
+  static constexpr int kWaves = kT / 64;
+  struct Room { float v[2][kN][kGroup / 64]; };
+  static __device__ __forceinline__ void run(float (&v)[kN], Room& room, int& turn) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      v[n] = row16_sum(v[n]);
+      if constexpr (kT >= 64) {
+        v[n] += __shfl_xor(v[n], 16);
+        v[n] += __shfl_xor(v[n], 32);
+      }
+    }
+    if constexpr (kT > 64) {
+      const int wave = threadIdx.x >> 6, first = wave / kWaves * kWaves;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) room.v[turn][n][wave] = v[n];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        float s = room.v[turn][n][first];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) s += room.v[turn][n][first + w];
+        v[n] = s;
+      }
+      turn ^= 1;
+    }
+  }
+};
+
+__device__ __forceinline__ float inverse_rms(float squares, const NormArgs& g) {
+  return 1.0f / sqrtf(squares / (float)g.D + g.eps);
+}
+
+// v of eight elements from those of r and y.
+__device__ __forceinline__ void joined(const NormArgs& g, const Drop& drop, uint64_t chunk, float iy, const float (&y)[8],
+                                       const float (&post)[8], const float (&gate)[8], float (&v)[8]) {
+  const uint32_t kept = kept_of(drop, chunk);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float z = g.post ? y[j] * iy * post[j] : y[j];
+    v[j] = g.scale * v[j] + gate[j] * (kept >> j & 1 ? z * drop.scale : 0.0f);
+  }
+}
+
+template <int kR, int kY>
+__device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t col, int valid, float iv,
+                                          const float (&v)[8], const float (&w)[8]) {
+  Held<FP64EMU_F32> x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x.v[0][j] = v[j] * iv * w[j];
+  if (g.x) store8<kY>(g.x, m * g.ld_x + col, valid, x.v[0]);
+  if (g.rows.q) {
+    // (All 16 lanes of a block come here or none: those past the row hold zeros.)
+    const float a = amax_of(row16_max(x.row_mag(0)));
+    put8(g.rows.q + m * g.rows.ld + col, valid, row_codes<FP64EMU_E4M3>(x, 0, inverse_scale<FP64EMU_E4M3>(a)));
+    const int64_t kb = col / kBlk;
+    if ((threadIdx.x & 15) == 0 && valid > 0) g.rows.s[m * g.rows.s_row + kb * g.rows.s_block] = scale_of<FP64EMU_E4M3>(a);
+  }
+}
+
+// Rows whose values stay in registers from the first sum to the last store.  A work group takes
+// rows blockIdx.x kRows + .., gridDim.x kRows apart, the weights in registers throughout and the next
+// row's values on their way.
+template <int kR, int kY, class S>
+__global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
+  constexpr int kT = S::kT;
+  using Sum = RowSum<kT, 1, S::kGroup>;
+  __shared__ typename Sum::Room room;
+  const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  const int64_t row_chunks = (g.D + 7) / 8;
+  const int col = 8 * t, left = (int)g.D - col, valid = left < 0 ? 0 : left < 8 ? left : 8;
+  float w[8], post[8], gate[8];
+  load8_any(g.w_type, g.w, col, valid, w);
+  load8_any(g.post_type, g.post, col, valid, post);
+  if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, valid, gate);
+  int turn = 0;
+  Eight<kR> r;
+  Eight<kY> y, gates;
+  auto fetch = [&](int64_t m) {
+    const int n = m < g.M ? valid : 0;
+    r.load(g.r, m * g.ld_r + col, n);
+    if (g.y) y.load(g.y, m * g.ld_y + col, n);
+    if (g.ld_gate) gates.load(g.gate, m * g.ld_gate + col, n);
+  };
+  const int64_t step = (int64_t)gridDim.x * S::kRows;
+  int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
+  fetch(m);
+  for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
+    float v[8], yv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = r.at(j);
+      if (g.y) yv[j] = y.at(j);
+      if (g.ld_gate) gate[j] = gates.at(j);
+    }
+    fetch(m + step);
+    float iy = 1.0f;
+    if (g.y) {
+      if (g.post) {
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] = fmaf(yv[j], yv[j], s[0]);
+        Sum::run(s, room, turn);
+        iy = inverse_rms(s[0], g);
+      }
+      joined(g, drop, (uint64_t)(m * row_chunks + t), iy, yv, post, gate, v);
+      if (g.out && m < g.M) store8<kR>(g.out, m * g.ld_out + col, valid, v);
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[0] = fmaf(v[j], v[j], s[0]);
+    Sum::run(s, room, turn);
+    const float iv = inverse_rms(s[0], g);
+    if (m < g.M) {
+      if (g.stats && t == 0) {
+        g.stats[m] = iv;
+        if (g.post) g.stats[g.M + m] = iy;
+      }
+      emit_norm<kR, kY>(g, m, col, valid, iv, v, w);
+    }
+  }
+}
+
+// Eight elements of v again from memory, for rows that do not stay in registers.
+template <int kR, int kY>
+__device__ __forceinline__ void joined_at(const NormArgs& g, const Drop& drop, int64_t m, int64_t col, int valid,
+                                          float iy, float (&v)[8]) {
+  load8<kR>(g.r, m * g.ld_r + col, valid, v);
+  if (!g.y) return;
+  float y[8], post[8], gate[8];
+  load8<kY>(g.y, m * g.ld_y + col, valid, y);
+  load8_any(g.post_type, g.post, col, valid, post);
+  load8_any(g.gate_type, g.gate, m * g.ld_gate + col, valid, gate);
+  joined(g, drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8), iy, y, post, gate, v);
+}
+
+// Rows of any length, a row to a work group of 1024, read once for each sum and once for x: past
+// the registers' 8192 elements a row's second and third reading come from L2.
+constexpr int kLong = 1024;
+
+template <int kR, int kY>
+__global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
+  using Sum = RowSum<kLong, 1, kLong>;
+  __shared__ typename Sum::Room room;
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  int turn = 0;
+  auto each = [&](auto fn) {
+    // (Whole blocks of 128 of the last round, so that emit_norm's 16 lanes are there together.)
+    for (int64_t col = 8 * threadIdx.x; col < g.blocks * kBlk; col += 8 * kLong) {
+      const int64_t left = g.D - col;
+      fn(col, left < 0 ? 0 : left < 8 ? (int)left : 8);
+    }
+  };
+  for (int64_t m = blockIdx.x; m < g.M; m += gridDim.x) {
+    float iy = 1.0f;
+    if (g.post) {
+      float s[1] = {0.0f};
+      each([&](int64_t col, int valid) {
+        float y[8];
+        load8<kY>(g.y, m * g.ld_y + col, valid, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] = fmaf(y[j], y[j], s[0]);
+      });
+      Sum::run(s, room, turn);
+      iy = inverse_rms(s[0], g);
+    }
+    float s[1] = {0.0f};
+    each([&](int64_t col, int valid) {
+      float v[8];
+      joined_at<kR, kY>(g, drop, m, col, valid, iy, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] = fmaf(v[j], v[j], s[0]);
+    });
+    Sum::run(s, room, turn);
+    const float iv = inverse_rms(s[0], g);
+    if (g.stats && threadIdx.x == 0) {
+      g.stats[m] = iv;
+      if (g.post) g.stats[g.M + m] = iy;
+    }
+    if (!g.out && !g.x && !g.rows.q) continue;
+    each([&](int64_t col, int valid) {
+      float v[8], w[8];
+      joined_at<kR, kY>(g, drop, m, col, valid, iy, v);
+      load8_any(g.w_type, g.w, col, valid, w);
+      // (r may be the new stream itself: its last reading is above.)
+      if (g.out) store8<kR>(g.out, m * g.ld_out + col, valid, v);
+      emit_norm<kR, kY>(g, m, col, valid, iv, v, w);
+    });
+  }
+}
+
+// Tiles of 128 x 128, once the rows' statistics are there: the new stream, x's rows and its columns.
+template <int kR, int kY>
+__global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
+  __shared__ TileLds lds;
+  const uint32_t blocks = (uint32_t)g.blocks;
+  const int64_t kb = blockIdx.x % blocks, mb = blockIdx.x / blocks;
+  const int64_t row0 = mb * kBlk, col0 = kb * kBlk, row = row0 + 8 * ((int)threadIdx.x >> 4);
+  const TilePlace t = tile_place(row0, col0, g.M, g.D);
+  const int64_t col = col0 + 8 * t.cl;
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  const int n = t.valid(0) > 0 ? (t.valid(0) < 8 ? t.valid(0) : 8) : 0;
+  // Lane cl of a row group has row cl % 8's statistics, i(v) in the lower eight lanes and i(y) in the
+  // upper ones: broadcast within the DPP row where they are used.
+  float stat = 0.0f;
+  if (8 * t.rg + (t.cl & 7) < t.rows && (t.cl < 8 || g.post)) stat = g.stats[(t.cl < 8 ? 0 : g.M) + row + (t.cl & 7)];
+  Held<FP64EMU_F32> x;
+  {
+    Held<kR> r;
+    Held<kY> y;
+    float w[8], post[8], gate[8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      r.load(p, g.r, (row + p) * g.ld_r + col, t.valid(p));
+      if (g.y) y.load(p, g.y, (row + p) * g.ld_y + col, t.valid(p));
+    }
+    load8_any(g.w_type, g.w, col, n, w);
+    load8_any(g.post_type, g.post, col, n, post);
+    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, n, gate);
+    const uint64_t chunk = (uint64_t)(row * ((g.D + 7) / 8) + col / 8);
+    auto each = [&](auto P) {
+      constexpr int p = decltype(P)::value;
+      const float iv = row16_lane<p>(stat), iy = row16_lane<8 + p>(stat);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = r.at(p, j);
+      if (g.y) {
+        float yv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) yv[j] = y.at(p, j);
+        if (g.ld_gate) load8<kY>(g.gate, (row + p) * g.ld_gate + col, t.valid(p), gate);
+        joined(g, drop, chunk + p * ((g.D + 7) / 8), iy, yv, post, gate, v);
+        if (g.out) store8<kR>(g.out, (row + p) * g.ld_out + col, t.valid(p), v);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v[p][j] = v[j] * iv * w[j];
+    };
+    each_row(each, std::make_integer_sequence<int, 8>{});
+  }
+  if (g.rows.q) emit_rows<FP64EMU_E4M3>(x, t, row0, col0, kb, g.rows);
+  emit_cols<FP64EMU_E4M3>(x, t, row0, col0, mb, g.cols, lds);
+}
+
+// ---------------------------------------------------------------------------
+// Gradient.  With vh = v i(v), yh = y i(y) and k drop's factor of an element:
+//
+//   e = dr + i(v) (dx w),   t = e - i(v) vh c1,       c1 = mean(dx w vh)     t: v's gradient
+//   dz = t gate k,  dy = i(y) (dz post - yh c2),      c2 = mean(dz post yh)
+//   dw = sum dx vh,  dpost = sum dz yh,  dgate = sum t k yh post    over the rows
+//
+// and scale t is r's gradient.  c2 is linear in c1: with u = gate k post yh, c2 = mean(u e) - c1
+// mean(u i(v) vh), so that one joint sum of three gives both and a row takes one barrier.
+// v is the stream as it is stored.
+
+// What eight elements give, first to the three sums and then, with the means, to the gradients; kept is
+// there before.
+struct GradPart {
+  float vh[8], e[8], yh[8];
+  uint32_t kept;
+};
+
+template <bool kPost>
+__device__ __forceinline__ void grad_sums(const Drop& drop, float iv, float iy, const float (&v)[8], const float (&y)[8],
+                                          const float (&dx)[8], const float (&dr)[8], const float (&w)[8],
+                                          const float (&post)[8], const float (&gate)[8], GradPart& p,
+                                          float (&s)[kPost ? 3 : 1]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float gw = dx[j] * w[j];
+    p.vh[j] = v[j] * iv;
+    p.e[j] = dr[j] + iv * gw;
+    s[0] = fmaf(gw, p.vh[j], s[0]);
+    if constexpr (kPost) {
+      p.yh[j] = y[j] * iy;
+      const float u = p.kept >> j & 1 ? gate[j] * drop.scale * post[j] * p.yh[j] : 0.0f;
+      s[1] = fmaf(u, p.e[j], s[1]);
+      s[2] = fmaf(u, iv * p.vh[j], s[2]);
+    } else {
+      p.yh[j] = y[j];
+    }
+  }
+}
+
+// t, dy and dgate of eight elements, and what they add to the sums over the rows.
+template <bool kPost>
+__device__ __forceinline__ void grad_values(const Drop& drop, const GradPart& p, float iv, float iy, float c1, float c2,
+                                            const float (&post)[8], const float (&gate)[8], float (&t)[8],
+                                            float (&dz)[8], float (&dy)[8], float (&dgate)[8]) {
+  const float back = iv * c1;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    t[j] = p.e[j] - back * p.vh[j];
+    const float k = p.kept >> j & 1 ? t[j] * drop.scale : 0.0f;
+    const bool in = p.kept >> j & 1;
+    dz[j] = k * gate[j];
+    dgate[j] = in ? k * (kPost ? p.yh[j] * post[j] : p.yh[j]) : 0.0f;
+    dy[j] = kPost ? iy * (dz[j] * post[j] - p.yh[j] * c2) : in ? dz[j] : 0.0f;
+  }
+}
+
+// A group's sums over its rows into its part of [groups][D] (or the result itself, with one group).
+template <class S, class Column>
+__device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& of, float* part, int64_t D, float* lds) {
+  constexpr int kT = S::kT;
+  const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
+  float* to = part + (int64_t)blockIdx.x * D;
+  if constexpr (S::kRows == 1) {
+    store8<FP64EMU_F32>(to, of.col, of.valid, sum);
+  } else {
+    __syncthreads();                         // (whatever the room held before)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds[j * S::kGroup + threadIdx.x] = sum[j];
+    __syncthreads();
+    if (sub == 0) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = lds[j * S::kGroup + t];
+#pragma unroll
+        for (int i = 1; i < S::kRows; ++i) v[j] += lds[j * S::kGroup + i * kT + t];
+      }
+      store8<FP64EMU_F32>(to, of.col, of.valid, v);
+    }
+  }
+}
+
+// Rows in registers, as norm_rows_kernel, but kC times eight elements a thread (element 8 (c kT + t) on):
+// 1024 threads a row leave 128 registers each, which the sums over the rows, kept a column to a thread,
+// do not fit.  A row's values stay as they came and are worked out again after its sums; with one
+// chunk the next row's are on their way meanwhile.  kPost: y has a norm; without it y may be absent, too.
+template <int kR, int kY, class S, int kC, bool kPost>
+__global__ void __launch_bounds__(S::kGroup) norm_grad_kernel(NormArgs g, NormGradArgs d) {
+  constexpr int kT = S::kT, kN = kPost ? 3 : 1;
+  constexpr bool kAhead = kC == 1;
+  using Sum = RowSum<kT, kN, S::kGroup>;
+  __shared__ typename Sum::Room room;
+  __shared__ float joint[S::kRows > 1 ? 8 * S::kGroup : 1];
+  const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  const int64_t row_chunks = (g.D + 7) / 8;
+  struct Column {
+    float w[8], post[8], gate[8], dw[8], dpost[8], dgate[8];
+    int col, valid;
+  } of[kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    Column& o = of[c];
+    o.col = 8 * (c * kT + t);
+    const int left = (int)g.D - o.col;
+    o.valid = left < 0 ? 0 : left < 8 ? left : 8;
+    load8_any(g.w_type, g.w, o.col, o.valid, o.w);
+    if constexpr (kPost) load8_any(g.post_type, g.post, o.col, o.valid, o.post);
+    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, o.col, o.valid, o.gate);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.dw[j] = o.dpost[j] = o.dgate[j] = 0.0f;
+  }
+  int turn = 0;
+  struct Row {
+    Eight<kR> v[kC], dr[kC];
+    Eight<kY> y[kC], dx[kC], gates[kC];
+    float iv, iy;
+  };
+  auto fetch = [&](int64_t m, Row& o) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int n = m < g.M ? of[c].valid : 0, col = of[c].col;
+      o.v[c].load(g.r, m * g.ld_r + col, n);
+      o.dx[c].load(d.dx, m * d.ld_dx + col, n);
+      o.dr[c].load(d.dr, m * d.ld_dr + col, d.dr ? n : 0);
+      o.y[c].load(g.y, m * g.ld_y + col, g.y ? n : 0);
+      if (g.ld_gate) o.gates[c].load(g.gate, m * g.ld_gate + col, n);
+    }
+    o.iv = m < g.M ? g.stats[m] : 0.0f;
+    o.iy = kPost && m < g.M ? g.stats[g.M + m] : 0.0f;
+  };
+  const int64_t step = (int64_t)gridDim.x * S::kRows;
+  int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
+  Row next;
+  if constexpr (kAhead) fetch(m, next);
+  for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
+    Row o;
+    if constexpr (kAhead) {
+      o = next;
+      fetch(m + step, next);
+    } else {
+      fetch(m, o);
+    }
+    GradPart p;
+    float s[kN] = {}, dx[8];
+    auto work_out = [&](int c, float (&s)[kN]) {
+      Column& k = of[c];
+      float v[8], y[8], dr[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = o.v[c].at(j);
+        dx[j] = o.dx[c].at(j);
+        dr[j] = o.dr[c].at(j);
+        y[j] = o.y[c].at(j);
+        if (g.ld_gate) k.gate[j] = o.gates[c].at(j);
+      }
+      grad_sums<kPost>(drop, o.iv, o.iy, v, y, dx, dr, k.w, k.post, k.gate, p, s);
+    };
+    uint32_t kept[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      p.kept = kept[c] = kept_of(drop, (uint64_t)(m * row_chunks + c * kT + t));
+      work_out(c, s);
+    }
+    Sum::run(s, room, turn);
+    const float c1 = s[0] / (float)g.D;
+    float c2 = 0.0f;
+    if constexpr (kPost) c2 = (s[1] - c1 * s[2]) / (float)g.D;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      Column& k = of[c];
+      o.v[c].again();
+      o.dx[c].again();
+      o.dr[c].again();
+      o.y[c].again();
+      o.gates[c].again();
+      p.kept = kept[c];
+      float none[kN], tv[8], dz[8], dy[8], dg[8];
+      work_out(c, none);
+      grad_values<kPost>(drop, p, o.iv, o.iy, c1, c2, k.post, k.gate, tv, dz, dy, dg);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        k.dw[j] = fmaf(dx[j], p.vh[j], k.dw[j]);
+        if constexpr (kPost) k.dpost[j] = fmaf(dz[j], p.yh[j], k.dpost[j]);
+        k.dgate[j] += dg[j];
+        tv[j] *= g.scale;
+      }
+      if (m < g.M) {
+        if (d.dr_out) store8<kR>(d.dr_out, m * d.ld_dr_out + k.col, k.valid, tv);
+        if (d.dy) store8<kY>(d.dy, m * d.ld_dy + k.col, k.valid, dy);
+        if (d.dgates) store8<kY>(d.dgates, m * d.ld_dgates + k.col, k.valid, dg);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    if (d.dw) join_rows<S>(of[c].dw, of[c], d.dw, g.D, joint);
+    if (kPost && d.dpost) join_rows<S>(of[c].dpost, of[c], d.dpost, g.D, joint);
+    if (d.dgate) join_rows<S>(of[c].dgate, of[c], d.dgate, g.D, joint);
+  }
+}
+
+// Rows of any length: the row's sums, then its gradients, from two readings of it; c1 is kept for
+// the sums over the rows, which another kernel makes.
+template <int kR, int kY, bool kPost>
+struct GradAt {
+  float v[8], dx[8], y[8], w[8], post[8], gate[8];
+  GradPart p;
+  __device__ __forceinline__ void load(const NormArgs& g, const NormGradArgs& d, const Drop& drop, int64_t m, int64_t col,
+                                       int valid, float iv, float iy, float (&s)[kPost ? 3 : 1]) {
+    float dr[8] = {};
+    load8<kR>(g.r, m * g.ld_r + col, valid, v);
+    load8<kY>(d.dx, m * d.ld_dx + col, valid, dx);
+    if (d.dr) load8<kR>(d.dr, m * d.ld_dr + col, valid, dr);
+    load8_any(kY, g.y, m * g.ld_y + col, valid, y);
+    load8_any(g.w_type, g.w, col, valid, w);
+    load8_any(g.post_type, g.post, col, valid, post);
+    load8_any(g.gate_type, g.gate, m * g.ld_gate + col, valid, gate);
+    p.kept = kept_of(drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8));
+    grad_sums<kPost>(drop, iv, iy, v, y, dx, dr, w, post, gate, p, s);
+  }
+};
+
+template <int kR, int kY, bool kPost>
+__global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormGradArgs d) {
+  constexpr int kN = kPost ? 3 : 1;
+  using Sum = RowSum<kLong, kN, kLong>;
+  __shared__ typename Sum::Room room;
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  int turn = 0;
+  for (int64_t m = blockIdx.x; m < g.M; m += gridDim.x) {
+    const float iv = g.stats[m], iy = kPost ? g.stats[g.M + m] : 1.0f;
+    float s[kN] = {};
+    for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
+      GradAt<kR, kY, kPost> a;
+      a.load(g, d, drop, m, col, g.D - col < 8 ? (int)(g.D - col) : 8, iv, iy, s);
+    }
+    Sum::run(s, room, turn);
+    const float c1 = s[0] / (float)g.D;
+    float c2 = 0.0f;
+    if constexpr (kPost) c2 = (s[1] - c1 * s[2]) / (float)g.D;
+    if (threadIdx.x == 0) d.c1[m] = c1;
+    for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
+      const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
+      GradAt<kR, kY, kPost> a;
+      float none[kN] = {}, t[8], dz[8], dy[8], dg[8];
+      a.load(g, d, drop, m, col, valid, iv, iy, none);
+      grad_values<kPost>(drop, a.p, iv, iy, c1, c2, a.post, a.gate, t, dz, dy, dg);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] *= g.scale;
+      if (d.dr_out) store8<kR>(d.dr_out, m * d.ld_dr_out + col, valid, t);
+      if (d.dy) store8<kY>(d.dy, m * d.ld_dy + col, valid, dy);
+      if (d.dgates) store8<kY>(d.dgates, m * d.ld_dgates + col, valid, dg);
+    }
+  }
+}
+
+// The sums over the rows blockIdx.x, + gridDim.x, ..  for the columns of blockIdx.y, from c1.
+template <int kR, int kY, bool kPost>
+__global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormArgs g, NormGradArgs d) {
+  const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
+  const int64_t col = 8 * ((int64_t)blockIdx.y * kThreads + threadIdx.x);
+  if (col >= g.D) return;
+  const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
+  float dw[8] = {}, dpost[8] = {}, dgate[8] = {};
+  for (int64_t m = blockIdx.x; m < g.M; m += gridDim.x) {
+    const float iv = g.stats[m], iy = kPost ? g.stats[g.M + m] : 1.0f;
+    GradAt<kR, kY, kPost> a;
+    float none[kPost ? 3 : 1] = {}, t[8], dz[8], dy[8], dg[8];
+    a.load(g, d, drop, m, col, valid, iv, iy, none);
+    grad_values<kPost>(drop, a.p, iv, iy, d.c1[m], 0.0f, a.post, a.gate, t, dz, dy, dg);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw[j] = fmaf(a.dx[j], a.p.vh[j], dw[j]);
+      dpost[j] = fmaf(dz[j], a.p.yh[j], dpost[j]);
+      dgate[j] += dg[j];
+    }
+  }
+  const int64_t to = (int64_t)blockIdx.x * g.D + col;
+  if (d.dw) store8<FP64EMU_F32>(d.dw, to, valid, dw);
+  if (kPost && d.dpost) store8<FP64EMU_F32>(d.dpost, to, valid, dpost);
+  if (d.dgate) store8<FP64EMU_F32>(d.dgate, to, valid, dgate);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+// Calls fn with the launch shape of rows of D elements, or with no shape (void) past the registers.
+template <class Fn>
+void for_rows(int64_t D, const Fn& fn) {
+  if (D <= 128) fn(RowShape<16>{});
+  else if (D <= 512) fn(RowShape<64>{});
+  else if (D <= 1024) fn(RowShape<128>{});
+  else if (D <= 2048) fn(RowShape<256>{});
+  else if (D <= 4096) fn(RowShape<512>{});
+  else fn(RowShape<1024>{});
+}
+constexpr int64_t kMaxHeld = 8192;           // elements of a row that stay in registers
+
+int64_t rows_a_group(int64_t D) {
+  int64_t rows = 1;
+  if (D <= kMaxHeld) for_rows(D, [&](auto s) { rows = decltype(s)::kRows; });
+  return rows;
+}
+
+// Work groups of a forward pass: each CU's threads eight times over.
+int64_t norm_groups(int64_t M, int64_t D) {
+  const int64_t rows = rows_a_group(D);
+  return std::min<int64_t>((M + rows - 1) / rows, 4096);
+}
+// Of a gradient, which leaves D floats for each group and weight.
+int64_t grad_groups(int64_t M, int64_t D) {
+  const int64_t rows = rows_a_group(D);
+  return std::min<int64_t>((M + rows - 1) / rows, 512);
+}
+
+template <int kR, int kY>
+int launch_norm(const NormArgs& g, bool tiles, hipStream_t s) {
+  NormArgs rows = g;
+  if (tiles) {                               // the statistics alone
+    rows.out = rows.x = nullptr;
+    rows.rows = Out8{};
+  }
+  const unsigned groups = (unsigned)norm_groups(g.M, g.D);
+  if (g.D > kMaxHeld) {
+    norm_long_kernel<kR, kY><<<groups, kLong, 0, s>>>(rows);
+  } else {
+    for_rows(g.D, [&](auto shape) {
+      using S = decltype(shape);
+      norm_rows_kernel<kR, kY, S><<<groups, S::kGroup, 0, s>>>(rows);
+    });
+  }
+  if (int st = check_hip(hipGetLastError(), "norm_f8 launch")) return st;
+  if (!tiles) return FP64EMU_OK;
+  norm_tile_kernel<kR, kY><<<(unsigned)((g.M + kBlk - 1) / kBlk * g.blocks), kThreads, 0, s>>>(g);
+  return check_hip(hipGetLastError(), "norm_f8 launch");
+}
+
+template <int kR, int kY, bool kPost>
+int launch_grad(const NormArgs& g, const NormGradArgs& d, hipStream_t s) {
+  const unsigned groups = (unsigned)grad_groups(g.M, g.D);
+  if (g.D > kMaxHeld) {
+    norm_grad_long_kernel<kR, kY, kPost><<<(unsigned)norm_groups(g.M, g.D), kLong, 0, s>>>(g, d);
+    if (int st = check_hip(hipGetLastError(), "norm_f8_backward launch")) return st;
+    const unsigned strips = (unsigned)((g.D + 8 * kThreads - 1) / (8 * kThreads));
+    norm_grad_columns_kernel<kR, kY, kPost><<<dim3(groups, strips), kThreads, 0, s>>>(g, d);
+  } else {
+    for_rows(g.D, [&](auto shape) {
+      using S = decltype(shape);
+      if constexpr (S::kT == 1024) norm_grad_kernel<kR, kY, RowShape<512>, 2, kPost><<<groups, 512, 0, s>>>(g, d);
+      else norm_grad_kernel<kR, kY, S, 1, kPost><<<groups, S::kGroup, 0, s>>>(g, d);
+    });
+  }
+  return check_hip(hipGetLastError(), "norm_f8_backward launch");
+}
+
+int check_norm(const fp64emu_norm_t* p) {
+  if (!p) return invalid("norm must not be NULL");
+  if (p->M < 0 || p->D < 0) return invalid("shapes must be non-negative");
+  if (p->M >= 1ll << 40 || p->D >= 1ll << 27) return invalid("shapes must be below 2^40 rows of 2^27 elements");
+  if (!known_dtype(p->r_dtype) || !known_dtype(p->y_dtype) || !known_dtype(p->w_dtype) ||
+      !known_dtype(p->post_dtype) || !known_dtype(p->gate_dtype))
+    return invalid("dtype must be FP64EMU_F32, FP64EMU_BF16 or FP64EMU_F16");
+  if (p->y_dtype != p->r_dtype && p->r_dtype != FP64EMU_F32)
+    return invalid("y's dtype must be r's, or r's FP64EMU_F32");
+  if (!(p->eps > 0.0f)) return invalid("eps must be positive");
+  if (p->drop < 0 || p->drop > 65535) return invalid("drop must be in 0 .. 65535");
+  if (p->M == 0 || p->D == 0) return FP64EMU_OK;              // (whose operands have no address)
+  if (!p->y && (p->post || p->gate || p->drop)) return invalid("post, gate and drop need y");
+  if (p->drop && !p->rng) return invalid("drop needs rng");
+  return FP64EMU_OK;
+}
+
+// Of a call with something to do.
+int norm_args(const fp64emu_norm_t* p, NormArgs* g) {
+  if (!p->r || !p->w) return invalid("null operand pointer");
+  if (p->ld_r < p->D || (p->y && p->ld_y < p->D)) return invalid("rows are shorter than D");
+  if (p->gate && p->ld_gate != 0 && p->ld_gate < p->D) return invalid("rows of gate are shorter than D");
+  *g = NormArgs{};
+  g->r = p->r;
+  g->y = p->y;
+  g->gate = p->gate;
+  g->w = p->w;
+  g->post = p->post;
+  g->rng = p->rng;
+  g->M = p->M;
+  g->D = p->D;
+  g->ld_r = p->ld_r;
+  g->ld_y = p->ld_y;
+  g->ld_gate = p->gate ? p->ld_gate : 0;
+  g->blocks = (p->D + kBlk - 1) / kBlk;
+  g->w_type = p->w_dtype;
+  g->post_type = p->post_dtype;
+  g->gate_type = p->gate_dtype;
+  g->threshold = (uint32_t)p->drop;
+  g->scale = p->scale;
+  g->eps = p->eps;
+  if (g->ld_gate && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
+  return FP64EMU_OK;
+}
+
+// Calls fn with r's and y's types as constants.
+template <class Fn>
+int for_types(int r, int y, const Fn& fn) {
+#define FP64EMU_TYPES(R, Y) \
+  if (r == R && y == Y) return fn(std::integral_constant<int, R>{}, std::integral_constant<int, Y>{});
+  FP64EMU_TYPES(FP64EMU_F32, FP64EMU_F32)
+  FP64EMU_TYPES(FP64EMU_BF16, FP64EMU_BF16)
+  FP64EMU_TYPES(FP64EMU_F16, FP64EMU_F16)
+  FP64EMU_TYPES(FP64EMU_F32, FP64EMU_BF16)
+  FP64EMU_TYPES(FP64EMU_F32, FP64EMU_F16)
+#undef FP64EMU_TYPES
+  return invalid("dtype");
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x, int64_t ld_x, float* stats,
+                    const fp64emu_f8_t* rows, const fp64emu_f8_t* cols, fp64emu_stream_t stream) {
+  if (int st = check_norm(p)) return st;
+  for (const fp64emu_f8_t* f : {rows, cols})
+    if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("outputs are e4m3 with scales by rows");
+  if (p->M == 0 || p->D == 0) return FP64EMU_OK;
+  if (!out && !x && !rows && !cols && !stats) return invalid("no output asked for");
+  if (out && !p->y) return invalid("a new stream needs y");
+  if (cols && !stats) return invalid("columns need stats");
+  if (cols && x) return invalid("columns come without x in its plain form");
+  if ((out && ld_out < p->D) || (x && ld_x < p->D)) return invalid("rows are shorter than D");
+  NormArgs g;
+  if (int st = norm_args(p, &g)) return st;
+  if (int st = out8(rows, p->D, &g.rows)) return st;
+  if (int st = out8(cols, p->M, &g.cols)) return st;
+  g.out = out;
+  g.ld_out = ld_out;
+  g.x = x;
+  g.ld_x = ld_x;
+  g.stats = stats;
+  if (cols && (p->M + kBlk - 1) / kBlk > ((1ll << 31) / kThreads) / g.blocks) return invalid("operand too large for one launch");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {
+    return launch_norm<decltype(r)::value, decltype(y)::value>(g, cols != nullptr, s);
+  });
+}
+
+size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p) {
+  if (check_norm(p) || p->M == 0 || p->D == 0) return 0;
+  const int64_t groups = grad_groups(p->M, p->D);
+  const size_t parts = groups > 1 ? 4 * (size_t)kMaxSums * (size_t)(groups * p->D) : 0;
+  return parts + (p->D > kMaxHeld ? 4 * (size_t)p->M : 0);
+}
+
+int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d, void* workspace,
+                             size_t workspace_bytes, fp64emu_stream_t stream) {
+  if (int st = check_norm(p)) return st;
+  if (!d) return invalid("gradient must not be NULL");
+  if (p->M > 0 && !p->y && (d->dy || d->dpost || d->dgate || d->dgates)) return invalid("gradients of what is absent");
+  if ((d->dpost && !p->post) || ((d->dgate || d->dgates) && !p->gate)) return invalid("gradients of what is absent");
+  if (d->dgate && d->dgates) return invalid("gate's gradient is a row or a matrix");
+  if (d->dgates && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
+  if (p->D == 0) return FP64EMU_OK;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  float* const sums[kMaxSums] = {d->dw, d->dpost, d->dgate};
+  Sums all{};
+  int count = 0;
+  if (p->M == 0) {                           // sums of nothing
+    for (float* to : sums)
+      if (to) all.out[count++] = to;
+    all.D = p->D;
+    return launch_sums(all, count, s);
+  }
+  if (!d->dx || !stats) return invalid("null operand pointer");
+  if (d->ld_dx < p->D || (d->dr && d->ld_dr < p->D) || (d->dr_out && d->ld_dr_out < p->D) || (d->dy && d->ld_dy < p->D) ||
+      (d->dgates && d->ld_dgates < p->D))
+    return invalid("rows are shorter than D");
+  NormArgs g;
+  if (int st = norm_args(p, &g)) return st;
+  const size_t need = fp64emu_norm_f8_backward_workspace(p);
+  if (need && (!workspace || workspace_bytes < need))
+    return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_norm_f8_backward_workspace");
+  if (need && !multiple(workspace, 4)) return invalid("workspace must be 4-byte aligned");
+  g.stats = const_cast<float*>(stats);
+  NormGradArgs a{};
+  a.dx = d->dx;
+  a.dr = d->dr;
+  a.ld_dx = d->ld_dx;
+  a.ld_dr = d->ld_dr;
+  a.dr_out = d->dr_out;
+  a.dy = d->dy;
+  a.dgates = d->dgates;
+  a.ld_dr_out = d->ld_dr_out;
+  a.ld_dy = d->ld_dy;
+  a.ld_dgates = d->ld_dgates;
+  const int64_t groups = grad_groups(p->M, p->D);
+  float* room = static_cast<float*>(workspace);
+  float** const to[kMaxSums] = {&a.dw, &a.dpost, &a.dgate};
+  for (int i = 0; i < kMaxSums; ++i) {
+    *to[i] = sums[i];
+    if (!sums[i] || groups == 1) continue;
+    *to[i] = room + (int64_t)count * groups * p->D;
+    all.part[count] = *to[i];
+    all.out[count++] = sums[i];
+  }
+  if (p->D > kMaxHeld) a.c1 = room + (groups > 1 ? kMaxSums * groups * p->D : 0);
+  all.groups = groups;
+  all.D = p->D;
+  const int st = for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {
+    return p->post ? launch_grad<decltype(r)::value, decltype(y)::value, true>(g, a, s)
+                   : launch_grad<decltype(r)::value, decltype(y)::value, false>(g, a, s);
+  });
+  return st ? st : launch_sums(all, count, s);
+}
+
+}  // extern "C"

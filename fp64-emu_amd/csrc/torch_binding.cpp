@@ -306,8 +306,56 @@ fp64emu_f8_t kept_of(const at::Tensor& like, const at::Tensor& hq, const at::Ten
 
 constexpr int64_t kPlain = 0, kRows = 1, kBoth = 2;    // what form an activation's result takes
 
+using Maybe = std::optional<at::Tensor>;
+
+// What a product's sums go through; keep: undefined or where bias makes them.
+struct EpilogueOf {
+  Maybe bias, residual;
+  int act = FP64EMU_ACT_NONE;
+  at::Tensor keep;
+};
+
+// A tensor that goes with `like`, on its device.
+void check_with(const at::Tensor& t, const at::Tensor& like, const char* what) {
+  TORCH_CHECK(t.device() == like.device(), what, " must be on the same device as the other operands");
+}
+
+// The C form of e for a product of out's shape; hold keeps what it points to.
+fp64emu_epilogue_t epilogue_of(const EpilogueOf& e, const at::Tensor& out, std::vector<at::Tensor>& hold) {
+  fp64emu_epilogue_t f{};
+  const int64_t d = out.dim(), N = out.size(d - 1);
+  f.act = e.act;
+  f.bias_dtype = FP64EMU_F32;
+  if (e.bias) {
+    check_with(*e.bias, out, "bias");
+    const int64_t b = e.bias->dim();
+    TORCH_CHECK(b >= 1 && e.bias->size(b - 1) == N && (b == 1 || (b == 2 && d == 3 && e.bias->size(0) == out.size(0))),
+                d == 3 ? "expect bias as [N] or [batch, N]" : "expect bias as [N]");
+    hold.push_back(e.bias->contiguous());
+    f.bias = hold.back().data_ptr();
+    f.bias_dtype = dtype_of(hold.back());
+    f.bias_stride = b == 2 ? N : 0;
+  }
+  if (e.residual) {
+    check_with(*e.residual, out, "residual");
+    TORCH_CHECK(e.residual->sizes() == out.sizes(), "residual must have the product's shape");
+    TORCH_CHECK(e.residual->scalar_type() == out.scalar_type(), "residual must have the product's dtype");
+    hold.push_back(in_rows(*e.residual));
+    const at::Tensor& r = hold.back();
+    f.residual = r.data_ptr();
+    f.ld_residual = row_stride(r);
+    f.stride_residual = d == 3 && r.size(0) > 1 ? r.stride(0) : 0;
+  }
+  if (e.keep.defined()) {
+    f.keep = e.keep.data_ptr();
+    f.ld_keep = row_stride(e.keep);
+    f.stride_keep = d == 3 && e.keep.size(0) > 1 ? e.keep.stride(0) : 0;
+  }
+  return f;
+}
+
 void product_f8(const at::Tensor& out, const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
-                const at::Tensor& sB, bool accumulate) {
+                const at::Tensor& sB, bool accumulate, const EpilogueOf* epilogue = nullptr) {
   TORCH_CHECK(A.dim() >= 2 && B.dim() >= 2 && out.dim() >= 2, "A, B and out are all 2-D or all 3-D");
   const at::Tensor qa = in_rows(A), qb = in_rows(B);
   fp64emu_mm_f8_t p{};
@@ -334,10 +382,14 @@ void product_f8(const at::Tensor& out, const at::Tensor& A, const at::Tensor& sA
   p.stride_o = d == 3 && p.batch > 1 ? out.stride(0) : 0;
   p.accumulate = accumulate;
   const c10::DeviceGuard guard(A.device());
-  const size_t bytes = fp64emu_mm_f8_workspace(&p);
+  std::vector<at::Tensor> hold;
+  fp64emu_epilogue_t e{};
+  if (epilogue) e = epilogue_of(*epilogue, out, hold);
+  const fp64emu_epilogue_t* ep = epilogue ? &e : nullptr;
+  const size_t bytes = fp64emu_mm_f8_epilogue_workspace(&p, ep);
   at::Tensor ws;
   if (bytes) ws = workspace(A, bytes);
-  check_status(fp64emu_mm_f8(&p, bytes ? ws.data_ptr() : nullptr, bytes, current_stream(A)));
+  check_status(fp64emu_mm_f8_epilogue(&p, ep, bytes ? ws.data_ptr() : nullptr, bytes, current_stream(A)));
 }
 
 }  // namespace
@@ -458,6 +510,233 @@ std::vector<at::Tensor> fp64_emu_swiglu_f8_backward(const at::Tensor& dy, const 
   return out;
 }
 
+// act(A B^T + bias) + residual as a new tensor of `dtype`; with keep also A B^T + bias.
+std::vector<at::Tensor> fp64_emu_mm_f8_epilogue(const at::Tensor& A, const at::Tensor& sA, const at::Tensor& B,
+                                                const at::Tensor& sB, at::ScalarType dtype, const Maybe& bias,
+                                                int64_t act, const Maybe& residual, bool keep) {
+  const int64_t d = A.dim();
+  TORCH_CHECK((d == 2 || d == 3) && B.dim() == d, "A, B and out are all 2-D or all 3-D");
+  const at::TensorOptions on = A.options().dtype(dtype);
+  const auto made = [&] {
+    return d == 3 ? at::empty({A.size(0), A.size(1), B.size(1)}, on) : at::empty({A.size(0), B.size(0)}, on);
+  };
+  std::vector<at::Tensor> out{made()};
+  EpilogueOf e;
+  e.bias = bias;
+  e.residual = residual;
+  e.act = (int)act;
+  if (keep) {
+    e.keep = made();
+    out.push_back(e.keep);
+  }
+  product_f8(out[0], A, sA, B, sB, false, &e);
+  return out;
+}
+
+namespace {
+
+// Outputs of a matrix [M, D] like v, plain, by rows or both ways.
+struct Asked {
+  at::Tensor x;
+  std::optional<NewF8> rows, cols;
+  std::vector<at::Tensor> out;
+  Asked(const at::Tensor& v, int64_t M, int64_t D, int64_t quant) {
+    if (quant == kPlain) {
+      x = at::empty({M, D}, v.options());
+      out.push_back(x);
+      return;
+    }
+    rows.emplace(v, nullptr, M, D, M, blocks_of(D), at::kFloat8_e4m3fn, false);
+    out.insert(out.end(), {rows->q, rows->s});
+    if (quant == kBoth) {
+      cols.emplace(v, nullptr, D, M, D, blocks_of(M), at::kFloat8_e4m3fn, false);
+      out.insert(out.end(), {cols->q, cols->s});
+    }
+  }
+  void* plain() const { return x.defined() ? x.data_ptr() : nullptr; }
+  const fp64emu_f8_t* by_rows() const { return rows ? &rows->f : nullptr; }
+  const fp64emu_f8_t* by_cols() const { return cols ? &cols->f : nullptr; }
+};
+
+void check_quant(int64_t quant) { TORCH_CHECK(quant >= kPlain && quant <= kBoth, "quant: 0 plain, 1 rows, 2 both"); }
+
+void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// The seed and offset, with drop > 0.
+const int64_t* rng_of(const Maybe& rng, int64_t drop, const at::Tensor& like) {
+  TORCH_CHECK(drop >= 0 && drop <= 65535, "drop: 0 .. 65535 of 65536");
+  if (drop == 0) return nullptr;
+  TORCH_CHECK(rng.has_value(), "a dropout needs rng, its seed and offset");
+  check_with(*rng, like, "rng");
+  TORCH_CHECK(rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous(),
+              "rng: two int64, the seed and the offset");
+  return rng->data_ptr<int64_t>();
+}
+
+// The C form of the norms around a block; hold keeps what it points to.
+fp64emu_norm_t norm_of(const at::Tensor& r, const at::Tensor& w, const Maybe& y, const Maybe& post, const Maybe& gate,
+                       double scale, int64_t drop, const Maybe& rng, double eps, std::vector<at::Tensor>& hold) {
+  TORCH_CHECK(r.dim() == 2, "expect r as [M, D]");
+  const int64_t M = r.size(0), D = r.size(1);
+  fp64emu_norm_t p{};
+  const auto rows = [&](const at::Tensor& t, const char* what, const void** to, int64_t* ld, int* type) {
+    check_with(t, r, what);
+    TORCH_CHECK(t.sizes() == r.sizes(), what, " must be [M, D] as r is");
+    hold.push_back(in_rows(t));
+    check_rows(hold.back(), what);
+    *to = hold.back().data_ptr();
+    *ld = row_stride(hold.back());
+    *type = dtype_of(t);
+  };
+  const auto vec = [&](const at::Tensor& t, const char* what, const void** to, int* type) {
+    check_with(t, r, what);
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == D, what, " must be [D]");
+    hold.push_back(t.contiguous());
+    *to = hold.back().data_ptr();
+    *type = dtype_of(t);
+  };
+  rows(r, "r", &p.r, &p.ld_r, &p.r_dtype);
+  vec(w, "w", &p.w, &p.w_dtype);
+  p.y_dtype = p.r_dtype;
+  if (y) rows(*y, "y", &p.y, &p.ld_y, &p.y_dtype);
+  TORCH_CHECK(y || (!post && !gate && drop == 0), "post, gate and a dropout are of y");
+  TORCH_CHECK(p.y_dtype == p.r_dtype || p.r_dtype == FP64EMU_F32, "y must have r's dtype, or r be float32");
+  if (post) vec(*post, "post", &p.post, &p.post_dtype);
+  if (gate && gate->dim() == 1) {
+    vec(*gate, "gate", &p.gate, &p.gate_dtype);
+  } else if (gate) {
+    rows(*gate, "gate", &p.gate, &p.ld_gate, &p.gate_dtype);
+    TORCH_CHECK(p.gate_dtype == p.y_dtype, "a gate for each row must have y's dtype");
+  }
+  p.rng = rng_of(rng, drop, r);
+  p.M = M;
+  p.D = D;
+  p.drop = (int)drop;
+  p.scale = (float)scale;
+  p.eps = (float)eps;
+  return p;
+}
+
+}  // namespace
+
+// dy act'(h): plain, its (q, s), or (q, s, qt, st); with bias then its sum over the rows.
+std::vector<at::Tensor> fp64_emu_act_f8_backward(const at::Tensor& dy, const Maybe& h, int64_t act, int64_t quant,
+                                                 bool bias) {
+  TORCH_CHECK(dy.dim() == 2, "expect dy as [M, N]");
+  check_quant(quant);
+  TORCH_CHECK(act == FP64EMU_ACT_NONE || h.has_value(), "an activation's gradient needs h");
+  const at::Tensor v = in_rows(dy);
+  check_rows(v, "dy");
+  const int dtype = dtype_of(v);
+  const int64_t M = v.size(0), N = v.size(1);
+  at::Tensor hv;
+  if (act != FP64EMU_ACT_NONE) {
+    check_with(*h, v, "h");
+    TORCH_CHECK(h->sizes() == v.sizes() && h->scalar_type() == v.scalar_type(), "h must have dy's shape and dtype");
+    hv = in_rows(*h);
+  }
+  const c10::DeviceGuard guard(v.device());
+  Asked a(v, M, N, quant);
+  at::Tensor db, ws;
+  size_t bytes = 0;
+  if (bias) {
+    db = at::empty({N}, v.options().dtype(at::kFloat));
+    a.out.push_back(db);
+    bytes = fp64emu_act_f8_backward_workspace(M, N, quant == kBoth);
+    if (bytes) ws = workspace(v, bytes);
+  }
+  check_status(fp64emu_act_f8_backward(v.data_ptr(), pointer(hv), dtype, (int)act, M, N, row_stride(v),
+                                       hv.defined() ? row_stride(hv) : 0, a.plain(), N, a.by_rows(), a.by_cols(),
+                                       bias ? db.data_ptr<float>() : nullptr, pointer(ws), bytes, current_stream(v)));
+  return a.out;
+}
+
+// x dropped: plain, its (q, s), or (q, s, qt, st).
+std::vector<at::Tensor> fp64_emu_dropout_f8(const at::Tensor& x, int64_t drop, const Maybe& rng, int64_t quant) {
+  TORCH_CHECK(x.dim() == 2, "expect x as [M, K]");
+  check_quant(quant);
+  const at::Tensor v = in_rows(x);
+  check_rows(v, "x");
+  const int dtype = dtype_of(v);
+  const int64_t M = v.size(0), K = v.size(1);
+  const int64_t* state = rng_of(rng, drop, v);
+  const c10::DeviceGuard guard(v.device());
+  Asked a(v, M, K, quant);
+  check_status(fp64emu_dropout_f8(v.data_ptr(), dtype, M, K, row_stride(v), (int)drop, state, a.plain(), K, a.by_rows(),
+                                  a.by_cols(), current_stream(v)));
+  return a.out;
+}
+
+// With y the new stream; then x, its (q, s), or (q, s, qt, st); then, with keep, the rows' statistics.
+std::vector<at::Tensor> fp64_emu_norm_f8(const at::Tensor& r, const at::Tensor& w, const Maybe& y, const Maybe& post,
+                                         const Maybe& gate, double scale, int64_t drop, const Maybe& rng, int64_t quant,
+                                         bool keep, double eps) {
+  check_quant(quant);
+  TORCH_CHECK(r.is_cuda(), "r must be on a GPU");
+  std::vector<at::Tensor> hold;
+  const fp64emu_norm_t p = norm_of(r, w, y, post, gate, scale, drop, rng, eps, hold);
+  const c10::DeviceGuard guard(r.device());
+  std::vector<at::Tensor> out;
+  at::Tensor stream, stats;
+  if (y) {
+    stream = at::empty({p.M, p.D}, r.options());
+    out.push_back(stream);
+  }
+  Asked a(y ? *y : r, p.M, p.D, quant);
+  out.insert(out.end(), a.out.begin(), a.out.end());
+  if (keep || quant == kBoth) stats = at::empty({post ? 2 : 1, p.M}, r.options().dtype(at::kFloat));
+  if (keep) out.push_back(stats);
+  check_status(fp64emu_norm_f8(&p, pointer(stream), p.D, a.plain(), p.D,
+                               stats.defined() ? stats.data_ptr<float>() : nullptr, a.by_rows(), a.by_cols(),
+                               current_stream(r)));
+  return out;
+}
+
+// Its gradient: dr, then, of what is there, dy, dw, dpost and dgate.
+std::vector<at::Tensor> fp64_emu_norm_f8_backward(const at::Tensor& dx, const Maybe& dr, const at::Tensor& r,
+                                                  const at::Tensor& w, const at::Tensor& stats, const Maybe& y,
+                                                  const Maybe& post, const Maybe& gate, double scale, int64_t drop,
+                                                  const Maybe& rng) {
+  TORCH_CHECK(r.is_cuda(), "r must be on a GPU");
+  std::vector<at::Tensor> hold;
+  const fp64emu_norm_t p = norm_of(r, w, y, post, gate, scale, drop, rng, 1.0, hold);
+  const at::Tensor& like = y ? *y : r;
+  fp64emu_norm_grad_t d{};
+  const auto rows = [&](const at::Tensor& t, at::ScalarType type, const char* what, int64_t* ld) -> const void* {
+    check_with(t, r, what);
+    TORCH_CHECK(t.sizes() == r.sizes() && t.scalar_type() == type, what, " must have the shape and dtype of its value");
+    hold.push_back(in_rows(t));
+    check_rows(hold.back(), what);
+    *ld = row_stride(hold.back());
+    return hold.back().data_ptr();
+  };
+  d.dx = rows(dx, like.scalar_type(), "dx", &d.ld_dx);
+  if (dr) d.dr = rows(*dr, r.scalar_type(), "dr", &d.ld_dr);
+  check_with(stats, r, "stats");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == (post ? 2 : 1) &&
+                  stats.size(1) == p.M && stats.is_contiguous(),
+              "stats: what the forward pass kept, float32 [", post ? 2 : 1, ", M]");
+  const c10::DeviceGuard guard(r.device());
+  const at::TensorOptions on = r.options();
+  std::vector<at::Tensor> out;
+  const auto made = [&](at::IntArrayRef shape, at::ScalarType type) {
+    out.push_back(at::empty(shape, on.dtype(type)));
+    return out.back().data_ptr();
+  };
+  d.ld_dr_out = d.ld_dy = d.ld_dgates = p.D;
+  d.dr_out = made({p.M, p.D}, r.scalar_type());
+  if (y) d.dy = made({p.M, p.D}, y->scalar_type());
+  d.dw = static_cast<float*>(made({p.D}, at::kFloat));
+  if (post) d.dpost = static_cast<float*>(made({p.D}, at::kFloat));
+  if (gate && gate->dim() == 1) d.dgate = static_cast<float*>(made({p.D}, at::kFloat));
+  else if (gate) d.dgates = made({p.M, p.D}, gate->scalar_type());
+  const size_t bytes = fp64emu_norm_f8_backward_workspace(&p);
+  at::Tensor ws;
+  if (bytes) ws = workspace(r, bytes);
+  check_status(fp64emu_norm_f8_backward(&p, stats.data_ptr<float>(), &d, pointer(ws), bytes, current_stream(r)));
+  return out;
+}
+
 TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_maxp() -> int", &fp64_emu_maxp);
   ops.def("fp64_emu_mm(Tensor! out, Tensor A, Tensor B, Tensor primes_cpu, Tensor inv_cpu, Tensor mu_cpu, bool exact, int bits=53, bool use_corr=True) -> ()");
@@ -468,6 +747,11 @@ TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_quant_f8(Tensor x, bool rows, bool cols, bool tiles, ScalarType fmt) -> Tensor[]");
   ops.def("fp64_emu_mm_f8(Tensor A, Tensor sA, Tensor B, Tensor sB, ScalarType dtype) -> Tensor");
   ops.def("fp64_emu_mm_f8_out(Tensor(a!) out, Tensor A, Tensor sA, Tensor B, Tensor sB, bool accumulate) -> ()");
+  ops.def("fp64_emu_mm_f8_epilogue(Tensor A, Tensor sA, Tensor B, Tensor sB, ScalarType dtype, Tensor? bias, int act, Tensor? residual, bool keep) -> Tensor[]");
+  ops.def("fp64_emu_act_f8_backward(Tensor dy, Tensor? h, int act, int quant, bool bias) -> Tensor[]");
+  ops.def("fp64_emu_dropout_f8(Tensor x, int drop, Tensor? rng, int quant) -> Tensor[]");
+  ops.def("fp64_emu_norm_f8(Tensor r, Tensor w, Tensor? y, Tensor? post, Tensor? gate, float scale, int drop, Tensor? rng, int quant, bool keep, float eps) -> Tensor[]");
+  ops.def("fp64_emu_norm_f8_backward(Tensor dx, Tensor? dr, Tensor r, Tensor w, Tensor stats, Tensor? y, Tensor? post, Tensor? gate, float scale, int drop, Tensor? rng) -> Tensor[]");
   ops.def("fp64_emu_swiglu_f8(Tensor h, int quant, bool keep) -> Tensor[]");
   ops.def("fp64_emu_swiglu_f8_backward(Tensor dy, Tensor hq, Tensor hs, int quant) -> Tensor[]");
 }
@@ -482,6 +766,11 @@ TORCH_LIBRARY_IMPL(fp64_emu, CUDA, ops) {
   ops.impl("fp64_emu_quant_f8", &fp64_emu_quant_f8);
   ops.impl("fp64_emu_mm_f8", &fp64_emu_mm_f8);
   ops.impl("fp64_emu_mm_f8_out", &fp64_emu_mm_f8_out);
+  ops.impl("fp64_emu_mm_f8_epilogue", &fp64_emu_mm_f8_epilogue);
+  ops.impl("fp64_emu_act_f8_backward", &fp64_emu_act_f8_backward);
+  ops.impl("fp64_emu_dropout_f8", &fp64_emu_dropout_f8);
+  ops.impl("fp64_emu_norm_f8", &fp64_emu_norm_f8);
+  ops.impl("fp64_emu_norm_f8_backward", &fp64_emu_norm_f8_backward);
   ops.impl("fp64_emu_swiglu_f8", &fp64_emu_swiglu_f8);
   ops.impl("fp64_emu_swiglu_f8_backward", &fp64_emu_swiglu_f8_backward);
 }
@@ -516,7 +805,9 @@ void mm_f8_out_written(c10::DispatchKeySet keys, at::Tensor& out, const at::Tens
 }  // namespace
 
 TORCH_LIBRARY_IMPL(fp64_emu, Autograd, ops) {
-  for (const char* name : {"fp64_emu_quant_f8", "fp64_emu_mm_f8", "fp64_emu_swiglu_f8", "fp64_emu_swiglu_f8_backward"})
+  for (const char* name : {"fp64_emu_quant_f8", "fp64_emu_mm_f8", "fp64_emu_swiglu_f8", "fp64_emu_swiglu_f8_backward",
+                           "fp64_emu_mm_f8_epilogue", "fp64_emu_act_f8_backward", "fp64_emu_dropout_f8",
+                           "fp64_emu_norm_f8", "fp64_emu_norm_f8_backward"})
     ops.impl(name, torch::autograd::autogradNotImplementedFallback());
   ops.impl("fp64_emu_mm_f8_out", &mm_f8_out_autograd);
 }

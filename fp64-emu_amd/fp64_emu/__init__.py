@@ -24,7 +24,8 @@ import torch
 
 from ._ops import ops
 from . import _meta  # noqa: F401  (fake kernels for torch.compile)
-from .f8 import (bmm_f8, linear_f8, mm_f8, quant_f8, quant_f8_tiles, swiglu_ckpt_f8, swiglu_f8,
+from .f8 import (act_f8_backward, bmm_f8, dropout_f8, linear_f8, mm_f8, norm_f8, norm_f8_backward, quant_f8,
+                 quant_f8_tiles, residual_norm_f8, seeded_dropout_f8, swiglu_ckpt_f8, swiglu_f8,
                  swiglu_f8_backward)
 
 # Pairwise-coprime moduli up to the balanced int8 ceiling of 256, largest
@@ -200,4 +201,5 @@ def plan(K: int, bits: int = 53) -> int:
 
 __all__ = ["mm", "mm_nt", "bmm", "bmm_nt", "mm_timed", "plan", "plan_config", "range_bits",
            "quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",
-           "linear_f8", "swiglu_ckpt_f8"]
+           "linear_f8", "swiglu_ckpt_f8", "act_f8_backward", "dropout_f8", "norm_f8", "norm_f8_backward",
+           "residual_norm_f8", "seeded_dropout_f8"]

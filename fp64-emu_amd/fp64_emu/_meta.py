@@ -67,6 +67,46 @@ def _swiglu_backward(dy, hq, hs, quant):
     return out
 
 
+def _asked(like, M, D, quant):
+    e4m3 = torch.float8_e4m3fn
+    if quant == 0:
+        return [like.new_empty((M, D))]
+    return _f8(like, (), M, D, M, _blocks(D), e4m3) + (_f8(like, (), D, M, D, _blocks(M), e4m3) if quant == 2 else [])
+
+
+def _mm_epilogue(A, sA, B, sB, dtype, bias, act, residual, keep):
+    return [_mm(A, sA, B, sB, dtype) for _ in range(2 if keep else 1)]
+
+
+def _act_backward(dy, h, act, quant, bias):
+    M, N = dy.shape
+    return _asked(dy, M, N, quant) + ([dy.new_empty((N,), dtype=torch.float32)] if bias else [])
+
+
+def _dropout(x, drop, rng, quant):
+    return _asked(x, *x.shape, quant)
+
+
+def _norm(r, w, y, post, gate, scale, drop, rng, quant, keep, eps):
+    M, D = r.shape
+    out = [] if y is None else [r.new_empty((M, D))]
+    out += _asked(r if y is None else y, M, D, quant)
+    return out + ([r.new_empty((1 if post is None else 2, M), dtype=torch.float32)] if keep else [])
+
+
+def _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng):
+    M, D = r.shape
+    out = [r.new_empty((M, D))] + ([] if y is None else [y.new_empty((M, D))])
+    out += [r.new_empty((D,), dtype=torch.float32) for _ in range(1 if post is None else 2)]
+    if gate is not None:
+        out.append(r.new_empty((D,), dtype=torch.float32) if gate.dim() == 1 else gate.new_empty((M, D)))
+    return out
+
+
+for _name, _fake in (("mm_f8_epilogue", _mm_epilogue), ("act_f8_backward", _act_backward), ("dropout_f8", _dropout),
+                     ("norm_f8", _norm), ("norm_f8_backward", _norm_backward)):
+    torch.library.register_fake("fp64_emu::fp64_emu_" + _name)(_fake)
+
 for _name, _fake in (("quant_f8", _quant), ("mm_f8", _mm), ("swiglu_f8", _swiglu),
                      ("swiglu_f8_backward", _swiglu_backward)):
     torch.library.register_fake("fp64_emu::fp64_emu_" + _name)(_fake)

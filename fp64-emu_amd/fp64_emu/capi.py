@@ -27,7 +27,9 @@ EXPORTS = ("fp64emu_maxp", "fp64emu_last_error", "fp64emu_workspace_size",
            "fp64emu_product_workspace", "fp64emu_product", "fp64emu_layout",
            "fp64emu_ddgemm_nt", "fp64emu_probe_mfma", "fp64emu_probe_stream", "fp64emu_quant_f8",
            "fp64emu_mm_f8_workspace", "fp64emu_mm_f8_plan", "fp64emu_mm_f8", "fp64emu_swiglu_f8",
-           "fp64emu_swiglu_f8_backward")
+           "fp64emu_swiglu_f8_backward", "fp64emu_mm_f8_epilogue_workspace", "fp64emu_mm_f8_epilogue",
+           "fp64emu_act_f8_backward_workspace", "fp64emu_act_f8_backward", "fp64emu_dropout_f8",
+           "fp64emu_norm_f8", "fp64emu_norm_f8_backward_workspace", "fp64emu_norm_f8_backward")
 
 NOALLOC_SCRATCH_BYTES = 64 << 20   # FP64EMU_NOALLOC_SCRATCH_BYTES
 
@@ -72,6 +74,27 @@ class MmF8(ctypes.Structure):
     _fields_ = [("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("stride_o", ctypes.c_int64),
                 ("dtype", ctypes.c_int), ("accumulate", ctypes.c_int), ("A", F8), ("B", F8)] + [
                     (n, ctypes.c_int64) for n in ("batch", "M", "N", "K")]
+
+
+class Epilogue(ctypes.Structure):
+    """Mirror of fp64emu_epilogue_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("bias", "residual", "keep")] + [
+        (n, ctypes.c_int64) for n in ("bias_stride", "ld_residual", "stride_residual", "ld_keep", "stride_keep")] + [
+            ("bias_dtype", ctypes.c_int), ("act", ctypes.c_int)]
+
+
+class Norm(ctypes.Structure):
+    """Mirror of fp64emu_norm_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("r", "y", "w", "post", "gate", "rng")] + [
+        (n, ctypes.c_int64) for n in ("M", "D", "ld_r", "ld_y", "ld_gate")] + [
+            (n, ctypes.c_int) for n in ("r_dtype", "y_dtype", "w_dtype", "post_dtype", "gate_dtype", "drop")] + [
+                ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class NormGrad(ctypes.Structure):
+    """Mirror of fp64emu_norm_grad_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dx", "dr", "dr_out", "dy", "dgates", "dw", "dpost", "dgate")] + [
+        (n, ctypes.c_int64) for n in ("ld_dx", "ld_dr", "ld_dr_out", "ld_dy", "ld_dgates")]
 
 
 class MmF8Plan(ctypes.Structure):
@@ -137,6 +160,23 @@ def lib():
     L.fp64emu_swiglu_f8.restype = i32
     L.fp64emu_swiglu_f8_backward.argtypes = [vp, i32, i64, i64, i64, f8, vp, i32, i64, f8, f8, vp]
     L.fp64emu_swiglu_f8_backward.restype = i32
+    mm, epi, norm = ctypes.POINTER(MmF8), ctypes.POINTER(Epilogue), ctypes.POINTER(Norm)
+    L.fp64emu_mm_f8_epilogue_workspace.argtypes = [mm, epi]
+    L.fp64emu_mm_f8_epilogue_workspace.restype = sz
+    L.fp64emu_mm_f8_epilogue.argtypes = [mm, epi, vp, sz, vp]
+    L.fp64emu_mm_f8_epilogue.restype = i32
+    L.fp64emu_act_f8_backward_workspace.argtypes = [i64, i64, i32]
+    L.fp64emu_act_f8_backward_workspace.restype = sz
+    L.fp64emu_act_f8_backward.argtypes = [vp, vp, i32, i32, i64, i64, i64, i64, vp, i64, f8, f8, vp, vp, sz, vp]
+    L.fp64emu_act_f8_backward.restype = i32
+    L.fp64emu_dropout_f8.argtypes = [vp, i32, i64, i64, i64, i32, vp, vp, i64, f8, f8, vp]
+    L.fp64emu_dropout_f8.restype = i32
+    L.fp64emu_norm_f8.argtypes = [norm, vp, i64, vp, i64, vp, f8, f8, vp]
+    L.fp64emu_norm_f8.restype = i32
+    L.fp64emu_norm_f8_backward_workspace.argtypes = [norm]
+    L.fp64emu_norm_f8_backward_workspace.restype = sz
+    L.fp64emu_norm_f8_backward.argtypes = [norm, vp, ctypes.POINTER(NormGrad), vp, sz, vp]
+    L.fp64emu_norm_f8_backward.restype = i32
     _LIB = L
     return L
 

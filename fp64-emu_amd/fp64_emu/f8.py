@@ -1,6 +1,7 @@
 """Matrices in 8-bit floating point with one float32 scale per block of 128:
-the quantiser, products of such matrices, and the gated activation whose
-checkpoint is held so.
+the quantiser, products of such matrices with what follows them in their epilogue,
+the gated activation whose checkpoint is held so, and what stands around the
+products of a block: norms with residual, gate and dropout.
 
 A quantised matrix is a pair (q, s) with x ~ q s: q holds float8_e4m3fn or
 float8_e5m2 codes, s one float32 scale for a block.  Blocks lie along K, 128
@@ -22,8 +23,14 @@ Products take their operands' rows along K, so a gradient needs its operands
 quantised along another dimension; the quantiser's "cols" form gives blocks
 along M with the codes laid transposed, in the same pass over x.
 
-Differentiable are linear_f8 and swiglu_ckpt_f8, once.  The other functions have no
-derivative: given tensors that require a gradient, their results raise in a
+A dropout's random bits come from an element's place and rng, two int64 on the GPU: a
+seed and an offset (Philox4x32-10, sixteen bits an element).  No mask is stored; the
+same rng gives the same one again, and a program that drops anew adds to the offset
+(in place, where a captured graph is to read it).  Of elements the share
+round(p 2^16) / 2^16 is dropped and the rest scaled by its exact inverse.
+
+Differentiable are linear_f8, swiglu_ckpt_f8, residual_norm_f8 and seeded_dropout_f8, once.
+The other functions have no derivative: given tensors that require a gradient, their results raise in a
 backward pass, and a product into `out` raises at once.
 
 No reference counterpart: the reference's products are float64 ones.  The
@@ -39,6 +46,7 @@ from ._ops import ops
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BLOCK = 128
 _FORMS = {None: 0, "rows": 1, "both": 2}
+_ACTS = {None: 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
 
 # The overloads themselves: resolving a packet's overload costs a microsecond a call.
 _quant = ops.fp64_emu_quant_f8.default
@@ -46,6 +54,11 @@ _mm = ops.fp64_emu_mm_f8.default
 _mm_out = ops.fp64_emu_mm_f8_out.default
 _swiglu = ops.fp64_emu_swiglu_f8.default
 _swiglu_backward = ops.fp64_emu_swiglu_f8_backward.default
+_mm_epilogue = ops.fp64_emu_mm_f8_epilogue.default
+_act_backward = ops.fp64_emu_act_f8_backward.default
+_dropout = ops.fp64_emu_dropout_f8.default
+_norm = ops.fp64_emu_norm_f8.default
+_norm_backward = ops.fp64_emu_norm_f8_backward.default
 
 
 def _check_x(x, fmt):
@@ -59,6 +72,22 @@ def _form(quant):
     if quant not in _FORMS:
         raise ValueError(f"quant must be one of {tuple(_FORMS)}, got {quant!r}")
     return _FORMS[quant]
+
+
+def _act(act):
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {tuple(_ACTS)}, got {act!r}")
+    return _ACTS[act]
+
+
+def _drop(p, rng):
+    """The share of 65536 that is dropped."""
+    drop = round(p * 65536) if 0.0 <= p <= 1.0 else -1
+    if not 0 <= drop <= 65535:
+        raise ValueError(f"p must be in 0 .. 1 - 2^-16, got {p}")
+    if drop and rng is None:
+        raise ValueError("a dropout needs rng: two int64 on the GPU, a seed and an offset")
+    return drop
 
 
 def quant_f8(x: torch.Tensor, rows: bool = True, cols: bool = False, fmt: torch.dtype = E4M3):
@@ -82,9 +111,14 @@ def quant_f8_tiles(x: torch.Tensor, transposed: bool = False, fmt: torch.dtype =
     return tuple(_quant(x, True, transposed, True, fmt))
 
 
-def _product(dim, A, sA, B, sB, out_dtype, out, accumulate):
+def _product(dim, A, sA, B, sB, out_dtype, out, accumulate, bias, act, residual, keep):
     if A.dim() != dim or B.dim() != dim:
         raise ValueError(f"expect {dim}-D operands, got {A.dim()}-D and {B.dim()}-D")
+    if bias is not None or act is not None or residual is not None or keep:
+        if out is not None or accumulate:
+            raise ValueError("out and accumulate go without bias, act, residual and keep")
+        got = _mm_epilogue(A, sA, B, sB, out_dtype, bias, _act(act), residual, keep)
+        return tuple(got) if keep else got[0]
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -95,20 +129,105 @@ def _product(dim, A, sA, B, sB, out_dtype, out, accumulate):
 
 def mm_f8(A: torch.Tensor, sA: torch.Tensor, B: torch.Tensor, sB: torch.Tensor,
           out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor = None,
-          accumulate: bool = False) -> torch.Tensor:
+          accumulate: bool = False, bias: torch.Tensor = None, act: str = None,
+          residual: torch.Tensor = None, keep: bool = False) -> torch.Tensor:
     """C = A @ B^T of quantised A [M, K] and B [N, K], A's scales by rows, B's by
     rows or tiles.  out: where to (float32, bfloat16 or float16, rows any
     distance apart; out_dtype is then out's); accumulate: C is added to it, the
     sum rounded once.  16-bit outputs of more than a few rows take less exact sums of a
-    block than float32 ones (the module's notes say how much)."""
-    return _product(2, A, sA, B, sB, out_dtype, out, accumulate)
+    block than float32 ones (the module's notes say how much).
+
+    bias [N], act ("relu", "relu2", "silu", "gelu", "gelu_tanh") and residual [M, N] in
+    out_dtype give act(C + bias) + residual instead, from the float32 sums and rounded once;
+    keep: then (that, C + bias), the second for act_f8_backward."""
+    return _product(2, A, sA, B, sB, out_dtype, out, accumulate, bias, act, residual, keep)
 
 
 def bmm_f8(A: torch.Tensor, sA: torch.Tensor, B: torch.Tensor, sB: torch.Tensor,
            out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor = None,
-           accumulate: bool = False) -> torch.Tensor:
-    """C[b] = A[b] @ B[b]^T, as mm_f8 for each member."""
-    return _product(3, A, sA, B, sB, out_dtype, out, accumulate)
+           accumulate: bool = False, bias: torch.Tensor = None, act: str = None,
+           residual: torch.Tensor = None, keep: bool = False) -> torch.Tensor:
+    """C[b] = A[b] @ B[b]^T, as mm_f8 for each member; bias [batch, N], or [N] for all."""
+    return _product(3, A, sA, B, sB, out_dtype, out, accumulate, bias, act, residual, keep)
+
+
+def act_f8_backward(dy: torch.Tensor, h: torch.Tensor = None, act: str = None, quant: str = None,
+                    bias: bool = False):
+    """dh = dy act'(h) for the h that mm_f8 kept, dy and h [M, N] of one type; without act,
+    dh = dy.  quant None: (dh,) in dy's type; "rows": (q, s); "both": (q, s, qt, st), quantised from
+    the float32 values.  bias: then also dbias [N], their float32 sum over the rows."""
+    code, form = _act(act), _form(quant)
+    if dy.dim() != 2:
+        raise ValueError(f"expect dy as [M, N], got {tuple(dy.shape)}")
+    if code and (h is None or h.shape != dy.shape):
+        raise ValueError(f"expect h with dy's shape {tuple(dy.shape)}")
+    return tuple(_act_backward(dy, h if code else None, code, form, bias))
+
+
+def dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor, quant: str = None):
+    """x [M, K] with a share p of its elements zero and the others scaled, by rng's bits (the
+    module's notes).  quant None: (y,) in x's type; "rows": (q, s); "both": (q, s, qt, st).
+    The same call on a gradient is the gradient."""
+    form, drop = _form(quant), _drop(p, rng)
+    if x.dim() != 2:
+        raise ValueError(f"expect x as [M, K], got {tuple(x.shape)}")
+    return tuple(_dropout(x, drop, rng, form))
+
+
+def _check_norm(r, w, y, post, gate, eps=1.0):
+    if r.dim() != 2 or w.shape != r.shape[1:]:
+        raise ValueError(f"expect r [M, D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
+    if y is None and (post is not None or gate is not None):
+        raise ValueError("post and gate are of y")
+    if y is not None and y.shape != r.shape:
+        raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")
+    if post is not None and post.shape != w.shape:
+        raise ValueError(f"expect post as [D], got {tuple(post.shape)}")
+    if gate is not None and gate.shape not in (w.shape, r.shape):
+        raise ValueError(f"expect gate as [D] or [M, D], got {tuple(gate.shape)}")
+    if not eps > 0.0:
+        raise ValueError(f"eps must be positive, got {eps}")
+
+
+def norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torch.Tensor = None,
+            gate: torch.Tensor = None, scale: float = 1.0, p: float = 0.0, rng: torch.Tensor = None,
+            quant: str = None, keep: bool = False, eps: float = 1e-6):
+    """Between two blocks: the block's output y joins the residual stream r, and the norm of
+    the new stream is the next block's input.  With i(v) = (mean(v^2) + eps)^-1/2 over a row of D,
+
+      z = y i(y) post,  r' = scale r + gate drop(z),  x = r' i(r') w
+
+    for r and y [M, D], w and post [D], gate [D] or [M, D]; z = y without post, r' = r without y.
+    x comes from r' before that is rounded to r's type.  y has r's type, or r is float32; x (and
+    a gate [M, D]) have y's.  p, rng: the dropout of z.
+
+    Returns (r',) with y; then quant None: (x,), "rows": (q, s), "both": (q, s, qt, st); then with keep
+    (stats,), i(r') and, with post, i(y) of each row, for norm_f8_backward.  Sums of squares are
+    float32 ones: rows past about 1e18 give x = 0."""
+    form, drop = _form(quant), _drop(p, rng)
+    _check_norm(r, w, y, post, gate, eps)
+    if y is None and (drop or scale != 1.0):
+        raise ValueError("scale and p go with y")
+    return tuple(_norm(r, w, y, post, gate, scale, drop, rng, form, keep, eps))
+
+
+def norm_f8_backward(dx: torch.Tensor, dr: torch.Tensor, r: torch.Tensor, w: torch.Tensor, stats: torch.Tensor,
+                     y: torch.Tensor = None, post: torch.Tensor = None, gate: torch.Tensor = None,
+                     scale: float = 1.0, p: float = 0.0, rng: torch.Tensor = None):
+    """The gradient of norm_f8 for dx (x's) and dr (the new stream's own, or None), from the
+    new stream r that it returned (with y None, r itself), its stats and its other arguments.
+
+    Returns (dr, dy, dw, dpost, dgate), None for what is absent: dr in r's type, dy in y's, dw, dpost
+    and the gradient of a gate [D] float32, that of a gate [M, D] in its type."""
+    drop = _drop(p, rng)
+    _check_norm(r, w, y, post, gate)
+    if dx.shape != r.shape or (dr is not None and dr.shape != r.shape):
+        raise ValueError(f"dx and dr must have r's shape {tuple(r.shape)}")
+    if y is None and (drop or scale != 1.0):
+        raise ValueError("scale and p go with y")
+    got = iter(_norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng))
+    out = [next(got) if there else None for there in (True, y is not None, True, post is not None)]
+    return (*out, next(got, None))
 
 
 def swiglu_f8(h: torch.Tensor, quant: str = None, keep: bool = True):
@@ -143,40 +262,60 @@ def _as_rows(t):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, wq, ws, wqt, wst, grad):
+    def forward(ctx, x, w, wq, ws, wqt, wst, bias, act, residual, grad):
         rows = _as_rows(x)
         # (needs_input_grad does not heed no_grad, and in here gradients are always off.)
-        wants_x, wants_w = (grad and n for n in ctx.needs_input_grad[:2])
+        wants_x, wants_w, wants_b = (grad and ctx.needs_input_grad[i] for i in (0, 1, 6))
         q, s, *kept = quant_f8(rows, cols=wants_w)
         if wq is None:
             wq, ws, *across = quant_f8_tiles(w.detach(), transposed=wants_x)
             wqt, wst = across if wants_x else (None, None)
         elif wants_x and wqt is None:
             raise ValueError("wq lacks the transposed half that x's gradient reads")
-        ctx.save_for_backward(*(kept if wants_w else (None, None)),
-                              *((wqt, wst) if wants_x else (None, None)))
+        ctx.act, ctx.wants_b = act, wants_b
         ctx.shape, ctx.w_dtype, ctx.x_dtype = x.shape, w.dtype, x.dtype
-        return mm_f8(q, s, wq, ws, out_dtype=x.dtype).view(*x.shape[:-1], w.size(0))
+        ctx.b_dtype = bias.dtype if bias is not None else None
+        shape, h = (*x.shape[:-1], w.size(0)), None
+        if bias is None and act is None and residual is None:
+            y = mm_f8(q, s, wq, ws, out_dtype=x.dtype)
+        else:
+            keep = act is not None and (wants_x or wants_w or wants_b)
+            added = _as_rows(residual) if residual is not None else None
+            y = mm_f8(q, s, wq, ws, out_dtype=x.dtype, bias=bias, act=act, residual=added, keep=keep)
+            y, h = y if keep else (y, None)
+        ctx.save_for_backward(*(kept if wants_w else (None, None)),
+                              *((wqt, wst) if wants_x else (None, None)), h)
+        return y.view(shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xqt, xst, wqt, wst = ctx.saved_tensors
+        xqt, xst, wqt, wst, h = ctx.saved_tensors
         rows = _as_rows(dy)
-        dx = dw = None
-        got = quant_f8(rows, rows=wqt is not None, cols=xqt is not None)
+        dx = dw = db = None
+        got = ()
+        if ctx.wants_b or h is not None:
+            quant = "both" if xqt is not None else "rows" if wqt is not None else None
+            got = act_f8_backward(rows, h, ctx.act, quant, bias=ctx.wants_b)
+            if ctx.wants_b:
+                *got, db = got
+                db = db.to(ctx.b_dtype)
+        elif wqt is not None or xqt is not None:
+            got = quant_f8(rows, rows=wqt is not None, cols=xqt is not None)
         if wqt is not None:
             dx = mm_f8(got[0], got[1], wqt, wst, out_dtype=ctx.x_dtype).view(ctx.shape)
         if xqt is not None:
             dw = mm_f8(got[-2], got[-1], xqt, xst, out_dtype=ctx.w_dtype)
-        return dx, dw, None, None, None, None, None
+        return dx, dw, None, None, None, None, db, None, dy if ctx.needs_input_grad[8] else None, None
 
 
-def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tensor:
-    """y = x @ w^T for x [.., K] and w [N, K], in x's type, by 8-bit products:
-    x by rows, w by tiles.  Differentiable once, in x and w; what is kept for w's
-    gradient is x in 8 bits (blocks along its rows' direction), not x.  Gradients:
-    dx = dy w with dy by rows, dw = dy^T x with dy and x by columns.
+def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None, bias: torch.Tensor = None, act: str = None,
+              residual: torch.Tensor = None) -> torch.Tensor:
+    """y = act(x @ w^T + bias) + residual for x [.., K] and w [N, K], in x's type, by 8-bit products:
+    x by rows, w by tiles.  Differentiable once, in x, w, bias [N] and residual [.., N] (in x's
+    type); what is kept for w's gradient is x in 8 bits (blocks along its rows' direction), not x, and
+    with act its argument in x's type.  Gradients: with dh = dy act', dx = dh w with dh by rows,
+    dw = dh^T x with dh and x by columns.
 
     wq: quant_f8_tiles(w, transposed=True) made earlier, for weights that stay
     (without the transposed half where x needs no gradient, or under no_grad)."""
@@ -187,7 +326,12 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None) -> torch.Tenso
         raise ValueError("wq: what quant_f8_tiles gives, two or four tensors")
     if wq and wq[0].shape != w.shape:
         raise ValueError(f"wq is of another weight: {tuple(wq[0].shape)} and {tuple(w.shape)}")
-    return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))), torch.is_grad_enabled())
+    _act(act)
+    if bias is not None and bias.shape != w.shape[:1]:
+        raise ValueError(f"expect bias as [N], got {tuple(bias.shape)}")
+    if residual is not None and (residual.shape != (*x.shape[:-1], w.size(0)) or residual.dtype != x.dtype):
+        raise ValueError(f"expect residual as {(*x.shape[:-1], w.size(0))} in x's type")
+    return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))), bias, act, residual, torch.is_grad_enabled())
 
 
 class _SwigluCkpt(torch.autograd.Function):
@@ -212,5 +356,79 @@ def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
     return _SwigluCkpt.apply(h, torch.is_grad_enabled())
 
 
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, r, w, y, post, gate, scale, p, rng, eps, grad):
+        flat = [_as_rows(t) if t is not None else None for t in (r, y)]
+        gates = _as_rows(gate) if gate is not None and gate.dim() > 1 else gate
+        keep = grad and any(ctx.needs_input_grad[:5])
+        got = norm_f8(flat[0], w, flat[1], post, gates, scale, p, rng, keep=keep, eps=eps)
+        ctx.scale, ctx.p, ctx.joined = scale, p, y is not None
+        if keep:
+            # (rng may go on in place before the backward pass.)
+            rng = rng.clone() if p else None
+            ctx.save_for_backward(got[0] if ctx.joined else flat[0], w, flat[1], post, gates, got[-1], rng)
+        ctx.set_materialize_grads(False)
+        out = tuple(t.view(r.shape) for t in got[:2 if ctx.joined else 1])
+        return out if ctx.joined else out[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        r, w, y, post, gate, stats, rng = ctx.saved_tensors
+        dr, dx = grads if ctx.joined else (None, grads[0])
+        shape = next((g.shape for g in (dr, dx) if g is not None), None)
+        if shape is None:
+            return (None,) * 10
+        dx = torch.zeros_like(r if y is None else y) if dx is None else _as_rows(dx)
+        dr = _as_rows(dr) if dr is not None else None
+        dr, dy, dw, dpost, dgate = norm_f8_backward(dx, dr, r, w, stats, y, post, gate, ctx.scale, ctx.p, rng)
+        dy = dy.view(shape) if dy is not None else None
+        dpost = dpost.to(post.dtype) if post is not None else None
+        if gate is not None:
+            dgate = dgate.to(gate.dtype) if gate.dim() == 1 else dgate.view(shape)
+        return dr.view(shape), dw.to(w.dtype), dy, dpost, dgate, None, None, None, None, None
+
+
+def residual_norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torch.Tensor = None,
+                     gate: torch.Tensor = None, scale: float = 1.0, p: float = 0.0, rng: torch.Tensor = None,
+                     eps: float = 1e-6):
+    """(r', x) of norm_f8 in their plain forms for r [.., D], x alone without y.  Differentiable once, in r,
+    w, y, post and gate: [D], or of a shape that spreads to r's, as a gate for each sequence or
+    token does.  What is kept is r', y, and two floats a row."""
+    if r.dim() < 1 or w.dim() != 1:
+        raise ValueError(f"expect r [.., D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
+    if gate is not None and gate.dim() > 1:
+        gate = gate.expand(r.shape)
+    if y is not None and y.shape != r.shape:
+        raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")
+    return _ResidualNorm.apply(r, w, y, post, gate, scale, p, rng, eps, torch.is_grad_enabled())
+
+
+class _SeededDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, rng, grad):
+        if grad and ctx.needs_input_grad[0]:
+            ctx.p = p
+            # (rng may go on in place before the backward pass.)
+            ctx.save_for_backward(rng.clone() if rng is not None else None)
+        return dropout_f8(_as_rows(x), p, rng)[0].view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rng, = ctx.saved_tensors
+        return dropout_f8(_as_rows(dy), ctx.p, rng)[0].view(dy.shape), None, None, None
+
+
+def seeded_dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
+    """dropout_f8's plain form for x [.., K], differentiable once: the gradient makes the mask again from
+    rng's value at the call."""
+    if x.dim() < 1:
+        raise ValueError(f"expect x as [.., K], got {tuple(x.shape)}")
+    return _SeededDropout.apply(x, p, rng, torch.is_grad_enabled())
+
+
 __all__ = ["quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",
-           "linear_f8", "swiglu_ckpt_f8"]
+           "linear_f8", "swiglu_ckpt_f8", "act_f8_backward", "dropout_f8", "norm_f8", "norm_f8_backward",
+           "residual_norm_f8", "seeded_dropout_f8"]

@@ -367,6 +367,89 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
                                const fp64emu_f8_t* rows, const fp64emu_f8_t* cols,
                                fp64emu_stream_t stream);
 
+/* The epilogue of a product: h = A B^T + bias, out = act(h) + residual, from the float32 sums and
+ * rounded once.  bias [batch, N] (bias_stride 0: one for all members) in any dtype; residual and
+ * keep, where h goes, [batch, M, N] in out's dtype.  Each may be NULL; residual may be out
+ * itself, other overlaps not.  With an epilogue, accumulate must be 0.  e NULL: fp64emu_mm_f8.
+ * gelu is h Phi(h), gelu_tanh h (1 + tanh(sqrt(2 / pi) (h + 0.044715 h^3))) / 2, relu2 max(h, 0)^2. */
+enum {
+  FP64EMU_ACT_NONE = 0, FP64EMU_ACT_RELU = 1, FP64EMU_ACT_RELU2 = 2, FP64EMU_ACT_SILU = 3,
+  FP64EMU_ACT_GELU = 4, FP64EMU_ACT_GELU_TANH = 5
+};
+
+typedef struct {
+  const void *bias, *residual;
+  void* keep;
+  int64_t bias_stride, ld_residual, stride_residual, ld_keep, stride_keep;
+  int bias_dtype, act;
+} fp64emu_epilogue_t;
+
+size_t fp64emu_mm_f8_epilogue_workspace(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e);
+
+int fp64emu_mm_f8_epilogue(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e, void* workspace,
+                           size_t workspace_bytes, fp64emu_stream_t stream);
+
+/* Its gradient at h: dh = dy act'(h) of dy and h [M, N] (h unread with FP64EMU_ACT_NONE), each output only
+ * where asked for: `dh` in dtype; `rows` and `cols` (as fp64emu_quant_f8's, from the float32 values; dh
+ * does not come with cols); dbias [N], dh's float32 sum over the rows, which takes the workspace. */
+size_t fp64emu_act_f8_backward_workspace(int64_t M, int64_t N, int cols /* asked for */);
+
+int fp64emu_act_f8_backward(const void* dy, const void* h, int dtype, int act, int64_t M, int64_t N,
+                            int64_t ld_dy, int64_t ld_h, void* dh, int64_t ld_dh, const fp64emu_f8_t* rows,
+                            const fp64emu_f8_t* cols, float* dbias, void* workspace, size_t workspace_bytes,
+                            fp64emu_stream_t stream);
+
+/* ---- Dropout from a counter.  An element of an M x D matrix gets sixteen random bits from its place, the seed
+ * rng[0] and the offset rng[1] (two int64 in device memory, read by the kernel): Philox4x32-10 with the
+ * counter (c, c >> 32, offset, offset >> 32), c = m ceil(D / 8) + d / 8, and the key (seed, seed >> 32)
+ * gives four words, element (m, d) has half d % 2 (0: the lower) of word d % 8 / 2.  Bits below `drop`
+ * (of 65536) make it 0, others multiply it by 65536 / (65536 - drop).  The same call on a gradient is
+ * the gradient. ---- */
+
+/* x [M, K] dropped, each output only where asked for: `y` in x's dtype; `rows` and `cols` (y does not come
+ * with cols).  rng may be NULL with drop = 0. */
+int fp64emu_dropout_f8(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int drop,
+                       const int64_t* rng /* device */, void* y, int64_t ldy, const fp64emu_f8_t* rows,
+                       const fp64emu_f8_t* cols, fp64emu_stream_t stream);
+
+/* ---- The norms before and after a block.  With i(v) = (mean(v^2) + eps)^-1/2 over a row of D:
+ * z = y i(y) post (y without post), v = scale r + gate drop(z) (r without y), x = v i(v) w, x from v
+ * before it is rounded to the stream's dtype. ---- */
+typedef struct {
+  const void *r, *y;            /* [M, D], rows ld_r and ld_y apart; y may be NULL */
+  const void *w, *post, *gate;  /* [D]; post and gate may be NULL; gate [M, D] with ld_gate >= D */
+  const int64_t* rng;           /* device; with drop > 0 */
+  int64_t M, D;                 /* D < 2^27 */
+  int64_t ld_r, ld_y, ld_gate;  /* ld_gate 0: one gate for all rows */
+  int r_dtype, y_dtype;         /* y_dtype: of y and x; r_dtype the same or FP64EMU_F32 */
+  int w_dtype, post_dtype, gate_dtype;  /* any; of a gate for each row: y_dtype */
+  int drop;                     /* of 65536 */
+  float scale, eps;             /* eps > 0 */
+} fp64emu_norm_t;
+
+/* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype (may be r itself);
+ * `x` [M, D] in y's dtype; stats, i(v) of each row, then with post i(y), M floats each; `rows` and `cols`,
+ * x quantised from its float32 values.  cols needs stats and comes without x. */
+int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x, int64_t ld_x, float* stats,
+                    const fp64emu_f8_t* rows, const fp64emu_f8_t* cols, fp64emu_stream_t stream);
+
+/* Its gradient.  p as forward, but r is the new stream v as it was stored; of dx [M, D] in y's dtype
+ * and dr, the new stream's own gradient in r's (NULL: zeros).  Each output only where asked for: dr_out in r's
+ * dtype, dy in y's, dw, dpost and dgate [D] float32, sums over the rows in an order that follows from
+ * the sizes, and dgates [M, D] in y's dtype instead of dgate for a gate for each row.  No output may
+ * overlap an input. */
+typedef struct {
+  const void *dx, *dr;
+  void *dr_out, *dy, *dgates;
+  float *dw, *dpost, *dgate;
+  int64_t ld_dx, ld_dr, ld_dr_out, ld_dy, ld_dgates;
+} fp64emu_norm_grad_t;
+
+size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p);
+
+int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d,
+                             void* workspace, size_t workspace_bytes, fp64emu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
