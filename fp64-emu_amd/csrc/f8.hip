@@ -465,9 +465,10 @@ __device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m,
   if (g.epilogue) {
     if (g.bias) v += read4(g.bias_type, g.bias, b * g.bias_stride + n, valid, vec);
     if (g.keep) write4(g.dtype, g.keep, b * g.stride_keep + m * g.ld_keep + n, valid, vec, v);
-    float a[4] = {v[0], v[1], v[2], v[3]};
-    activate(g.act, a);
-    v = v4f{a[0], a[1], a[2], a[3]};
+    with_act(g.act, [&](auto act) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = activated<decltype(act)::value, true>(v[j]);
+    });
     if (g.residual) v += read4(g.dtype, g.residual, b * g.stride_res + m * g.ld_res + n, valid, vec);
   }
   if (g.accumulate) v += read4(g.dtype, g.out, i, valid, vec);
@@ -655,10 +656,12 @@ __device__ __forceinline__ void store16_past(void* p, const void* w) {
 // wave's room in LDS, half of its rows at a time, so that what is kept, the residual and the
 // output go by whole lines.  The activation works there in a loop of its own, once in the code for
 // all of a half's values (unrolled over the registers its five forms would not fit the
-// instruction cache); the residual's lines are read before it and used after it.
+// instruction cache); the residual's lines are read before it and used after it, the second half's
+// into the first's registers.
+// `bias`: the wave's columns' in LDS.
 template <class S, bool kExact>
-__device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64_t m0, int64_t n0, int b, int wave, int lane,
-                                            v4f (&acc)[S::kTN][S::kTM]) {
+__device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, const float* bias, int64_t m0, int64_t n0, int b,
+                                            int wave, int lane, v4f (&acc)[S::kTN][S::kTM]) {
   using T = std::conditional_t<kExact, float, unsigned short>;
   constexpr int kEach = 16 / (int)sizeof(T), kLanes = S::kTN * 16 / kEach, kRows = 64 / kLanes;
   constexpr int kHalf = S::kTM / 2, kSteps = kHalf * 16 / kRows;
@@ -666,13 +669,30 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64
   static_assert(S::kWaves * kHalf * 16 * kRow <= 2 * S::kStage, "the waves' rooms in the stages'");
   const int fr = lane & 15, fg = lane >> 4;
   uint8_t* room = lds + wave * (kHalf * 16 * kRow);
+  const int64_t n = n0 + (lane % kLanes) * kEach, line0 = m0 + lane / kLanes;    // step i: row line0 + i kRows
+  const int valid = (int)(g.N - n < kEach ? g.N - n : kEach);
+  T old[kSteps][kEach];
+  auto read_old = [&](int half, int i) {
+    const int64_t m = line0 + half * kHalf * 16 + i * kRows;
+    if (m >= g.M) return;
+    const T* q = static_cast<const T*>(g.residual) + b * g.stride_res + m * g.ld_res + n;
+    if (valid == kEach) {
+      __builtin_memcpy(old[i], q, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach - 1; ++j) old[i][j] = j < valid ? q[j] : T{};
+    }
+  };
+  if (g.residual) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) read_old(0, i);
+  }
   if (g.bias) {
 #pragma unroll
     for (int x = 0; x < S::kTN; ++x) {
-      const int64_t n = n0 + x * 16 + 4 * fg, left = g.N - n;
-      const v4f bias = read4(g.bias_type, g.bias, b * g.bias_stride + n, (int)(left < 4 ? left : 4), g.vec_o && left >= 4);
+      const v4f add = *reinterpret_cast<const v4f*>(bias + x * 16 + 4 * fg);
 #pragma unroll
-      for (int y = 0; y < S::kTM; ++y) acc[x][y] += bias;
+      for (int y = 0; y < S::kTM; ++y) acc[x][y] += add;
     }
   }
   // Other lanes of the wave read what a lane wrote: not before it is written, whatever the
@@ -689,8 +709,6 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64
       else w[j] = g.dtype == FP64EMU_BF16 ? bf16_round(v[j]) : __builtin_bit_cast(unsigned short, (_Float16)v[j]);
     }
   };
-  const int64_t n = n0 + (lane % kLanes) * kEach;
-  const int valid = (int)(g.N - n < kEach ? g.N - n : kEach);
   auto put_line = [&](void* out, int64_t i, const T (&w)[kEach]) {
     T* to = static_cast<T*>(out) + i;
     if (valid == kEach) {
@@ -704,22 +722,7 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64
   uint8_t* const line = room + (lane / kLanes) * kRow + (lane % kLanes) * kEach * 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int64_t first = m0 + half * kHalf * 16 + lane / kLanes;    // step i: row first + i kRows
-    T old[kSteps][kEach];
-    if (g.residual) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int64_t m = first + i * kRows;
-        const T* q = static_cast<const T*>(g.residual) + b * g.stride_res + m * g.ld_res + n;
-        if (m >= g.M) break;
-        if (valid == kEach) {
-          __builtin_memcpy(old[i], q, 16);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kEach - 1; ++j) old[i][j] = j < valid ? q[j] : T{};
-        }
-      }
-    }
+    const int64_t first = line0 + half * kHalf * 16;
     if (half) handed();                                        // the first half's lines are read
 #pragma unroll
     for (int y = 0; y < kHalf; ++y)
@@ -730,20 +733,28 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64
     auto get = [&](int i, float (&v)[kEach]) {
       __builtin_memcpy(v, __builtin_assume_aligned(line + i * kRows * kRow, 16), 4 * kEach);
     };
-    if (g.keep || g.act) {
-#pragma unroll 1
+    if (g.keep) {
+#pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const int64_t m = first + i * kRows;
         float v[kEach];
+        T w[kEach];
         get(i, v);
-        if (g.keep && m < g.M) {
-          T w[kEach];
-          round(v, w);
-          put_line(g.keep, b * g.stride_keep + m * g.ld_keep + n, w);
-        }
-        activate(g.act, v);
-        __builtin_memcpy(__builtin_assume_aligned(line + i * kRows * kRow, 16), v, 4 * kEach);
+        round(v, w);
+        if (m < g.M) put_line(g.keep, b * g.stride_keep + m * g.ld_keep + n, w);
       }
+    }
+    if (g.act) {
+      with_act(g.act, [&](auto act) {
+#pragma unroll 1
+        for (int i = 0; i < kSteps; ++i) {
+          float v[kEach];
+          get(i, v);
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) v[j] = activated<decltype(act)::value, kExact>(v[j]);
+          __builtin_memcpy(__builtin_assume_aligned(line + i * kRows * kRow, 16), v, 4 * kEach);
+        }
+      });
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -754,11 +765,12 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, int64
       if (g.residual) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-          if constexpr (kExact) v[j] += old[i][j];
-          else v[j] += g.dtype == FP64EMU_BF16 ? bf16_value(old[i][j])
-                                               : (float)__builtin_bit_cast(_Float16, old[i][j]);
+          const T w = old[i][j];
+          if constexpr (kExact) v[j] += w;
+          else v[j] += g.dtype == FP64EMU_BF16 ? bf16_value(w) : (float)__builtin_bit_cast(_Float16, w);
         }
       }
+      if (g.residual && half == 0) read_old(1, i);             // the next half's, in the place of this one's
       T w[kEach];
       round(v, w);
       put_line(g.out, b * g.stride_o + m * g.ldo + n, w);
@@ -771,7 +783,9 @@ template <class S, bool kExact, int kFA, int kFB, bool kRowB, bool kEpilogue>
 __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   // The two stages, or the waves' rows of out.
   constexpr int kOut = S::kWaves * S::kTM * 16 * (S::kTN * 16 * (kExact ? 4 : 2) + 16);
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kOut > 2 * S::kStage ? kOut : 2 * S::kStage];
+  constexpr int kRoom = kOut > 2 * S::kStage && !kEpilogue ? kOut : 2 * S::kStage;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRoom + (kEpilogue ? 4 * S::kBN : 0)];
+  float* const bias = reinterpret_cast<float*>(lds + kRoom);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
@@ -832,6 +846,11 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
       sp = g.sA + b * g.sA_str + (m0 + r) * g.sA_row;
     }
     sp += kb0 * sblk;
+  }
+
+  if constexpr (kEpilogue) {           // seen past the first block's barrier
+    const int t = threadIdx.x;
+    if (g.bias && t < S::kBN) bias[t] = t < rowsB ? read4(g.bias_type, g.bias, b * g.bias_stride + n0 + t, 1, false)[0] : 0.0f;
   }
 
   // Block kb into stage st.  The block's offset is part of each lane's where it
@@ -1037,7 +1056,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   }
   if constexpr (kEpilogue) {
     barrier_lds();                                           // every wave is done with the stages
-    finish_tile<S, kExact>(g, lds, m0 + wm * S::kTM * 16, n0 + wn * S::kTN * 16, b, wave, lane, acc);
+    finish_tile<S, kExact>(g, lds, bias + wn * S::kTN * 16, m0 + wm * S::kTM * 16, n0 + wn * S::kTN * 16, b, wave, lane, acc);
     return;
   }
   // Through LDS, so that a store writes whole lines of out past the caches: 8192 x

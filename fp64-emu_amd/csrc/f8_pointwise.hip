@@ -13,7 +13,7 @@ struct ActGradArgs {
   const void *dy, *h;
   int64_t M, N, ld_dy, ld_h;
   int64_t blocks;                            // of 128 along a row
-  int act, per;                              // per: rows of a thread (rows kernel)
+  int per;                                   // rows of a thread (rows kernel)
   void* dh;
   int64_t ld_dh;
   float* part;                               // sums over the rows of a group: [groups][N], or null
@@ -39,7 +39,7 @@ __device__ __forceinline__ void emit_sums(const float (&mine)[8], int cols, floa
 
 // One work group per 128 x 128 tile, for columns: dh in both orientations and its sums over the
 // tile's rows from one reading.
-template <int kT>
+template <int kT, int kAct>
 __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_tile_kernel(ActGradArgs a) {
   __shared__ TileLds lds;
   __shared__ ColumnRoom room;
@@ -55,17 +55,13 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_
 #pragma unroll
     for (int p = 0; p < 8; ++p, ++row) {
       dy.load(p, a.dy, row * a.ld_dy + col, t.valid(p));
-      if (a.act) h.load(p, a.h, row * a.ld_h + col, t.valid(p));
+      if (kAct) h.load(p, a.h, row * a.ld_h + col, t.valid(p));
     }
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        d.v[p][j] = dy.at(p, j);
-        x[j] = a.act ? h.at(p, j) : 0.0f;
-      }
-      activate_back(a.act, x, d.v[p]);
+      for (int j = 0; j < 8; ++j) d.v[p][j] = activated_back<kAct, kT == FP64EMU_F32>(h.at(p, j), dy.at(p, j));
+      __builtin_amdgcn_sched_barrier(0);     // (a row's temporaries at a time)
     }
   }
   if (a.part) {
@@ -84,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_
 
 // Without columns: a work group has 16 x per rows of one block of 128 columns, a row's block on 16
 // lanes, 16 rows at a time.
-template <int kT>
+template <int kT, int kAct>
 __global__ void __launch_bounds__(kThreads) act_grad_rows_kernel(ActGradArgs a) {
   __shared__ ColumnRoom room;
   const uint32_t blocks = (uint32_t)a.blocks;
@@ -99,15 +95,10 @@ __global__ void __launch_bounds__(kThreads) act_grad_rows_kernel(ActGradArgs a) 
   for (int i = 0; i < a.per && u.row < a.M; ++i, u.row += 16) {
     Held<kT> dy, h;
     dy.load(0, a.dy, u.row * a.ld_dy + u.col, u.valid);
-    if (a.act) h.load(0, a.h, u.row * a.ld_h + u.col, u.valid);
+    if (kAct) h.load(0, a.h, u.row * a.ld_h + u.col, u.valid);
     Held<FP64EMU_F32> d;
-    float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d.v[0][j] = dy.at(0, j);
-      x[j] = a.act ? h.at(0, j) : 0.0f;
-    }
-    activate_back(a.act, x, d.v[0]);
+    for (int j = 0; j < 8; ++j) d.v[0][j] = activated_back<kAct, kT == FP64EMU_F32>(h.at(0, j), dy.at(0, j));
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] += d.v[0][j];
     if (a.dh) store8<kT>(a.dh, u.row * a.ld_dh + u.col, u.valid, d.v[0]);
@@ -232,7 +223,6 @@ int fp64emu_act_f8_backward(const void* dy, const void* h, int dtype, int act, i
   a.ld_dy = ld_dy;
   a.ld_h = ld_h;
   a.blocks = (N + kBlk - 1) / kBlk;
-  a.act = act;
   a.per = rows_per(M, a.blocks);
   a.dh = dh;
   a.ld_dh = ld_dh;
@@ -247,17 +237,20 @@ int fp64emu_act_f8_backward(const void* dy, const void* h, int dtype, int act, i
     sums.part[0] = a.part;
   }
   const unsigned groups = (unsigned)(sums.groups * a.blocks);
-#define FP64EMU_ACT_GRAD(T)                                             \
-  case T:                                                               \
-    if (cols) act_grad_tile_kernel<T><<<groups, kThreads, 0, s>>>(a);   \
-    else act_grad_rows_kernel<T><<<groups, kThreads, 0, s>>>(a);        \
+  with_act(act, [&](auto which) {
+    constexpr int kAct = decltype(which)::value;
+#define FP64EMU_ACT_GRAD(T)                                                   \
+  case T:                                                                     \
+    if (cols) act_grad_tile_kernel<T, kAct><<<groups, kThreads, 0, s>>>(a);   \
+    else act_grad_rows_kernel<T, kAct><<<groups, kThreads, 0, s>>>(a);        \
     break;
-  switch (dtype) {
-    FP64EMU_ACT_GRAD(FP64EMU_F32)
-    FP64EMU_ACT_GRAD(FP64EMU_BF16)
-    FP64EMU_ACT_GRAD(FP64EMU_F16)
-  }
+    switch (dtype) {
+      FP64EMU_ACT_GRAD(FP64EMU_F32)
+      FP64EMU_ACT_GRAD(FP64EMU_BF16)
+      FP64EMU_ACT_GRAD(FP64EMU_F16)
+    }
 #undef FP64EMU_ACT_GRAD
+  });
   if (int st = check_hip(hipGetLastError(), "act_f8_backward launch")) return st;
   return launch_sums(sums, dbias && sums.groups > 1 ? 1 : 0, s);
 }

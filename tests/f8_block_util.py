@@ -97,23 +97,24 @@ def _far(u):
     return 72 * (u.abs() > 87.3).to(u.dtype)
 
 
-# A sigmoid below 2^-126 comes as zero (the hardware's reciprocal): off by that, and what it is a factor of by
+# A sigmoid or e^(-h^2 / 2) below 2^-126 comes as zero (the hardware's reciprocal and 2^x): off by that, and what it is a factor of by
 # that times the other factors.
 LEAST = 2.0 ** -126
 
 
 def act_error(h, name):
     """Of act(h) in float32.  sigmoid(u): e^-u within 4 U of itself and u's own error, a reciprocal: 8 U + |u's
-    error| of itself.  u of gelu_tanh: three products and a sum, with two rounded constants, 6 U of
-    itself.  Phi(h) by erfc: 16 last places, and its argument's two roundings by its slope."""
+    error| of itself, and for 16-bit values 1.25 U |u| more, u log2 e being rounded once (and log2 e, by 0.22 U).  u of gelu_tanh: three products and a sum, with two rounded constants, 6 U of
+    itself.  Phi(-x) by a fit: 8 U, a reciprocal, a product and e^(-x^2 / 2), whose
+    argument's roundings are 2.3 U of x^2 / 2, below 4 U x phi / Phi; the other side is 1 less that."""
     a = h.abs()
     if name == "silu":
-        return (12 + _far(h)) * U * (h * torch.sigmoid(h)).abs() + a * LEAST
+        return (12 + 1.25 * a + _far(h)) * U * (h * torch.sigmoid(h)).abs() + a * LEAST
     if name == "gelu":
-        return U * a * (40 * _cdf(h) + 4 * a * _phi(h))
+        return U * a * (40 * _cdf(h) + 4 * a * _phi(h)) + a * LEAST
     if name == "gelu_tanh":
         u = _tanh_arg(h)[0]
-        return U * (h * torch.sigmoid(u)).abs() * (12 + 6 * u.abs() + _far(u)) + a * LEAST
+        return U * (h * torch.sigmoid(u)).abs() * (12 + 7.25 * u.abs() + _far(u)) + a * LEAST
     return 2 * U * act(h, name).abs()
 
 
@@ -121,15 +122,15 @@ def slope_error(h, name):
     a = h.abs()
     if name == "silu":
         s = torch.sigmoid(h)
-        return (24 + _far(h)) * U * s * (1 + a) + (1 + a) * LEAST
+        return (24 + 2.5 * a + _far(h)) * U * s * (1 + a) + (1 + a) * LEAST
     if name == "gelu":
         # (exp of -h^2 / 2, which has two roundings of itself)
-        return U * (40 * _cdf(h) + 4 * a * _phi(h) + a * _phi(h) * (8 + 2 * h * h))
+        return U * (40 * _cdf(h) + 4 * a * _phi(h) + a * _phi(h) * (8 + 2 * h * h)) + (1 + a) * LEAST
     if name == "gelu_tanh":
         u, du = _tanh_arg(h)
         s = torch.sigmoid(u)
         # (1 - s is within U of 1 absolutely where s nears it, so s (1 - s) is within s U)
-        return U * (s * (12 + 6 * u.abs() + _far(u)) + a * du * s * (4 + (1 - s) * (24 + 12 * u.abs() + _far(u)))) + (1 + a * du) * LEAST
+        return U * (s * (12 + 7.25 * u.abs() + _far(u)) + a * du * s * (4 + (1 - s) * (24 + 14.5 * u.abs() + _far(u)))) + (1 + a * du) * LEAST
     return 2 * U * slope(h, name).abs()
 
 
