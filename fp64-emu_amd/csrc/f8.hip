@@ -277,6 +277,7 @@ struct MmArgs {
   int vec_o;                         // out's rows start at multiples of 4 elements
   // What a product's sums go through before they are rounded: + bias, (kept,) act, + residual.
   int epilogue;                      // any of it
+  int touch;                         // the residual's rows are 16-byte aligned and within 32-bit offsets
   int act, bias_type;
   const void *bias, *residual;       // residual and keep have out's dtype
   void* keep;
@@ -784,8 +785,9 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
   // The two stages, or the waves' rows of out.
   constexpr int kOut = S::kWaves * S::kTM * 16 * (S::kTN * 16 * (kExact ? 4 : 2) + 16);
   constexpr int kRoom = kOut > 2 * S::kStage && !kEpilogue ? kOut : 2 * S::kStage;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRoom + (kEpilogue ? 4 * S::kBN : 0)];
-  float* const bias = reinterpret_cast<float*>(lds + kRoom);
+  // (With an epilogue then a kilobyte a wave that nothing reads, and the bias.)
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRoom + (kEpilogue ? S::kWaves * 1024 + 4 * S::kBN : 0)];
+  float* const bias = reinterpret_cast<float*>(lds + kRoom + S::kWaves * 1024);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
@@ -869,6 +871,38 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     if (wave * 64 >= S::kBN + S::kBM) return;
     __builtin_amdgcn_global_load_lds(sp, (lds_u8*)lds + st * S::kStage + S::kOffS + wave * 256, 4, 0, 0);
     sp += sblk;
+  };
+  // The residual's lines on their way from memory while it has little else to do: in the last two blocks
+  // the wave reads its lines into LDS, eight a block, where nothing looks at them; the epilogue then
+  // finds most of them in the caches.  8192^3 with a residual took 48 us more than without, with this 32 to 36
+  // (its bytes are 26); one line a block 40, two 34, all sixteen at once 35, in the blocks before
+  // the last 33 to 38; with a residual that never left the caches 12.
+  constexpr int kSize = kExact ? 4 : 2, kLines = S::kTM * 16 * (S::kTN * 16 * kSize / 16) / 64, kTouch = 8, kTouched = kLines / kTouch;
+  static_assert(kLines % kTouch == 0, "whole blocks of touches");
+  const bool touches = kEpilogue && g.touch;
+  __amdgpu_buffer_rsrc_t srcR = srcA;
+  uint32_t offR = 0, stepR = 0;
+  if constexpr (kEpilogue) {
+    if (touches) {
+      constexpr int kLanes = S::kTN * 16 * kSize / 16;
+      const uint8_t* R = static_cast<const uint8_t*>(g.residual) + (b * g.stride_res + m0 * g.ld_res + n0) * kSize;
+      srcR = buffer_src(R, (uint32_t)(((rowsA - 1) * g.ld_res + rowsB) * kSize));
+      offR = (uint32_t)(((wm * S::kTM * 16 + lane / kLanes) * g.ld_res + wn * S::kTN * 16) * kSize + lane % kLanes * 16);
+      stepR = (uint32_t)(64 / kLanes * g.ld_res * kSize);
+    }
+  }
+  // kTouch lines, if block i is one of those; past them in the source order nothing of the block is copied.
+  auto touch = [&](int i) {
+    if constexpr (kEpilogue) {
+      const int j = i - (nk - kTouched);
+      if (!touches || j < 0) return false;
+      lds_u8* to = (lds_u8*)lds + kRoom + wave * 1024;
+#pragma unroll
+      for (int q = 0; q < kTouch; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(srcR, to, 16, (int)(offR + (kTouch * j + q) * stepR), 0, 0, 0);
+      return true;
+    }
+    return false;
   };
   constexpr int kParts = 4, kPer = (kAll + kParts - 1) / kParts;
   auto issue = [&](int kb, int st, int part) {
@@ -972,6 +1006,8 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
     v4f p[2][S::kTM], sb[2];
     float sa_next[S::kTM], power_b = 1.0f;
     constexpr int kLast = S::kTN - 1;
+    bool touched = false;
+    static_assert(kLast >= kParts - 1, "a block's copies before its touches");
     if constexpr (kSplit) {
       const Split one = split_scale(scale(stage, rowB));       // of a tile of B
       power_b = one.power;
@@ -997,7 +1033,8 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
         power_b = split_scale(scale(stage, rowB + x * 16 + fr)).power;
       }
       if (x == kLast) {
-        wait_vm_lgkm0<0>();
+        if (kEpilogue && touched) wait_vm_lgkm0<kTouch>();     // (the touches are the latest)
+        else wait_vm_lgkm0<0>();
         barrier_lds();
         if (i + 2 < nk) issue(kb0 + i + 2, i & 1, 0);
         if (tail && i + 2 == nk && kb1 == g.nkb) clear_tail((i + 1) & 1);
@@ -1007,6 +1044,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g) {
         next = frag(stage, fragB + (x + 1) * 16 * kBlk);
       }
       if (x + 1 < kParts && i + 1 < nk) issue(kb0 + i + 1, (i + 1) & 1, x + 1);
+      if (x + 1 == kLast) touched = touch(i);
       Frag<kExact, kFB> fbx;
       if constexpr (kSplit) fbx = Frag<kExact, kFB>(fb, power_b);
       else fbx = Frag<kExact, kFB>(fb);
@@ -1580,6 +1618,9 @@ int fp64emu_mm_f8_epilogue(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e
     g.keep = e->keep;
     g.ld_keep = e->ld_keep;
     g.stride_keep = e->stride_keep;
+    const int64_t ld_bytes = e->ld_residual * (quad / 4);
+    g.touch = e->residual && multiple(e->residual, 16) && ld_bytes % 16 == 0 && ld_bytes < (1ll << 31) / 256 &&
+              e->stride_residual * (quad / 4) % 16 == 0;
     const auto fours = [](const void* q, int size, int64_t ld, int64_t stride) {
       return !q || (multiple(q, 4 * size) && ld % 4 == 0 && stride % 4 == 0);
     };

@@ -36,16 +36,61 @@ struct NormGradArgs {
   void *dr_out, *dy, *dgates;
   int64_t ld_dr_out, ld_dy, ld_dgates;
   float *dw, *dpost, *dgate;                 // [D], or a group's part of them, [groups][D] each
-  float* c1;                                 // rows of any length: a row's first mean
+  float* back;                               // rows of any length: a row's, as GradRow has it
+};
+
+// Eight elements of a row as they came.  A launch's kernels load whole ones of all their operands behind one
+// branch and the last, partial ones of a row behind another, element by element: a branch for each operand
+// took 60 registers of addresses and masks more.
+template <int kT>
+struct Eight {
+  v4u w;
+  __device__ __forceinline__ void whole(const void* p, int64_t i) {
+    __builtin_memcpy(&w, static_cast<const unsigned short*>(p) + i, 16);
+  }
+  __device__ __forceinline__ void part(const void* p, int64_t i, int valid) {
+    const unsigned short* q = static_cast<const unsigned short*>(p) + i;
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int j = valid - 1; j >= 0; --j) {
+      hi = hi << 16 | lo >> 48;
+      lo = lo << 16 | q[j];
+    }
+    w = v4u{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+  __device__ __forceinline__ void zero() { w = v4u{0u, 0u, 0u, 0u}; }
+  __device__ __forceinline__ float at(int j) const {
+    const uint32_t h = w[j >> 1] >> (16 * (j & 1));
+    return kT == FP64EMU_BF16 ? bf16_value((unsigned short)h) : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+  }
+  // Makes the compiler unpack element j on from here on, and not before: it unpacked all elements of a row's
+  // operands at once and kept them.
+  __device__ __forceinline__ void from_here(int j) { asm volatile("" : "+v"(w[j >> 1])); }
+};
+template <>
+struct Eight<FP64EMU_F32> {
+  v4f v[2];
+  __device__ __forceinline__ void whole(const void* p, int64_t i) {
+    __builtin_memcpy(v, static_cast<const float*>(p) + i, 32);
+  }
+  __device__ __forceinline__ void part(const void* p, int64_t i, int valid) {
+    const float* q = static_cast<const float*>(p) + i;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = j < valid ? q[j] : 0.0f;
+  }
+  __device__ __forceinline__ void zero() { v[0] = v[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f}; }
+  __device__ __forceinline__ float at(int j) const { return v[j >> 2][j & 3]; }
+  __device__ __forceinline__ void from_here(int) {}
 };
 
 // Eight elements from i on, those past `valid` as zeros.
 template <int kT>
 __device__ __forceinline__ void load8(const void* p, int64_t i, int valid, float (&v)[8]) {
-  Held<kT> h;
-  h.load(0, p, i, valid);
+  Eight<kT> e;
+  if (valid >= 8) e.whole(p, i);
+  else e.part(p, i, valid);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = h.at(0, j);
+  for (int j = 0; j < 8; ++j) v[j] = e.at(j);
 }
 // The same of any type, or ones.
 __device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, int valid, float (&v)[8]) {
@@ -54,10 +99,15 @@ __device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, in
     for (int j = 0; j < 8; ++j) v[j] = 1.0f;
   } else if (type == FP64EMU_F32) {
     load8<FP64EMU_F32>(p, i, valid, v);
-  } else if (type == FP64EMU_BF16) {
-    load8<FP64EMU_BF16>(p, i, valid, v);
   } else {
-    load8<FP64EMU_F16>(p, i, valid, v);
+    Eight<FP64EMU_BF16> e;
+    if (valid >= 8) e.whole(p, i);
+    else e.part(p, i, valid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t h = e.w[j >> 1] >> (16 * (j & 1));
+      v[j] = type == FP64EMU_BF16 ? bf16_value((unsigned short)h) : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+    }
   }
 }
 
@@ -73,23 +123,28 @@ __device__ __forceinline__ float row16_sum(float v) {
   return v + dpp<0x121>(v);
 }
 
-// Eight elements of a row as they came.
-template <int kT>
-struct Eight {
-  Held<kT> h;
-  __device__ __forceinline__ void load(const void* p, int64_t i, int valid) { h.load(0, p, i, valid); }
-  __device__ __forceinline__ float at(int j) const { return h.at(0, j); }
-  // Makes the compiler unpack the words again instead of keeping eight floats beside them.
-  __device__ __forceinline__ void again() {
-    if constexpr (kT != FP64EMU_F32) asm volatile("" : "+v"(h.w[0]));
-  }
-};
-
 // How a launch lays rows on threads: kT threads a row, eight elements each (so 16 neighbouring
 // lanes hold a block of 128), work groups of 256 threads or one row.
 template <int kT_>
 struct RowShape {
   static constexpr int kT = kT_, kGroup = kT > kThreads ? kT : kThreads, kRows = kGroup / kT;
+  // Which of the group's rows a thread has: the same for a wave, where it is, so that addresses of rows are scalar.
+  static __device__ __forceinline__ int sub() {
+    if constexpr (kRows == 1) return 0;
+    const int s = threadIdx.x / kT;
+    return kT >= 64 ? __builtin_amdgcn_readfirstlane(s) : s;
+  }
+  // Row m of a matrix of rows of ld elements of T.  Scalar where a wave has one row: the compiler kept
+  // a pointer for each operand in vector registers from row to row.
+  template <int kType>
+  static __device__ __forceinline__ uint8_t* row(const void* p, int64_t m, int64_t ld) {
+    uint64_t a = reinterpret_cast<uint64_t>(p) + (uint64_t)(m * ld) * (kType == FP64EMU_F32 ? 4 : 2);
+    if constexpr (kT >= 64) {
+      const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+      a = (uint64_t)hi << 32 | lo;
+    }
+    return reinterpret_cast<uint8_t*>(a);
+  }
 };
 
 // Sums over the threads of a row, in all of them; `turn` alternates from call to call, so that one
@@ -165,7 +220,7 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   constexpr int kT = S::kT;
   using Sum = RowSum<kT, 1, S::kGroup>;
   __shared__ typename Sum::Room room;
-  const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
+  const int t = threadIdx.x % kT, sub = S::sub();
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
   const int64_t row_chunks = (g.D + 7) / 8;
   const int col = 8 * t, left = (int)g.D - col, valid = left < 0 ? 0 : left < 8 ? left : 8;
@@ -178,9 +233,15 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   Eight<kY> y, gates;
   auto fetch = [&](int64_t m) {
     const int n = m < g.M ? valid : 0;
-    r.load(g.r, m * g.ld_r + col, n);
-    if (g.y) y.load(g.y, m * g.ld_y + col, n);
-    if (g.ld_gate) gates.load(g.gate, m * g.ld_gate + col, n);
+    if (n == 8) {
+      r.whole(g.r, m * g.ld_r + col);
+      if (g.y) y.whole(g.y, m * g.ld_y + col);
+      if (g.ld_gate) gates.whole(g.gate, m * g.ld_gate + col);
+    } else {
+      r.part(g.r, m * g.ld_r + col, n);
+      y.part(g.y, m * g.ld_y + col, g.y ? n : 0);
+      gates.part(g.gate, m * g.ld_gate + col, g.ld_gate ? n : 0);
+    }
   };
   const int64_t step = (int64_t)gridDim.x * S::kRows;
   int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
@@ -344,58 +405,64 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
 // ---------------------------------------------------------------------------
 // Gradient.  With vh = v i(v), yh = y i(y) and k drop's factor of an element:
 //
-//   e = dr + i(v) (dx w),   t = e - i(v) vh c1,       c1 = mean(dx w vh)     t: v's gradient
+//   t = dr + i(v) (dx w - vh c1),                     c1 = mean(dx w vh)     t: v's gradient
 //   dz = t gate k,  dy = i(y) (dz post - yh c2),      c2 = mean(dz post yh)
 //   dw = sum dx vh,  dpost = sum dz yh,  dgate = sum t k yh post    over the rows
 //
-// and scale t is r's gradient.  c2 is linear in c1: with u = gate k post yh, c2 = mean(u e) - c1
-// mean(u i(v) vh), so that one joint sum of three gives both and a row takes one barrier.
-// v is the stream as it is stored.
+// and scale t is r's gradient.  c2 is linear in c1: with e = dr + i(v) dx w and q = gate k post y, it is
+// i(y) (mean(q e) - i(v)^2 c1 mean(q v)), so that one joint sum of three gives both and a row takes
+// one barrier.  v is the stream as it is stored.
 
-// What eight elements give, first to the three sums and then, with the means, to the gradients; kept is
-// there before.
-struct GradPart {
-  float vh[8], e[8], yh[8];
-  uint32_t kept;
-};
-
+// The three sums of eight elements: of (dx w) v, and with k what remains of gate and drop (0 where dropped),
+// q = k post y, of q e and of q v.  The rows' own factors i(v) and i(y) join them at their ends.
 template <bool kPost>
-__device__ __forceinline__ void grad_sums(const Drop& drop, float iv, float iy, const float (&v)[8], const float (&y)[8],
-                                          const float (&dx)[8], const float (&dr)[8], const float (&w)[8],
-                                          const float (&post)[8], const float (&gate)[8], GradPart& p,
-                                          float (&s)[kPost ? 3 : 1]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float gw = dx[j] * w[j];
-    p.vh[j] = v[j] * iv;
-    p.e[j] = dr[j] + iv * gw;
-    s[0] = fmaf(gw, p.vh[j], s[0]);
+struct GradSums {
+  static constexpr int kN = kPost ? 3 : 1;
+  static __device__ __forceinline__ void add(float v, float dx, float dr, float w, float iv, float kept_gate, float post,
+                                             float y, float (&s)[kN]) {
+    const float gw = dx * w;
+    s[0] = fmaf(gw, v, s[0]);
     if constexpr (kPost) {
-      p.yh[j] = y[j] * iy;
-      const float u = p.kept >> j & 1 ? gate[j] * drop.scale * post[j] * p.yh[j] : 0.0f;
-      s[1] = fmaf(u, p.e[j], s[1]);
-      s[2] = fmaf(u, iv * p.vh[j], s[2]);
-    } else {
-      p.yh[j] = y[j];
+      const float q = kept_gate * post * y, e = fmaf(iv, gw, dr);
+      s[1] = fmaf(q, e, s[1]);
+      s[2] = fmaf(q, v, s[2]);
     }
   }
+};
+
+// A row's factors once its sums are there: t = dr + iv dx w - back v; dy = iy dz post - c2 y.
+struct GradRow { float iv, iy, back, c2; };
+
+template <bool kPost>
+__device__ __forceinline__ GradRow grad_row(const float (&s)[kPost ? 3 : 1], float iv, float iy, int64_t D) {
+  GradRow r{iv, iy, 0.0f, 0.0f};
+  const float n = (float)D, c1 = s[0] * iv / n;                // mean(dx w vh)
+  r.back = iv * iv * c1;
+  // mean(dz post yh) is i(y) (s1 - back s2) / D
+  if constexpr (kPost) r.c2 = iy * iy * (iy * ((s[1] - r.back * s[2]) / n));
+  return r;
 }
 
-// t, dy and dgate of eight elements, and what they add to the sums over the rows.
+struct GradOut { float t, dy, dz, z, dgate; };
+
+// An element's gradients: kept_scale is drop's factor, 0 where dropped.
 template <bool kPost>
-__device__ __forceinline__ void grad_values(const Drop& drop, const GradPart& p, float iv, float iy, float c1, float c2,
-                                            const float (&post)[8], const float (&gate)[8], float (&t)[8],
-                                            float (&dz)[8], float (&dy)[8], float (&dgate)[8]) {
-  const float back = iv * c1;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    t[j] = p.e[j] - back * p.vh[j];
-    const float k = p.kept >> j & 1 ? t[j] * drop.scale : 0.0f;
-    const bool in = p.kept >> j & 1;
-    dz[j] = k * gate[j];
-    dgate[j] = in ? k * (kPost ? p.yh[j] * post[j] : p.yh[j]) : 0.0f;
-    dy[j] = kPost ? iy * (dz[j] * post[j] - p.yh[j] * c2) : in ? dz[j] : 0.0f;
+__device__ __forceinline__ GradOut grad_of(const GradRow& r, float v, float dx, float dr, float w, float kept_scale,
+                                           float gate, float post, float y) {
+  GradOut o;
+  o.t = fmaf(-r.back, v, fmaf(r.iv, dx * w, dr));
+  const float u = o.t * kept_scale;
+  o.dz = u * gate;
+  if constexpr (kPost) {
+    o.z = y * r.iy;                                            // (yh)
+    o.dy = fmaf(-r.c2, y, r.iy * (o.dz * post));
+    o.dgate = u * (o.z * post);
+  } else {
+    o.z = kept_scale != 0.0f ? y : 0.0f;                       // (whatever a dropped y was)
+    o.dy = o.dz;
+    o.dgate = u * o.z;
   }
+  return o;
 }
 
 // A group's sums over its rows into its part of [groups][D] (or the result itself, with one group).
@@ -405,7 +472,7 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
   const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
   float* to = part + (int64_t)blockIdx.x * D;
   if constexpr (S::kRows == 1) {
-    store8<FP64EMU_F32>(to, of.col, of.valid, sum);
+    if (of.in) store8<FP64EMU_F32>(to, of.col, 8, sum);
   } else {
     __syncthreads();                         // (whatever the room held before)
 #pragma unroll
@@ -419,7 +486,7 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
 #pragma unroll
         for (int i = 1; i < S::kRows; ++i) v[j] += lds[j * S::kGroup + i * kT + t];
       }
-      store8<FP64EMU_F32>(to, of.col, of.valid, v);
+      if (of.in) store8<FP64EMU_F32>(to, of.col, 8, v);
     }
   }
 }
@@ -427,30 +494,37 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
 // Rows in registers, as norm_rows_kernel, but kC times eight elements a thread (element 8 (c kT + t) on):
 // 1024 threads a row leave 128 registers each, which the sums over the rows, kept a column to a thread,
 // do not fit.  A row's values stay as they came and are worked out again after its sums; with one
-// chunk the next row's are on their way meanwhile.  kPost: y has a norm; without it y may be absent, too.
-template <int kR, int kY, class S, int kC, bool kPost>
-__global__ void __launch_bounds__(S::kGroup) norm_grad_kernel(NormArgs g, NormGradArgs d) {
+// chunk the next row's are on their way meanwhile.  A row's last, partial eight elements are its last eight: what the
+// thread beside has of them comes out the same from both and counts once in the sums (with loads and stores
+// of parts the kernel took 195 registers).  kPost: y has a norm; without it y may be absent, too.  kGates: a gate
+// for each row, whose values and gradient do not fit 128 registers as the rest does.
+template <int kR, int kY, class S, int kC, bool kPost, bool kGates>
+__global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU_F32 && S::kT >= 64 ? 4 : 2)
+    norm_grad_kernel(NormArgs g, NormGradArgs d) {
   constexpr int kT = S::kT, kN = kPost ? 3 : 1;
   constexpr bool kAhead = kC == 1;
   using Sum = RowSum<kT, kN, S::kGroup>;
   __shared__ typename Sum::Room room;
   __shared__ float joint[S::kRows > 1 ? 8 * S::kGroup : 1];
-  const int t = threadIdx.x % kT, sub = threadIdx.x / kT;
+  const int t = threadIdx.x % kT, sub = S::sub();
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
   const int64_t row_chunks = (g.D + 7) / 8;
   struct Column {
     float w[8], post[8], gate[8], dw[8], dpost[8], dgate[8];
-    int col, valid;
+    int col, again;                          // first column; leading elements that another thread has, too
+    bool in;
   } of[kC];
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
     Column& o = of[c];
-    o.col = 8 * (c * kT + t);
-    const int left = (int)g.D - o.col;
-    o.valid = left < 0 ? 0 : left < 8 ? left : 8;
-    load8_any(g.w_type, g.w, o.col, o.valid, o.w);
-    if constexpr (kPost) load8_any(g.post_type, g.post, o.col, o.valid, o.post);
-    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, o.col, o.valid, o.gate);
+    const int col = 8 * (c * kT + t), left = (int)g.D - col;
+    o.in = left > 0;
+    o.again = left > 0 && left < 8 ? 8 - left : 0;
+    o.col = col - o.again;
+    const int valid = o.in ? 8 : 0;
+    load8_any(g.w_type, g.w, o.col, valid, o.w);
+    if constexpr (kPost) load8_any(g.post_type, g.post, o.col, valid, o.post);
+    if constexpr (!kGates) load8_any(g.gate_type, g.gate, o.col, valid, o.gate);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o.dw[j] = o.dpost[j] = o.dgate[j] = 0.0f;
   }
@@ -459,16 +533,29 @@ __global__ void __launch_bounds__(S::kGroup) norm_grad_kernel(NormArgs g, NormGr
     Eight<kR> v[kC], dr[kC];
     Eight<kY> y[kC], dx[kC], gates[kC];
     float iv, iy;
+    __device__ __forceinline__ void from_here(int c, int j) {
+      v[c].from_here(j);
+      dr[c].from_here(j);
+      y[c].from_here(j);
+      dx[c].from_here(j);
+    }
   };
   auto fetch = [&](int64_t m, Row& o) {
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const int n = m < g.M ? of[c].valid : 0, col = of[c].col;
-      o.v[c].load(g.r, m * g.ld_r + col, n);
-      o.dx[c].load(d.dx, m * d.ld_dx + col, n);
-      o.dr[c].load(d.dr, m * d.ld_dr + col, d.dr ? n : 0);
-      o.y[c].load(g.y, m * g.ld_y + col, g.y ? n : 0);
-      if (g.ld_gate) o.gates[c].load(g.gate, m * g.ld_gate + col, n);
+      const int col = of[c].col;
+      o.v[c].zero();
+      o.dx[c].zero();
+      o.dr[c].zero();
+      o.y[c].zero();
+      if constexpr (kGates) o.gates[c].zero();
+      if (m < g.M && of[c].in) {
+        o.v[c].whole(S::template row<kR>(g.r, m, g.ld_r), col);
+        o.dx[c].whole(S::template row<kY>(d.dx, m, d.ld_dx), col);
+        if (d.dr) o.dr[c].whole(S::template row<kR>(d.dr, m, d.ld_dr), col);
+        if (g.y) o.y[c].whole(S::template row<kY>(g.y, m, g.ld_y), col);
+        if constexpr (kGates) o.gates[c].whole(S::template row<kY>(g.gate, m, g.ld_gate), col);
+      }
     }
     o.iv = m < g.M ? g.stats[m] : 0.0f;
     o.iy = kPost && m < g.M ? g.stats[g.M + m] : 0.0f;
@@ -485,54 +572,60 @@ __global__ void __launch_bounds__(S::kGroup) norm_grad_kernel(NormArgs g, NormGr
     } else {
       fetch(m, o);
     }
-    GradPart p;
-    float s[kN] = {}, dx[8];
-    auto work_out = [&](int c, float (&s)[kN]) {
-      Column& k = of[c];
-      float v[8], y[8], dr[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = o.v[c].at(j);
-        dx[j] = o.dx[c].at(j);
-        dr[j] = o.dr[c].at(j);
-        y[j] = o.y[c].at(j);
-        if (g.ld_gate) k.gate[j] = o.gates[c].at(j);
-      }
-      grad_sums<kPost>(drop, o.iv, o.iy, v, y, dx, dr, k.w, k.post, k.gate, p, s);
-    };
+    float s[kN] = {};
     uint32_t kept[kC];
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      p.kept = kept[c] = kept_of(drop, (uint64_t)(m * row_chunks + c * kT + t));
-      work_out(c, s);
+      Column& k = of[c];
+      const uint64_t chunk = (uint64_t)(m * row_chunks + c * kT + t);
+      kept[c] = kept_of(drop, chunk);
+      if (k.again) kept[c] = (kept_of(drop, chunk - 1) | kept[c] << 8) >> (8 - k.again) & 0xff;
+      float mine[kN] = {};
+      auto element = [&](int j) {
+        GradSums<kPost>::add(o.v[c].at(j), o.dx[c].at(j), o.dr[c].at(j), k.w[j], o.iv,
+                             kept[c] >> j & 1 ? k.gate[j] * drop.scale : 0.0f, k.post[j], o.y[c].at(j), mine);
+      };
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j % 2 == 0) o.from_here(c, j);
+        if constexpr (kGates) k.gate[j] = o.gates[c].at(j);
+        element(j);
+        asm volatile("" : "+v"(mine[0]));
+      }
+      if (k.again) {                         // (a wave's last thread, at most)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) mine[i] = 0.0f;
+#pragma unroll
+        for (int j = 1; j < 8; ++j)
+          if (j >= k.again) element(j);
+      }
+#pragma unroll
+      for (int i = 0; i < kN; ++i) s[i] += mine[i];
     }
     Sum::run(s, room, turn);
-    const float c1 = s[0] / (float)g.D;
-    float c2 = 0.0f;
-    if constexpr (kPost) c2 = (s[1] - c1 * s[2]) / (float)g.D;
+    const GradRow row = grad_row<kPost>(s, o.iv, o.iy, g.D);
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       Column& k = of[c];
-      o.v[c].again();
-      o.dx[c].again();
-      o.dr[c].again();
-      o.y[c].again();
-      o.gates[c].again();
-      p.kept = kept[c];
-      float none[kN], tv[8], dz[8], dy[8], dg[8];
-      work_out(c, none);
-      grad_values<kPost>(drop, p, o.iv, o.iy, c1, c2, k.post, k.gate, tv, dz, dy, dg);
+      float tv[8], dy[8], dg[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        k.dw[j] = fmaf(dx[j], p.vh[j], k.dw[j]);
-        if constexpr (kPost) k.dpost[j] = fmaf(dz[j], p.yh[j], k.dpost[j]);
-        k.dgate[j] += dg[j];
-        tv[j] *= g.scale;
+        if (j % 2 == 0) o.from_here(c, j);
+        const float v = o.v[c].at(j), dx = o.dx[c].at(j);
+        const GradOut e = grad_of<kPost>(row, v, dx, o.dr[c].at(j), k.w[j], kept[c] >> j & 1 ? drop.scale : 0.0f, k.gate[j],
+                                         kPost ? k.post[j] : 1.0f, o.y[c].at(j));
+        k.dw[j] = fmaf(dx, v * o.iv, k.dw[j]);
+        if constexpr (kPost) k.dpost[j] = fmaf(e.dz, e.z, k.dpost[j]);
+        if constexpr (!kGates) k.dgate[j] += e.dgate;
+        tv[j] = e.t * g.scale;
+        dy[j] = e.dy;
+        dg[j] = e.dgate;
+        asm volatile("" : "+v"(k.dw[j]), "+v"(k.dpost[j]), "+v"(k.dgate[j]));      // (here, and not at the end)
       }
-      if (m < g.M) {
-        if (d.dr_out) store8<kR>(d.dr_out, m * d.ld_dr_out + k.col, k.valid, tv);
-        if (d.dy) store8<kY>(d.dy, m * d.ld_dy + k.col, k.valid, dy);
-        if (d.dgates) store8<kY>(d.dgates, m * d.ld_dgates + k.col, k.valid, dg);
+      if (m < g.M && k.in) {
+        if (d.dr_out) store8<kR>(S::template row<kR>(d.dr_out, m, d.ld_dr_out), k.col, 8, tv);
+        if (d.dy) store8<kY>(S::template row<kY>(d.dy, m, d.ld_dy), k.col, 8, dy);
+        if (kGates && d.dgates) store8<kY>(S::template row<kY>(d.dgates, m, d.ld_dgates), k.col, 8, dg);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -541,28 +634,29 @@ __global__ void __launch_bounds__(S::kGroup) norm_grad_kernel(NormArgs g, NormGr
   for (int c = 0; c < kC; ++c) {
     if (d.dw) join_rows<S>(of[c].dw, of[c], d.dw, g.D, joint);
     if (kPost && d.dpost) join_rows<S>(of[c].dpost, of[c], d.dpost, g.D, joint);
-    if (d.dgate) join_rows<S>(of[c].dgate, of[c], d.dgate, g.D, joint);
+    if (!kGates && d.dgate) join_rows<S>(of[c].dgate, of[c], d.dgate, g.D, joint);
   }
 }
 
-// Rows of any length: the row's sums, then its gradients, from two readings of it; c1 is kept for
-// the sums over the rows, which another kernel makes.
+// Rows of any length: the row's sums, then its gradients, from two readings of it; its `back` is kept
+// for the sums over the rows, which another kernel makes.
 template <int kR, int kY, bool kPost>
 struct GradAt {
-  float v[8], dx[8], y[8], w[8], post[8], gate[8];
-  GradPart p;
-  __device__ __forceinline__ void load(const NormArgs& g, const NormGradArgs& d, const Drop& drop, int64_t m, int64_t col,
-                                       int valid, float iv, float iy, float (&s)[kPost ? 3 : 1]) {
-    float dr[8] = {};
+  float v[8], dx[8], dr[8], y[8], w[8], post[8], gate[8];
+  uint32_t kept;
+  __device__ __forceinline__ GradAt(const NormArgs& g, const NormGradArgs& d, const Drop& drop, int64_t m, int64_t col) {
+    const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
     load8<kR>(g.r, m * g.ld_r + col, valid, v);
     load8<kY>(d.dx, m * d.ld_dx + col, valid, dx);
-    if (d.dr) load8<kR>(d.dr, m * d.ld_dr + col, valid, dr);
-    load8_any(kY, g.y, m * g.ld_y + col, valid, y);
+    load8<kR>(d.dr, m * d.ld_dr + col, d.dr ? valid : 0, dr);
+    load8<kY>(g.y, m * g.ld_y + col, g.y ? valid : 0, y);
     load8_any(g.w_type, g.w, col, valid, w);
     load8_any(g.post_type, g.post, col, valid, post);
     load8_any(g.gate_type, g.gate, m * g.ld_gate + col, valid, gate);
-    p.kept = kept_of(drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8));
-    grad_sums<kPost>(drop, iv, iy, v, y, dx, dr, w, post, gate, p, s);
+    kept = kept_of(drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8));
+  }
+  __device__ __forceinline__ GradOut at(const GradRow& r, const Drop& drop, int j) const {
+    return grad_of<kPost>(r, v[j], dx[j], dr[j], w[j], kept >> j & 1 ? drop.scale : 0.0f, gate[j], post[j], y[j]);
   }
 };
 
@@ -570,6 +664,7 @@ template <int kR, int kY, bool kPost>
 __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormGradArgs d) {
   constexpr int kN = kPost ? 3 : 1;
   using Sum = RowSum<kLong, kN, kLong>;
+  using At = GradAt<kR, kY, kPost>;
   __shared__ typename Sum::Room room;
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
   int turn = 0;
@@ -577,22 +672,26 @@ __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormG
     const float iv = g.stats[m], iy = kPost ? g.stats[g.M + m] : 1.0f;
     float s[kN] = {};
     for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
-      GradAt<kR, kY, kPost> a;
-      a.load(g, d, drop, m, col, g.D - col < 8 ? (int)(g.D - col) : 8, iv, iy, s);
+      const At a(g, d, drop, m, col);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        GradSums<kPost>::add(a.v[j], a.dx[j], a.dr[j], a.w[j], iv, a.kept >> j & 1 ? a.gate[j] * drop.scale : 0.0f,
+                             a.post[j], a.y[j], s);
     }
     Sum::run(s, room, turn);
-    const float c1 = s[0] / (float)g.D;
-    float c2 = 0.0f;
-    if constexpr (kPost) c2 = (s[1] - c1 * s[2]) / (float)g.D;
-    if (threadIdx.x == 0) d.c1[m] = c1;
+    const GradRow row = grad_row<kPost>(s, iv, iy, g.D);
+    if (threadIdx.x == 0) d.back[m] = row.back;
     for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
       const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
-      GradAt<kR, kY, kPost> a;
-      float none[kN] = {}, t[8], dz[8], dy[8], dg[8];
-      a.load(g, d, drop, m, col, valid, iv, iy, none);
-      grad_values<kPost>(drop, a.p, iv, iy, c1, c2, a.post, a.gate, t, dz, dy, dg);
+      const At a(g, d, drop, m, col);
+      float t[8], dy[8], dg[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] *= g.scale;
+      for (int j = 0; j < 8; ++j) {
+        const GradOut e = a.at(row, drop, j);
+        t[j] = e.t * g.scale;
+        dy[j] = e.dy;
+        dg[j] = e.dgate;
+      }
       if (d.dr_out) store8<kR>(d.dr_out, m * d.ld_dr_out + col, valid, t);
       if (d.dy) store8<kY>(d.dy, m * d.ld_dy + col, valid, dy);
       if (d.dgates) store8<kY>(d.dgates, m * d.ld_dgates + col, valid, dg);
@@ -600,7 +699,7 @@ __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormG
   }
 }
 
-// The sums over the rows blockIdx.x, + gridDim.x, ..  for the columns of blockIdx.y, from c1.
+// The sums over the rows blockIdx.x, + gridDim.x, ..  for the columns of blockIdx.y, from `back`.
 template <int kR, int kY, bool kPost>
 __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormArgs g, NormGradArgs d) {
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
@@ -609,16 +708,14 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormArgs g,
   const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
   float dw[8] = {}, dpost[8] = {}, dgate[8] = {};
   for (int64_t m = blockIdx.x; m < g.M; m += gridDim.x) {
-    const float iv = g.stats[m], iy = kPost ? g.stats[g.M + m] : 1.0f;
-    GradAt<kR, kY, kPost> a;
-    float none[kPost ? 3 : 1] = {}, t[8], dz[8], dy[8], dg[8];
-    a.load(g, d, drop, m, col, valid, iv, iy, none);
-    grad_values<kPost>(drop, a.p, iv, iy, d.c1[m], 0.0f, a.post, a.gate, t, dz, dy, dg);
+    const GradRow row{g.stats[m], kPost ? g.stats[g.M + m] : 1.0f, d.back[m], 0.0f};
+    const GradAt<kR, kY, kPost> a(g, d, drop, m, col);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      dw[j] = fmaf(a.dx[j], a.p.vh[j], dw[j]);
-      dpost[j] = fmaf(dz[j], a.p.yh[j], dpost[j]);
-      dgate[j] += dg[j];
+      const GradOut e = a.at(row, drop, j);
+      dw[j] = fmaf(a.dx[j], a.v[j] * row.iv, dw[j]);
+      dpost[j] = fmaf(e.dz, e.z, dpost[j]);
+      dgate[j] += e.dgate;
     }
   }
   const int64_t to = (int64_t)blockIdx.x * g.D + col;
@@ -641,6 +738,7 @@ void for_rows(int64_t D, const Fn& fn) {
   else fn(RowShape<1024>{});
 }
 constexpr int64_t kMaxHeld = 8192;           // elements of a row that stay in registers
+bool grad_held(int64_t D) { return D >= 8 && D <= kMaxHeld; }
 
 int64_t rows_a_group(int64_t D) {
   int64_t rows = 1;
@@ -684,16 +782,17 @@ int launch_norm(const NormArgs& g, bool tiles, hipStream_t s) {
 template <int kR, int kY, bool kPost>
 int launch_grad(const NormArgs& g, const NormGradArgs& d, hipStream_t s) {
   const unsigned groups = (unsigned)grad_groups(g.M, g.D);
-  if (g.D > kMaxHeld) {
+  if (!grad_held(g.D)) {
     norm_grad_long_kernel<kR, kY, kPost><<<(unsigned)norm_groups(g.M, g.D), kLong, 0, s>>>(g, d);
     if (int st = check_hip(hipGetLastError(), "norm_f8_backward launch")) return st;
     const unsigned strips = (unsigned)((g.D + 8 * kThreads - 1) / (8 * kThreads));
     norm_grad_columns_kernel<kR, kY, kPost><<<dim3(groups, strips), kThreads, 0, s>>>(g, d);
   } else {
     for_rows(g.D, [&](auto shape) {
-      using S = decltype(shape);
-      if constexpr (S::kT == 1024) norm_grad_kernel<kR, kY, RowShape<512>, 2, kPost><<<groups, 512, 0, s>>>(g, d);
-      else norm_grad_kernel<kR, kY, S, 1, kPost><<<groups, S::kGroup, 0, s>>>(g, d);
+      using S = std::conditional_t<decltype(shape)::kT == 1024, RowShape<512>, decltype(shape)>;
+      constexpr int kC = decltype(shape)::kT == 1024 ? 2 : 1;
+      if (g.ld_gate) norm_grad_kernel<kR, kY, S, kC, kPost, true><<<groups, S::kGroup, 0, s>>>(g, d);
+      else norm_grad_kernel<kR, kY, S, kC, kPost, false><<<groups, S::kGroup, 0, s>>>(g, d);
     });
   }
   return check_hip(hipGetLastError(), "norm_f8_backward launch");
@@ -793,7 +892,7 @@ size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p) {
   if (check_norm(p) || p->M == 0 || p->D == 0) return 0;
   const int64_t groups = grad_groups(p->M, p->D);
   const size_t parts = groups > 1 ? 4 * (size_t)kMaxSums * (size_t)(groups * p->D) : 0;
-  return parts + (p->D > kMaxHeld ? 4 * (size_t)p->M : 0);
+  return parts + (grad_held(p->D) ? 0 : 4 * (size_t)p->M);
 }
 
 int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d, void* workspace,
@@ -821,6 +920,8 @@ int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const 
     return invalid("rows are shorter than D");
   NormArgs g;
   if (int st = norm_args(p, &g)) return st;
+  if ((d->dgate && p->ld_gate != 0) || (d->dgates && p->ld_gate == 0))
+    return invalid("dgate is of one gate, dgates of a gate for each row");
   const size_t need = fp64emu_norm_f8_backward_workspace(p);
   if (need && (!workspace || workspace_bytes < need))
     return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_norm_f8_backward_workspace");
@@ -847,7 +948,7 @@ int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const 
     all.part[count] = *to[i];
     all.out[count++] = sums[i];
   }
-  if (p->D > kMaxHeld) a.c1 = room + (groups > 1 ? kMaxSums * groups * p->D : 0);
+  if (!grad_held(p->D)) a.back = room + (groups > 1 ? kMaxSums * groups * p->D : 0);
   all.groups = groups;
   all.D = p->D;
   const int st = for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {

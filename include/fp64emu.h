@@ -436,7 +436,7 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
 /* Its gradient.  p as forward, but r is the new stream v as it was stored; of dx [M, D] in y's dtype
  * and dr, the new stream's own gradient in r's (NULL: zeros).  Each output only where asked for: dr_out in r's
  * dtype, dy in y's, dw, dpost and dgate [D] float32, sums over the rows in an order that follows from
- * the sizes, and dgates [M, D] in y's dtype instead of dgate for a gate for each row.  No output may
+ * the sizes, and, for a gate for each row, dgates [M, D] in y's dtype instead of dgate.  No output may
  * overlap an input. */
 typedef struct {
   const void *dx, *dr;

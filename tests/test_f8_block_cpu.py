@@ -123,7 +123,8 @@ def test_norm_grad_refusals():
                      (dict(grad={"ld_dr": 255}), "shorter"), (dict(grad={"ld_dr_out": 255}), "shorter"), (dict(grad={"ld_dy": 255}), "shorter"),
                      (dict(post=None), "absent"), (dict(gate=None), "absent"), (dict(grad={"dgates": P}), "a row or a matrix"),
                      (dict(grad={"dgates": P, "dgate": None}), "y's dtype"), (dict(y=None, post=None, gate=None), "absent"),
-                     (dict(M=300), "workspace too small"), (dict(M=300, ws=0x1002, n=1 << 30), "aligned")):
+                     (dict(ld_gate=256, gate_dtype=BF16), "of one gate"),
+                     (dict(gate_dtype=BF16, grad={"dgates": P, "dgate": None}), "of one gate"), (dict(M=300), "workspace too small"), (dict(M=300, ws=0x1002, n=1 << 30), "aligned")):
         _says(call(**kw), text)
     assert L.fp64emu_norm_f8_backward(R(_norm()), P, None, None, 0, None) == EINVAL
     assert L.fp64emu_norm_f8_backward_workspace(R(_norm(M=0))) == 0
