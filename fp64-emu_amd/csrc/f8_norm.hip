@@ -22,7 +22,7 @@ struct NormArgs {
   int64_t blocks;                            // of 128 along a row
   int w_type, post_type, gate_type;
   uint32_t threshold;
-  float scale, eps;
+  float scale, eps, over_d;                  // over_d: 1 / D
   void* out;                                 // the new stream
   void* x;
   int64_t ld_out, ld_x;
@@ -111,9 +111,9 @@ __device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, in
   }
 }
 
-template <int kCtrl>
-__device__ __forceinline__ float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, false));
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ float dpp(float v) {         // 0 in the rows that are masked out
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRowMask, 0xf, false));
 }
 // The sum over the 16 lanes of a DPP row, the same bits in all of them.
 __device__ __forceinline__ float row16_sum(float v) {
@@ -121,6 +121,13 @@ __device__ __forceinline__ float row16_sum(float v) {
   v += dpp<0x124>(v);
   v += dpp<0x122>(v);
   return v + dpp<0x121>(v);
+}
+// Over a wave, scalar: on vector instructions alone, where lane exchanges go through the LDS unit.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = row16_sum(v);
+  v += dpp<0x142, 0xa>(v);                   // row_bcast:15: rows 1 and 3 add the row before
+  v += dpp<0x143, 0xc>(v);                   // row_bcast:31: rows 2 and 3 add the half before
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // How a launch lays rows on threads: kT threads a row, eight elements each (so 16 neighbouring
@@ -152,16 +159,10 @@ struct RowShape {
 template <int kT, int kN, int kGroup>
 struct RowSum {
   static constexpr int kWaves = kT / 64;
-  struct Room { float v[2][kN][kGroup / 64]; };
+  struct alignas(16) Room { float v[2][kN][kGroup / 64]; };
   static __device__ __forceinline__ void run(float (&v)[kN], Room& room, int& turn) {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      v[n] = row16_sum(v[n]);
-      if constexpr (kT >= 64) {
-        v[n] += __shfl_xor(v[n], 16);
-        v[n] += __shfl_xor(v[n], 32);
-      }
-    }
+    for (int n = 0; n < kN; ++n) v[n] = kT >= 64 ? wave_sum(v[n]) : row16_sum(v[n]);
     if constexpr (kT > 64) {
       const int wave = threadIdx.x >> 6, first = wave / kWaves * kWaves;
       if ((threadIdx.x & 63) == 0) {
@@ -181,8 +182,10 @@ struct RowSum {
   }
 };
 
+// The hardware's 1 / sqrt, within one ulp, and a Newton step.
 __device__ __forceinline__ float inverse_rms(float squares, const NormArgs& g) {
-  return 1.0f / sqrtf(squares / (float)g.D + g.eps);
+  const float m = fmaf(squares, g.over_d, g.eps), y = __builtin_amdgcn_rsqf(m);
+  return m < __builtin_inff() ? fmaf(y * 0.5f, fmaf(-m * y, y, 1.0f), y) : y;      // (past that inf 0)
 }
 
 // v of eight elements from those of r and y.
@@ -212,10 +215,10 @@ __device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t 
   }
 }
 
-// Rows whose values stay in registers from the first sum to the last store.  A work group takes
-// rows blockIdx.x kRows + .., gridDim.x kRows apart, the weights in registers throughout and the next
-// row's values on their way.
-template <int kR, int kY, class S>
+// Rows whose values stay in registers from the first sum to the last store, kC times eight elements a
+// thread (element 8 (c kT + t) on).  A work group takes rows blockIdx.x kRows + .., gridDim.x kRows
+// apart, the weights in registers throughout and the next row's values on their way.
+template <int kR, int kY, class S, int kC>
 __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   constexpr int kT = S::kT;
   using Sum = RowSum<kT, 1, S::kGroup>;
@@ -223,53 +226,73 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   const int t = threadIdx.x % kT, sub = S::sub();
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
   const int64_t row_chunks = (g.D + 7) / 8;
-  const int col = 8 * t, left = (int)g.D - col, valid = left < 0 ? 0 : left < 8 ? left : 8;
-  float w[8], post[8], gate[8];
-  load8_any(g.w_type, g.w, col, valid, w);
-  load8_any(g.post_type, g.post, col, valid, post);
-  if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, valid, gate);
+  float w[kC][8], post[kC][8], gate[kC][8];
+  int valid[kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const int col = 8 * (c * kT + t), left = (int)g.D - col;
+    valid[c] = left < 0 ? 0 : left < 8 ? left : 8;
+    load8_any(g.w_type, g.w, col, valid[c], w[c]);
+    load8_any(g.post_type, g.post, col, valid[c], post[c]);
+    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, valid[c], gate[c]);
+  }
   int turn = 0;
-  Eight<kR> r;
-  Eight<kY> y, gates;
+  Eight<kR> r[kC];
+  Eight<kY> y[kC], gates[kC];
   auto fetch = [&](int64_t m) {
-    const int n = m < g.M ? valid : 0;
-    if (n == 8) {
-      r.whole(g.r, m * g.ld_r + col);
-      if (g.y) y.whole(g.y, m * g.ld_y + col);
-      if (g.ld_gate) gates.whole(g.gate, m * g.ld_gate + col);
-    } else {
-      r.part(g.r, m * g.ld_r + col, n);
-      y.part(g.y, m * g.ld_y + col, g.y ? n : 0);
-      gates.part(g.gate, m * g.ld_gate + col, g.ld_gate ? n : 0);
+    const uint8_t* pr = S::template row<kR>(g.r, m, g.ld_r);
+    const uint8_t* py = S::template row<kY>(g.y, m, g.ld_y);
+    const uint8_t* pg = S::template row<kY>(g.gate, m, g.ld_gate);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int n = m < g.M ? valid[c] : 0, col = 8 * (c * kT + t);
+      if (n == 8) {
+        r[c].whole(pr, col);
+        if (g.y) y[c].whole(py, col);
+        if (g.ld_gate) gates[c].whole(pg, col);
+      } else {
+        r[c].part(pr, col, n);
+        y[c].part(py, col, g.y ? n : 0);
+        gates[c].part(pg, col, g.ld_gate ? n : 0);
+      }
     }
   };
   const int64_t step = (int64_t)gridDim.x * S::kRows;
   int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
   fetch(m);
   for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
-    float v[8], yv[8];
+    float v[kC][8], yv[kC][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = r.at(j);
-      if (g.y) yv[j] = y.at(j);
-      if (g.ld_gate) gate[j] = gates.at(j);
-    }
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] = r[c].at(j);
+        if (g.y) yv[c][j] = y[c].at(j);
+        if (g.ld_gate) gate[c][j] = gates[c].at(j);
+      }
     fetch(m + step);
     float iy = 1.0f;
     if (g.y) {
       if (g.post) {
         float s[1] = {0.0f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[0] = fmaf(yv[j], yv[j], s[0]);
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[0] = fmaf(yv[c][j], yv[c][j], s[0]);
         Sum::run(s, room, turn);
         iy = inverse_rms(s[0], g);
       }
-      joined(g, drop, (uint64_t)(m * row_chunks + t), iy, yv, post, gate, v);
-      if (g.out && m < g.M) store8<kR>(g.out, m * g.ld_out + col, valid, v);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        joined(g, drop, (uint64_t)(m * row_chunks + c * kT + t), iy, yv[c], post[c], gate[c], v[c]);
+        if (g.out && m < g.M) store8<kR>(S::template row<kR>(g.out, m, g.ld_out), 8 * (c * kT + t), valid[c], v[c]);
+      }
     }
     float s[1] = {0.0f};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] = fmaf(v[j], v[j], s[0]);
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] = fmaf(v[c][j], v[c][j], s[0]);
     Sum::run(s, room, turn);
     const float iv = inverse_rms(s[0], g);
     if (m < g.M) {
@@ -277,7 +300,8 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
         g.stats[m] = iv;
         if (g.post) g.stats[g.M + m] = iy;
       }
-      emit_norm<kR, kY>(g, m, col, valid, iv, v, w);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) emit_norm<kR, kY>(g, m, 8 * (c * kT + t), valid[c], iv, v[c], w[c]);
     }
   }
 }
@@ -350,7 +374,9 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
   }
 }
 
-// Tiles of 128 x 128, once the rows' statistics are there: the new stream, x's rows and its columns.
+// x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
+// else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways TODO us; with the
+// statistics alone from that kernel and all outputs from this one 113).
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;
@@ -391,14 +417,12 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
         for (int j = 0; j < 8; ++j) yv[j] = y.at(p, j);
         if (g.ld_gate) load8<kY>(g.gate, (row + p) * g.ld_gate + col, t.valid(p), gate);
         joined(g, drop, chunk + p * ((g.D + 7) / 8), iy, yv, post, gate, v);
-        if (g.out) store8<kR>(g.out, (row + p) * g.ld_out + col, t.valid(p), v);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) x.v[p][j] = v[j] * iv * w[j];
     };
     each_row(each, std::make_integer_sequence<int, 8>{});
   }
-  if (g.rows.q) emit_rows<FP64EMU_E4M3>(x, t, row0, col0, kb, g.rows);
   emit_cols<FP64EMU_E4M3>(x, t, row0, col0, mb, g.cols, lds);
 }
 
@@ -434,12 +458,12 @@ struct GradSums {
 struct GradRow { float iv, iy, back, c2; };
 
 template <bool kPost>
-__device__ __forceinline__ GradRow grad_row(const float (&s)[kPost ? 3 : 1], float iv, float iy, int64_t D) {
+__device__ __forceinline__ GradRow grad_row(const float (&s)[kPost ? 3 : 1], float iv, float iy, float over_d) {
   GradRow r{iv, iy, 0.0f, 0.0f};
-  const float n = (float)D, c1 = s[0] * iv / n;                // mean(dx w vh)
+  const float c1 = s[0] * iv * over_d;                         // mean(dx w vh)
   r.back = iv * iv * c1;
   // mean(dz post yh) is i(y) (s1 - back s2) / D
-  if constexpr (kPost) r.c2 = iy * iy * (iy * ((s[1] - r.back * s[2]) / n));
+  if constexpr (kPost) r.c2 = iy * iy * (iy * ((s[1] - r.back * s[2]) * over_d));
   return r;
 }
 
@@ -603,7 +627,7 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
       for (int i = 0; i < kN; ++i) s[i] += mine[i];
     }
     Sum::run(s, room, turn);
-    const GradRow row = grad_row<kPost>(s, o.iv, o.iy, g.D);
+    const GradRow row = grad_row<kPost>(s, o.iv, o.iy, g.over_d);
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       Column& k = of[c];
@@ -679,7 +703,7 @@ __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormG
                              a.post[j], a.y[j], s);
     }
     Sum::run(s, room, turn);
-    const GradRow row = grad_row<kPost>(s, iv, iy, g.D);
+    const GradRow row = grad_row<kPost>(s, iv, iy, g.over_d);
     if (threadIdx.x == 0) d.back[m] = row.back;
     for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
       const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;
@@ -727,72 +751,87 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormArgs g,
 // ---------------------------------------------------------------------------
 // Host side.
 
-// Calls fn with the launch shape of rows of D elements, or with no shape (void) past the registers.
-template <class Fn>
-void for_rows(int64_t D, const Fn& fn) {
-  if (D <= 128) fn(RowShape<16>{});
-  else if (D <= 512) fn(RowShape<64>{});
-  else if (D <= 1024) fn(RowShape<128>{});
-  else if (D <= 2048) fn(RowShape<256>{});
-  else if (D <= 4096) fn(RowShape<512>{});
-  else fn(RowShape<1024>{});
-}
 constexpr int64_t kMaxHeld = 8192;           // elements of a row that stay in registers
 bool grad_held(int64_t D) { return D >= 8 && D <= kMaxHeld; }
 
-int64_t rows_a_group(int64_t D) {
-  int64_t rows = 1;
-  if (D <= kMaxHeld) for_rows(D, [&](auto s) { rows = decltype(s)::kRows; });
-  return rows;
+template <int kT, int kC_>
+struct Launch : RowShape<kT> {
+  using Shape = RowShape<kT>;
+  static constexpr int kC = kC_;
+};
+
+// Calls fn with the launch shape of rows of D <= kMaxHeld elements.  Forward, sixteen elements a thread: half the
+// waves that meet at a row's barriers, and twice the rows on a CU (TODO).
+template <class Fn>
+void for_norm(int64_t D, const Fn& fn) {
+  if (D <= 128) fn(Launch<16, 1>{});
+  else if (D <= 512) fn(Launch<64, 1>{});
+  else if (D <= 1024) fn(Launch<64, 2>{});
+  else if (D <= 2048) fn(Launch<128, 2>{});
+  else if (D <= 4096) fn(Launch<256, 2>{});
+  else fn(Launch<512, 2>{});
+}
+template <class Fn>
+void for_grad(int64_t D, const Fn& fn) {
+  if (D <= 128) fn(Launch<16, 1>{});
+  else if (D <= 512) fn(Launch<64, 1>{});
+  else if (D <= 1024) fn(Launch<128, 1>{});
+  else if (D <= 2048) fn(Launch<256, 1>{});
+  else if (D <= 4096) fn(Launch<512, 1>{});
+  else fn(Launch<512, 2>{});
 }
 
-// Work groups of a forward pass: each CU's threads eight times over.
+// Work groups of a forward pass: 2^19 threads, what the card holds twice over, so that a group loads its weights
+// once for many rows (8192 x 8192 both ways 200 us, 229 with eight times as many groups).
 int64_t norm_groups(int64_t M, int64_t D) {
-  const int64_t rows = rows_a_group(D);
-  return std::min<int64_t>((M + rows - 1) / rows, 4096);
+  int64_t groups = std::min<int64_t>(M, 512);
+  if (D <= kMaxHeld)
+    for_norm(D, [&](auto s) { groups = std::min<int64_t>((M + s.kRows - 1) / s.kRows, (1 << 19) / s.kGroup); });
+  return groups;
 }
-// Of a gradient, which leaves D floats for each group and weight.
-int64_t grad_groups(int64_t M, int64_t D) {
-  const int64_t rows = rows_a_group(D);
-  return std::min<int64_t>((M + rows - 1) / rows, 512);
+// Of a gradient, as many as run at once, since each leaves D floats for each weight: 16 waves a CU where the
+// kernel keeps to 128 registers, else 8 (8192 x 4096: 101 us, float32 116; 129 and 160 with four times as many,
+// 114 with half).
+int64_t grad_groups(const fp64emu_norm_t* p) {
+  if (!grad_held(p->D)) return std::min<int64_t>(p->M, 512);
+  int64_t groups = 0;
+  for_grad(p->D, [&](auto s) {
+    const bool lean = s.kC == 1 && s.kT >= 64 && p->ld_gate == 0 && p->r_dtype != FP64EMU_F32;
+    groups = std::min<int64_t>((p->M + s.kRows - 1) / s.kRows, 256 * (lean ? 1024 : 512) / s.kGroup);
+  });
+  return groups;
 }
 
 template <int kR, int kY>
-int launch_norm(const NormArgs& g, bool tiles, hipStream_t s) {
-  NormArgs rows = g;
-  if (tiles) {                               // the statistics alone
-    rows.out = rows.x = nullptr;
-    rows.rows = Out8{};
-  }
+int launch_norm(const NormArgs& g, bool cols, hipStream_t s) {
   const unsigned groups = (unsigned)norm_groups(g.M, g.D);
   if (g.D > kMaxHeld) {
-    norm_long_kernel<kR, kY><<<groups, kLong, 0, s>>>(rows);
+    norm_long_kernel<kR, kY><<<groups, kLong, 0, s>>>(g);
   } else {
-    for_rows(g.D, [&](auto shape) {
-      using S = decltype(shape);
-      norm_rows_kernel<kR, kY, S><<<groups, S::kGroup, 0, s>>>(rows);
+    for_norm(g.D, [&](auto shape) {
+      using L = decltype(shape);
+      norm_rows_kernel<kR, kY, typename L::Shape, L::kC><<<groups, L::kGroup, 0, s>>>(g);
     });
   }
   if (int st = check_hip(hipGetLastError(), "norm_f8 launch")) return st;
-  if (!tiles) return FP64EMU_OK;
+  if (!cols) return FP64EMU_OK;
   norm_tile_kernel<kR, kY><<<(unsigned)((g.M + kBlk - 1) / kBlk * g.blocks), kThreads, 0, s>>>(g);
   return check_hip(hipGetLastError(), "norm_f8 launch");
 }
 
 template <int kR, int kY, bool kPost>
-int launch_grad(const NormArgs& g, const NormGradArgs& d, hipStream_t s) {
-  const unsigned groups = (unsigned)grad_groups(g.M, g.D);
+int launch_grad(const NormArgs& g, const NormGradArgs& d, unsigned groups, hipStream_t s) {
   if (!grad_held(g.D)) {
-    norm_grad_long_kernel<kR, kY, kPost><<<(unsigned)norm_groups(g.M, g.D), kLong, 0, s>>>(g, d);
+    norm_grad_long_kernel<kR, kY, kPost><<<(unsigned)std::min<int64_t>(g.M, 512), kLong, 0, s>>>(g, d);
     if (int st = check_hip(hipGetLastError(), "norm_f8_backward launch")) return st;
     const unsigned strips = (unsigned)((g.D + 8 * kThreads - 1) / (8 * kThreads));
     norm_grad_columns_kernel<kR, kY, kPost><<<dim3(groups, strips), kThreads, 0, s>>>(g, d);
   } else {
-    for_rows(g.D, [&](auto shape) {
-      using S = std::conditional_t<decltype(shape)::kT == 1024, RowShape<512>, decltype(shape)>;
-      constexpr int kC = decltype(shape)::kT == 1024 ? 2 : 1;
-      if (g.ld_gate) norm_grad_kernel<kR, kY, S, kC, kPost, true><<<groups, S::kGroup, 0, s>>>(g, d);
-      else norm_grad_kernel<kR, kY, S, kC, kPost, false><<<groups, S::kGroup, 0, s>>>(g, d);
+    for_grad(g.D, [&](auto shape) {
+      using L = decltype(shape);
+      using S = typename L::Shape;
+      if (g.ld_gate) norm_grad_kernel<kR, kY, S, L::kC, kPost, true><<<groups, L::kGroup, 0, s>>>(g, d);
+      else norm_grad_kernel<kR, kY, S, L::kC, kPost, false><<<groups, L::kGroup, 0, s>>>(g, d);
     });
   }
   return check_hip(hipGetLastError(), "norm_f8_backward launch");
@@ -839,6 +878,7 @@ int norm_args(const fp64emu_norm_t* p, NormArgs* g) {
   g->threshold = (uint32_t)p->drop;
   g->scale = p->scale;
   g->eps = p->eps;
+  g->over_d = 1.0f / (float)p->D;
   if (g->ld_gate && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
   return FP64EMU_OK;
 }
@@ -871,6 +911,7 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
   if (out && !p->y) return invalid("a new stream needs y");
   if (cols && !stats) return invalid("columns need stats");
   if (cols && x) return invalid("columns come without x in its plain form");
+  if (cols && out && out == p->r) return invalid("columns need r as it was: out must be elsewhere");
   if ((out && ld_out < p->D) || (x && ld_x < p->D)) return invalid("rows are shorter than D");
   NormArgs g;
   if (int st = norm_args(p, &g)) return st;
@@ -890,7 +931,7 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
 
 size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p) {
   if (check_norm(p) || p->M == 0 || p->D == 0) return 0;
-  const int64_t groups = grad_groups(p->M, p->D);
+  const int64_t groups = grad_groups(p);
   const size_t parts = groups > 1 ? 4 * (size_t)kMaxSums * (size_t)(groups * p->D) : 0;
   return parts + (grad_held(p->D) ? 0 : 4 * (size_t)p->M);
 }
@@ -938,7 +979,7 @@ int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const 
   a.ld_dr_out = d->ld_dr_out;
   a.ld_dy = d->ld_dy;
   a.ld_dgates = d->ld_dgates;
-  const int64_t groups = grad_groups(p->M, p->D);
+  const int64_t groups = grad_groups(p);
   float* room = static_cast<float*>(workspace);
   float** const to[kMaxSums] = {&a.dw, &a.dpost, &a.dgate};
   for (int i = 0; i < kMaxSums; ++i) {
@@ -952,8 +993,8 @@ int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const 
   all.groups = groups;
   all.D = p->D;
   const int st = for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {
-    return p->post ? launch_grad<decltype(r)::value, decltype(y)::value, true>(g, a, s)
-                   : launch_grad<decltype(r)::value, decltype(y)::value, false>(g, a, s);
+    return p->post ? launch_grad<decltype(r)::value, decltype(y)::value, true>(g, a, (unsigned)groups, s)
+                   : launch_grad<decltype(r)::value, decltype(y)::value, false>(g, a, (unsigned)groups, s);
   });
   return st ? st : launch_sums(all, count, s);
 }

@@ -427,7 +427,7 @@ typedef struct {
   float scale, eps;             /* eps > 0 */
 } fp64emu_norm_t;
 
-/* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype (may be r itself);
+/* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype (may be r itself, without cols);
  * `x` [M, D] in y's dtype; stats, i(v) of each row, then with post i(y), M floats each; `rows` and `cols`,
  * x quantised from its float32 values.  cols needs stats and comes without x. */
 int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x, int64_t ld_x, float* stats,

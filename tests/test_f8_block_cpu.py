@@ -102,7 +102,8 @@ def test_norm_refusals():
     plain = dict(y=None, post=None, gate=None)
     for kw, text in ((dict(out=None, x=None, stats=None), "no output"), (dict(**plain), "needs y"), (dict(ldo=255), "shorter"),
                      (dict(ldx=255), "shorter"), (dict(cols=_f8(256, 4)), "plain form"),
-                     (dict(x=None, stats=None, cols=_f8(256, 4)), "need stats"), (dict(rows=_f8(4, 256, fmt=1)), "e4m3"),
+                     (dict(x=None, stats=None, cols=_f8(256, 4)), "need stats"),
+                     (dict(x=None, cols=_f8(256, 4)), "elsewhere"), (dict(rows=_f8(4, 256, fmt=1)), "e4m3"),
                      (dict(rows=_f8(4, 256, tiles=1)), "e4m3"), (dict(rows=_f8(4, 256, s=None)), "null 8-bit")):
         _says(call(**kw), text)
     assert call(M=0) == 0 and L.fp64emu_norm_f8(None, P, 1, P, 1, P, None, None, None) == EINVAL
