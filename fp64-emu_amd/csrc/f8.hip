@@ -458,19 +458,30 @@ __device__ __forceinline__ void write4(int type, void* p, int64_t i, int valid, 
     if (j < valid) q[j] = r[j];
 }
 
-// Four successive outputs (m, n .. n + 3).
-__device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v) {
+// What an epilogue adds to four successive outputs (m, n .. n + 3).
+struct Added { v4f bias, residual; };
+
+__device__ __forceinline__ Added read_added(const MmArgs& g, int64_t b, int64_t m, int64_t n) {
   const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
   const bool vec = g.vec_o && valid == 4;    // of every operand of the epilogue, too
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  return {g.bias ? read4(g.bias_type, g.bias, b * g.bias_stride + n, valid, vec) : zero,
+          g.residual ? read4(g.dtype, g.residual, b * g.stride_res + m * g.ld_res + n, valid, vec) : zero};
+}
+
+// Four successive outputs (m, n .. n + 3).
+__device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v, const Added& added) {
+  const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
+  const bool vec = g.vec_o && valid == 4;
   const int64_t i = b * g.stride_o + m * g.ldo + n;
   if (g.epilogue) {
-    if (g.bias) v += read4(g.bias_type, g.bias, b * g.bias_stride + n, valid, vec);
+    if (g.bias) v += added.bias;
     if (g.keep) write4(g.dtype, g.keep, b * g.stride_keep + m * g.ld_keep + n, valid, vec, v);
     with_act(g.act, [&](auto act) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = activated<decltype(act)::value, true>(v[j]);
     });
-    if (g.residual) v += read4(g.dtype, g.residual, b * g.stride_res + m * g.ld_res + n, valid, vec);
+    if (g.residual) v += added.residual;
   }
   if (g.accumulate) v += read4(g.dtype, g.out, i, valid, vec);
   write4(g.dtype, g.out, i, valid, vec, v);
@@ -507,7 +518,8 @@ __global__ void __launch_bounds__(kThreads) sum_parts_kernel(MmArgs g) {
         for (int j = 0; j < 4; ++j)
           if (j < left) v[j] += p[s * one + j];
     }
-    store_out(g, bm / g.M, bm % g.M, n, v);
+    const int64_t b = bm / g.M, m = bm % g.M;
+    store_out(g, b, m, n, v, g.epilogue ? read_added(g, b, m, n) : Added{});
   }
 }
 
@@ -1284,6 +1296,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
     }
   };
 
+  // A wave stores at most one of the tiles; what the epilogue adds to it is read ahead of the loop (one
+  // token through 8192 x 8192 with bias and residual 14.2 us, 14.7 with it read at the end, 13.8 to 14.4 without either).
+  static_assert(kTN * kTM <= kFewWaves, "a tile a wave");
+  const int64_t m_out = m0 + (wave % kTM) * 16 + fr, n_out = n0 + (wave / kTM) * 16 + 4 * fg;
+  const bool stores = wave < kTN * kTM && m_out < g.M && n_out < g.N;
+  Added added{};
+  if (g.epilogue && stores && g.splits == 1) added = read_added(g, b, m_out, n_out);
+
   const int full = (int)(g.K / kBlk) < kb1 ? (int)(g.K / kBlk) : kb1;    // blocks before it are whole
   int kb = kb0 + wave;
   for (; kb + (kU - 1) * kFewWaves < full; kb += kU * kFewWaves) {
@@ -1315,15 +1335,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
 #pragma unroll
     for (int y = 0; y < kTM; ++y) red[wave][x * kTM + y][lane] = acc[x][y];
   __syncthreads();
-  for (int t = wave; t < kTN * kTM; t += kFewWaves) {
-    v4f v = red[0][t][lane];
+  if (!stores) return;
+  v4f v = red[0][wave][lane];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) v += red[w][t][lane];
-    const int64_t m = m0 + (t % kTM) * 16 + fr, n = n0 + (t / kTM) * 16 + 4 * fg;
-    if (m >= g.M || n >= g.N) continue;
-    if (g.splits > 1) store_part(g, split, b, m, n, v);
-    else store_out(g, b, m, n, v);
-  }
+  for (int w = 1; w < kFewWaves; ++w) v += red[w][wave][lane];
+  if (g.splits > 1) store_part(g, split, b, m_out, n_out, v);
+  else store_out(g, b, m_out, n_out, v, added);
 }
 
 // ---------------------------------------------------------------------------

@@ -174,19 +174,25 @@ def dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor, quant: str = None):
     return tuple(_dropout(x, drop, rng, form))
 
 
-def _check_norm(r, w, y, post, gate, eps=1.0):
-    if r.dim() != 2 or w.shape != r.shape[1:]:
-        raise ValueError(f"expect r [M, D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
-    if y is None and (post is not None or gate is not None):
-        raise ValueError("post and gate are of y")
-    if y is not None and y.shape != r.shape:
-        raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")
-    if post is not None and post.shape != w.shape:
+def _check_norm(r, w, y, post, gate, scale, drop, eps=1.0):
+    shape = r.shape                         # (a tensor's shape is made anew each time it is asked for)
+    width = shape[1:]
+    if len(shape) != 2 or w.shape != width:
+        raise ValueError(f"expect r [M, D] and w [D], got {tuple(shape)} and {tuple(w.shape)}")
+    if y is None:
+        if post is not None or gate is not None or drop or scale != 1.0:
+            raise ValueError("post, gate, scale and p are of y")
+    elif y.shape != shape:
+        raise ValueError(f"y must have r's shape {tuple(shape)}, got {tuple(y.shape)}")
+    if post is not None and post.shape != width:
         raise ValueError(f"expect post as [D], got {tuple(post.shape)}")
-    if gate is not None and gate.shape not in (w.shape, r.shape):
-        raise ValueError(f"expect gate as [D] or [M, D], got {tuple(gate.shape)}")
+    if gate is not None:
+        have = gate.shape
+        if have != width and have != shape:
+            raise ValueError(f"expect gate as [D] or [M, D], got {tuple(have)}")
     if not eps > 0.0:
         raise ValueError(f"eps must be positive, got {eps}")
+    return shape
 
 
 def norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torch.Tensor = None,
@@ -205,9 +211,7 @@ def norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torc
     (stats,), i(r') and, with post, i(y) of each row, for norm_f8_backward.  Sums of squares are
     float32 ones: rows past about 1e18 give x = 0."""
     form, drop = _form(quant), _drop(p, rng)
-    _check_norm(r, w, y, post, gate, eps)
-    if y is None and (drop or scale != 1.0):
-        raise ValueError("scale and p go with y")
+    _check_norm(r, w, y, post, gate, scale, drop, eps)
     return tuple(_norm(r, w, y, post, gate, scale, drop, rng, form, keep, eps))
 
 
@@ -220,14 +224,13 @@ def norm_f8_backward(dx: torch.Tensor, dr: torch.Tensor, r: torch.Tensor, w: tor
     Returns (dr, dy, dw, dpost, dgate), None for what is absent: dr in r's type, dy in y's, dw, dpost
     and the gradient of a gate [D] float32, that of a gate [M, D] in its type."""
     drop = _drop(p, rng)
-    _check_norm(r, w, y, post, gate)
-    if dx.shape != r.shape or (dr is not None and dr.shape != r.shape):
-        raise ValueError(f"dx and dr must have r's shape {tuple(r.shape)}")
-    if y is None and (drop or scale != 1.0):
-        raise ValueError("scale and p go with y")
-    got = iter(_norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng))
-    out = [next(got) if there else None for there in (True, y is not None, True, post is not None)]
-    return (*out, next(got, None))
+    shape = _check_norm(r, w, y, post, gate, scale, drop)
+    if dx.shape != shape or (dr is not None and dr.shape != shape):
+        raise ValueError(f"dx and dr must have r's shape {tuple(shape)}")
+    got = _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng)
+    if y is None:
+        return got[0], None, got[1], None, None
+    return got[0], got[1], got[2], None if post is None else got[3], None if gate is None else got[-1]
 
 
 def swiglu_f8(h: torch.Tensor, quant: str = None, keep: bool = True):
