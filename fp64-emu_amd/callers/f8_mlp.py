@@ -16,6 +16,10 @@ One training step:
 
 Serving a token: x's rows, h, y's rows, out; nothing kept.
 
+`Block` is that MLP in a residual stream, between the norms before and after it, with a gate and
+dropout (fp64_emu.norm_f8 and its gradient): x comes from the norm in 8 bits both ways, and
+the next block's input from the norm of the stream that out has joined.
+
     python fp64-emu_amd/callers/f8_mlp.py [d=4096] [f=4096] [tokens=8192]
 """
 import argparse
@@ -49,7 +53,10 @@ class GatedMlp:
 
     def forward(self, x):
         """(out, what backward takes): x [tokens, d] in bfloat16."""
-        q, s, *x_cols = emu.quant_f8(x, cols=True)
+        return self.forward_f8(*emu.quant_f8(x, cols=True))
+
+    def forward_f8(self, q, s, *x_cols):
+        """The same for x quantised both ways."""
         h = emu.mm_f8(q, s, *self.q1[:2])
         yq, ys, yqt, yst, hq, hs = emu.swiglu_f8(h, quant="both")
         return emu.mm_f8(yq, ys, *self.q2[:2]), (x_cols, (yqt, yst), (hq, hs))
@@ -66,7 +73,10 @@ class GatedMlp:
 
     def serve(self, x):
         """out for tokens that nothing is kept of."""
-        h = emu.mm_f8(*emu.quant_f8(x), *self.q1[:2])
+        return self.serve_f8(*emu.quant_f8(x))
+
+    def serve_f8(self, q, s):
+        h = emu.mm_f8(q, s, *self.q1[:2])
         return emu.mm_f8(*emu.swiglu_f8(h, quant="rows", keep=False), *self.q2[:2])
 
     def sgd(self, rate):
@@ -75,6 +85,43 @@ class GatedMlp:
         self.g1.zero_()
         self.g2.zero_()
         self.quantise()
+
+
+class Block:
+    """r -> (r', x'): x = norm(r) w0, y = mlp(x), r' = r + gate drop(norm(y) post), x' = norm(r') w1,
+    for a bfloat16 stream r [tokens, d]; w0, post, gate and w1 [d] float32, their gradients added to g."""
+
+    NAMES = ("w0", "post", "gate", "w1")
+
+    def __init__(self, d, f, seed=0, p=0.1, device="cuda"):
+        self.mlp, self.p = GatedMlp(d, f, seed, device), p
+        gen = torch.Generator().manual_seed(seed + 100)
+        for name, mean in zip(self.NAMES, (1.0, 1.0, 0.5, 1.0)):
+            setattr(self, name, (mean + 0.1 * torch.randn(d, generator=gen)).to(device))
+        self.g = {name: torch.zeros(d, device=device) for name in self.NAMES}
+
+    def forward(self, r, rng):
+        """(r', x', what backward takes).  rng is the call's own: not to go on before the backward pass."""
+        *x, stats0 = emu.norm_f8(r, self.w0, quant="both", keep=True)
+        y, kept = self.mlp.forward_f8(*x)
+        new, out, stats1 = emu.norm_f8(r, self.w1, y, self.post, self.gate, p=self.p, rng=rng, keep=True)
+        return new, out, (r, stats0, kept, y, new, stats1, rng)
+
+    def backward(self, dnew, dout, kept):
+        """dr."""
+        r, stats0, mlp_kept, y, new, stats1, rng = kept
+        dr, dy, dw1, dpost, dgate = emu.norm_f8_backward(dout, dnew, new, self.w1, stats1, y, self.post, self.gate,
+                                                         p=self.p, rng=rng)
+        dx = self.mlp.backward(dy, mlp_kept)
+        dr, _, dw0, _, _ = emu.norm_f8_backward(dx, dr, r, self.w0, stats0)
+        for name, grad in zip(self.NAMES, (dw0, dpost, dgate, dw1)):
+            self.g[name] += grad
+        return dr
+
+    def serve(self, r):
+        """(r', x') for tokens that nothing is kept or dropped of."""
+        y = self.mlp.serve_f8(*emu.norm_f8(r, self.w0, quant="rows"))
+        return emu.norm_f8(r, self.w1, y, self.post, self.gate)
 
 
 class PlainMlp:
@@ -137,10 +184,18 @@ def run(d, f, tokens, device="cuda"):
         _, kept = net.forward(x)
         net.backward(dout, kept)
 
+    block = Block(d, f, device=device)
+    rng = torch.tensor([1, 0], device=device)
+
+    def block_step():
+        _, _, kept = block.forward(x, rng)
+        block.backward(dout, dout, kept)
+
     _, kept = net.forward(x)
     held = sum(t.numel() * t.element_size() for pair in kept for t in pair)
     train_s, token_s = _time(step), _time(lambda: net.serve(x[:1]))
-    return {"step_ms": train_s * 1e3, "step_tflops": 18 * tokens * d * f / train_s / 1e12,
+    block_s, block_token_s = _time(block_step), _time(lambda: block.serve(x[:1]))
+    return {"block_ms": block_s * 1e3, "block_token_us": block_token_s * 1e6, "step_ms": train_s * 1e3, "step_tflops": 18 * tokens * d * f / train_s / 1e12,
             "token_us": token_s * 1e6, "held_mb": held / 1e6,
             "held_bf16_mb": 2 * tokens * (d + 3 * f) / 1e6}
 
@@ -155,6 +210,8 @@ def main():
     print(f"{torch.cuda.get_device_name(0)} | d={a.d} f={a.f} tokens={a.tokens}", flush=True)
     print(f"forward and backward {r['step_ms']:.3f} ms, {r['step_tflops']:.0f} TFLOP/s | held for the backward pass "
           f"{r['held_mb']:.1f} MB ({r['held_bf16_mb']:.1f} MB in bfloat16) | one token {r['token_us']:.1f} us",
+          flush=True)
+    print(f"the block around it: forward and backward {r['block_ms']:.3f} ms | one token {r['block_token_us']:.1f} us",
           flush=True)
     print("losses after 60 steps:", {k: round(v, 5) for k, v in train().items()}, flush=True)
 

@@ -758,16 +758,26 @@ __device__ __forceinline__ void finish_tile(const MmArgs& g, uint8_t* lds, const
       }
     }
     if (g.act) {
+      // Without a residual the loop stores, too.
+      const bool last = !g.residual;
       with_act(g.act, [&](auto act) {
 #pragma unroll 1
         for (int i = 0; i < kSteps; ++i) {
+          const int64_t m = first + i * kRows;
           float v[kEach];
           get(i, v);
 #pragma unroll
           for (int j = 0; j < kEach; ++j) v[j] = activated<decltype(act)::value, kExact>(v[j]);
-          __builtin_memcpy(__builtin_assume_aligned(line + i * kRows * kRow, 16), v, 4 * kEach);
+          if (last) {
+            T w[kEach];
+            round(v, w);
+            if (m < g.M) put_line(g.out, b * g.stride_o + m * g.ldo + n, w);
+          } else {
+            __builtin_memcpy(__builtin_assume_aligned(line + i * kRows * kRow, 16), v, 4 * kEach);
+          }
         }
       });
+      if (last) continue;
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {

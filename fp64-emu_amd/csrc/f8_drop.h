@@ -35,6 +35,9 @@ __device__ __forceinline__ Drop drop_of(uint32_t threshold, const int64_t* rng) 
 __device__ __forceinline__ v4u random_bits(const Drop& d, uint64_t chunk) {
   uint32_t x0 = (uint32_t)chunk, x1 = (uint32_t)(chunk >> 32), x2 = d.offset[0], x3 = d.offset[1];
   uint32_t k0 = d.seed[0], k1 = d.seed[1];
+  // (The ten rounds' keys anew for each chunk: kept from one to the next they and a kernel's pointers do
+  // not fit the scalar registers.)
+  asm("" : "+s"(k0), "+s"(k1) : "v"((uint32_t)chunk));
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)x0 * 0xd2511f53u, b = (uint64_t)x2 * 0xcd9e8d57u;
@@ -48,14 +51,24 @@ __device__ __forceinline__ v4u random_bits(const Drop& d, uint64_t chunk) {
   return v4u{x0, x1, x2, x3};
 }
 
-// Which of a chunk's elements stay, a bit each.
+// A chunk's bits, and which of its elements stay: compared where they are, the higher half of a word as
+// the whole word, which takes half the instructions of a mask of eight bits made first and asked later.
+struct Kept {
+  v4u w;
+  uint32_t threshold;                        // in the higher half
+  __device__ __forceinline__ Kept(const Drop& d, uint64_t chunk) : threshold(d.threshold << 16) {
+    w = d.threshold ? random_bits(d, chunk) : v4u{0u, 0u, 0u, 0u};
+  }
+  __device__ __forceinline__ bool at(int j) const { return (j & 1 ? w[j >> 1] : w[j >> 1] << 16) >= threshold; }
+};
+
+// The same as a mask, a bit each, where it is kept from one use to the next.
 __device__ __forceinline__ uint32_t kept_of(const Drop& d, uint64_t chunk) {
   if (d.threshold == 0) return 0xffu;
-  const v4u w = random_bits(d, chunk);
+  const Kept k(d, chunk);
   uint32_t kept = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    kept |= (uint32_t)((w[j >> 1] >> (16 * (j & 1)) & 0xffffu) >= d.threshold) << j;
+  for (int j = 0; j < 8; ++j) kept |= (uint32_t)k.at(j) << j;
   return kept;
 }
 

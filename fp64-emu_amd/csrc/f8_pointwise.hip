@@ -120,9 +120,9 @@ struct DropArgs {
 
 template <int kT>
 __device__ __forceinline__ void dropped(const Held<kT>& x, int p, const Drop& drop, uint64_t chunk, float (&y)[8]) {
-  const uint32_t kept = kept_of(drop, chunk);
+  const Kept kept(drop, chunk);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = kept >> j & 1 ? x.at(p, j) * drop.scale : 0.0f;
+  for (int j = 0; j < 8; ++j) y[j] = kept.at(j) ? x.at(p, j) * drop.scale : 0.0f;
 }
 
 template <int kT>

@@ -190,8 +190,8 @@ def _check_norm(r, w, y, post, gate, scale, drop, eps=1.0):
         have = gate.shape
         if have != width and have != shape:
             raise ValueError(f"expect gate as [D] or [M, D], got {tuple(have)}")
-    if not eps > 0.0:
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not eps >= 2.0 ** -126:
+        raise ValueError(f"eps must be positive and not denormal, got {eps}")
     return shape
 
 

@@ -424,7 +424,7 @@ typedef struct {
   int r_dtype, y_dtype;         /* y_dtype: of y and x; r_dtype the same or FP64EMU_F32 */
   int w_dtype, post_dtype, gate_dtype;  /* any; of a gate for each row: y_dtype */
   int drop;                     /* of 65536 */
-  float scale, eps;             /* eps > 0 */
+  float scale, eps;             /* eps at least 2^-126 */
 } fp64emu_norm_t;
 
 /* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype (may be r itself, without cols);

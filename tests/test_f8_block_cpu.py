@@ -84,7 +84,7 @@ def _norm(M=4, D=256, **kw):
 NORM_REFUSALS = [
     (dict(M=-1), "non-negative"), (dict(D=1 << 27), "2^27"), (dict(M=1 << 40), "2^40"), (dict(r_dtype=4), "dtype must"),
     (dict(w_dtype=4), "dtype must"), (dict(post_dtype=-1), "dtype must"), (dict(gate_dtype=3), "dtype must"),
-    (dict(r_dtype=BF16, y_dtype=F32), "y's dtype"), (dict(r_dtype=F16, y_dtype=BF16), "y's dtype"), (dict(eps=0.0), "eps"),
+    (dict(r_dtype=BF16, y_dtype=F32), "y's dtype"), (dict(r_dtype=F16, y_dtype=BF16), "y's dtype"), (dict(eps=0.0), "eps"), (dict(eps=1e-40), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(drop=65536), "0 .. 65535"), (dict(drop=-1), "0 .. 65535"), (dict(y=None), "need y"),
     (dict(y=None, post=None, gate=None, drop=7), "need y"), (dict(drop=7, rng=None), "needs rng"), (dict(r=None), "null"),
     (dict(w=None), "null"), (dict(ld_r=255), "shorter than D"), (dict(ld_y=255), "shorter than D"),
