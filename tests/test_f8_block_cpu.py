@@ -236,3 +236,23 @@ def test_plain_norm_gradient(post, gates, p):
     names = ["dr", "dy", "dw"] + (["dpost"] if post else []) + ["dgate" if gates else "dgate sum"]
     for n, t in zip(names, want):
         assert torch.allclose(got[n][0], t, rtol=1e-9, atol=1e-11), n
+
+
+def test_no_derivative_is_said():
+    """Results of the ops for tensors that require a gradient raise in the backward pass; under no_grad, or
+    where nothing requires one, they have no history."""
+    e = fp64_emu
+    with FakeTensorMode():
+        x = torch.empty(8, 256, device="cuda")
+        w, h = torch.empty(256, device="cuda"), torch.empty(8, 256, device="cuda", requires_grad=True)
+        q, s = e.quant_f8(x)
+        rng, stats = torch.empty(2, dtype=torch.int64, device="cuda"), torch.empty(1, 8, device="cuda")
+        calls = (lambda t: e.norm_f8(t, w), lambda t: e.norm_f8(x, w, t), lambda t: e.norm_f8_backward(t, x, x, w, stats)[:1],
+                 lambda t: e.act_f8_backward(t, x, "silu"), lambda t: e.dropout_f8(t, 0.5, rng),
+                 lambda t: [e.mm_f8(q, s, q, s, torch.float32, bias=t[0, :8], act="relu")])
+        for call in calls:
+            for out in call(h):
+                assert out.requires_grad and out.grad_fn.name().endswith("NotImplemented")
+            assert not any(t.requires_grad for t in call(x))
+            with torch.no_grad():
+                assert not any(t.requires_grad for t in call(h))
