@@ -390,8 +390,9 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
 }
 
 // x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
-// else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways TODO us; with the
-// statistics alone from that kernel and all outputs from this one 113).
+// else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways 110 us, with the
+// statistics alone from that kernel and all outputs from this one 113; since then 97 to 102, 61 and 37
+// of them, the generator 14).  Bound by its bytes: r and y again and a byte a value, 4.7 TB/s.
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;
@@ -535,7 +536,9 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
 // do not fit.  A row's values stay as they came and are worked out again after its sums; with one
 // chunk the next row's are on their way meanwhile.  A row's last, partial eight elements are its last eight: what the
 // thread beside has of them comes out the same from both and counts once in the sums (with loads and stores
-// of parts the kernel took 195 registers).  kPost: y has a norm; without it y may be absent, too.  kGates: a gate
+// of parts the kernel took 195 registers).  8192 x 4096 bfloat16 with everything 90 to 96 us, the last sums' 5 among
+// them: 4.2 to 4.5 TB/s of the copy's 5.2; two work groups of 512 on a CU share its vector units, which take about half
+// that time, and each waits for its row's one barrier.  kPost: y has a norm; without it y may be absent, too.  kGates: a gate
 // for each row, whose values and gradient do not fit 128 registers as the rest does.
 template <int kR, int kY, class S, int kC, bool kPost, bool kGates>
 __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU_F32 && S::kT >= 64 ? 4 : 2)
@@ -855,6 +858,7 @@ int launch_grad(const NormArgs& g, const NormGradArgs& d, unsigned groups, hipSt
 int check_norm(const fp64emu_norm_t* p) {
   if (!p) return invalid("norm must not be NULL");
   if (p->M < 0 || p->D < 0) return invalid("shapes must be non-negative");
+  if (p->D == 0) return invalid("rows of nothing have no norm");
   if (p->M >= 1ll << 40 || p->D >= 1ll << 27) return invalid("shapes must be below 2^40 rows of 2^27 elements");
   if (!known_dtype(p->r_dtype) || !known_dtype(p->y_dtype) || !known_dtype(p->w_dtype) ||
       !known_dtype(p->post_dtype) || !known_dtype(p->gate_dtype))
@@ -863,7 +867,7 @@ int check_norm(const fp64emu_norm_t* p) {
     return invalid("y's dtype must be r's, or r's FP64EMU_F32");
   if (!(p->eps >= 0x1p-126f)) return invalid("eps must be positive and not denormal");
   if (p->drop < 0 || p->drop > 65535) return invalid("drop must be in 0 .. 65535");
-  if (p->M == 0 || p->D == 0) return FP64EMU_OK;              // (whose operands have no address)
+  if (p->M == 0) return FP64EMU_OK;                           // (operands that have no address)
   if (!p->y && (p->post || p->gate || p->drop)) return invalid("post, gate and drop need y");
   if (p->drop && !p->rng) return invalid("drop needs rng");
   return FP64EMU_OK;
@@ -921,7 +925,7 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
   if (int st = check_norm(p)) return st;
   for (const fp64emu_f8_t* f : {rows, cols})
     if (f && (f->fmt != FP64EMU_E4M3 || f->tiles)) return invalid("outputs are e4m3 with scales by rows");
-  if (p->M == 0 || p->D == 0) return FP64EMU_OK;
+  if (p->M == 0) return FP64EMU_OK;
   if (!out && !x && !rows && !cols && !stats) return invalid("no output asked for");
   if (out && !p->y) return invalid("a new stream needs y");
   if (cols && !stats) return invalid("columns need stats");
@@ -945,7 +949,7 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
 }
 
 size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p) {
-  if (check_norm(p) || p->M == 0 || p->D == 0) return 0;
+  if (check_norm(p) || p->M == 0) return 0;
   const int64_t groups = grad_groups(p);
   const size_t parts = groups > 1 ? 4 * (size_t)kMaxSums * (size_t)(groups * p->D) : 0;
   return parts + (grad_held(p->D) ? 0 : 4 * (size_t)p->M);
@@ -959,7 +963,6 @@ int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const 
   if ((d->dpost && !p->post) || ((d->dgate || d->dgates) && !p->gate)) return invalid("gradients of what is absent");
   if (d->dgate && d->dgates) return invalid("gate's gradient is a row or a matrix");
   if (d->dgates && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
-  if (p->D == 0) return FP64EMU_OK;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   float* const sums[kMaxSums] = {d->dw, d->dpost, d->dgate};
   Sums all{};

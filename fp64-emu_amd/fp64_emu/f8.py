@@ -177,7 +177,7 @@ def dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor, quant: str = None):
 def _check_norm(r, w, y, post, gate, scale, drop, eps=1.0):
     shape = r.shape                         # (a tensor's shape is made anew each time it is asked for)
     width = shape[1:]
-    if len(shape) != 2 or w.shape != width:
+    if len(shape) != 2 or w.shape != width or not width[0]:
         raise ValueError(f"expect r [M, D] and w [D], got {tuple(shape)} and {tuple(w.shape)}")
     if y is None:
         if post is not None or gate is not None or drop or scale != 1.0:

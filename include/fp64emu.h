@@ -419,7 +419,7 @@ typedef struct {
   const void *r, *y;            /* [M, D], rows ld_r and ld_y apart; y may be NULL */
   const void *w, *post, *gate;  /* [D]; post and gate may be NULL; gate [M, D] with ld_gate >= D */
   const int64_t* rng;           /* device; with drop > 0 */
-  int64_t M, D;                 /* D < 2^27 */
+  int64_t M, D;                 /* 0 < D < 2^27 */
   int64_t ld_r, ld_y, ld_gate;  /* ld_gate 0: one gate for all rows */
   int r_dtype, y_dtype;         /* y_dtype: of y and x; r_dtype the same or FP64EMU_F32 */
   int w_dtype, post_dtype, gate_dtype;  /* any; of a gate for each row: y_dtype */

@@ -82,7 +82,7 @@ def _norm(M=4, D=256, **kw):
 
 
 NORM_REFUSALS = [
-    (dict(M=-1), "non-negative"), (dict(D=1 << 27), "2^27"), (dict(M=1 << 40), "2^40"), (dict(r_dtype=4), "dtype must"),
+    (dict(M=-1), "non-negative"), (dict(D=0), "no norm"), (dict(D=1 << 27), "2^27"), (dict(M=1 << 40), "2^40"), (dict(r_dtype=4), "dtype must"),
     (dict(w_dtype=4), "dtype must"), (dict(post_dtype=-1), "dtype must"), (dict(gate_dtype=3), "dtype must"),
     (dict(r_dtype=BF16, y_dtype=F32), "y's dtype"), (dict(r_dtype=F16, y_dtype=BF16), "y's dtype"), (dict(eps=0.0), "eps"), (dict(eps=1e-40), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(drop=65536), "0 .. 65535"), (dict(drop=-1), "0 .. 65535"), (dict(y=None), "need y"),
@@ -146,7 +146,7 @@ def test_python_refusals():
                  lambda: e.dropout_f8(x[0], 0.5, rng), lambda: e.dropout_f8(x, 0.5, rng, "cols"), lambda: e.norm_f8(x[0], w),
                  lambda: e.norm_f8(x, w[:3]), lambda: e.norm_f8(x, w, post=w), lambda: e.norm_f8(x, w, gate=w),
                  lambda: e.norm_f8(x, w, x[:2]), lambda: e.norm_f8(x, w, x, post=x), lambda: e.norm_f8(x, w, x, gate=w[:5]),
-                 lambda: e.norm_f8(x, w, eps=0.0), lambda: e.norm_f8(x, w, scale=2.0), lambda: e.norm_f8(x, w, p=0.5, rng=rng),
+                 lambda: e.norm_f8(x, w, eps=0.0), lambda: e.norm_f8(x[:, :0], w[:0]), lambda: e.norm_f8(x, w, scale=2.0), lambda: e.norm_f8(x, w, p=0.5, rng=rng),
                  lambda: e.norm_f8(x, w, x, p=0.5), lambda: e.norm_f8(x, w, quant="cols"),
                  lambda: e.norm_f8_backward(x[:2], None, x, w, x), lambda: e.norm_f8_backward(x, x[:2], x, w, x),
                  lambda: e.norm_f8_backward(x, None, x, w, x, post=w), lambda: e.norm_f8_backward(x, None, x, w, x, scale=0.5),

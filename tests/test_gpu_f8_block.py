@@ -479,3 +479,17 @@ def test_block_refusals(dev):
                  lambda: fp64_emu.mm_f8(q, s, q, s, F32, bias=leaf[0, :4])):
         with pytest.raises(RuntimeError):
             call().sum().backward()
+
+
+@pytest.mark.parametrize("shape,N", [((0, 256), 70), ((5, 0), 70), ((2, 0, 128), 40), ((3, 128), 0)])
+def test_linear_epilogue_of_nothing(dev, shape, N):
+    """No rows, no depth, no columns: an empty sum's epilogue and gradients of zeros."""
+    print("case linear of nothing", shape, N, flush=True)
+    K = shape[-1]
+    x, w, b = (torch.ones(s, device=dev).requires_grad_() for s in (shape, (N, K), (N,)))
+    r = torch.ones(*shape[:-1], N, device=dev).requires_grad_()
+    y = fp64_emu.linear_f8(x, w, bias=b, act="relu", residual=r)
+    assert y.shape == r.shape and (K != 0 or torch.equal(y, torch.full_like(y, 2.0)))
+    grads = torch.autograd.grad(y, (x, w, b, r), torch.ones_like(y))
+    assert [g.shape for g in grads] == [t.shape for t in (x, w, b, r)]
+    assert torch.equal(grads[2], torch.full_like(b, float(y.numel() // max(N, 1)))) and not grads[1].any()
