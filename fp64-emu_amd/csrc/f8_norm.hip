@@ -92,23 +92,53 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int valid, float
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = e.at(j);
 }
-// The same of any type, or ones.
-__device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, int valid, float (&v)[8]) {
-  if (!p) {
+// Eight elements of a weight of any type, as they came (ones without one): loaded first, told apart where
+// they are used.  With the type's branch around load and conversion a kernel waited for each weight before it
+// asked for the next, six memory latencies for a row of 8192 (one row 6.4 us, now 5.8).
+struct EightAny {
+  v4u a, b;
+  __device__ __forceinline__ void load(int type, const void* p, int64_t i, int valid) {
+    a = b = v4u{0u, 0u, 0u, 0u};
+    if (!p || valid <= 0) return;
+    if (valid < 8) {
+      if (type == FP64EMU_F32) {
+        const uint32_t* q = static_cast<const uint32_t*>(p) + i;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 1.0f;
-  } else if (type == FP64EMU_F32) {
-    load8<FP64EMU_F32>(p, i, valid, v);
-  } else {
-    Eight<FP64EMU_BF16> e;
-    if (valid >= 8) e.whole(p, i);
-    else e.part(p, i, valid);
+        for (int j = 0; j < 7; ++j)
+          if (j < valid) (j < 4 ? a : b)[j & 3] = q[j];
+      } else {
+        const unsigned short* q = static_cast<const unsigned short*>(p) + i;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t h = e.w[j >> 1] >> (16 * (j & 1));
-      v[j] = type == FP64EMU_BF16 ? bf16_value((unsigned short)h) : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+        for (int j = 0; j < 7; ++j)
+          if (j < valid) a[j >> 1] |= (uint32_t)q[j] << (16 * (j & 1));
+      }
+    } else if (type == FP64EMU_F32) {
+      __builtin_memcpy(&a, static_cast<const float*>(p) + i, 16);
+      __builtin_memcpy(&b, static_cast<const float*>(p) + i + 4, 16);
+    } else {
+      __builtin_memcpy(&a, static_cast<const unsigned short*>(p) + i, 16);
     }
   }
+  __device__ __forceinline__ void values(int type, const void* p, float (&v)[8]) const {
+    if (!p) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 1.0f;
+    } else if (type == FP64EMU_F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_bit_cast(float, j < 4 ? a[j & 3] : b[j & 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t h = a[j >> 1] >> (16 * (j & 1));
+        v[j] = type == FP64EMU_BF16 ? bf16_value((unsigned short)h) : (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+      }
+    }
+  }
+};
+__device__ __forceinline__ void load8_any(int type, const void* p, int64_t i, int valid, float (&v)[8]) {
+  EightAny e;
+  e.load(type, p, i, valid);
+  e.values(type, p, v);
 }
 
 template <int kCtrl, int kRowMask = 0xf>
@@ -218,9 +248,9 @@ __device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t 
 // Rows whose values stay in registers from the first sum to the last store, kC times eight elements a
 // thread (element 8 (c kT + t) on).  A work group takes rows blockIdx.x kRows + .., gridDim.x kRows
 // apart, the weights in registers throughout and the next row's values on their way.  Bound by its
-// bytes: 8192 x 4096 bfloat16 with everything 54 us in 8 bits (4.4 TB/s), 52 plain (5.1, as a copy).  512 threads
-// a row keep to 128 registers, so that two rows are on a CU (8192 x 8192 182 us both ways, else 195); for
-// fewer threads the spills cost more (62 us).
+// bytes: 8192 x 4096 bfloat16 with everything 51 us in 8 bits (4.6 TB/s), 49 plain (5.5: some of it stays in the
+// 256 MB cache).  512 threads a row keep to 128 registers, so that two rows are on a CU (8192 x 8192 182 us both
+// ways, else 195); for fewer threads the spills cost more (8192 x 4096 62 us where 54 without).
 template <int kR, int kY, class S, int kC>
 __global__ void __launch_bounds__(S::kGroup, S::kT == 512 && kR != FP64EMU_F32 ? 4 : 1) norm_rows_kernel(NormArgs g) {
   constexpr int kT = S::kT;
@@ -233,11 +263,8 @@ __global__ void __launch_bounds__(S::kGroup, S::kT == 512 && kR != FP64EMU_F32 ?
   int valid[kC];
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
-    const int col = 8 * (c * kT + t), left = (int)g.D - col;
+    const int left = (int)g.D - 8 * (c * kT + t);
     valid[c] = left < 0 ? 0 : left < 8 ? left : 8;
-    load8_any(g.w_type, g.w, col, valid[c], w[c]);
-    load8_any(g.post_type, g.post, col, valid[c], post[c]);
-    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, valid[c], gate[c]);
   }
   int turn = 0;
   Eight<kR> r[kC];
@@ -264,6 +291,22 @@ __global__ void __launch_bounds__(S::kGroup, S::kT == 512 && kR != FP64EMU_F32 ?
   const int64_t step = (int64_t)gridDim.x * S::kRows;
   int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
   fetch(m);
+  {
+    EightAny ew[kC], ep[kC], eg[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int col = 8 * (c * kT + t);
+      ep[c].load(g.post_type, g.post, col, valid[c]);
+      eg[c].load(g.gate_type, g.ld_gate == 0 ? g.gate : nullptr, col, valid[c]);
+      ew[c].load(g.w_type, g.w, col, valid[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      ep[c].values(g.post_type, g.post, post[c]);
+      eg[c].values(g.gate_type, g.gate, gate[c]);
+      ew[c].values(g.w_type, g.w, w[c]);
+    }
+  }
   for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
     Eight<kR> ro[kC];
     Eight<kY> yo[kC], go[kC];
@@ -563,10 +606,6 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
     o.in = left > 0;
     o.again = left > 0 && left < 8 ? 8 - left : 0;
     o.col = col - o.again;
-    const int valid = o.in ? 8 : 0;
-    load8_any(g.w_type, g.w, o.col, valid, o.w);
-    if constexpr (kPost) load8_any(g.post_type, g.post, o.col, valid, o.post);
-    if constexpr (!kGates) load8_any(g.gate_type, g.gate, o.col, valid, o.gate);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o.dw[j] = o.dpost[j] = o.dgate[j] = 0.0f;
   }
@@ -606,6 +645,22 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
   int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
   Row next;
   if constexpr (kAhead) fetch(m, next);
+  {
+    EightAny ew[kC], ep[kC], eg[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int col = of[c].col, valid = of[c].in ? 8 : 0;
+      ew[c].load(g.w_type, g.w, col, valid);
+      if constexpr (kPost) ep[c].load(g.post_type, g.post, col, valid);
+      if constexpr (!kGates) eg[c].load(g.gate_type, g.gate, col, valid);
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      ew[c].values(g.w_type, g.w, of[c].w);
+      if constexpr (kPost) ep[c].values(g.post_type, g.post, of[c].post);
+      if constexpr (!kGates) eg[c].values(g.gate_type, g.gate, of[c].gate);
+    }
+  }
   for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
     Row o;
     if constexpr (kAhead) {
