@@ -94,7 +94,7 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int valid, float
 }
 // Eight elements of a weight of any type, as they came (ones without one): loaded first, told apart where
 // they are used.  With the type's branch around load and conversion a kernel waited for each weight before it
-// asked for the next, six memory latencies for a row of 8192 (one row 6.4 us, now 5.8).
+// asked for the next (8192 x 4096 rows 54 us, 51 without).
 struct EightAny {
   v4u a, b;
   __device__ __forceinline__ void load(int type, const void* p, int64_t i, int valid) {
@@ -245,112 +245,82 @@ __device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t 
   }
 }
 
-// Rows whose values stay in registers from the first sum to the last store, kC times eight elements a
-// thread (element 8 (c kT + t) on).  A work group takes rows blockIdx.x kRows + .., gridDim.x kRows
-// apart, the weights in registers throughout and the next row's values on their way.  Bound by its
-// bytes: 8192 x 4096 bfloat16 with everything 51 us in 8 bits (4.6 TB/s), 49 plain (5.5: some of it stays in the
-// 256 MB cache).  512 threads a row keep to 128 registers, so that two rows are on a CU (8192 x 8192 182 us both
-// ways, else 195); for fewer threads the spills cost more (8192 x 4096 62 us where 54 without).
-template <int kR, int kY, class S, int kC>
-__global__ void __launch_bounds__(S::kGroup, S::kT == 512 && kR != FP64EMU_F32 ? 4 : 1) norm_rows_kernel(NormArgs g) {
+// Rows whose values stay in registers from the first sum to the last store.  A work group takes
+// rows blockIdx.x kRows + .., gridDim.x kRows apart, the weights in registers throughout and the next
+// row's values on their way.  Bound by its bytes: 8192 x 4096 bfloat16 with everything 50 us in 8 bits
+// (4.7 TB/s), 48 plain (5.6: some of it stays in the 256 MB cache).  (Sixteen elements a thread: as fast, and one row
+// of 8192 5.6 us where this takes 4.4.)
+template <int kR, int kY, class S>
+__global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   constexpr int kT = S::kT;
   using Sum = RowSum<kT, 1, S::kGroup>;
   __shared__ typename Sum::Room room;
   const int t = threadIdx.x % kT, sub = S::sub();
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
   const int64_t row_chunks = (g.D + 7) / 8;
-  float w[kC][8], post[kC][8], gate[kC][8];
-  int valid[kC];
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    const int left = (int)g.D - 8 * (c * kT + t);
-    valid[c] = left < 0 ? 0 : left < 8 ? left : 8;
-  }
+  const int col = 8 * t, left = (int)g.D - col, valid = left < 0 ? 0 : left < 8 ? left : 8;
   int turn = 0;
-  Eight<kR> r[kC];
-  Eight<kY> y[kC], gates[kC];
+  Eight<kR> r;
+  Eight<kY> y, gates;
   auto fetch = [&](int64_t m) {
     const uint8_t* pr = S::template row<kR>(g.r, m, g.ld_r);
     const uint8_t* py = S::template row<kY>(g.y, m, g.ld_y);
     const uint8_t* pg = S::template row<kY>(g.gate, m, g.ld_gate);
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      const int n = m < g.M ? valid[c] : 0, col = 8 * (c * kT + t);
-      if (n == 8) {
-        r[c].whole(pr, col);
-        y[c].zero();
-        if (g.y) y[c].whole(py, col);
-        if (g.ld_gate) gates[c].whole(pg, col);
-      } else {
-        r[c].part(pr, col, n);
-        y[c].part(py, col, g.y ? n : 0);
-        gates[c].part(pg, col, g.ld_gate ? n : 0);
-      }
+    const int n = m < g.M ? valid : 0;
+    y.zero();
+    gates.zero();
+    if (n == 8) {
+      r.whole(pr, col);
+      if (g.y) y.whole(py, col);
+      if (g.ld_gate) gates.whole(pg, col);
+    } else {
+      r.part(pr, col, n);
+      if (g.y) y.part(py, col, n);
+      if (g.ld_gate) gates.part(pg, col, n);
     }
   };
   const int64_t step = (int64_t)gridDim.x * S::kRows;
   int64_t m = (int64_t)blockIdx.x * S::kRows + sub;
   fetch(m);
+  float w[8], post[8], gate[8];
   {
-    EightAny ew[kC], ep[kC], eg[kC];
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      const int col = 8 * (c * kT + t);
-      ep[c].load(g.post_type, g.post, col, valid[c]);
-      eg[c].load(g.gate_type, g.ld_gate == 0 ? g.gate : nullptr, col, valid[c]);
-      ew[c].load(g.w_type, g.w, col, valid[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      ep[c].values(g.post_type, g.post, post[c]);
-      eg[c].values(g.gate_type, g.gate, gate[c]);
-      ew[c].values(g.w_type, g.w, w[c]);
-    }
+    EightAny ew, ep, eg;
+    ep.load(g.post_type, g.post, col, valid);
+    eg.load(g.gate_type, g.ld_gate == 0 ? g.gate : nullptr, col, valid);
+    ew.load(g.w_type, g.w, col, valid);
+    ep.values(g.post_type, g.post, post);
+    eg.values(g.gate_type, g.gate, gate);
+    ew.values(g.w_type, g.w, w);
   }
   for (int64_t first = (int64_t)blockIdx.x * S::kRows; first < g.M; first += step, m += step) {
-    Eight<kR> ro[kC];
-    Eight<kY> yo[kC], go[kC];
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      ro[c] = r[c];
-      yo[c] = y[c];
-      go[c] = gates[c];
-    }
+    Eight<kR> ro = r;
+    Eight<kY> yo = y, go = gates;
     fetch(m + step);
-    float v[kC][8];
-    float iy = 1.0f;
+    float v[8], yv[8], iy = 1.0f;
     if (g.post) {
       float s[1] = {0.0f};
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[0] = fmaf(yo[c].at(j), yo[c].at(j), s[0]);
+      for (int j = 0; j < 8; ++j) s[0] = fmaf(yo.at(j), yo.at(j), s[0]);
       Sum::run(s, room, turn);
       iy = inverse_rms(s[0], g);
     }
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      float yv[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j % 2 == 0) {
-          ro[c].from_here(j);
-          yo[c].from_here(j);
-        }
-        v[c][j] = ro[c].at(j);
-        yv[j] = yo[c].at(j);
-        if (g.ld_gate) gate[c][j] = go[c].at(j);
+    for (int j = 0; j < 8; ++j) {
+      if (j % 2 == 0) {
+        ro.from_here(j);
+        yo.from_here(j);
       }
-      if (g.y) {
-        joined(g, drop, (uint64_t)(m * row_chunks + c * kT + t), iy, yv, post[c], gate[c], v[c]);
-        if (g.out && m < g.M) store8<kR>(S::template row<kR>(g.out, m, g.ld_out), 8 * (c * kT + t), valid[c], v[c]);
-      }
+      v[j] = ro.at(j);
+      yv[j] = yo.at(j);
+      if (g.ld_gate) gate[j] = go.at(j);
+    }
+    if (g.y) {
+      joined(g, drop, (uint64_t)(m * row_chunks + t), iy, yv, post, gate, v);
+      if (g.out && m < g.M) store8<kR>(S::template row<kR>(g.out, m, g.ld_out), col, valid, v);
     }
     float s[1] = {0.0f};
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] = fmaf(v[c][j], v[c][j], s[0]);
+    for (int j = 0; j < 8; ++j) s[0] = fmaf(v[j], v[j], s[0]);
     Sum::run(s, room, turn);
     const float iv = inverse_rms(s[0], g);
     if (m < g.M) {
@@ -358,8 +328,7 @@ __global__ void __launch_bounds__(S::kGroup, S::kT == 512 && kR != FP64EMU_F32 ?
         g.stats[m] = iv;
         if (g.post) g.stats[g.M + m] = iy;
       }
-#pragma unroll
-      for (int c = 0; c < kC; ++c) emit_norm<kR, kY>(g, m, 8 * (c * kT + t), valid[c], iv, v[c], w[c]);
+      emit_norm<kR, kY>(g, m, col, valid, iv, v, w);
     }
   }
 }
@@ -574,7 +543,7 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
   }
 }
 
-// Rows in registers, as norm_rows_kernel, but kC times eight elements a thread (element 8 (c kT + t) on):
+// Rows in registers, as norm_rows_kernel, but kC times eight elements a thread (element 8 (c kT + t) on) for rows past 4096:
 // 1024 threads a row leave 128 registers each, which the sums over the rows, kept a column to a thread,
 // do not fit.  A row's values stay as they came and are worked out again after its sums; with one
 // chunk the next row's are on their way meanwhile.  A row's last, partial eight elements are its last eight: what the
@@ -827,35 +796,27 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormArgs g,
 constexpr int64_t kMaxHeld = 8192;           // elements of a row that stay in registers
 bool grad_held(int64_t D) { return D >= 8 && D <= kMaxHeld; }
 
-template <int kT, int kC_>
-struct Launch : RowShape<kT> {
-  using Shape = RowShape<kT>;
-  static constexpr int kC = kC_;
-};
-
-// Calls fn with the launch shape of rows of D <= kMaxHeld elements.  Forward, sixteen elements a thread: half the
-// waves that meet at a row's barriers, and more rows on a CU (8192 x 4096 in 8 bits 59 us, with eight 68).
+// Calls fn with the launch shape of rows of D <= kMaxHeld elements.
 template <class Fn>
 void for_norm(int64_t D, const Fn& fn) {
-  if (D <= 128) fn(Launch<16, 1>{});
-  else if (D <= 512) fn(Launch<64, 1>{});
-  else if (D <= 1024) fn(Launch<64, 2>{});
-  else if (D <= 2048) fn(Launch<128, 2>{});
-  else if (D <= 4096) fn(Launch<256, 2>{});
-  else fn(Launch<512, 2>{});
+  if (D <= 128) fn(RowShape<16>{});
+  else if (D <= 512) fn(RowShape<64>{});
+  else if (D <= 1024) fn(RowShape<128>{});
+  else if (D <= 2048) fn(RowShape<256>{});
+  else if (D <= 4096) fn(RowShape<512>{});
+  else fn(RowShape<1024>{});
 }
+// The gradient's, and the chunks a thread has.
 template <class Fn>
 void for_grad(int64_t D, const Fn& fn) {
-  if (D <= 128) fn(Launch<16, 1>{});
-  else if (D <= 512) fn(Launch<64, 1>{});
-  else if (D <= 1024) fn(Launch<128, 1>{});
-  else if (D <= 2048) fn(Launch<256, 1>{});
-  else if (D <= 4096) fn(Launch<512, 1>{});
-  else fn(Launch<512, 2>{});
+  if (D <= 4096) for_norm(D, [&](auto s) {
+    if constexpr (s.kT < 1024) fn(s, std::integral_constant<int, 1>{});
+  });
+  else fn(RowShape<512>{}, std::integral_constant<int, 2>{});
 }
 
 // Work groups of a forward pass: 2^19 threads, what the card holds twice over, so that a group loads its weights
-// once for many rows (8192 x 8192 both ways 200 us, 229 with eight times as many groups).
+// once for many rows (8192 x 8192 both ways 179 us; an earlier kernel took 14% more with eight times as many).
 int64_t norm_groups(int64_t M, int64_t D) {
   int64_t groups = std::min<int64_t>(M, 512);
   if (D <= kMaxHeld)
@@ -868,8 +829,8 @@ int64_t norm_groups(int64_t M, int64_t D) {
 int64_t grad_groups(const fp64emu_norm_t* p) {
   if (!grad_held(p->D)) return std::min<int64_t>(p->M, 512);
   int64_t groups = 0;
-  for_grad(p->D, [&](auto s) {
-    const bool lean = s.kC == 1 && s.kT >= 64 && p->ld_gate == 0 && p->r_dtype != FP64EMU_F32;
+  for_grad(p->D, [&](auto s, auto chunks) {
+    const bool lean = chunks() == 1 && s.kT >= 64 && p->ld_gate == 0 && p->r_dtype != FP64EMU_F32;
     groups = std::min<int64_t>((p->M + s.kRows - 1) / s.kRows, 256 * (lean ? 1024 : 512) / s.kGroup);
   });
   return groups;
@@ -882,8 +843,8 @@ int launch_norm(const NormArgs& g, bool cols, hipStream_t s) {
     norm_long_kernel<kR, kY><<<groups, kLong, 0, s>>>(g);
   } else {
     for_norm(g.D, [&](auto shape) {
-      using L = decltype(shape);
-      norm_rows_kernel<kR, kY, typename L::Shape, L::kC><<<groups, L::kGroup, 0, s>>>(g);
+      using S = decltype(shape);
+      norm_rows_kernel<kR, kY, S><<<groups, S::kGroup, 0, s>>>(g);
     });
   }
   if (int st = check_hip(hipGetLastError(), "norm_f8 launch")) return st;
@@ -900,11 +861,11 @@ int launch_grad(const NormArgs& g, const NormGradArgs& d, unsigned groups, hipSt
     const unsigned strips = (unsigned)((g.D + 8 * kThreads - 1) / (8 * kThreads));
     norm_grad_columns_kernel<kR, kY, kPost><<<dim3(groups, strips), kThreads, 0, s>>>(g, d);
   } else {
-    for_grad(g.D, [&](auto shape) {
-      using L = decltype(shape);
-      using S = typename L::Shape;
-      if (g.ld_gate) norm_grad_kernel<kR, kY, S, L::kC, kPost, true><<<groups, L::kGroup, 0, s>>>(g, d);
-      else norm_grad_kernel<kR, kY, S, L::kC, kPost, false><<<groups, L::kGroup, 0, s>>>(g, d);
+    for_grad(g.D, [&](auto shape, auto chunks) {
+      using S = decltype(shape);
+      constexpr int kC = decltype(chunks)::value;
+      if (g.ld_gate) norm_grad_kernel<kR, kY, S, kC, kPost, true><<<groups, S::kGroup, 0, s>>>(g, d);
+      else norm_grad_kernel<kR, kY, S, kC, kPost, false><<<groups, S::kGroup, 0, s>>>(g, d);
     });
   }
   return check_hip(hipGetLastError(), "norm_f8_backward launch");
