@@ -403,8 +403,8 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
 
 // x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
 // else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways 110 us, with the
-// statistics alone from that kernel and all outputs from this one 113; since then 97 to 102, 61 and 37
-// of them, the generator 14).  Bound by its bytes: r and y again and a byte a value, 4.7 TB/s.
+// statistics alone from that kernel and all outputs from this one 113; since then 97 to 104, 58 and 42
+// of them, the generator 15).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;
@@ -423,15 +423,20 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
   {
     Held<kR> r;
     Held<kY> y;
+    // The weights before the rows: behind them the tile took 7 us more of 40.
     float w[8], post[8], gate[8];
+    EightAny ew, ep, eg;
+    ew.load(g.w_type, g.w, col, n);
+    ep.load(g.post_type, g.post, col, n);
+    eg.load(g.gate_type, g.ld_gate == 0 ? g.gate : nullptr, col, n);
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       r.load(p, g.r, (row + p) * g.ld_r + col, t.valid(p));
       if (g.y) y.load(p, g.y, (row + p) * g.ld_y + col, t.valid(p));
     }
-    load8_any(g.w_type, g.w, col, n, w);
-    load8_any(g.post_type, g.post, col, n, post);
-    if (g.ld_gate == 0) load8_any(g.gate_type, g.gate, col, n, gate);
+    ew.values(g.w_type, g.w, w);
+    ep.values(g.post_type, g.post, post);
+    eg.values(g.gate_type, g.gate, gate);
     const uint64_t chunk = (uint64_t)(row * ((g.D + 7) / 8) + col / 8);
     auto each = [&](auto P) {
       constexpr int p = decltype(P)::value;
