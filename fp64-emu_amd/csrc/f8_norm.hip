@@ -218,14 +218,14 @@ __device__ __forceinline__ float inverse_rms(float squares, const NormArgs& g) {
   return m < __builtin_inff() ? fmaf(y * 0.5f, fmaf(-m * y, y, 1.0f), y) : y;      // (past that inf 0)
 }
 
-// v of eight elements from those of r and y.
-__device__ __forceinline__ void joined(const NormArgs& g, const Drop& drop, uint64_t chunk, float iy, const float (&y)[8],
+// v of eight elements from those of r and y; kept(j): whether element j stays.
+template <class Kept>
+__device__ __forceinline__ void joined(const NormArgs& g, const Drop& drop, const Kept& kept, float iy, const float (&y)[8],
                                        const float (&post)[8], const float (&gate)[8], float (&v)[8]) {
-  const Kept kept(drop, chunk);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float z = g.post ? y[j] * iy * post[j] : y[j];
-    v[j] = g.scale * v[j] + gate[j] * (kept.at(j) ? z * drop.scale : 0.0f);
+    v[j] = g.scale * v[j] + gate[j] * (kept(j) ? z * drop.scale : 0.0f);
   }
 }
 
@@ -247,8 +247,8 @@ __device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t 
 
 // Rows whose values stay in registers from the first sum to the last store.  A work group takes
 // rows blockIdx.x kRows + .., gridDim.x kRows apart, the weights in registers throughout and the next
-// row's values on their way.  Bound by its bytes: 8192 x 4096 bfloat16 with everything 50 us in 8 bits
-// (4.7 TB/s), 48 plain (5.6: some of it stays in the 256 MB cache).  (Sixteen elements a thread: as fast, and one row
+// row's values on their way.  Bound by its bytes: 8192 x 4096 bfloat16 with y, post and gate 49 us in 8 bits
+// (4.9 TB/s), 46 plain (5.8: some of it stays in the 256 MB cache); the generator adds 7.  (Sixteen elements a thread: as fast, and one row
 // of 8192 5.6 us where this takes 4.4.)
 template <int kR, int kY, class S>
 __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
@@ -296,6 +296,8 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
     Eight<kR> ro = r;
     Eight<kY> yo = y, go = gates;
     fetch(m + step);
+    // (The generator works while the row is on its way.)
+    const Kept kept(drop, (uint64_t)(m * row_chunks + t));
     float v[8], yv[8], iy = 1.0f;
     if (g.post) {
       float s[1] = {0.0f};
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
       if (g.ld_gate) gate[j] = go.at(j);
     }
     if (g.y) {
-      joined(g, drop, (uint64_t)(m * row_chunks + t), iy, yv, post, gate, v);
+      joined(g, drop, [&](int j) { return kept.at(j); }, iy, yv, post, gate, v);
       if (g.out && m < g.M) store8<kR>(S::template row<kR>(g.out, m, g.ld_out), col, valid, v);
     }
     float s[1] = {0.0f};
@@ -343,7 +345,8 @@ __device__ __forceinline__ void joined_at(const NormArgs& g, const Drop& drop, i
   load8<kY>(g.y, m * g.ld_y + col, valid, y);
   load8_any(g.post_type, g.post, col, valid, post);
   load8_any(g.gate_type, g.gate, m * g.ld_gate + col, valid, gate);
-  joined(g, drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8), iy, y, post, gate, v);
+  const Kept kept(drop, (uint64_t)(m * ((g.D + 7) / 8) + col / 8));
+  joined(g, drop, [&](int j) { return kept.at(j); }, iy, y, post, gate, v);
 }
 
 // Rows of any length, a row to a work group of 1024, read once for each sum and once for x: past
@@ -403,8 +406,8 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
 
 // x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
 // else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways 110 us, with the
-// statistics alone from that kernel and all outputs from this one 113; since then 97 to 104, 58 and 42
-// of them, the generator 15).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
+// statistics alone from that kernel and all outputs from this one 113; since then 96 to 101, 58 and 42
+// of them, the generator 17).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;
@@ -437,7 +440,15 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
     ew.values(g.w_type, g.w, w);
     ep.values(g.post_type, g.post, post);
     eg.values(g.gate_type, g.gate, gate);
-    const uint64_t chunk = (uint64_t)(row * ((g.D + 7) / 8) + col / 8);
+    // The generator works while the rows are on their way: a byte of a mask for each row.
+    uint32_t mask[2] = {~0u, ~0u};
+    if (drop.threshold) {
+      const uint64_t chunk = (uint64_t)(row * ((g.D + 7) / 8) + col / 8);
+      mask[0] = mask[1] = 0;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) mask[p >> 2] |= kept_of(drop, chunk + p * ((g.D + 7) / 8)) << (8 * (p & 3));
+    }
+    asm volatile("" : "+v"(mask[0]), "+v"(mask[1]));
     auto each = [&](auto P) {
       constexpr int p = decltype(P)::value;
       const float iv = row16_lane<p>(stat), iy = row16_lane<8 + p>(stat);
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
 #pragma unroll
         for (int j = 0; j < 8; ++j) yv[j] = y.at(p, j);
         if (g.ld_gate) load8<kY>(g.gate, (row + p) * g.ld_gate + col, t.valid(p), gate);
-        joined(g, drop, chunk + p * ((g.D + 7) / 8), iy, yv, post, gate, v);
+        joined(g, drop, [&](int j) { return (mask[p >> 2] >> (8 * (p & 3) + j) & 1) != 0; }, iy, yv, post, gate, v);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) x.v[p][j] = v[j] * iv * w[j];
