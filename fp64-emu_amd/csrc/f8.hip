@@ -469,12 +469,13 @@ __device__ __forceinline__ Added read_added(const MmArgs& g, int64_t b, int64_t 
           g.residual ? read4(g.dtype, g.residual, b * g.stride_res + m * g.ld_res + n, valid, vec) : zero};
 }
 
-// Four successive outputs (m, n .. n + 3).
+// Four successive outputs (m, n .. n + 3); kEpilogue in kernels of their own, so that plain ones keep their size.
+template <bool kEpilogue>
 __device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m, int64_t n, v4f v, const Added& added) {
   const int valid = (int)(g.N - n < 4 ? g.N - n : 4);
   const bool vec = g.vec_o && valid == 4;
   const int64_t i = b * g.stride_o + m * g.ldo + n;
-  if (g.epilogue) {
+  if constexpr (kEpilogue) {
     if (g.bias) v += added.bias;
     if (g.keep) write4(g.dtype, g.keep, b * g.stride_keep + m * g.ld_keep + n, valid, vec, v);
     with_act(g.act, [&](auto act) {
@@ -482,8 +483,9 @@ __device__ __forceinline__ void store_out(const MmArgs& g, int64_t b, int64_t m,
       for (int j = 0; j < 4; ++j) v[j] = activated<decltype(act)::value, true>(v[j]);
     });
     if (g.residual) v += added.residual;
+  } else if (g.accumulate) {
+    v += read4(g.dtype, g.out, i, valid, vec);
   }
-  if (g.accumulate) v += read4(g.dtype, g.out, i, valid, vec);
   write4(g.dtype, g.out, i, valid, vec, v);
 }
 
@@ -501,6 +503,7 @@ __device__ __forceinline__ void store_part(const MmArgs& g, int split, int64_t b
 }
 
 // Sum of the splits' partial sums, in their order.
+template <bool kEpilogue>
 __global__ void __launch_bounds__(kThreads) sum_parts_kernel(MmArgs g) {
   const int64_t row_quads = (g.N + 3) / 4, total = (int64_t)g.batch * g.M * row_quads;
   const int64_t step = (int64_t)gridDim.x * kThreads;
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(kThreads) sum_parts_kernel(MmArgs g) {
           if (j < left) v[j] += p[s * one + j];
     }
     const int64_t b = bm / g.M, m = bm % g.M;
-    store_out(g, b, m, n, v, g.epilogue ? read_added(g, b, m, n) : Added{});
+    store_out<kEpilogue>(g, b, m, n, v, kEpilogue ? read_added(g, b, m, n) : Added{});
   }
 }
 
@@ -1221,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const uint8_t* q, i
 // small (333 x 501 x 777: 6.4 us, 11.2 on 128 x 128 tiles).
 constexpr int kFewWaves = 8;
 
-template <int kTM, int kTN, int kU, int kFA, int kFB, bool kRowB>
+template <int kTM, int kTN, int kU, int kFA, int kFB, bool kRowB, bool kEpilogue>
 __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   __shared__ v4f red[kFewWaves][kTN * kTM][64];
   const int lane = threadIdx.x & 63;
@@ -1312,7 +1315,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   const int64_t m_out = m0 + (wave % kTM) * 16 + fr, n_out = n0 + (wave / kTM) * 16 + 4 * fg;
   const bool stores = wave < kTN * kTM && m_out < g.M && n_out < g.N;
   Added added{};
-  if (g.epilogue && stores && g.splits == 1) added = read_added(g, b, m_out, n_out);
+  if (kEpilogue && stores) added = read_added(g, b, m_out, n_out);
 
   const int full = (int)(g.K / kBlk) < kb1 ? (int)(g.K / kBlk) : kb1;    // blocks before it are whole
   int kb = kb0 + wave;
@@ -1349,8 +1352,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) mm_few_kernel(MmArgs g) {
   v4f v = red[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < kFewWaves; ++w) v += red[w][wave][lane];
-  if (g.splits > 1) store_part(g, split, b, m_out, n_out, v);
-  else store_out(g, b, m_out, n_out, v, added);
+  if (!kEpilogue && g.part) store_part(g, split, b, m_out, n_out, v);
+  else store_out<kEpilogue>(g, b, m_out, n_out, v, added);
 }
 
 // ---------------------------------------------------------------------------
@@ -1462,7 +1465,7 @@ int launch_quant(QuantArgs g, int64_t batch, int64_t mblocks, bool tiles, hipStr
   return FP64EMU_OK;
 }
 
-// Operands whose tile kernels finish a product with an epilogue themselves: e4m3 on both sides, what
+// Operands whose kernels finish a product with an epilogue themselves: e4m3 on both sides, what
 // activations and weights are held in.  With e5m2 (gradients) the sums go through the
 // workspace, as with splits, at 8 bytes an output more.
 template <int kFA, int kFB>
@@ -1483,8 +1486,16 @@ void launch_tile(const MmArgs& g, unsigned groups, hipStream_t s) {
 
 template <int kTM, int kTN, int kU, int kFA, int kFB>
 void launch_few(const MmArgs& g, unsigned groups, hipStream_t s) {
-  if (g.b_tiles) mm_few_kernel<kTM, kTN, kU, kFA, kFB, false><<<groups, 64 * kFewWaves, 0, s>>>(g);
-  else mm_few_kernel<kTM, kTN, kU, kFA, kFB, true><<<groups, 64 * kFewWaves, 0, s>>>(g);
+  constexpr int kT = 64 * kFewWaves;
+  if constexpr (kFusedFmt<kFA, kFB>) {
+    if (g.epilogue && !g.part) {
+      if (g.b_tiles) mm_few_kernel<kTM, kTN, kU, kFA, kFB, false, true><<<groups, kT, 0, s>>>(g);
+      else mm_few_kernel<kTM, kTN, kU, kFA, kFB, true, true><<<groups, kT, 0, s>>>(g);
+      return;
+    }
+  }
+  if (g.b_tiles) mm_few_kernel<kTM, kTN, kU, kFA, kFB, false, false><<<groups, kT, 0, s>>>(g);
+  else mm_few_kernel<kTM, kTN, kU, kFA, kFB, true, false><<<groups, kT, 0, s>>>(g);
 }
 
 template <int kFA, int kFB>
@@ -1511,7 +1522,7 @@ MmRoom mm_room(const fp64emu_mm_f8_t* p, const MmPlan& plan, bool epilogue) {
   MmRoom r{};
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const bool fused = p->A.fmt == FP64EMU_E4M3 && p->B.fmt == FP64EMU_E4M3;       // kFusedFmt
-  if (plan.splits > 1 || (epilogue && plan.form != kFew && !fused)) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
+  if (plan.splits > 1 || (epilogue && !fused)) r.parts = up((size_t)plan.splits * 4 * (size_t)(p->batch * p->M * p->N));
   const size_t ld = (size_t)((p->K + 15) / 16 * 16);
   if (plan.form != kFew && !copyable(p->A)) r.A = up((size_t)(p->batch * p->M) * ld);
   if (plan.form != kFew && !copyable(p->B)) r.B = up((size_t)(p->batch * p->N) * ld);
@@ -1665,8 +1676,12 @@ int fp64emu_mm_f8_epilogue(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e
   }
   const int64_t quads = p->batch * p->M * ((p->N + 3) / 4);
   const unsigned sum_groups = (unsigned)std::min<int64_t>((quads + kThreads - 1) / kThreads, 65536);
+  const auto sum_parts = [&] {
+    if (g.epilogue) sum_parts_kernel<true><<<sum_groups, kThreads, 0, s>>>(g);
+    else sum_parts_kernel<false><<<sum_groups, kThreads, 0, s>>>(g);
+  };
   if (p->K == 0) {
-    sum_parts_kernel<<<sum_groups, kThreads, 0, s>>>(g);
+    sum_parts();
     return check_hip(hipGetLastError(), "mm_f8 launch");
   }
   const MmPlan plan = plan_mm(p->batch, p->M, p->N, p->K, p->dtype);
@@ -1722,7 +1737,7 @@ int fp64emu_mm_f8_epilogue(const fp64emu_mm_f8_t* p, const fp64emu_epilogue_t* e
   }
   if (int st = check_hip(hipGetLastError(), "mm_f8 launch")) return st;
   if (g.part) {
-    sum_parts_kernel<<<sum_groups, kThreads, 0, s>>>(g);
+    sum_parts();
     return check_hip(hipGetLastError(), "mm_f8 launch");
   }
   return FP64EMU_OK;
