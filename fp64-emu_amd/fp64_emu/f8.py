@@ -401,7 +401,7 @@ def residual_norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, p
     token does.  What is kept is r', y, and two floats a row."""
     if r.dim() < 1 or w.dim() != 1:
         raise ValueError(f"expect r [.., D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
-    if gate is not None and gate.dim() > 1:
+    if gate is not None and gate.shape != r.shape[-1:] and (gate.dim() != 1 or gate.numel() == 1):
         gate = gate.expand(r.shape)
     if y is not None and y.shape != r.shape:
         raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")

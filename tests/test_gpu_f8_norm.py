@@ -297,6 +297,23 @@ def test_residual_norm(dev, lead):
         assert u.shape == t[name].shape and (u.double() - o).norm() <= 2.0 ** -14 * o.norm() + 1e-12, name
 
 
+@pytest.mark.parametrize("shape", [(), (1,), (3, 1), (1, 64), (64,)])
+def test_residual_norm_gate_spreads(shape, dev):
+    """A gate of any shape that spreads to r's does what the spread one does, and its gradient is the sum."""
+    print("case residual norm gate", shape, flush=True)
+    r, y, w, a, b = (randn(*s, seed=i).to(dev) for i, s in enumerate([(3, 64), (3, 64), (64,), (3, 64), (3, 64)]))
+    gate = randn(*shape, seed=9).to(dev).requires_grad_()
+    whole = gate.detach().expand(3, 64).contiguous().requires_grad_()
+    got, want = (fp64_emu.residual_norm_f8(r, w, y, gate=g) for g in (gate, whole))
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+    g, = torch.autograd.grad(got, gate, (a, b))
+    each, = torch.autograd.grad(want, whole, (a, b))
+    o = each.double().sum_to_size(shape)
+    # two orders of sums of at most 192 float32 terms
+    assert g.shape == gate.shape
+    assert ((g.double() - o).abs() <= 192 * 2.0 ** -24 * each.double().abs().sum_to_size(shape)).all()
+
+
 def test_residual_norm_parts(dev):
     """x alone, only one of the results used, nothing kept without gradients, no second derivative."""
     print("case residual norm parts", flush=True)
