@@ -219,6 +219,25 @@ def test_act_gradient(dev, M, N, name):
         assert torch.equal(fp64_emu.act_f8_backward(dy, bias=True)[1], fp64_emu.act_f8_backward(dy, h, bias=True)[1])
 
 
+@pytest.mark.parametrize("M,N,K,ld", [(3, 264, 300, 2 ** 30 + 8), (1000, 1101, 300, 2 ** 22 + 8)])
+def test_far_offsets(dev, M, N, K, ld):
+    """Rows whose elements lie past 2^31 elements (and 2^32 bytes) from the first."""
+    print("case far offsets", M, N, K, ld, flush=True)
+    buf = torch.zeros((M - 1) * ld + N, dtype=BF16, device=dev)
+    far = buf.as_strided((M, N), (ld, 1))
+    near, h = (randn(M, N, seed=i, dtype=BF16).to(dev) for i in (96, 97))
+    far.copy_(near)
+    qa, sa = operand((M, K), 1, device=dev)
+    qb, sb = operand((N, K), 2, device=dev)
+    assert torch.equal(*(fp64_emu.mm_f8(qa, sa, qb, sb, act="relu", residual=t) for t in (far, near)))
+    state = rng(5, 6, dev)
+    for quant in (None, "rows", "both"):
+        for call in (lambda t: fp64_emu.act_f8_backward(t, h, "silu", quant, bias=True),
+                     lambda t: fp64_emu.act_f8_backward(h, t, "silu", quant, bias=True),
+                     lambda t: fp64_emu.dropout_f8(t, 0.3, state, quant)):
+            assert all(torch.equal(u.float(), v.float()) for u, v in zip(call(far), call(near)))
+
+
 def test_act_gradient_layouts(dev):
     print("case act gradient layouts", flush=True)
     M, N = 150, 200
