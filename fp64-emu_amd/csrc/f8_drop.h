@@ -31,6 +31,11 @@ __device__ __forceinline__ Drop drop_of(uint32_t threshold, const int64_t* rng) 
   return d;
 }
 
+// a ^ b ^ c in one instruction (0x96 is that function's truth table).
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 // Sixteen bits for each of a chunk's eight elements: element j's are half j % 2 of word j / 2.
 __device__ __forceinline__ v4u random_bits(const Drop& d, uint64_t chunk) {
   uint32_t x0 = (uint32_t)chunk, x1 = (uint32_t)(chunk >> 32), x2 = d.offset[0], x3 = d.offset[1];
@@ -41,9 +46,9 @@ __device__ __forceinline__ v4u random_bits(const Drop& d, uint64_t chunk) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)x0 * 0xd2511f53u, b = (uint64_t)x2 * 0xcd9e8d57u;
-    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
+    x0 = xor3((uint32_t)(b >> 32), x1, k0);
     x1 = (uint32_t)b;
-    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
+    x2 = xor3((uint32_t)(a >> 32), x3, k1);
     x3 = (uint32_t)a;
     k0 += 0x9e3779b9u;
     k1 += 0xbb67ae85u;

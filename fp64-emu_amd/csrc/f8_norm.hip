@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
 
 // x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
 // else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways 110 us, with the
-// statistics alone from that kernel and all outputs from this one 113; since then 96 to 101, 58 and 42
-// of them, the generator 17).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
+// statistics alone from that kernel and all outputs from this one 113; since then 93 to 99, 56 to 62 and 42
+// of them, the generator 16).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;

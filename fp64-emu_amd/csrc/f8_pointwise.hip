@@ -128,8 +128,8 @@ __device__ __forceinline__ void dropped(const Held<kT>& x, int p, const Drop& dr
   for (int j = 0; j < 8; ++j) y[j] = kept.at(j) ? x.at(p, j) * drop.scale : 0.0f;
 }
 
-// A block of a row on 16 lanes.  8192 x 8192 bfloat16 plain 45 us (6 TB/s: what of it the 256 MB cache holds
-// from call to call is faster than memory), in 8 bits 49: the generator's twenty wide products for eight
+// A block of a row on 16 lanes.  8192 x 8192 bfloat16 plain 44 us (6.1 TB/s: what of it the 256 MB cache holds
+// from call to call is faster than memory), in 8 bits 47: the generator's twenty wide products for eight
 // elements hide behind the memory.
 template <int kT>
 __global__ void __launch_bounds__(kThreads) dropout_rows_kernel(DropArgs a) {
