@@ -247,8 +247,9 @@ def _run_own(s):
         return f8.dropout_f8(s["x"], s["p"], s["rng"], quant=quant)
     if op == "act_grad":
         return f8.act_f8_backward(s["dy"], s["h"], s["act"], quant=quant, bias="bias" in s["parts"])
-    around = {"y": s.get("y"), "post": s.get("post"), "gate": s.get("gate"), "scale": s["scale"], "p": s["p"],
-              "rng": s.get("rng")}
+    # (scale is of the stream that y joins: without y there is none to pass.)
+    around = {"y": s["y"], "post": s.get("post"), "gate": s.get("gate"), "scale": s["scale"], "p": s["p"],
+              "rng": s["rng"]} if "y" in s else {}
     if op == "norm":
         return f8.norm_f8(s["r"], s["w"], **around, quant=quant, keep="keep" in s["parts"], eps=EPS)
     got = f8.norm_f8_backward(s["dx"], s["dr"], s["r"], s["w"], s["stats"], **around)
