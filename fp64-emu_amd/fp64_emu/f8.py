@@ -205,7 +205,8 @@ def norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torc
 
     for r and y [M, D], w and post [D], gate [D] or [M, D]; z = y without post, r' = r without y.
     x comes from r' before that is rounded to r's type.  y has r's type, or r is float32; x (and
-    a gate [M, D]) have y's.  p, rng: the dropout of z.
+    a gate [M, D]) have y's.  p, rng: the dropout of z.  post, gate, scale and p are of y: without it they are
+    refused, a scale of 1 aside.
 
     Returns (r',) with y; then quant None: (x,), "rows": (q, s), "both": (q, s, qt, st); then with keep
     (stats,), i(r') and, with post, i(y) of each row, for norm_f8_backward.  Sums of squares are
