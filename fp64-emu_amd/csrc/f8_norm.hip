@@ -927,7 +927,7 @@ int norm_args(const fp64emu_norm_t* p, NormArgs* g) {
   g->post_type = p->post_dtype;
   g->gate_type = p->gate_dtype;
   g->threshold = (uint32_t)p->drop;
-  g->scale = p->scale;
+  g->scale = p->y ? p->scale : 1.0f;         // (v = r without y)
   g->eps = p->eps;
   g->over_d = 1.0f / (float)p->D;
   if (g->ld_gate && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");

@@ -413,8 +413,8 @@ int fp64emu_dropout_f8(const void* x, int dtype, int64_t M, int64_t K, int64_t l
                        const fp64emu_f8_t* cols, fp64emu_stream_t stream);
 
 /* ---- The norms before and after a block.  With i(v) = (mean(v^2) + eps)^-1/2 over a row of D:
- * z = y i(y) post (y without post), v = scale r + gate drop(z) (r without y), x = v i(v) w, x from v
- * before it is rounded to the stream's dtype. ---- */
+ * z = y i(y) post (y without post), v = scale r + gate drop(z) (r without y, scale unread), x = v i(v) w,
+ * x from v before it is rounded to the stream's dtype. ---- */
 typedef struct {
   const void *r, *y;            /* [M, D], rows ld_r and ld_y apart; y may be NULL */
   const void *w, *post, *gate;  /* [D]; post and gate may be NULL; gate [M, D] with ld_gate >= D */

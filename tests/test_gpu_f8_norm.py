@@ -1,10 +1,13 @@
 """GPU tier: the norms around a block and their gradient against float64, at row lengths around every
 launch shape (16 threads a row up to rows that do not stay in registers), ragged and odd ones, all
 types, and a run of both through autograd."""
+import ctypes
+
 import pytest
 import torch
 
 import fp64_emu
+from fp64_emu import capi
 from f8_block_util import F64, close, close_codes, factors, inverse_rms, norm, norm_grad, randn, rng
 from f8_util import quantised, same_codes
 
@@ -347,3 +350,41 @@ def test_norm_refusals(dev):
                  lambda: fp64_emu.norm_f8_backward(x, None, x, w, x[:2, :4].contiguous())):
         with pytest.raises(RuntimeError):
             call()
+
+
+# ---- The C entry points by themselves.
+
+CODE = {F32: 0, BF16: 1, FP16: 2}
+
+
+def _c_norm(r, w, y=None, scale=1.0, gate=None):
+    M, D = r.shape
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    kind = lambda t: CODE[(r if t is None else t).dtype]  # noqa: E731
+    return capi.Norm(at(r), at(y), at(w), None, at(gate), None, M, D, r.stride(0), 0 if y is None else y.stride(0),
+                     0 if gate is None else gate.stride(0), kind(r), kind(y), CODE[w.dtype], 0, kind(gate), 0, scale, EPS)
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+@pytest.mark.parametrize("D", [5, 300, 8200])
+def test_norm_alone_has_no_scale(dev, D):
+    """Without y the stream is r, whatever scale the structure holds: forward and backward give scale 1's bits."""
+    print("case norm alone, scale", D, flush=True)
+    L, M = capi.lib(), 9
+    r, w, dx, dr = randn(M, D, seed=1).to(dev), randn(D, seed=2).to(dev), randn(M, D, seed=3).to(dev), randn(M, D, seed=4).to(dev)
+    want = None
+    for scale in (1.0, 0.75, 0.0):
+        p = _c_norm(r, w, scale=scale)
+        x, stats = torch.empty(M, D, device=dev), torch.empty(M, device=dev)
+        out, dw = torch.empty(M, D, device=dev), torch.empty(D, device=dev)
+        assert L.fp64emu_norm_f8(ctypes.byref(p), None, 0, x.data_ptr(), D, stats.data_ptr(), None, None, _stream()) == 0
+        d = capi.NormGrad(dx=dx.data_ptr(), dr=dr.data_ptr(), dr_out=out.data_ptr(), dw=dw.data_ptr(), ld_dx=D, ld_dr=D, ld_dr_out=D)
+        need = L.fp64emu_norm_f8_backward_workspace(ctypes.byref(p))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        assert L.fp64emu_norm_f8_backward(ctypes.byref(p), stats.data_ptr(), ctypes.byref(d), ws.data_ptr(), need, _stream()) == 0
+        got = (x, stats, out, dw)
+        want = want or [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), scale
