@@ -370,7 +370,7 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.scale, ctx.p, ctx.joined = scale, p, y is not None
         if keep:
             # (rng may go on in place before the backward pass.)
-            rng = rng.clone() if p else None
+            rng = rng.clone() if p and rng is not None else None
             ctx.save_for_backward(got[0] if ctx.joined else flat[0], w, flat[1], post, gates, got[-1], rng)
         ctx.set_materialize_grads(False)
         out = tuple(t.view(r.shape) for t in got[:2 if ctx.joined else 1])

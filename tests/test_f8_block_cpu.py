@@ -256,3 +256,16 @@ def test_no_derivative_is_said():
             assert not any(t.requires_grad for t in call(x))
             with torch.no_grad():
                 assert not any(t.requires_grad for t in call(h))
+
+
+@pytest.mark.parametrize("p", [0.0, 1e-6, 2.0 ** -17])
+def test_shares_that_round_to_none_need_no_rng(p):
+    """A share of at most 2^-17 drops nothing: rng may be absent, with gradients and without."""
+    with FakeTensorMode():
+        r = torch.empty(4, 256, device="cuda", requires_grad=True)
+        w = torch.empty(256, device="cuda")
+        new, x = fp64_emu.residual_norm_f8(r, w, r, p=p)
+        assert new.requires_grad and x.shape == r.shape
+        assert fp64_emu.seeded_dropout_f8(r, p, None).requires_grad
+        with torch.no_grad():
+            assert fp64_emu.residual_norm_f8(r, w, r, p=p)[1].shape == r.shape
