@@ -934,6 +934,39 @@ int norm_args(const fp64emu_norm_t* p, NormArgs* g) {
   return FP64EMU_OK;
 }
 
+// A matrix of M rows as bytes.
+struct Place { const void* p; int64_t width, pitch; };
+
+bool same_place(const Place& a, const Place& b, int64_t M) {
+  return a.p == b.p && a.width == b.width && (M == 1 || a.pitch == b.pitch);
+}
+// Whether two of them have a byte in common; of different pitches, whether their ranges have.
+bool overlap(Place a, Place b, int64_t M) {
+  if (reinterpret_cast<uintptr_t>(b.p) < reinterpret_cast<uintptr_t>(a.p)) std::swap(a, b);
+  const uint64_t d = reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p);
+  if (d >= (uint64_t)((M - 1) * a.pitch + a.width)) return false;
+  if (M == 1 || a.pitch != b.pitch) return true;
+  const uint64_t side = d % (uint64_t)a.pitch;                // rows side by side in one buffer do not
+  return side < (uint64_t)a.width || (uint64_t)a.pitch - side < (uint64_t)b.width;
+}
+
+// out and x may be an operand itself, whose elements a thread reads before it writes them in their place; any other overlap, and,
+// with columns, which read the operands again, any at all, gives rows that were overwritten.
+int check_places(const fp64emu_norm_t* p, const void* out, int64_t ld_out, const void* x, int64_t ld_x, bool cols) {
+  const auto place = [&](const void* q, int dtype, int64_t ld) { return Place{q, p->D * size_of(dtype), ld * size_of(dtype)}; };
+  const Place in[] = {place(p->r, p->r_dtype, p->ld_r), place(p->y, p->y_dtype, p->ld_y),
+                      place(p->gate && p->ld_gate ? p->gate : nullptr, p->gate_dtype, p->ld_gate)};
+  const Place to[] = {place(out, p->r_dtype, ld_out), place(x, p->y_dtype, ld_x)};
+  for (const Place& o : to)
+    for (const Place& i : in) {
+      if (!o.p || !i.p || !overlap(o, i, p->M)) continue;
+      if (cols) return invalid("columns need the operands as they were: out must be elsewhere");
+      if (!same_place(o, i, p->M)) return invalid("outputs are an operand itself, rows and all, or apart from it");
+    }
+  if (out && x && overlap(to[0], to[1], p->M)) return invalid("outputs overlap");
+  return FP64EMU_OK;
+}
+
 // Calls fn with r's and y's types as constants.
 template <class Fn>
 int for_types(int r, int y, const Fn& fn) {
@@ -962,12 +995,12 @@ int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x,
   if (out && !p->y) return invalid("a new stream needs y");
   if (cols && !stats) return invalid("columns need stats");
   if (cols && x) return invalid("columns come without x in its plain form");
-  if (cols && out && out == p->r) return invalid("columns need r as it was: out must be elsewhere");
   if ((out && ld_out < p->D) || (x && ld_x < p->D)) return invalid("rows are shorter than D");
   NormArgs g;
   if (int st = norm_args(p, &g)) return st;
   if (int st = out8(rows, p->D, &g.rows)) return st;
   if (int st = out8(cols, p->M, &g.cols)) return st;
+  if (int st = check_places(p, out, ld_out, x, ld_x, cols != nullptr)) return st;
   g.out = out;
   g.ld_out = ld_out;
   g.x = x;

@@ -427,9 +427,10 @@ typedef struct {
   float scale, eps;             /* eps at least 2^-126 */
 } fp64emu_norm_t;
 
-/* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype (may be r itself, without cols);
- * `x` [M, D] in y's dtype; stats, i(v) of each row, then with post i(y), M floats each; `rows` and `cols`,
- * x quantised from its float32 values.  cols needs stats and comes without x. */
+/* Each output only where asked for: `out`, the new stream v [M, D] in r's dtype; `x` [M, D] in y's dtype; stats, i(v)
+ * of each row, then with post i(y), M floats each; `rows` and `cols`, x quantised from its float32 values.  cols needs
+ * stats and comes without x.  Without cols, out and x may be r, y or a gate for each row itself (same address, row distance and element size);
+ * no outputs overlap otherwise, neither one another nor an operand. */
 int fp64emu_norm_f8(const fp64emu_norm_t* p, void* out, int64_t ld_out, void* x, int64_t ld_x, float* stats,
                     const fp64emu_f8_t* rows, const fp64emu_f8_t* cols, fp64emu_stream_t stream);
 

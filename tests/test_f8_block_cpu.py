@@ -269,3 +269,27 @@ def test_shares_that_round_to_none_need_no_rng(p):
         assert fp64_emu.seeded_dropout_f8(r, p, None).requires_grad
         with torch.no_grad():
             assert fp64_emu.residual_norm_f8(r, w, r, p=p)[1].shape == r.shape
+
+
+def test_norm_places():
+    """Outputs on their operands: the same rows at the same distance without columns, or rows side by side in one buffer."""
+    L, M, D = capi.lib(), 4, 256
+    r, y, g, o, x = (0x100000 * (i + 1) for i in range(5))
+
+    def call(out=o, ldo=D, x=x, ldx=D, cols=None, **kw):
+        kw = {"r": r, "y": y, "gate": g, "ld_gate": D, "gate_dtype": BF16, **kw}
+        return L.fp64emu_norm_f8(R(_norm(M, D, **kw)), out, ldo, x, ldx, P, None, cols and R(cols), None)
+
+    cols = _f8(D, M)
+    for at in (r, y, g):
+        _says(call(out=at, x=None, cols=cols), "elsewhere")
+        _says(call(out=at + 2 * D, x=None, cols=cols), "elsewhere")
+        for kw in (dict(out=at, ldo=D + 8), dict(out=at + 2), dict(out=at + 2 * D), dict(out=at - 2 * D), dict(x=at, ldx=D + 8),
+                   dict(x=at + 2 * (M * D - 1))):
+            _says(call(**kw), "operand itself")
+    _says(call(out=r, r_dtype=F32, y=r, ld_y=2 * D), "operand itself")          # the same start and pitch, half the width
+    _says(call(out=o, x=o), "outputs overlap")
+    _says(call(out=o, x=o + 2 * D), "outputs overlap")
+    # Side by side: half a row's distance away, an element into the neighbour's.
+    _says(call(ld_r=2 * D, out=r + 2 * D - 2, ldo=2 * D), "operand itself")
+    _says(call(ld_r=2 * D, out=r + 2 * D + 2, ldo=2 * D), "operand itself")

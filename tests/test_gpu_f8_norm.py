@@ -388,3 +388,36 @@ def test_norm_alone_has_no_scale(dev, D):
         got = (x, stats, out, dw)
         want = want or [t.clone() for t in got]
         assert all(torch.equal(a, b) for a, b in zip(got, want)), scale
+
+
+@pytest.mark.parametrize("form", ["x", "rows"])
+@pytest.mark.parametrize("D", [40, 300, 5000, 8200])
+def test_norm_in_place(dev, D, form):
+    """The new stream in r's, y's or the gates' place, x in y's, the new stream beside r in one buffer: the bits of
+    outputs of their own."""
+    print("case norm in place", D, form, flush=True)
+    L, M = capi.lib(), 70
+    w = randn(D, seed=1).to(dev)
+    fresh = [randn(M, D, seed=i, dtype=BF16).to(dev) for i in (2, 3, 4)]
+    want = fp64_emu.norm_f8(fresh[0], w, fresh[1], gate=fresh[2], scale=0.5, eps=EPS, quant=None if form == "x" else "rows")
+
+    def run(r, y, gate, out, x=None):
+        p = _c_norm(r, w, y, 0.5, gate)
+        q, s = torch.empty(M, D, device=dev, dtype=torch.uint8), torch.empty(M, -(-D // 128), device=dev)
+        rows = capi.F8(q.data_ptr(), s.data_ptr(), D, 0, s.stride(0), 1, 0, 0, 0)
+        st = L.fp64emu_norm_f8(ctypes.byref(p), out.data_ptr(), out.stride(0), None if x is None else x.data_ptr(), D, None,
+                               None if x is not None else ctypes.byref(rows), None, _stream())
+        assert st == 0, L.fp64emu_last_error()
+        assert torch.equal(out, want[0])
+        if x is not None:
+            assert torch.equal(x, want[1])
+        else:
+            assert torch.equal(q, want[1].view(torch.uint8)) and torch.equal(s, want[2])
+
+    for at in range(3):
+        t = [v.clone() for v in fresh]
+        x = None if form == "rows" else t[1] if at != 1 else torch.empty(M, D, dtype=BF16, device=dev)
+        run(*t, t[at], x)
+    both = torch.cat([fresh[0], torch.zeros_like(fresh[0])], 1)
+    run(both[:, :D], fresh[1], fresh[2], both[:, D:], torch.empty(M, D, dtype=BF16, device=dev) if form == "x" else None)
+    assert torch.equal(both[:, :D], fresh[0])
