@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d.v[p][j] = activated_back<kAct, kT == FP64EMU_F32>(h.at(p, j), dy.at(p, j));
+      for (int j = 0; j < 8; ++j) d.v[p][j] = activated_back<kAct>(h.at(p, j), dy.at(p, j));
       __builtin_amdgcn_sched_barrier(0);     // (a row's temporaries at a time)
     }
   }
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) act_grad_rows_kernel(ActGradArgs a) 
     if (kAct) h.load(0, a.h, u.row * a.ld_h + u.col, u.valid);
     Held<FP64EMU_F32> d;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d.v[0][j] = activated_back<kAct, kT == FP64EMU_F32>(h.at(0, j), dy.at(0, j));
+    for (int j = 0; j < 8; ++j) d.v[0][j] = activated_back<kAct>(h.at(0, j), dy.at(0, j));
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] += d.v[0][j];
     if (a.dh) store8<kT>(a.dh, u.row * a.ld_dh + u.col, u.valid, d.v[0]);

@@ -219,6 +219,22 @@ def test_act_gradient(dev, M, N, name):
         assert torch.equal(fp64_emu.act_f8_backward(dy, bias=True)[1], fp64_emu.act_f8_backward(dy, h, bias=True)[1])
 
 
+@pytest.mark.parametrize("name", ACTS[1:])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_act_gradient_in_float32(dev, dtype, name):
+    """16-bit operands are float32 values: codes, scales and dbias have the bits that the same values in float32 give,
+    the plain gradient theirs rounded."""
+    print("case act gradient in float32", dtype, name, flush=True)
+    for M, N in ((5, 300), (700, 520)):
+        dy, h = randn(M, N, seed=1, dtype=dtype).to(dev), randn(M, N, seed=2, dtype=dtype, scale=3.0).to(dev)
+        for quant in ("rows", "both", None):
+            got = fp64_emu.act_f8_backward(dy, h, name, quant, bias=True)
+            want = fp64_emu.act_f8_backward(dy.float(), h.float(), name, quant, bias=True)
+            if quant is None:
+                want = (want[0].to(dtype), want[1])
+            assert _same(got, want), (M, N, quant)
+
+
 @pytest.mark.parametrize("M,N,K,ld", [(3, 264, 300, 2 ** 30 + 8), (1000, 1101, 300, 2 ** 22 + 8)])
 def test_far_offsets(dev, M, N, K, ld):
     """Rows whose elements lie past 2^31 elements (and 2^32 bytes) from the first."""
