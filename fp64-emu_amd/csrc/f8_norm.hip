@@ -145,19 +145,52 @@ template <int kCtrl, int kRowMask = 0xf>
 __device__ __forceinline__ float dpp(float v) {         // 0 in the rows that are masked out
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRowMask, 0xf, false));
 }
-// The sum over the 16 lanes of a DPP row, the same bits in all of them.
-__device__ __forceinline__ float row16_sum(float v) {
+template <int kCtrl, int kRowMask = 0xf>
+__device__ __forceinline__ double dpp(double v) {
+  v2u w = __builtin_bit_cast(v2u, v);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[i], kCtrl, kRowMask, 0xf, false);
+  return __builtin_bit_cast(double, w);
+}
+__device__ __forceinline__ float from_lane(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+  v2u w = __builtin_bit_cast(v2u, v);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w[i] = (uint32_t)__builtin_amdgcn_readlane((int)w[i], lane);
+  return __builtin_bit_cast(double, w);
+}
+// The sum over the 16 lanes of a DPP row, the same bits in all of them; T: float or double.
+template <class T>
+__device__ __forceinline__ T row16_sum(T v) {
   v += dpp<0x128>(v);                        // row_ror:8
   v += dpp<0x124>(v);
   v += dpp<0x122>(v);
   return v + dpp<0x121>(v);
 }
 // Over a wave, scalar: on vector instructions alone, where lane exchanges go through the LDS unit.
-__device__ __forceinline__ float wave_sum(float v) {
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
   v = row16_sum(v);
   v += dpp<0x142, 0xa>(v);                   // row_bcast:15: rows 1 and 3 add the row before
   v += dpp<0x143, 0xc>(v);                   // row_bcast:31: rows 2 and 3 add the half before
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+  return from_lane(v, 63);
+}
+// Of two values over a wave, scalar: a in the lower 32 lanes and b in the upper ones from the first step on, which
+// takes half the steps of one after the other.
+__device__ __forceinline__ void wave_sums(double& a, double& b) {
+  v2u x = __builtin_bit_cast(v2u, a), y = __builtin_bit_cast(v2u, b);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x[i], y[i], false, false);
+    x[i] = r[0];                             // a's lower lanes, b's lower lanes
+    y[i] = r[1];                             // a's upper lanes, b's upper lanes
+  }
+  double v = row16_sum(__builtin_bit_cast(double, x) + __builtin_bit_cast(double, y));
+  v += dpp<0x142, 0xa>(v);
+  a = from_lane(v, 31);
+  b = from_lane(v, 63);
 }
 
 // How a launch lays rows on threads: kT threads a row, eight elements each (so 16 neighbouring
@@ -186,13 +219,19 @@ struct RowShape {
 
 // Sums over the threads of a row, in all of them; `turn` alternates from call to call, so that one
 // barrier is enough.
-template <int kT, int kN, int kGroup>
+template <int kT, int kN, int kGroup, class T = float>
 struct RowSum {
   static constexpr int kWaves = kT / 64;
-  struct alignas(16) Room { float v[2][kN][kGroup / 64]; };
-  static __device__ __forceinline__ void run(float (&v)[kN], Room& room, int& turn) {
+  struct alignas(16) Room { T v[2][kN][kGroup / 64]; };
+  static __device__ __forceinline__ void run(T (&v)[kN], Room& room, int& turn) {
+    if constexpr (sizeof(T) == 8 && kT >= 64) {
+      static_assert(kN == 3, "the gradient's sums");
+      v[0] = wave_sum((float)v[0]);          // (nothing is taken off the first of them)
+      wave_sums(v[1], v[2]);
+    } else {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) v[n] = kT >= 64 ? wave_sum(v[n]) : row16_sum(v[n]);
+      for (int n = 0; n < kN; ++n) v[n] = kT >= 64 ? wave_sum(v[n]) : row16_sum(v[n]);
+    }
     if constexpr (kT > 64) {
       const int wave = threadIdx.x >> 6, first = wave / kWaves * kWaves;
       if ((threadIdx.x & 63) == 0) {
@@ -200,9 +239,20 @@ struct RowSum {
         for (int n = 0; n < kN; ++n) room.v[turn][n][wave] = v[n];
       }
       __syncthreads();
+      if constexpr (sizeof(T) == 8) {
+        // A DPP row for each sum, a lane for each wave's part of it: in each thread the parts would take 48 registers.
+        static_assert(kN <= 4 && kWaves <= 16, "a wave has them all");
+        const int lane = threadIdx.x & 63, n = lane >> 4, w = lane & 15;
+        T s = n < kN && w < kWaves ? room.v[turn][n < kN ? n : 0][first + (w < kWaves ? w : 0)] : T{};
+        s = row16_sum(s);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = from_lane(s, 16 * i);
+        turn ^= 1;
+        return;
+      }
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        float s = room.v[turn][n][first];
+        T s = room.v[turn][n][first];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) s += room.v[turn][n][first + w];
         v[n] = s;
@@ -479,13 +529,16 @@ __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile
 //
 // and scale t is r's gradient.  c2 is linear in c1: with e = dr + i(v) dx w and q = gate k post y, it is
 // i(y) (mean(q e) - i(v)^2 c1 mean(q v)), so that one joint sum of three gives both and a row takes
-// one barrier.  v is the stream as it is stored.
+// one barrier.  Where the stream is mostly the branch's output and dx lies along it, the two cancel: the threads'
+// sums are then joined, and subtracted, in 64 bits, which leaves dy as far from the formula as a second pass over what is
+// left would (joined in 32 bits, 2.4 to 2.7 times as far).  v is the stream as it is stored.
 
 // The three sums of eight elements: of (dx w) v, and with k what remains of gate and drop (0 where dropped),
 // q = k post y, of q e and of q v.  The rows' own factors i(v) and i(y) join them at their ends.
 template <bool kPost>
 struct GradSums {
   static constexpr int kN = kPost ? 3 : 1;
+  using Joint = std::conditional_t<kPost, double, float>;      // what the threads' sums are joined in
   static __device__ __forceinline__ void add(float v, float dx, float dr, float w, float iv, float kept_gate, float post,
                                              float y, float (&s)[kN]) {
     const float gw = dx * w;
@@ -502,13 +555,24 @@ struct GradSums {
 struct GradRow { float iv, iy, back, c2; };
 
 template <bool kPost>
-__device__ __forceinline__ GradRow grad_row(const float (&s)[kPost ? 3 : 1], float iv, float iy, float over_d) {
+__device__ __forceinline__ GradRow grad_row(const typename GradSums<kPost>::Joint (&s)[GradSums<kPost>::kN], float iv, float iy,
+                                            float over_d) {
   GradRow r{iv, iy, 0.0f, 0.0f};
-  const float c1 = s[0] * iv * over_d;                         // mean(dx w vh)
+  const float c1 = (float)s[0] * iv * over_d;                  // mean(dx w vh)
   r.back = iv * iv * c1;
-  // mean(dz post yh) is i(y) (s1 - back s2) / D
-  if constexpr (kPost) r.c2 = iy * iy * (iy * ((s[1] - r.back * s[2]) * over_d));
+  // mean(dz post yh) is i(y) (s1 - back s2) / D, of the same rounded back that t takes
+  if constexpr (kPost) r.c2 = iy * iy * (iy * ((float)fma(-(double)r.back, s[2], s[1]) * over_d));
   return r;
+}
+// A row's sums over its threads from a thread's own.
+template <class Sum, bool kPost>
+__device__ __forceinline__ GradRow joined_row(const float (&mine)[GradSums<kPost>::kN], typename Sum::Room& room, int& turn, float iv,
+                                              float iy, float over_d) {
+  typename GradSums<kPost>::Joint s[GradSums<kPost>::kN];
+#pragma unroll
+  for (int i = 0; i < GradSums<kPost>::kN; ++i) s[i] = mine[i];
+  Sum::run(s, room, turn);
+  return grad_row<kPost>(s, iv, iy, over_d);
 }
 
 struct GradOut { float t, dy, dz, z, dgate; };
@@ -573,7 +637,7 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
     norm_grad_kernel(NormArgs g, NormGradArgs d) {
   constexpr int kT = S::kT, kN = kPost ? 3 : 1;
   constexpr bool kAhead = kC == 1;
-  using Sum = RowSum<kT, kN, S::kGroup>;
+  using Sum = RowSum<kT, kN, S::kGroup, typename GradSums<kPost>::Joint>;
   __shared__ typename Sum::Room room;
   __shared__ float joint[S::kRows > 1 ? 8 * S::kGroup : 1];
   const int t = threadIdx.x % kT, sub = S::sub();
@@ -684,8 +748,7 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
 #pragma unroll
       for (int i = 0; i < kN; ++i) s[i] += mine[i];
     }
-    Sum::run(s, room, turn);
-    const GradRow row = grad_row<kPost>(s, o.iv, o.iy, g.over_d);
+    const GradRow row = joined_row<Sum, kPost>(s, room, turn, o.iv, o.iy, g.over_d);
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       Column& k = of[c];
@@ -745,7 +808,7 @@ struct GradAt {
 template <int kR, int kY, bool kPost>
 __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormGradArgs d) {
   constexpr int kN = kPost ? 3 : 1;
-  using Sum = RowSum<kLong, kN, kLong>;
+  using Sum = RowSum<kLong, kN, kLong, typename GradSums<kPost>::Joint>;
   using At = GradAt<kR, kY, kPost>;
   __shared__ typename Sum::Room room;
   const Drop drop = drop_of(g.y ? g.threshold : 0, g.rng);
@@ -760,8 +823,7 @@ __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormG
         GradSums<kPost>::add(a.v[j], a.dx[j], a.dr[j], a.w[j], iv, a.kept >> j & 1 ? a.gate[j] * drop.scale : 0.0f,
                              a.post[j], a.y[j], s);
     }
-    Sum::run(s, room, turn);
-    const GradRow row = grad_row<kPost>(s, iv, iy, g.over_d);
+    const GradRow row = joined_row<Sum, kPost>(s, room, turn, iv, iy, g.over_d);
     if (threadIdx.x == 0) d.back[m] = row.back;
     for (int64_t col = 8 * threadIdx.x; col < g.D; col += 8 * kLong) {
       const int valid = g.D - col < 8 ? (int)(g.D - col) : 8;

@@ -153,6 +153,40 @@ def test_norm_gradient_differences(dev):
         assert abs(have - want) <= 60 * 2.0 ** -20 / h + 10 * h * h + 1e-3 * abs(want), (name, have, want)
 
 
+@pytest.mark.parametrize("D,each", [(1003, 8), (4096, 8), (8192, 16), (20001, 24)])
+def test_norm_gradient_cancels(dev, D, each):
+    """The stream mostly the branch's output, dx along it: dr + i(v) dx w and what is taken off it are large beside what is
+    left.  dy has no part along y but what c2's error and the elements' roundings leave.
+
+    Sum dy y over a row, against the formula's: an element's term of magnitude m = i(y) |gate post y| (|dr + i(v) dx w| +
+    i(v) |vh c1|) has eight roundings, uniform within U m, so of deviation U m / 3^1/2; a thread's sum of `each` terms as many
+    of its partial sums, which grow evenly: (each / 9)^1/2 U of the thread's sum of m, at most each^1/2 times the root of
+    its m^2, twice.  Sums over threads in 64 bits have none.  c2 has five of itself.  Over 64 rows the root mean square of
+    the errors in deviations is below 1.4 (1 + 5 (2 / 64)^1/2 is its square's fifth deviation).  Sums joined in 32 bits
+    give 3 to 4 from 4096 on."""
+    print("case norm gradient cancels", D, flush=True)
+    M, U = 64, 2.0 ** -24
+    y = randn(M, D, seed=1).to(dev)
+    r = 4 * y + randn(M, D, seed=2, scale=0.01).to(dev)
+    dx = 0.5 * r + randn(M, D, seed=3, scale=0.01).to(dev)
+    dr = randn(M, D, seed=4, scale=0.01).to(dev)
+    w, post, gate = ((a + b * randn(D, seed=5 + i)).to(dev) for i, (a, b) in enumerate([(1, 0.1), (1, 0.1), (0.3, 0.05)]))
+    stats = torch.stack([inverse_rms(v.to(F64), EPS)[:, 0] for v in (r, y)]).float()
+    got = fp64_emu.norm_f8_backward(dx, dr, r, w, stats, y, post, gate)[1]
+    r, y, dx, dr, w, post, gate, iv, iy = (t.to(F64) for t in (r, y, dx, dr, w, post, gate, stats[0][:, None], stats[1][:, None]))
+    want = norm_grad(dx, dr, r, w, iv, y, iy, post, gate)["dy"][0]
+    mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
+    back = iv * iv * iv * mean(dx * w * r) * r
+    m = iy * (gate * post * y).abs() * ((dr + iv * dx * w).abs() + back.abs())
+    c2 = mean((dr + iv * dx * w - back) * gate * post * y * iy)
+    roundings = (8 / 3) ** 0.5 + 2 ** 0.5 * (each / 9) ** 0.5 * each ** 0.5
+    deviation = U * (roundings ** 2 * m.square().sum(-1) + 5 / 3 * (iy * c2 * (y * y * iy).sum(-1, keepdim=True))[:, 0] ** 2).sqrt()
+    off = ((got.to(F64) - want) * y).sum(-1) / deviation
+    rms = off.square().mean().sqrt().item()
+    print("root mean square", rms, flush=True)
+    assert rms <= 1.4
+
+
 @pytest.mark.parametrize("what", ["rows apart", "odd start", "transposed", "expanded gate", "one row of many"])
 def test_norm_layouts(dev, what):
     print("case norm layouts", what, flush=True)
