@@ -35,6 +35,7 @@ struct NormGradArgs {
   int64_t ld_dx, ld_dr;
   void *dr_out, *dy, *dgates;
   int64_t ld_dr_out, ld_dy, ld_dgates;
+  int wide;                                  // dgates is float32
   float *dw, *dpost, *dgate;                 // [D], or a group's part of them, [groups][D] each
   float* back;                               // rows of any length: a row's, as GradRow has it
 };
@@ -597,6 +598,13 @@ __device__ __forceinline__ GradOut grad_of(const GradRow& r, float v, float dx, 
   return o;
 }
 
+// Eight elements of a gate's gradient for each row, in y's type or float32.
+template <int kY>
+__device__ __forceinline__ void put_gates(const NormGradArgs& d, int64_t m, int64_t col, int valid, const float (&v)[8]) {
+  if (kY == FP64EMU_F32 || d.wide) store8<FP64EMU_F32>(d.dgates, m * d.ld_dgates + col, valid, v);
+  else store8<kY>(d.dgates, m * d.ld_dgates + col, valid, v);
+}
+
 // A group's sums over its rows into its part of [groups][D] (or the result itself, with one group).
 template <class S, class Column>
 __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& of, float* part, int64_t D, float* lds) {
@@ -770,7 +778,7 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
       if (m < g.M && k.in) {
         if (d.dr_out) store8<kR>(S::template row<kR>(d.dr_out, m, d.ld_dr_out), k.col, 8, tv);
         if (d.dy) store8<kY>(S::template row<kY>(d.dy, m, d.ld_dy), k.col, 8, dy);
-        if (kGates && d.dgates) store8<kY>(S::template row<kY>(d.dgates, m, d.ld_dgates), k.col, 8, dg);
+        if (kGates && d.dgates) put_gates<kY>(d, m, k.col, 8, dg);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -838,7 +846,7 @@ __global__ void __launch_bounds__(kLong) norm_grad_long_kernel(NormArgs g, NormG
       }
       if (d.dr_out) store8<kR>(d.dr_out, m * d.ld_dr_out + col, valid, t);
       if (d.dy) store8<kY>(d.dy, m * d.ld_dy + col, valid, dy);
-      if (d.dgates) store8<kY>(d.dgates, m * d.ld_dgates + col, valid, dg);
+      if (d.dgates) put_gates<kY>(d, m, col, valid, dg);
     }
   }
 }
@@ -1043,6 +1051,70 @@ int for_types(int r, int y, const Fn& fn) {
   return invalid("dtype");
 }
 
+// wide: dgates is float32.
+int norm_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d, int wide, void* workspace,
+                  size_t workspace_bytes, fp64emu_stream_t stream) {
+  if (int st = check_norm(p)) return st;
+  if (!d) return invalid("gradient must not be NULL");
+  if (p->M > 0 && !p->y && (d->dy || d->dpost || d->dgate || d->dgates)) return invalid("gradients of what is absent");
+  if ((d->dpost && !p->post) || ((d->dgate || d->dgates) && !p->gate)) return invalid("gradients of what is absent");
+  if (d->dgate && d->dgates) return invalid("gate's gradient is a row or a matrix");
+  if (d->dgates && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  float* const sums[kMaxSums] = {d->dw, d->dpost, d->dgate};
+  Sums all{};
+  int count = 0;
+  if (p->M == 0) {                           // sums of nothing
+    for (float* to : sums)
+      if (to) all.out[count++] = to;
+    all.D = p->D;
+    return launch_sums(all, count, s);
+  }
+  if (!d->dx || !stats) return invalid("null operand pointer");
+  if (d->ld_dx < p->D || (d->dr && d->ld_dr < p->D) || (d->dr_out && d->ld_dr_out < p->D) || (d->dy && d->ld_dy < p->D) ||
+      (d->dgates && d->ld_dgates < p->D))
+    return invalid("rows are shorter than D");
+  NormArgs g;
+  if (int st = norm_args(p, &g)) return st;
+  if ((d->dgate && p->ld_gate != 0) || (d->dgates && p->ld_gate == 0))
+    return invalid("dgate is of one gate, dgates of a gate for each row");
+  const size_t need = fp64emu_norm_f8_backward_workspace(p);
+  if (need && (!workspace || workspace_bytes < need))
+    return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_norm_f8_backward_workspace");
+  if (need && !multiple(workspace, 4)) return invalid("workspace must be 4-byte aligned");
+  g.stats = const_cast<float*>(stats);
+  NormGradArgs a{};
+  a.dx = d->dx;
+  a.dr = d->dr;
+  a.ld_dx = d->ld_dx;
+  a.ld_dr = d->ld_dr;
+  a.dr_out = d->dr_out;
+  a.dy = d->dy;
+  a.dgates = d->dgates;
+  a.wide = wide;
+  a.ld_dr_out = d->ld_dr_out;
+  a.ld_dy = d->ld_dy;
+  a.ld_dgates = d->ld_dgates;
+  const int64_t groups = grad_groups(p);
+  float* room = static_cast<float*>(workspace);
+  float** const to[kMaxSums] = {&a.dw, &a.dpost, &a.dgate};
+  for (int i = 0; i < kMaxSums; ++i) {
+    *to[i] = sums[i];
+    if (!sums[i] || groups == 1) continue;
+    *to[i] = room + (int64_t)count * groups * p->D;
+    all.part[count] = *to[i];
+    all.out[count++] = sums[i];
+  }
+  if (!grad_held(p->D)) a.back = room + (groups > 1 ? kMaxSums * groups * p->D : 0);
+  all.groups = groups;
+  all.D = p->D;
+  const int st = for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {
+    return p->post ? launch_grad<decltype(r)::value, decltype(y)::value, true>(g, a, (unsigned)groups, s)
+                   : launch_grad<decltype(r)::value, decltype(y)::value, false>(g, a, (unsigned)groups, s);
+  });
+  return st ? st : launch_sums(all, count, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1084,64 +1156,12 @@ size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p) {
 
 int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d, void* workspace,
                              size_t workspace_bytes, fp64emu_stream_t stream) {
-  if (int st = check_norm(p)) return st;
-  if (!d) return invalid("gradient must not be NULL");
-  if (p->M > 0 && !p->y && (d->dy || d->dpost || d->dgate || d->dgates)) return invalid("gradients of what is absent");
-  if ((d->dpost && !p->post) || ((d->dgate || d->dgates) && !p->gate)) return invalid("gradients of what is absent");
-  if (d->dgate && d->dgates) return invalid("gate's gradient is a row or a matrix");
-  if (d->dgates && p->gate_dtype != p->y_dtype) return invalid("a gate for each row has y's dtype");
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  float* const sums[kMaxSums] = {d->dw, d->dpost, d->dgate};
-  Sums all{};
-  int count = 0;
-  if (p->M == 0) {                           // sums of nothing
-    for (float* to : sums)
-      if (to) all.out[count++] = to;
-    all.D = p->D;
-    return launch_sums(all, count, s);
-  }
-  if (!d->dx || !stats) return invalid("null operand pointer");
-  if (d->ld_dx < p->D || (d->dr && d->ld_dr < p->D) || (d->dr_out && d->ld_dr_out < p->D) || (d->dy && d->ld_dy < p->D) ||
-      (d->dgates && d->ld_dgates < p->D))
-    return invalid("rows are shorter than D");
-  NormArgs g;
-  if (int st = norm_args(p, &g)) return st;
-  if ((d->dgate && p->ld_gate != 0) || (d->dgates && p->ld_gate == 0))
-    return invalid("dgate is of one gate, dgates of a gate for each row");
-  const size_t need = fp64emu_norm_f8_backward_workspace(p);
-  if (need && (!workspace || workspace_bytes < need))
-    return fp64emu_fail(FP64EMU_EWORKSPACE, "workspace too small: see fp64emu_norm_f8_backward_workspace");
-  if (need && !multiple(workspace, 4)) return invalid("workspace must be 4-byte aligned");
-  g.stats = const_cast<float*>(stats);
-  NormGradArgs a{};
-  a.dx = d->dx;
-  a.dr = d->dr;
-  a.ld_dx = d->ld_dx;
-  a.ld_dr = d->ld_dr;
-  a.dr_out = d->dr_out;
-  a.dy = d->dy;
-  a.dgates = d->dgates;
-  a.ld_dr_out = d->ld_dr_out;
-  a.ld_dy = d->ld_dy;
-  a.ld_dgates = d->ld_dgates;
-  const int64_t groups = grad_groups(p);
-  float* room = static_cast<float*>(workspace);
-  float** const to[kMaxSums] = {&a.dw, &a.dpost, &a.dgate};
-  for (int i = 0; i < kMaxSums; ++i) {
-    *to[i] = sums[i];
-    if (!sums[i] || groups == 1) continue;
-    *to[i] = room + (int64_t)count * groups * p->D;
-    all.part[count] = *to[i];
-    all.out[count++] = sums[i];
-  }
-  if (!grad_held(p->D)) a.back = room + (groups > 1 ? kMaxSums * groups * p->D : 0);
-  all.groups = groups;
-  all.D = p->D;
-  const int st = for_types(p->r_dtype, p->y_dtype, [&](auto r, auto y) {
-    return p->post ? launch_grad<decltype(r)::value, decltype(y)::value, true>(g, a, (unsigned)groups, s)
-                   : launch_grad<decltype(r)::value, decltype(y)::value, false>(g, a, (unsigned)groups, s);
-  });
-  return st ? st : launch_sums(all, count, s);
+  return norm_backward(p, stats, d, 0, workspace, workspace_bytes, stream);
+}
+
+int fp64emu_norm_f8_backward_wide(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d, void* workspace,
+                                  size_t workspace_bytes, fp64emu_stream_t stream) {
+  return norm_backward(p, stats, d, 1, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

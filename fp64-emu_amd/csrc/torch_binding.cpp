@@ -316,6 +316,7 @@ fp64emu_f8_t kept_of(const at::Tensor& like, const at::Tensor& hq, const at::Ten
 }
 
 constexpr int64_t kPlain = 0, kRows = 1, kBoth = 2;    // what form an activation's result takes
+constexpr int64_t kNone = 3;                           // act_f8_backward: the sums alone
 
 using Maybe = std::optional<at::Tensor>;
 
@@ -550,6 +551,7 @@ struct Asked {
   std::optional<NewF8> rows, cols;
   std::vector<at::Tensor> out;
   Asked(const at::Tensor& v, int64_t M, int64_t D, int64_t quant) {
+    if (quant == kNone) return;
     if (quant == kPlain) {
       x = fresh({M, D}, v.scalar_type(), v);
       out.push_back(x);
@@ -628,11 +630,11 @@ fp64emu_norm_t norm_of(const at::Tensor& r, const at::Tensor& w, const Maybe& y,
 
 }  // namespace
 
-// dy act'(h): plain, its (q, s), or (q, s, qt, st); with bias then its sum over the rows.
+// dy act'(h): plain, its (q, s), (q, s, qt, st), or nothing; with bias then its sum over the rows.
 std::vector<at::Tensor> fp64_emu_act_f8_backward(const at::Tensor& dy, const Maybe& h, int64_t act, int64_t quant,
                                                  bool bias) {
   TORCH_CHECK(dy.dim() == 2, "expect dy as [M, N]");
-  check_quant(quant);
+  if (quant != kNone || !bias) check_quant(quant);
   TORCH_CHECK(act == FP64EMU_ACT_NONE || h.has_value(), "an activation's gradient needs h");
   const at::Tensor v = in_rows(dy);
   check_rows(v, "dy");
@@ -701,11 +703,11 @@ std::vector<at::Tensor> fp64_emu_norm_f8(const at::Tensor& r, const at::Tensor& 
   return out;
 }
 
-// Its gradient: dr, then, of what is there, dy, dw, dpost and dgate.
+// Its gradient: dr, then, of what is there, dy, dw, dpost and dgate; that of a gate for each row in its type, or with wide in float32.
 std::vector<at::Tensor> fp64_emu_norm_f8_backward(const at::Tensor& dx, const Maybe& dr, const at::Tensor& r,
                                                   const at::Tensor& w, const at::Tensor& stats, const Maybe& y,
                                                   const Maybe& post, const Maybe& gate, double scale, int64_t drop,
-                                                  const Maybe& rng) {
+                                                  const Maybe& rng, bool wide) {
   TORCH_CHECK(r.is_cuda(), "r must be on a GPU");
   std::vector<at::Tensor> hold;
   const fp64emu_norm_t p = norm_of(r, w, y, post, gate, scale, drop, rng, 1.0, hold);
@@ -738,11 +740,12 @@ std::vector<at::Tensor> fp64_emu_norm_f8_backward(const at::Tensor& dx, const Ma
   d.dw = static_cast<float*>(made({p.D}, at::kFloat));
   if (post) d.dpost = static_cast<float*>(made({p.D}, at::kFloat));
   if (gate && gate->dim() == 1) d.dgate = static_cast<float*>(made({p.D}, at::kFloat));
-  else if (gate) d.dgates = made({p.M, p.D}, gate->scalar_type());
+  else if (gate) d.dgates = made({p.M, p.D}, wide ? at::kFloat : gate->scalar_type());
   const size_t bytes = fp64emu_norm_f8_backward_workspace(&p);
   at::Tensor ws;
   if (bytes) ws = workspace(r, bytes);
-  check_status(fp64emu_norm_f8_backward(&p, stats.data_ptr<float>(), &d, pointer(ws), bytes, current_stream(r)));
+  const auto backward = wide ? fp64emu_norm_f8_backward_wide : fp64emu_norm_f8_backward;
+  check_status(backward(&p, stats.data_ptr<float>(), &d, pointer(ws), bytes, current_stream(r)));
   return out;
 }
 
@@ -760,7 +763,7 @@ TORCH_LIBRARY(fp64_emu, ops) {
   ops.def("fp64_emu_act_f8_backward(Tensor dy, Tensor? h, int act, int quant, bool bias) -> Tensor[]");
   ops.def("fp64_emu_dropout_f8(Tensor x, int drop, Tensor? rng, int quant) -> Tensor[]");
   ops.def("fp64_emu_norm_f8(Tensor r, Tensor w, Tensor? y, Tensor? post, Tensor? gate, float scale, int drop, Tensor? rng, int quant, bool keep, float eps) -> Tensor[]");
-  ops.def("fp64_emu_norm_f8_backward(Tensor dx, Tensor? dr, Tensor r, Tensor w, Tensor stats, Tensor? y, Tensor? post, Tensor? gate, float scale, int drop, Tensor? rng) -> Tensor[]");
+  ops.def("fp64_emu_norm_f8_backward(Tensor dx, Tensor? dr, Tensor r, Tensor w, Tensor stats, Tensor? y, Tensor? post, Tensor? gate, float scale, int drop, Tensor? rng, bool wide=False) -> Tensor[]");
   ops.def("fp64_emu_swiglu_f8(Tensor h, int quant, bool keep) -> Tensor[]");
   ops.def("fp64_emu_swiglu_f8_backward(Tensor dy, Tensor hq, Tensor hs, int quant) -> Tensor[]");
 }

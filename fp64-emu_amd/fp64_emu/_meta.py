@@ -69,8 +69,8 @@ def _swiglu_backward(dy, hq, hs, quant):
 
 def _asked(like, M, D, quant):
     e4m3 = torch.float8_e4m3fn
-    if quant == 0:
-        return [like.new_empty((M, D))]
+    if quant in (0, 3):
+        return [like.new_empty((M, D))] if quant == 0 else []
     return _f8(like, (), M, D, M, _blocks(D), e4m3) + (_f8(like, (), D, M, D, _blocks(M), e4m3) if quant == 2 else [])
 
 
@@ -94,12 +94,13 @@ def _norm(r, w, y, post, gate, scale, drop, rng, quant, keep, eps):
     return out + ([r.new_empty((1 if post is None else 2, M), dtype=torch.float32)] if keep else [])
 
 
-def _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng):
+def _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng, wide=False):
     M, D = r.shape
     out = [r.new_empty((M, D))] + ([] if y is None else [y.new_empty((M, D))])
     out += [r.new_empty((D,), dtype=torch.float32) for _ in range(1 if post is None else 2)]
     if gate is not None:
-        out.append(r.new_empty((D,), dtype=torch.float32) if gate.dim() == 1 else gate.new_empty((M, D)))
+        shape = (D,) if gate.dim() == 1 else (M, D)
+        out.append(gate.new_empty(shape, dtype=torch.float32 if wide or gate.dim() == 1 else gate.dtype))
     return out
 
 

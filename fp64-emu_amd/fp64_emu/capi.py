@@ -29,7 +29,8 @@ EXPORTS = ("fp64emu_maxp", "fp64emu_last_error", "fp64emu_workspace_size",
            "fp64emu_mm_f8_workspace", "fp64emu_mm_f8_plan", "fp64emu_mm_f8", "fp64emu_swiglu_f8",
            "fp64emu_swiglu_f8_backward", "fp64emu_mm_f8_epilogue_workspace", "fp64emu_mm_f8_epilogue",
            "fp64emu_act_f8_backward_workspace", "fp64emu_act_f8_backward", "fp64emu_dropout_f8",
-           "fp64emu_norm_f8", "fp64emu_norm_f8_backward_workspace", "fp64emu_norm_f8_backward")
+           "fp64emu_norm_f8", "fp64emu_norm_f8_backward_workspace", "fp64emu_norm_f8_backward",
+           "fp64emu_norm_f8_backward_wide")
 
 NOALLOC_SCRATCH_BYTES = 64 << 20   # FP64EMU_NOALLOC_SCRATCH_BYTES
 
@@ -175,8 +176,9 @@ def lib():
     L.fp64emu_norm_f8.restype = i32
     L.fp64emu_norm_f8_backward_workspace.argtypes = [norm]
     L.fp64emu_norm_f8_backward_workspace.restype = sz
-    L.fp64emu_norm_f8_backward.argtypes = [norm, vp, ctypes.POINTER(NormGrad), vp, sz, vp]
-    L.fp64emu_norm_f8_backward.restype = i32
+    for backward in (L.fp64emu_norm_f8_backward, L.fp64emu_norm_f8_backward_wide):
+        backward.argtypes = [norm, vp, ctypes.POINTER(NormGrad), vp, sz, vp]
+        backward.restype = i32
     _LIB = L
     return L
 

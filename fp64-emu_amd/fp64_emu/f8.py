@@ -46,6 +46,7 @@ from ._ops import ops
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BLOCK = 128
 _FORMS = {None: 0, "rows": 1, "both": 2}
+_SUMS = 3                                   # act_f8_backward's form without dh, dbias alone
 _ACTS = {None: 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
 
 # The overloads themselves: resolving a packet's overload costs a microsecond a call.
@@ -224,11 +225,16 @@ def norm_f8_backward(dx: torch.Tensor, dr: torch.Tensor, r: torch.Tensor, w: tor
 
     Returns (dr, dy, dw, dpost, dgate), None for what is absent: dr in r's type, dy in y's, dw, dpost
     and the gradient of a gate [D] float32, that of a gate [M, D] in its type."""
+    return _norm_gradients(dx, dr, r, w, stats, y, post, gate, scale, p, rng, False)
+
+
+def _norm_gradients(dx, dr, r, w, stats, y, post, gate, scale, p, rng, wide):
+    """norm_f8_backward; wide: the gradient of a gate [M, D] in float32."""
     drop = _drop(p, rng)
     shape = _check_norm(r, w, y, post, gate, scale, drop)
     if dx.shape != shape or (dr is not None and dr.shape != shape):
         raise ValueError(f"dx and dr must have r's shape {tuple(shape)}")
-    got = _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng)
+    got = _norm_backward(dx, dr, r, w, stats, y, post, gate, scale, drop, rng, wide)
     if y is None:
         return got[0], None, got[1], None, None
     return got[0], got[1], got[2], None if post is None else got[3], None if gate is None else got[-1]
@@ -360,18 +366,46 @@ def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
     return _SwigluCkpt.apply(h, torch.is_grad_enabled())
 
 
+def _gate_rows(gate, shape, dtype):
+    """A gate that spreads to `shape` [.., D] as norm_f8 takes it: [D] where all rows have one, else a row for each, in dtype."""
+    if gate is None or gate.shape == shape[-1:] or (gate.dim() == 1 and gate.numel() != 1):
+        return gate
+    if gate.shape[-1:] == shape[-1:] and gate.numel() == shape[-1] and gate.dim() <= len(shape):
+        return gate.reshape(shape[-1:])
+    return _as_rows(gate.to(dtype).expand(shape))
+
+
+def _column_sums(t):
+    """Of float32 [M, N]: by act_f8_backward's kernels, in an order that the sizes say, and without the memset that a library's
+    sum leaves in a captured graph."""
+    return _act_backward(t, None, 0, _SUMS, True)[0]
+
+
+def _sum_to(t, shape):
+    """Float32 t summed over the dimensions along which a tensor of `shape` spreads to t's."""
+    full, lead = t.shape, (1,) * (t.dim() - len(shape)) + tuple(shape)
+    over = [i for i in range(len(full) - 1) if lead[i] != full[i]]
+    rest = [i for i in range(len(full)) if i not in over]
+    if over:
+        count = math.prod([full[i] for i in over])
+        t = _column_sums(t.permute(over + rest).reshape(count, math.prod([full[i] for i in rest])))
+    if lead[-1] != full[-1]:
+        t = _column_sums(t.reshape(math.prod([full[i] for i in rest[:-1]]), full[-1]).t())
+    return t.reshape(shape)
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, r, w, y, post, gate, scale, p, rng, eps, grad):
         flat = [_as_rows(t) if t is not None else None for t in (r, y)]
-        gates = _as_rows(gate) if gate is not None and gate.dim() > 1 else gate
+        gates = _gate_rows(gate, r.shape, (r if y is None else y).dtype)
         keep = grad and any(ctx.needs_input_grad[:5])
         got = norm_f8(flat[0], w, flat[1], post, gates, scale, p, rng, keep=keep, eps=eps)
         ctx.scale, ctx.p, ctx.joined = scale, p, y is not None
         if keep:
             # (rng may go on in place before the backward pass.)
             rng = rng.clone() if p and rng is not None else None
-            ctx.save_for_backward(got[0] if ctx.joined else flat[0], w, flat[1], post, gates, got[-1], rng)
+            ctx.save_for_backward(got[0] if ctx.joined else flat[0], w, flat[1], post, gate, got[-1], rng)
         ctx.set_materialize_grads(False)
         out = tuple(t.view(r.shape) for t in got[:2 if ctx.joined else 1])
         return out if ctx.joined else out[0]
@@ -386,11 +420,14 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 10
         dx = torch.zeros_like(r if y is None else y) if dx is None else _as_rows(dx)
         dr = _as_rows(dr) if dr is not None else None
-        dr, dy, dw, dpost, dgate = norm_f8_backward(dx, dr, r, w, stats, y, post, gate, ctx.scale, ctx.p, rng)
+        gates = _gate_rows(gate, shape, (r if y is None else y).dtype)
+        # (Of a gate that rows share, or of another type than y, in float32 until it is what is returned.)
+        wide = gates is not None and gates.dim() == 2 and (gate.shape != shape or gate.dtype != y.dtype)
+        dr, dy, dw, dpost, dgate = _norm_gradients(dx, dr, r, w, stats, y, post, gates, ctx.scale, ctx.p, rng, wide)
         dy = dy.view(shape) if dy is not None else None
         dpost = dpost.to(post.dtype) if post is not None else None
         if gate is not None:
-            dgate = dgate.to(gate.dtype) if gate.dim() == 1 else dgate.view(shape)
+            dgate = (_sum_to(dgate.view(shape), gate.shape) if gates.dim() == 2 else dgate.view(gate.shape)).to(gate.dtype)
         return dr.view(shape), dw.to(w.dtype), dy, dpost, dgate, None, None, None, None, None
 
 
@@ -399,11 +436,11 @@ def residual_norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, p
                      eps: float = 1e-6):
     """(r', x) of norm_f8 in their plain forms for r [.., D], x alone without y.  Differentiable once, in r,
     w, y, post and gate: [D], or of a shape that spreads to r's, as a gate for each sequence or
-    token does.  What is kept is r', y, and two floats a row."""
+    token does.  A gate that is not one row for all is rounded to y's type, and spread to [.., D] for each
+    pass; its gradient is summed in float32 and rounded once to its own type.  What is kept is r', y, w, post, gate as
+    it was given, and two floats a row."""
     if r.dim() < 1 or w.dim() != 1:
         raise ValueError(f"expect r [.., D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
-    if gate is not None and gate.shape != r.shape[-1:] and (gate.dim() != 1 or gate.numel() == 1):
-        gate = gate.expand(r.shape)
     if y is not None and y.shape != r.shape:
         raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")
     return _ResidualNorm.apply(r, w, y, post, gate, scale, p, rng, eps, torch.is_grad_enabled())

@@ -451,6 +451,11 @@ size_t fp64emu_norm_f8_backward_workspace(const fp64emu_norm_t* p);
 int fp64emu_norm_f8_backward(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d,
                              void* workspace, size_t workspace_bytes, fp64emu_stream_t stream);
 
+/* The same with dgates [M, D] in float32, whatever y's dtype: of a gate that rows share, whose gradient is its
+ * sum over them. */
+int fp64emu_norm_f8_backward_wide(const fp64emu_norm_t* p, const float* stats, const fp64emu_norm_grad_t* d,
+                                  void* workspace, size_t workspace_bytes, fp64emu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -77,3 +77,32 @@ def test_compiled_operators(dev, backend):
     torch._dynamo.reset()
     got = torch.compile(step, backend=backend, fullgraph=True)(r, y, w, state)
     assert len(got) == len(want) and all(torch.equal(a.float(), b.float()) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_shared_gates(dev, backend):
+    print("case compiled shared gates", backend, flush=True)
+    t = [randn(*s, seed=i).to(dev) for i, s in enumerate([(3, 50, 256), (256,), (3, 50, 256), (3, 1, 256), (3, 50, 1)])]
+    leaves = [v.requires_grad_() for v in t]
+
+    def net(r, w, y, g, h):
+        new, x = fp64_emu.residual_norm_f8(r, w, y, gate=g)
+        return fp64_emu.residual_norm_f8(new, w, x.to(BF16), gate=h)
+
+    want = net(*leaves)
+    dy = [randn(3, 50, 256, seed=9 + i, dtype=v.dtype).to(dev) for i, v in enumerate(want)]
+    grads = torch.autograd.grad(want, leaves, dy)
+    torch._dynamo.reset()
+    got = torch.compile(net, backend=backend, fullgraph=True)(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, dy), grads))
+
+
+def test_layouts_of_fakes_of_sums(dev):
+    """The forms that autograd uses: a gate's gradient in float32, a bias's gradient alone."""
+    print("case fakes of sums", flush=True)
+    r, w, stats = randn(70, 300, seed=1).to(dev), randn(300, seed=2).to(dev), torch.ones(1, 70, device=dev)
+    y = r.to(BF16)
+    ops = torch.ops.fp64_emu
+    _same_layout(lambda r, w, y, s: ops.fp64_emu_norm_f8_backward(y, r, r, w, s, y, None, y, 1.0, 0, None, True), r, w, y, stats)
+    _same_layout(lambda r: ops.fp64_emu_act_f8_backward(r, None, 0, 3, True), r)

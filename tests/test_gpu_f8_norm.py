@@ -455,3 +455,87 @@ def test_norm_in_place(dev, D, form):
     both = torch.cat([fresh[0], torch.zeros_like(fresh[0])], 1)
     run(both[:, :D], fresh[1], fresh[2], both[:, D:], torch.empty(M, D, dtype=BF16, device=dev) if form == "x" else None)
     assert torch.equal(both[:, :D], fresh[0])
+
+
+# ---- Gates that rows share.
+
+GATES = [(), (1,), (1, 1, 96), (96,), (3, 1, 96), (1, 700, 96), (3, 700, 1), (3, 1, 1), (1, 1, 1), (700, 96), (3, 700, 96)]
+
+
+@pytest.mark.parametrize("gate_type", [F32, BF16, FP16])
+@pytest.mark.parametrize("shape", GATES)
+def test_shared_gates(dev, shape, gate_type):
+    """Beside a bfloat16 branch a gate of any shape and type: what it gives is what its spread rows in bfloat16 (or the one row
+    for all as it is) give, its gradient the float32 sum of theirs, rounded once to its own type."""
+    print("case shared gates", shape, gate_type, flush=True)
+    lead, D = (3, 700), 96
+    M, U = 2100, 2.0 ** -24
+    r, y = randn(*lead, D, seed=1).to(dev), randn(*lead, D, seed=2, dtype=BF16).to(dev)
+    w, post = (1 + 0.1 * randn(D, seed=3)).to(dev), (1 + 0.1 * randn(D, seed=4)).to(dev)
+    gate = (0.3 + randn(*shape, seed=5, scale=0.2)).to(dev, gate_type).requires_grad_()
+    a, b = randn(*lead, D, seed=6).to(dev), randn(*lead, D, seed=7, dtype=BF16).to(dev)
+    state = rng(3, 1, dev)
+    got = fp64_emu.residual_norm_f8(r, w, y, post, gate, 0.75, 0.25, state)
+    grad, = torch.autograd.grad(got, gate, (a, b))
+    one = shape in ((1, 1, 96), (96,))
+    rows = gate.detach().reshape(D) if one else gate.detach().to(BF16).expand(*lead, D).reshape(M, D).contiguous()
+    new, x, stats = fp64_emu.norm_f8(r.view(M, D), w, y.view(M, D), post, rows, 0.75, 0.25, state, keep=True)
+    assert torch.equal(got[0].view(M, D), new) and torch.equal(got[1].view(M, D), x)
+    wide = [t.to(F64) for t in (b.view(M, D), a.view(M, D), new, w, stats[0][:, None], y.view(M, D), stats[1][:, None], post, rows)]
+    each, err = norm_grad(*wide, scale=0.75, drop=factors(3, 1, 0.25, M, D).to(dev))["dgate"]
+    to = lambda t: t.view(*lead, D).sum_to_size(shape)  # noqa: E731
+    assert grad.shape == shape and grad.dtype == gate_type
+    # Of a sum of n rows: a thread's (16), two exchanges of lanes, four waves, and of the n / 16 groups' parts a sixteenth and then
+    # 16 waves' one after the other, 40 + n / 256 and for columns 40 more: at most 120 roundings of what is summed so far.  (With
+    # terms rounded to bfloat16 those of 700 rows would be off by 700^1/2 2^-9 / 3^1/2 = 0.03 of one; this is 700 200 U = 0.008.)
+    close(grad, to(each), to(err) + 120 * U * to(each.abs() + err))
+
+
+def test_shared_gate_keeps_the_gate_alone(dev):
+    """For the backward pass the gate is kept as it was given, not spread."""
+    print("case shared gate kept", flush=True)
+    r, y, w = randn(4, 500, 256, seed=1).to(dev), randn(4, 500, 256, seed=2).to(dev), torch.ones(256, device=dev)
+    gate = randn(4, 1, 256, seed=3).to(dev).requires_grad_()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        fp64_emu.residual_norm_f8(r, w, y, gate=gate)
+    assert sum(t.numel() for t in kept) == 2 * r.numel() + 2000 + w.numel() + gate.numel()
+
+
+def test_shared_gates_captured(dev):
+    """Forward and backward in a graph, with gates whose gradients are sums over rows, columns and both: each replay gives the
+    eager bits."""
+    print("case shared gates captured", flush=True)
+    B, S, D = 3, 900, 320
+    t = {"r": randn(B, S, D, seed=1, dtype=BF16).to(dev), "w": randn(D, seed=2).to(dev), "y": randn(B, S, D, seed=3, dtype=BF16).to(dev),
+         "post": randn(D, seed=4).to(dev)}
+    gates = [randn(*s, seed=5 + i).to(dev) for i, s in enumerate([(B, 1, D), (B, S, 1), (1, S, D), ()])]
+    a, b = randn(B, S, D, seed=9, dtype=BF16).to(dev), randn(B, S, D, seed=10, dtype=BF16).to(dev)
+    state = rng(1, 2, dev)
+
+    def step():
+        out = []
+        for gate in gates:
+            leaves = [v.detach().requires_grad_() for v in (*t.values(), gate)]
+            got = fp64_emu.residual_norm_f8(*leaves, 0.5, 0.25, state)
+            out += [*(v.detach() for v in got), *torch.autograd.grad(got, leaves, (a, b))]
+        return out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(3):
+        t["y"].mul_(0.5)
+        gates[turn].add_(0.25)
+        state += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = [v.clone() for v in got]
+        assert all(torch.equal(u, v) for u, v in zip(seen, step())), turn
+        torch.cuda.synchronize()
