@@ -270,50 +270,58 @@ def _as_rows(t):
     return t.reshape(math.prod(t.shape[:-1]), t.size(-1))
 
 
+# The functions below take and give matrices: flattened and unfolded around them, results are no views made inside,
+# which could not be written in place.
+
+def _flat(t):
+    return t if t is None or t.dim() == 2 else _as_rows(t)
+
+
+def _unfold(t, lead):
+    return t if len(lead) == 1 else t.view(*lead, t.size(1))
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, wq, ws, wqt, wst, bias, act, residual, grad):
-        rows = _as_rows(x)
         # (needs_input_grad does not heed no_grad, and in here gradients are always off.)
         wants_x, wants_w, wants_b = (grad and ctx.needs_input_grad[i] for i in (0, 1, 6))
-        q, s, *kept = quant_f8(rows, cols=wants_w)
+        q, s, *kept = quant_f8(x, cols=wants_w)
         if wq is None:
             wq, ws, *across = quant_f8_tiles(w.detach(), transposed=wants_x)
             wqt, wst = across if wants_x else (None, None)
         elif wants_x and wqt is None:
             raise ValueError("wq lacks the transposed half that x's gradient reads")
         ctx.act, ctx.wants_b = act, wants_b
-        ctx.shape, ctx.w_dtype, ctx.x_dtype = x.shape, w.dtype, x.dtype
+        ctx.w_dtype, ctx.x_dtype = w.dtype, x.dtype
         ctx.b_dtype = bias.dtype if bias is not None else None
-        shape, h = (*x.shape[:-1], w.size(0)), None
+        h = None
         if bias is None and act is None and residual is None:
             y = mm_f8(q, s, wq, ws, out_dtype=x.dtype)
         else:
             keep = act is not None and (wants_x or wants_w or wants_b)
-            added = _as_rows(residual) if residual is not None else None
-            y = mm_f8(q, s, wq, ws, out_dtype=x.dtype, bias=bias, act=act, residual=added, keep=keep)
+            y = mm_f8(q, s, wq, ws, out_dtype=x.dtype, bias=bias, act=act, residual=residual, keep=keep)
             y, h = y if keep else (y, None)
         ctx.save_for_backward(*(kept if wants_w else (None, None)),
                               *((wqt, wst) if wants_x else (None, None)), h)
-        return y.view(shape)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xqt, xst, wqt, wst, h = ctx.saved_tensors
-        rows = _as_rows(dy)
         dx = dw = db = None
         got = ()
         if ctx.wants_b or h is not None:
             quant = "both" if xqt is not None else "rows" if wqt is not None else None
-            got = act_f8_backward(rows, h, ctx.act, quant, bias=ctx.wants_b)
+            got = act_f8_backward(dy, h, ctx.act, quant, bias=ctx.wants_b)
             if ctx.wants_b:
                 *got, db = got
                 db = db.to(ctx.b_dtype)
         elif wqt is not None or xqt is not None:
-            got = quant_f8(rows, rows=wqt is not None, cols=xqt is not None)
+            got = quant_f8(dy, rows=wqt is not None, cols=xqt is not None)
         if wqt is not None:
-            dx = mm_f8(got[0], got[1], wqt, wst, out_dtype=ctx.x_dtype).view(ctx.shape)
+            dx = mm_f8(got[0], got[1], wqt, wst, out_dtype=ctx.x_dtype)
         if xqt is not None:
             dw = mm_f8(got[-2], got[-1], xqt, xst, out_dtype=ctx.w_dtype)
         return dx, dw, None, None, None, None, db, None, dy if ctx.needs_input_grad[8] else None, None
@@ -341,21 +349,21 @@ def linear_f8(x: torch.Tensor, w: torch.Tensor, wq: tuple = None, bias: torch.Te
         raise ValueError(f"expect bias as [N], got {tuple(bias.shape)}")
     if residual is not None and (residual.shape != (*x.shape[:-1], w.size(0)) or residual.dtype != x.dtype):
         raise ValueError(f"expect residual as {(*x.shape[:-1], w.size(0))} in x's type")
-    return _Linear.apply(x, w, *(wq + (None,) * (4 - len(wq))), bias, act, residual, torch.is_grad_enabled())
+    y = _Linear.apply(_flat(x), w, *(wq + (None,) * (4 - len(wq))), bias, act, _flat(residual), torch.is_grad_enabled())
+    return _unfold(y, x.shape[:-1])
 
 
 class _SwigluCkpt(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, grad):
-        y, *kept = swiglu_f8(_as_rows(h), keep=grad and ctx.needs_input_grad[0])
+        y, *kept = swiglu_f8(h, keep=grad and ctx.needs_input_grad[0])
         ctx.save_for_backward(*kept)
-        ctx.shape = h.shape
-        return y.view(*h.shape[:-1], y.size(1))
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return swiglu_f8_backward(_as_rows(dy), *ctx.saved_tensors).view(ctx.shape), None
+        return swiglu_f8_backward(dy, *ctx.saved_tensors), None
 
 
 def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
@@ -363,7 +371,7 @@ def swiglu_ckpt_f8(h: torch.Tensor) -> torch.Tensor:
     backward pass reads an 8-bit checkpoint of h instead of h."""
     if h.dim() < 1 or h.size(-1) % 2:
         raise ValueError(f"expect h as [.., 2 F], got {tuple(h.shape)}")
-    return _SwigluCkpt.apply(h, torch.is_grad_enabled())
+    return _unfold(_SwigluCkpt.apply(_flat(h), torch.is_grad_enabled()), h.shape[:-1])
 
 
 def _gate_rows(gate, shape, dtype):
@@ -396,39 +404,36 @@ def _sum_to(t, shape):
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, r, w, y, post, gate, scale, p, rng, eps, grad):
-        flat = [_as_rows(t) if t is not None else None for t in (r, y)]
-        gates = _gate_rows(gate, r.shape, (r if y is None else y).dtype)
+    def forward(ctx, r, w, y, post, gate, shape, scale, p, rng, eps, grad):
+        gates = _gate_rows(gate, shape, (r if y is None else y).dtype)
         keep = grad and any(ctx.needs_input_grad[:5])
-        got = norm_f8(flat[0], w, flat[1], post, gates, scale, p, rng, keep=keep, eps=eps)
-        ctx.scale, ctx.p, ctx.joined = scale, p, y is not None
+        got = norm_f8(r, w, y, post, gates, scale, p, rng, keep=keep, eps=eps)
+        ctx.shape, ctx.scale, ctx.p, ctx.joined = shape, scale, p, y is not None
         if keep:
             # (rng may go on in place before the backward pass.)
             rng = rng.clone() if p and rng is not None else None
-            ctx.save_for_backward(got[0] if ctx.joined else flat[0], w, flat[1], post, gate, got[-1], rng)
+            ctx.save_for_backward(got[0] if ctx.joined else r, w, y, post, gate, got[-1], rng)
         ctx.set_materialize_grads(False)
-        out = tuple(t.view(r.shape) for t in got[:2 if ctx.joined else 1])
-        return out if ctx.joined else out[0]
+        return got[:2] if ctx.joined else got[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         r, w, y, post, gate, stats, rng = ctx.saved_tensors
         dr, dx = grads if ctx.joined else (None, grads[0])
-        shape = next((g.shape for g in (dr, dx) if g is not None), None)
-        if shape is None:
-            return (None,) * 10
-        dx = torch.zeros_like(r if y is None else y) if dx is None else _as_rows(dx)
-        dr = _as_rows(dr) if dr is not None else None
+        if dr is None and dx is None:
+            return (None,) * 11
+        if dx is None:
+            dx = torch.zeros_like(r if y is None else y)
+        shape = ctx.shape
         gates = _gate_rows(gate, shape, (r if y is None else y).dtype)
         # (Of a gate that rows share, or of another type than y, in float32 until it is what is returned.)
         wide = gates is not None and gates.dim() == 2 and (gate.shape != shape or gate.dtype != y.dtype)
         dr, dy, dw, dpost, dgate = _norm_gradients(dx, dr, r, w, stats, y, post, gates, ctx.scale, ctx.p, rng, wide)
-        dy = dy.view(shape) if dy is not None else None
         dpost = dpost.to(post.dtype) if post is not None else None
         if gate is not None:
             dgate = (_sum_to(dgate.view(shape), gate.shape) if gates.dim() == 2 else dgate.view(gate.shape)).to(gate.dtype)
-        return dr.view(shape), dw.to(w.dtype), dy, dpost, dgate, None, None, None, None, None
+        return dr, dw.to(w.dtype), dy, dpost, dgate, None, None, None, None, None, None
 
 
 def residual_norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, post: torch.Tensor = None,
@@ -438,12 +443,14 @@ def residual_norm_f8(r: torch.Tensor, w: torch.Tensor, y: torch.Tensor = None, p
     w, y, post and gate: [D], or of a shape that spreads to r's, as a gate for each sequence or
     token does.  A gate that is not one row for all is rounded to y's type, and spread to [.., D] for each
     pass; its gradient is summed in float32 and rounded once to its own type.  What is kept is r', y, w, post, gate as
-    it was given, and two floats a row."""
+    it was given, and two floats a row: r' is not to be changed in place before the backward pass, x may be."""
     if r.dim() < 1 or w.dim() != 1:
         raise ValueError(f"expect r [.., D] and w [D], got {tuple(r.shape)} and {tuple(w.shape)}")
     if y is not None and y.shape != r.shape:
         raise ValueError(f"y must have r's shape {tuple(r.shape)}, got {tuple(y.shape)}")
-    return _ResidualNorm.apply(r, w, y, post, gate, scale, p, rng, eps, torch.is_grad_enabled())
+    lead = r.shape[:-1]
+    got = _ResidualNorm.apply(_flat(r), w, _flat(y), post, gate, r.shape, scale, p, rng, eps, torch.is_grad_enabled())
+    return _unfold(got, lead) if y is None else (_unfold(got[0], lead), _unfold(got[1], lead))
 
 
 class _SeededDropout(torch.autograd.Function):
@@ -453,13 +460,13 @@ class _SeededDropout(torch.autograd.Function):
             ctx.p = p
             # (rng may go on in place before the backward pass.)
             ctx.save_for_backward(rng.clone() if rng is not None else None)
-        return dropout_f8(_as_rows(x), p, rng)[0].view(x.shape)
+        return dropout_f8(x, p, rng)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         rng, = ctx.saved_tensors
-        return dropout_f8(_as_rows(dy), ctx.p, rng)[0].view(dy.shape), None, None, None
+        return dropout_f8(dy, ctx.p, rng)[0], None, None, None
 
 
 def seeded_dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
@@ -467,7 +474,7 @@ def seeded_dropout_f8(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Ten
     rng's value at the call."""
     if x.dim() < 1:
         raise ValueError(f"expect x as [.., K], got {tuple(x.shape)}")
-    return _SeededDropout.apply(x, p, rng, torch.is_grad_enabled())
+    return _unfold(_SeededDropout.apply(_flat(x), p, rng, torch.is_grad_enabled()), x.shape[:-1])
 
 
 __all__ = ["quant_f8", "quant_f8_tiles", "mm_f8", "bmm_f8", "swiglu_f8", "swiglu_f8_backward",

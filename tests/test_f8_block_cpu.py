@@ -293,3 +293,20 @@ def test_norm_places():
     # Side by side: half a row's distance away, an element into the neighbour's.
     _says(call(ld_r=2 * D, out=r + 2 * D - 2, ldo=2 * D), "operand itself")
     _says(call(ld_r=2 * D, out=r + 2 * D + 2, ldo=2 * D), "operand itself")
+
+
+@pytest.mark.parametrize("lead", [(6,), (2, 3), ()])
+def test_results_may_be_written_in_place(lead):
+    """Results of the differentiable functions are tensors of their own, as a plain operator's; the new stream, which is
+    kept, is so for a program that has no gradients."""
+    e = fp64_emu
+    with FakeTensorMode():
+        x = torch.empty(*lead, 256, device="cuda", requires_grad=True)
+        w, v = torch.empty(256, device="cuda"), torch.empty(64, 256, device="cuda", requires_grad=True)
+        state = torch.empty(2, dtype=torch.int64, device="cuda")
+        for call in (lambda: e.seeded_dropout_f8(x, 0.5, state), lambda: e.linear_f8(x, v, act="relu"), lambda: e.linear_f8(x, v),
+                     lambda: e.swiglu_ckpt_f8(x), lambda: e.residual_norm_f8(x, w), lambda: e.residual_norm_f8(x, w, x)[1]):
+            out = call()
+            assert out.requires_grad and out.mul_(2.0).shape[:-1] == x.shape[:-1]
+        with torch.no_grad():
+            e.residual_norm_f8(x, w, x)[0].mul_(2.0)

@@ -528,3 +528,20 @@ def test_linear_epilogue_of_nothing(dev, shape, N):
     grads = torch.autograd.grad(y, (x, w, b, r), torch.ones_like(y))
     assert [g.shape for g in grads] == [t.shape for t in (x, w, b, r)]
     assert torch.equal(grads[2], torch.full_like(b, float(y.numel() // max(N, 1)))) and not grads[1].any()
+
+
+@pytest.mark.parametrize("lead", [(6,), (2, 3), ()])
+def test_results_in_place(dev, lead):
+    """Results written in place before the backward pass: values and gradients of the same step out of place."""
+    print("case results in place", lead, flush=True)
+    x, w, v = randn(*lead, 256, seed=1).to(dev).requires_grad_(), randn(256, seed=2).to(dev), randn(64, 256, seed=3).to(dev).requires_grad_()
+    state = rng(3, 4, dev)
+    for call in (lambda: fp64_emu.seeded_dropout_f8(x, 0.5, state), lambda: fp64_emu.linear_f8(x, v, act="silu"),
+                 lambda: fp64_emu.swiglu_ckpt_f8(x), lambda: fp64_emu.residual_norm_f8(x, w), lambda: fp64_emu.residual_norm_f8(x, w, x)[1]):
+        a, b = call().mul(2.0), call().mul_(2.0)
+        dy = randn(*a.shape, seed=5).to(dev)
+        assert torch.equal(a, b) and torch.equal(*(torch.autograd.grad(t, x, dy)[0] for t in (a, b)))
+    new, out = fp64_emu.residual_norm_f8(x, w, x)
+    new.add_(1.0)                           # (kept, and therefore said)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, x, torch.ones_like(out))
