@@ -313,8 +313,8 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         got = ()
         if ctx.wants_b or h is not None:
-            quant = "both" if xqt is not None else "rows" if wqt is not None else None
-            got = act_f8_backward(dy, h, ctx.act, quant, bias=ctx.wants_b)
+            form = _FORMS["both"] if xqt is not None else _FORMS["rows"] if wqt is not None else _SUMS
+            got = _act_backward(dy, h, _act(ctx.act), form, ctx.wants_b)
             if ctx.wants_b:
                 *got, db = got
                 db = db.to(ctx.b_dtype)

@@ -545,3 +545,14 @@ def test_results_in_place(dev, lead):
     new.add_(1.0)                           # (kept, and therefore said)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("name", [None, "silu"])
+def test_linear_bias_alone(dev, name):
+    """Where the bias alone wants a gradient dh is not written; its sum is act_f8_backward's, of plain dh's order."""
+    print("case linear bias alone", name, flush=True)
+    x, w, b = randn(70, 200, seed=1).to(dev), randn(130, 200, seed=2).to(dev), randn(130, seed=3).to(dev).requires_grad_()
+    y, dy = fp64_emu.linear_f8(x, w, bias=b, act=name), randn(70, 130, seed=4).to(dev)
+    q, s = fp64_emu.quant_f8(x)
+    _, h = fp64_emu.mm_f8(q, s, *fp64_emu.quant_f8_tiles(w), F32, bias=b.detach(), act=name, keep=True)
+    assert torch.equal(torch.autograd.grad(y, b, dy)[0], fp64_emu.act_f8_backward(dy, h, name, bias=True)[1])
