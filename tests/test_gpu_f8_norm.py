@@ -153,6 +153,15 @@ def test_norm_gradient_differences(dev):
         assert abs(have - want) <= 60 * 2.0 ** -20 / h + 10 * h * h + 1e-3 * abs(want), (name, have, want)
 
 
+@pytest.mark.parametrize("options", ["plain", "y gate", "y post gate p", "y post gates p"])
+@pytest.mark.parametrize("D", [4097, 5003, 8191])
+def test_norm_ragged_long_rows(dev, D, options):
+    """Rows of two chunks a thread whose last eight elements overlap another chunk's, forward and back."""
+    test_norm(dev, 3, D, options)
+    test_norm_gradient(dev, 2, D, options)
+    test_norm_gradient(dev, 530, D, options)        # more than a row to a work group
+
+
 @pytest.mark.parametrize("D,each", [(1003, 8), (4096, 8), (8192, 16), (20001, 24)])
 def test_norm_gradient_cancels(dev, D, each):
     """The stream mostly the branch's output, dx along it: dr + i(v) dx w and what is taken off it are large beside what is
