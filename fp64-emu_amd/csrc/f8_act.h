@@ -76,15 +76,30 @@ __device__ __forceinline__ float activated(float h) {
   return h;
 }
 
+// sigmoid(g) and 1 - sigmoid(g), the second as e^-g times the first where that nears 1: taken from 1 it would keep nothing of
+// itself there, and gelu_tanh multiplies it by up to 500 (h from 4 to 8: its slope was off by up to 32 2^-24, now by 2).  Below
+// that 1 - s is the nearer one: its error and s's go against each other.
+struct Logistic { float s, rest; };
+__device__ __forceinline__ Logistic logistic(float g) {
+  // e^-g as sigmoid() has it, but the rounding of the argument goes in as a factor, which an infinite 2^t stands; past 100,
+  // where s is 0 or 1, there is none to carry.
+  constexpr float kL = 1.44269502f, kLlo = 1.92596303e-8f;
+  const float c = __builtin_amdgcn_fmed3f(g, -100.0f, 100.0f), t = -c * kL;
+  const float lo = fmaf(-c, kLlo, fmaf(-c, kL, -t));
+  const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, 0.693147182f, 1.0f);
+  const float s = __builtin_amdgcn_rcpf(1.0f + e);
+  return {s, c > 2.0f ? e * s : 1.0f - s};
+}
+
 // d times the slope at h, to float32 accuracy whatever the operands' type: the bias's gradient and the 8-bit forms come
-// from float32 values (with 2^t coarse for 16-bit operands dbias was 1.6 times as far from 64 bits).
+// from float32 values.
 template <int kAct>
 __device__ __forceinline__ float activated_back(float h, float d) {
   if constexpr (kAct == FP64EMU_ACT_RELU) return h > 0.0f ? d : 0.0f;
   if constexpr (kAct == FP64EMU_ACT_RELU2) return d * (2.0f * (h < 0.0f ? 0.0f : h));
   if constexpr (kAct == FP64EMU_ACT_SILU) {
-    const float s = sigmoid(h);
-    return d * (s * fmaf(h, 1.0f - s, 1.0f));
+    const Logistic l = logistic(h);
+    return d * (l.s * fmaf(h, l.rest, 1.0f));
   }
   if constexpr (kAct == FP64EMU_ACT_GELU) {
     const float e = bell<true>(h);
@@ -93,8 +108,8 @@ __device__ __forceinline__ float activated_back(float h, float d) {
   if constexpr (kAct == FP64EMU_ACT_GELU_TANH) {
     // (s (1 - s) is zero long before the clamp, which keeps its factor finite.)
     const float c = __builtin_amdgcn_fmed3f(h, -100.0f, 100.0f);
-    const float s = sigmoid(h * fmaf(kTanh3 * h, h, kTanh1));
-    return d * fmaf(h * (s * (1.0f - s)), fmaf(3.0f * kTanh3 * c, c, kTanh1), s);
+    const Logistic l = logistic(h * fmaf(kTanh3 * h, h, kTanh1));
+    return d * fmaf(h * (l.s * l.rest), fmaf(3.0f * kTanh3 * c, c, kTanh1), l.s);
   }
   return d;
 }

@@ -185,6 +185,29 @@ def test_activation_values(dev, name):
     assert y[0, 0] == float("inf") and torch.isnan(y[0, 1])
 
 
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh"])
+def test_slopes_near_one(dev, name):
+    """Where sigmoid(u) nears 1 what is left of 1 keeps its own accuracy.  In roundings U of 2^-24: u of gelu_tanh is off by 6 of
+    itself, e^-u by 4 and u's, sigmoid by 3 and (1 - s) of e^-u's, s (1 - s) by 8 and e^-u's, gelu_tanh's derivative of u by 4, products and
+    sums by one each; up to u = 2, where it is taken from 1, 1 - s by what s is.  So taken everywhere, slopes were off by 31 U
+    (gelu_tanh) and 8.5 U (silu) past h = 4."""
+    print("case slopes near one", name, flush=True)
+    h = torch.linspace(-8, 8, 2 ** 20 + 1).to(dev)[None]
+    got, = fp64_emu.act_f8_backward(torch.ones_like(h), h, name)
+    x = h.to(F64)
+    want = slope(x, name)
+    if name == "silu":
+        s = torch.sigmoid(x)
+        err = 6 * want.abs() + s * (1 - s) * (8 * x.abs() + 4) + (x <= 2) * x.abs() * s * s * (3 + 4 * (1 - s))
+    else:
+        c = 2 * (2 / torch.pi) ** 0.5
+        u, du = c * (x + 0.044715 * x ** 3), c * (1 + 3 * 0.044715 * x * x)
+        s, rest = torch.sigmoid(u), torch.sigmoid(-u)
+        err = 2 * want.abs() + 3 * s + s * rest * ((6 * u.abs() + 4) + x.abs() * du * (6 * u.abs() + 17))
+        err += (u <= 2) * x.abs() * du * s * s * (3 + rest * (6 * u.abs() + 4))
+    assert ((got.to(F64) - want).abs() <= U * err).all()
+
+
 # ---- The gradient of an activation and its bias.
 
 GRAD = [(1, 1), (1, 300), (5, 17), (16, 128), (17, 129), (333, 777), (130, 1000), (300, 256), (2100, 264)]
