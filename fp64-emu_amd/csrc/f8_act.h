@@ -80,15 +80,14 @@ __device__ __forceinline__ float activated(float h) {
 // itself there, and gelu_tanh multiplies it by up to 500 (h from 4 to 8: its slope was off by up to 32 2^-24, now by 2).  Below
 // that 1 - s is the nearer one: its error and s's go against each other.
 struct Logistic { float s, rest; };
+// (|g| below 2^23: e^-g is as sigmoid() has it, but what its argument's rounding was goes in as a factor, which stays positive
+// up to there and which an infinite 2^t stands.)
 __device__ __forceinline__ Logistic logistic(float g) {
-  // e^-g as sigmoid() has it, but the rounding of the argument goes in as a factor, which an infinite 2^t stands; past 100,
-  // where s is 0 or 1, there is none to carry.
   constexpr float kL = 1.44269502f, kLlo = 1.92596303e-8f;
-  const float c = __builtin_amdgcn_fmed3f(g, -100.0f, 100.0f), t = -c * kL;
-  const float lo = fmaf(-c, kLlo, fmaf(-c, kL, -t));
+  const float t = -g * kL, lo = fmaf(-g, kLlo, fmaf(-g, kL, -t));
   const float e = __builtin_amdgcn_exp2f(t) * fmaf(lo, 0.693147182f, 1.0f);
   const float s = __builtin_amdgcn_rcpf(1.0f + e);
-  return {s, c > 2.0f ? e * s : 1.0f - s};
+  return {s, g > 2.0f ? e * s : 1.0f - s};
 }
 
 // d times the slope at h, to float32 accuracy whatever the operands' type: the bias's gradient and the 8-bit forms come
@@ -98,7 +97,7 @@ __device__ __forceinline__ float activated_back(float h, float d) {
   if constexpr (kAct == FP64EMU_ACT_RELU) return h > 0.0f ? d : 0.0f;
   if constexpr (kAct == FP64EMU_ACT_RELU2) return d * (2.0f * (h < 0.0f ? 0.0f : h));
   if constexpr (kAct == FP64EMU_ACT_SILU) {
-    const Logistic l = logistic(h);
+    const Logistic l = logistic(__builtin_amdgcn_fmed3f(h, -100.0f, 100.0f));
     return d * (l.s * fmaf(h, l.rest, 1.0f));
   }
   if constexpr (kAct == FP64EMU_ACT_GELU) {
@@ -106,10 +105,11 @@ __device__ __forceinline__ float activated_back(float h, float d) {
     return d * fmaf(h * 0.398942280f, e, normal_cdf(h, e));
   }
   if constexpr (kAct == FP64EMU_ACT_GELU_TANH) {
-    // (s (1 - s) is zero long before the clamp, which keeps its factor finite.)
+    // (s (1 - s) is zero long before the clamp, which keeps its factor finite; h itself brings a NaN along.)
     const float c = __builtin_amdgcn_fmed3f(h, -100.0f, 100.0f);
-    const Logistic l = logistic(h * fmaf(kTanh3 * h, h, kTanh1));
-    return d * fmaf(h * (l.s * l.rest), fmaf(3.0f * kTanh3 * c, c, kTanh1), l.s);
+    const float q = c * c;
+    const Logistic l = logistic(c * fmaf(kTanh3, q, kTanh1));
+    return d * fmaf(h * (l.s * l.rest), fmaf(3.0f * kTanh3, q, kTanh1), l.s);
   }
   return d;
 }
