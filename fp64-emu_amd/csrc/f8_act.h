@@ -26,7 +26,8 @@ constexpr float kTanh1 = 1.59576912f, kTanh3 = 0.0713548163f;
 
 // kFine: float32 accuracy over the whole range.  Without it 2^t is taken of t rounded once, off by |g| 1.25
 // 2^-24 of itself more: 2^-17 where an activation's tail ends, nothing beside the rounding of
-// 16-bit values, and 5 instructions instead of 11 (8192^3 with silu: 7 us less).
+// 16-bit values, and 5 instructions instead of 11 (8192^3 with silu: 7 us less).  So products to 16 bits on tiles
+// without splits take it; few rows and sums of parts, where it would save nothing, and all float32 outputs do not.
 template <bool kFine>
 __device__ __forceinline__ float sigmoid_of(float g) {
   if constexpr (kFine) return sigmoid(g);

@@ -298,9 +298,9 @@ __device__ __forceinline__ void emit_norm(const NormArgs& g, int64_t m, int64_t 
 
 // Rows whose values stay in registers from the first sum to the last store.  A work group takes
 // rows blockIdx.x kRows + .., gridDim.x kRows apart, the weights in registers throughout and the next
-// row's values on their way.  Bound by its bytes: 8192 x 4096 bfloat16 with y, post and gate 49 us in 8 bits
-// (4.9 TB/s), 46 plain (5.8: some of it stays in the 256 MB cache); the generator adds 7.  (Sixteen elements a thread: as fast, and one row
-// of 8192 5.6 us where this takes 4.4.)
+// row's values on their way.  Bound by its bytes: 8192 x 4096 bfloat16 with y, post and gate 50 us in 8 bits
+// (4.75 TB/s), 46 plain (5.8, more than the copy's 5.2); its vector units are busy for 62% of it, with the generator, which adds
+// 6% to its cycles, for 66%.  (Sixteen elements a thread: as fast, and one row of 8192 5.6 us where this takes 4.4.)
 template <int kR, int kY, class S>
 __global__ void __launch_bounds__(S::kGroup) norm_rows_kernel(NormArgs g) {
   constexpr int kT = S::kT;
@@ -401,7 +401,9 @@ __device__ __forceinline__ void joined_at(const NormArgs& g, const Drop& drop, i
 }
 
 // Rows of any length, a row to a work group of 1024, read once for each sum and once for x: past
-// the registers' 8192 elements a row's second and third reading come from L2.
+// the registers' 8192 elements a row's second and third reading come from L2 (8192 x 16384 bfloat16 with y and post
+// fetches 546 MB, r and y once being 537).  435 us by rows, 2.2 TB/s: it unpacks and joins every element three times, and its vector
+// units are busy for 64% of that.
 constexpr int kLong = 1024;
 
 template <int kR, int kY>
@@ -456,9 +458,9 @@ __global__ void __launch_bounds__(kLong) norm_long_kernel(NormArgs g) {
 }
 
 // x's columns by tiles of 128 x 128, once the rows' statistics are there.  The rows' kernel writes everything
-// else: it waits for its sums, and the stores cost it little (8192 x 4096 both ways 110 us, with the
-// statistics alone from that kernel and all outputs from this one 113; since then 93 to 99, 56 to 62 and 42
-// of them, the generator 16).  Bound by its bytes: r and y again and a byte a value, 4 TB/s.
+// else: it waits for its sums, and the stores cost it little (with the statistics alone from that kernel and all outputs
+// from this one 8192 x 4096 both ways took 3% more).  Bound by its bytes: r and y again and a byte a value, 41 to 47 us there,
+// 3.6 to 4 TB/s, of 91 both ways and 82 to 85 without the generator, which adds 14% to this kernel's cycles.
 template <int kR, int kY>
 __global__ void __launch_bounds__(kThreads, kR == FP64EMU_F32 ? 2 : 3) norm_tile_kernel(NormArgs g) {
   __shared__ TileLds lds;
@@ -636,8 +638,8 @@ __device__ __forceinline__ void join_rows(const float (&sum)[8], const Column& o
 // do not fit.  A row's values stay as they came and are worked out again after its sums; with one
 // chunk the next row's are on their way meanwhile.  A row's last, partial eight elements are its last eight: what the
 // thread beside has of them comes out the same from both and counts once in the sums (with loads and stores
-// of parts the kernel took 195 registers).  8192 x 4096 bfloat16 with everything 90 to 96 us, the last sums' 5 among
-// them: 4.2 to 4.5 TB/s of the copy's 5.2; two work groups of 512 on a CU share its vector units, which take about half
+// of parts the kernel took 195 registers).  8192 x 4096 bfloat16 with everything 90 to 97 us, the last sums' 5 among
+// them: 4.2 to 4.5 TB/s of the copy's 5.2; two work groups of 512 on a CU share its vector units, which are busy for 65% of
 // that time, and each waits for its row's one barrier.  kPost: y has a norm; without it y may be absent, too.  kGates: a gate
 // for each row, whose values and gradient do not fit 128 registers as the rest does.
 template <int kR, int kY, class S, int kC, bool kPost, bool kGates>
@@ -791,7 +793,8 @@ __global__ void __launch_bounds__(S::kGroup, kC == 1 && !kGates && kR != FP64EMU
   }
 }
 
-// Rows of any length: the row's sums, then its gradients, from two readings of it; its `back` is kept
+// Rows of any length: the row's sums, then its gradients, from two readings of it, mostly from memory both times (8192 x 16384
+// bfloat16 fetches 1971 MB, four operands once being 1074); 460 us there, and 250 the columns' kernel.  A row's `back` is kept
 // for the sums over the rows, which another kernel makes.
 template <int kR, int kY, bool kPost>
 struct GradAt {
@@ -902,7 +905,7 @@ void for_grad(int64_t D, const Fn& fn) {
 }
 
 // Work groups of a forward pass: 2^19 threads, what the card holds twice over, so that a group loads its weights
-// once for many rows (8192 x 8192 both ways 179 us; an earlier kernel took 14% more with eight times as many).
+// once for many rows (8192 x 8192 both ways 173 us; 205 with eight times as many, 180 with half).
 int64_t norm_groups(int64_t M, int64_t D) {
   int64_t groups = std::min<int64_t>(M, 512);
   if (D <= kMaxHeld)
@@ -910,8 +913,8 @@ int64_t norm_groups(int64_t M, int64_t D) {
   return groups;
 }
 // Of a gradient, as many as run at once, since each leaves D floats for each weight: 16 waves a CU where the
-// kernel keeps to 128 registers, else 8 (8192 x 4096: 101 us, float32 116; 129 and 160 with four times as many,
-// 114 with half).
+// kernel keeps to 128 registers, else 8 (8192 x 4096: 95 us, float32 117; 119 and 136 with four times as many, 103 and
+// 181 with half).
 int64_t grad_groups(const fp64emu_norm_t* p) {
   if (!grad_held(p->D)) return std::min<int64_t>(p->M, 512);
   int64_t groups = 0;

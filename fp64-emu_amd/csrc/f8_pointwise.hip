@@ -39,7 +39,8 @@ __device__ __forceinline__ void emit_sums(const float (&mine)[8], int cols, floa
 
 // One work group per 128 x 128 tile, for columns: dh in both orientations and its sums over the
 // tile's rows from one reading.  Bound by its bytes: 8192 x 8192 bfloat16 with gelu_tanh and the bias's
-// gradient 91 to 97 us, 4.2 to 4.5 TB/s of the copy's 5.2, with relu 89; the sums and their last kernel take 4 of them.
+// gradient 91 to 97 us, 4.2 to 4.5 TB/s of the copy's 5.2, with relu 90, gelu 96; the sums and their last kernel take 4 of them.
+// (Its vector units are busy for 77% of it.)
 // A kernel for each activation: with the choice in it, it spilled 250 registers and took 137.
 template <int kT, int kAct>
 __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_tile_kernel(ActGradArgs a) {
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, kT == FP64EMU_F32 ? 2 : 4) act_grad_
 }
 
 // Without columns: a work group has 16 x per rows of one block of 128 columns, a row's block on 16
-// lanes, 16 rows at a time.  8192 x 8192 plain 91 us (4.4 TB/s); 333 x 777 4.1 and the last sums' 2.5, where
+// lanes, 16 rows at a time.  8192 x 8192 plain 93 us (4.3 TB/s); 333 x 777 4.1 and the last sums' 2.5, where
 // two launches take the host 6.
 template <int kT, int kAct>
 __global__ void __launch_bounds__(kThreads) act_grad_rows_kernel(ActGradArgs a) {
@@ -128,9 +129,8 @@ __device__ __forceinline__ void dropped(const Held<kT>& x, int p, const Drop& dr
   for (int j = 0; j < 8; ++j) y[j] = kept.at(j) ? x.at(p, j) * drop.scale : 0.0f;
 }
 
-// A block of a row on 16 lanes.  8192 x 8192 bfloat16 plain 44 us (6.1 TB/s: what of it the 256 MB cache holds
-// from call to call is faster than memory), in 8 bits 47: the generator's twenty wide products for eight
-// elements hide behind the memory.
+// A block of a row on 16 lanes.  8192 x 8192 bfloat16 plain 43 us (6.2 TB/s, more than the copy's 5.2), in 8 bits 47: the
+// generator's twenty wide products for eight elements hide behind the memory.
 template <int kT>
 __global__ void __launch_bounds__(kThreads) dropout_rows_kernel(DropArgs a) {
   const Drop drop = drop_of(a.threshold, a.rng);

@@ -140,7 +140,9 @@ def mm_f8(A: torch.Tensor, sA: torch.Tensor, B: torch.Tensor, sB: torch.Tensor,
 
     bias [N], act ("relu", "relu2", "silu", "gelu", "gelu_tanh") and residual [M, N] in
     out_dtype give act(C + bias) + residual instead, from the float32 sums and rounded once;
-    keep: then (that, C + bias), the second for act_f8_backward."""
+    keep: then (that, C + bias), the second for act_f8_backward.  Which kernel a product takes follows from its sizes, and
+    with it the last bits of a 16-bit output: beside the block sums, the activation's exponential, whose argument is rounded
+    once on tiles and exact to float32 elsewhere (2^-17 of itself at most)."""
     return _product(2, A, sA, B, sB, out_dtype, out, accumulate, bias, act, residual, keep)
 
 

@@ -371,6 +371,8 @@ int fp64emu_swiglu_f8_backward(const void* dy, int dtype, int64_t M, int64_t F, 
  * rounded once.  bias [batch, N] (bias_stride 0: one for all members) in any dtype; residual and
  * keep, where h goes, [batch, M, N] in out's dtype.  Each may be NULL; residual may be out
  * itself, other overlaps not.  With an epilogue, accumulate must be 0.  e NULL: fp64emu_mm_f8.
+ * Activations of float32 outputs are float32 ones; of 16-bit outputs that a plan has on tiles without splits, the
+ * exponential's argument is rounded once (2^-17 of the result at most).
  * gelu is h Phi(h), gelu_tanh h (1 + tanh(sqrt(2 / pi) (h + 0.044715 h^3))) / 2, relu2 max(h, 0)^2. */
 enum {
   FP64EMU_ACT_NONE = 0, FP64EMU_ACT_RELU = 1, FP64EMU_ACT_RELU2 = 2, FP64EMU_ACT_SILU = 3,
