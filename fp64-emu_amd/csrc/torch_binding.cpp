@@ -257,7 +257,8 @@ fp64emu_f8_t f8_of(const at::Tensor& q, const at::Tensor& s, const char* what) {
 void check_rows(const at::Tensor& t, const char* what) {
   const int64_t d = t.dim();
   TORCH_CHECK(t.is_cuda(), what, " must be on a GPU");
-  TORCH_CHECK(t.size(d - 1) <= 1 || t.stride(d - 1) == 1, what, " must be contiguous along its rows");
+  // (A tensor of nothing keeps its strides in contiguous(), those of an expanded one.)
+  TORCH_CHECK(t.numel() == 0 || t.size(d - 1) <= 1 || t.stride(d - 1) == 1, what, " must be contiguous along its rows");
 }
 
 int64_t row_stride(const at::Tensor& t) {

@@ -310,3 +310,16 @@ def test_results_may_be_written_in_place(lead):
             assert out.requires_grad and out.mul_(2.0).shape[:-1] == x.shape[:-1]
         with torch.no_grad():
             e.residual_norm_f8(x, w, x)[0].mul_(2.0)
+
+
+def test_norm_grad_wide_refusals():
+    """The entry point with a gate's gradient in float32 refuses as the other does."""
+    L = capi.lib()
+    call = lambda p, d, stats=P: L.fp64emu_norm_f8_backward_wide(R(p), stats, d and R(d), P, 1 << 40, None)  # noqa: E731
+    lds = dict.fromkeys(("ld_dx", "ld_dr", "ld_dr_out", "ld_dy", "ld_dgates"), 256)
+    _says(call(_norm(), None), "NULL")
+    _says(call(_norm(), capi.NormGrad(dx=P, dgates=P, **lds)), "y's dtype")
+    _says(call(_norm(gate_dtype=BF16), capi.NormGrad(dx=P, dgates=P, **lds)), "of one gate")
+    _says(call(_norm(gate_dtype=BF16, ld_gate=256), capi.NormGrad(dx=P, dgates=P, dgate=P, **lds)), "a row or a matrix")
+    _says(call(_norm(gate_dtype=BF16, ld_gate=256), capi.NormGrad(dx=P, dgates=P, **{**lds, "ld_dgates": 255})), "shorter")
+    _says(call(_norm(gate_dtype=BF16, ld_gate=256), capi.NormGrad(dx=P, dgates=P, **lds), None), "null")

@@ -208,6 +208,16 @@ def test_slopes_near_one(dev, name):
     assert ((got.to(F64) - want).abs() <= U * err).all()
 
 
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh"])
+def test_slopes_far_out(dev, name):
+    """From far out on slopes are 1 and 0, however large h (an e^-u that is not quite 0 would be multiplied by it)."""
+    print("case slopes far out", name, flush=True)
+    h = torch.tensor([2.0 ** i for i in range(7, 128)]).to(dev)[None]
+    for sign, want in ((1, 1.0), (-1, 0.0)):
+        got, = fp64_emu.act_f8_backward(torch.ones_like(h), sign * h, name)
+        assert torch.equal(got, torch.full_like(got, want))
+
+
 # ---- The gradient of an activation and its bias.
 
 GRAD = [(1, 1), (1, 300), (5, 17), (16, 128), (17, 129), (333, 777), (130, 1000), (300, 256), (2100, 264)]
@@ -579,3 +589,20 @@ def test_linear_bias_alone(dev, name):
     q, s = fp64_emu.quant_f8(x)
     _, h = fp64_emu.mm_f8(q, s, *fp64_emu.quant_f8_tiles(w), F32, bias=b.detach(), act=name, keep=True)
     assert torch.equal(torch.autograd.grad(y, b, dy)[0], fp64_emu.act_f8_backward(dy, h, name, bias=True)[1])
+
+
+def test_expanded_operands_of_nothing(dev):
+    """No rows, spread from a scalar, as the gradient of a sum over them comes."""
+    print("case expanded operands of nothing", flush=True)
+    x = torch.ones((), device=dev).expand(0, 256)
+    w = torch.ones(256, device=dev)
+    assert x.stride() == (0, 0)
+    assert [t.shape for t in fp64_emu.quant_f8(x, cols=True)] == [(0, 256), (0, 2), (256, 0), (256, 0)]
+    assert fp64_emu.dropout_f8(x, 0.5, rng(1, 2, dev))[0].shape == (0, 256)
+    assert not fp64_emu.act_f8_backward(x, x, "silu", bias=True)[1].any()
+    assert fp64_emu.norm_f8(x, w, x, gate=x)[1].shape == (0, 256)
+    leaf = torch.ones(0, 256, device=dev).requires_grad_()
+    for call in (lambda: fp64_emu.residual_norm_f8(leaf, w), lambda: fp64_emu.seeded_dropout_f8(leaf, 0.5, rng(1, 2, dev)),
+                 lambda: fp64_emu.linear_f8(leaf, torch.ones(8, 256, device=dev), act="silu"), lambda: fp64_emu.swiglu_ckpt_f8(leaf)):
+        g, = torch.autograd.grad(call().sum(), leaf)
+        assert g.shape == leaf.shape

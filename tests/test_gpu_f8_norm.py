@@ -548,3 +548,12 @@ def test_shared_gates_captured(dev):
         seen = [v.clone() for v in got]
         assert all(torch.equal(u, v) for u, v in zip(seen, step())), turn
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lead,shape", [((0,), ()), ((0,), (1, 64)), ((0, 5), (0, 1, 64)), ((3, 0), (3, 1, 64)), ((3, 0), (3, 1, 1)), ((3, 0), (1,))])
+def test_shared_gates_of_no_rows(dev, lead, shape):
+    print("case shared gates of no rows", lead, shape, flush=True)
+    r, w, gate = torch.ones(*lead, 64, device=dev), torch.ones(64, device=dev), torch.ones(shape, device=dev).requires_grad_()
+    new, x = fp64_emu.residual_norm_f8(r, w, r, gate=gate)
+    grad, = torch.autograd.grad((new, x), gate, (new, x))
+    assert x.shape == r.shape and grad.shape == gate.shape and not grad.any()
