@@ -98,7 +98,7 @@ __device__ __forceinline__ float activated_back(float h, float d) {
   if constexpr (kAct == FP64EMU_ACT_RELU) return h > 0.0f ? d : 0.0f;
   if constexpr (kAct == FP64EMU_ACT_RELU2) return d * (2.0f * (h < 0.0f ? 0.0f : h));
   if constexpr (kAct == FP64EMU_ACT_SILU) {
-    const Logistic l = logistic(__builtin_amdgcn_fmed3f(h, -100.0f, 100.0f));
+    const Logistic l = logistic(__builtin_amdgcn_fmed3f(h, -1000.0f, 1000.0f));
     return d * (l.s * fmaf(h, l.rest, 1.0f));
   }
   if constexpr (kAct == FP64EMU_ACT_GELU) {
